@@ -40,7 +40,7 @@ const char* sgl_status_string(int status);
 
 /* Library version, to check that the loaded .so matches this header. */
 int sgl_abi_version(void);
-#define SGL_ABI_VERSION 16
+#define SGL_ABI_VERSION 17
 
 /* ------------------------------------------------------------------ */
 /* KV-cache store                                                      */
@@ -212,6 +212,85 @@ int sgl_fused_qknorm_rope_store(void* qkv, int64_t qkv_stride_token,
                                 int num_kv_heads, int head_dim, float eps,
                                 int flags, void* stream);
 #define SGL_FUSED_NO_K_WRITEBACK 1
+
+/*
+ * cos/sin tables of a rotary embedding scaled for contexts longer than it was
+ * trained on: cos[p, i] = m cos(p f_i), sin[p, i] = m sin(p f_i) for p < max_pos,
+ * i < rotary_dim / 2, fp32 [max_pos, rotary_dim / 2], the angle p f_i in 64 bits
+ * (sgl_rope_cos_sin_cache rounds it to fp32 as the reference does). With
+ * f_i = base^(-2 i / rotary_dim), L = original_max_position, s = factor:
+ *   NONE    f_i (scaling NULL too)
+ *   LINEAR  f_i / s
+ *   NTK     base replaced by base s^(rotary_dim / (rotary_dim - 2))
+ *   YARN    f_i (g_i / s + 1 - g_i), g_i = clamp((i - lo) / (hi - lo), 0, 1), lo and hi
+ *           the pairs that turn beta_fast and beta_slow times over L positions,
+ *           rotary_dim ln(L / (2 pi beta)) / (2 ln base), rounded down and up and
+ *           kept inside [0, rotary_dim - 1]; m = attention_factor, or, where that is 0,
+ *           0.1 ln s + 1 (1 for s <= 1)
+ *   BANDS   f_i ((1 - w_i) / s + w_i), w_i = clamp((L f_i / (2 pi) - low_freq_factor) /
+ *           (high_freq_factor - low_freq_factor), 0, 1)
+ * m is 1 for the others. rotary_dim at most 512.
+ * Replaces: RotaryEmbedding ctor cache build (src/layers/rotary_embedding.cu:75-94),
+ *           which has no scaling.
+ */
+#define SGL_ROPE_SCALING_NONE 0
+#define SGL_ROPE_SCALING_LINEAR 1
+#define SGL_ROPE_SCALING_NTK 2
+#define SGL_ROPE_SCALING_YARN 3
+#define SGL_ROPE_SCALING_BANDS 4
+typedef struct {
+  int32_t kind;
+  int32_t original_max_position;
+  double factor;
+  double beta_fast, beta_slow;
+  double low_freq_factor, high_freq_factor;
+  double attention_factor;
+} sgl_rope_scaling_t;
+int sgl_rope_scaled_cache(float* cos_cache, float* sin_cache, int64_t max_pos, int rotary_dim,
+                          double base, const sgl_rope_scaling_t* scaling, void* stream);
+
+/*
+ * One pass that rotates q and k and appends k and v to the paged pool, for any
+ * head_dim up to 1024, rotary_dim up to it (even; elements from it on pass through)
+ * and both layouts of a pair: (x[i], x[i + rotary_dim / 2]), or with
+ * SGL_ROPE_INTERLEAVED (x[2 i], x[2 i + 1]). Per token t at position positions[t]:
+ *   q_out[t] = rotated q[t];  k_cache[out_loc[t]] = rotated k[t];  v_cache[out_loc[t]] = v[t]
+ * fp32 arithmetic, one rounding per element; cos and sin are fp32 [max_pos,
+ * rotary_dim / 2] tables. q, k, v, q_out are [tokens, heads, head_dim] with strides
+ * (last dim contiguous), the caches [num_slots, num_kv_heads, head_dim] likewise.
+ * q_out may be q (same strides) and the cache rows k's own (rotation in place); other
+ * overlaps are the caller's error. A token whose slot is outside [0, num_slots) (padding)
+ * is not appended; one whose position is outside [0, max_pos) gets NaN in the rotated
+ * elements. Tokens with the same slot: which of them it then holds is open. out_loc NULL:
+ * token t goes to slot t. v and v_cache both NULL: no v. No q with num_qo_heads 0, no k
+ * and v with num_kv_heads 0.
+ * Replaces: RotaryEmbedding::forward_inplace, then MHAKVCache::store_kv
+ *           (src/layers/rotary_embedding.cu:96-178, src/kvcache/mha_kvcache.cu:111-155); the
+ *           reference has the half layout over the whole head only.
+ */
+typedef struct {
+  const void* q;
+  void* q_out;
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const float* cos;
+  const float* sin;
+  const int32_t* positions;
+  const void* out_loc;
+  int64_t tokens, num_slots, max_pos;
+  int64_t q_stride_token, q_stride_head, q_out_stride_token, q_out_stride_head;
+  int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+  int64_t kv_stride_slot, kv_stride_head;
+  int32_t num_qo_heads, num_kv_heads, head_dim, rotary_dim;
+  int32_t dtype;       /* SGL_DTYPE_BF16 or SGL_DTYPE_F16: q, k, v and the caches */
+  int32_t index_dtype; /* of out_loc: SGL_INDEX_I32 or SGL_INDEX_I64 */
+  int32_t flags;       /* 0 or SGL_ROPE_INTERLEAVED */
+  int32_t reserved;
+} sgl_rope_append_t;
+#define SGL_ROPE_INTERLEAVED 1
+int sgl_rope_append(const sgl_rope_append_t* args, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Paged attention                                                     */
@@ -463,6 +542,60 @@ int sgl_paged_mixed(const sgl_decode_plan_t* plan, const void* q,
                     int64_t o_stride_token, int64_t o_stride_head,
                     void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * Attention of a batch whose requests share a prefix (samples of one prompt, users of
+ * one system prompt, drafted tokens being verified), the prefix's K/V read once for
+ * the whole batch instead of once per request. Request r's kv sequence is the
+ * prefix_len slots prefix_indices[0 .. prefix_len), then its own
+ * indices[kv_indptr[r] .. kv_indptr[r + 1]); its query tokens are rows
+ * [qo_indptr[r], qo_indptr[r + 1]) of q, at most max_qo_len of them (qo_len), and query
+ * i sees kv j with j <= i + kv_len - qo_len, kv_len = prefix_len + own length: the
+ * result of sgl_paged_prefill over the joined sequences (of sgl_paged_decode for one
+ * query token). A row that sees nothing is zero. K and V of tokens a row does not see
+ * never reach it, whatever they hold.
+ *   sgl_prefix_plan: host plan for up to batch_size requests with up to max_tokens query
+ *     tokens together (max_qo_len of one request at most SGL_PREFIX_MAX_QO). It does not
+ *     depend on the requests' own lengths, so it serves every step of a batch (graph
+ *     capture and replay) behind a prefix of prefix_len.
+ *   sgl_prefix_attention: q and o have max_tokens rows here (at most the plan's);
+ *     rows outside [qo_indptr[0], qo_indptr[batch_size]) are left as they were. The
+ *     offsets may start past 0 (a part of a larger batch); they must not decrease. A
+ *     request whose own do, or leave the batch's or [0, max_tokens], or whose qo_len
+ *     exceeds the plan's, gets NaN rows. workspace: plan->workspace_bytes, 16-byte aligned, written before it is
+ *     read; calls that share one must be stream-ordered.
+ * q, o: bf16 [max_tokens, num_qo_heads, 128], caches one layer's bf16 [slots,
+ * num_kv_heads, 128]; strides multiples of 8 elements; 1 to 64 query heads per kv head.
+ * Replaces: no counterpart in the reference, whose batches walk every request's whole kv
+ *           (src/attention/flashinfer_backend.cu:553-679) though its radix cache shares the
+ *           slots (src/kvcache/radix_tree.cc).
+ */
+typedef struct {
+  int32_t prefix_len;
+  int32_t batch_size;
+  int32_t max_tokens;
+  int32_t max_qo_len;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t num_units;    /* workgroups that walk equal shares of the tokens */
+  int32_t tile_rows;    /* packed query rows of a walk over the prefix */
+  int32_t num_tiles;    /* such walks of the units (0: the prefix has launches of its own) */
+  int32_t num_shares;   /* shares of the prefix's own launch */
+  int32_t reserved;
+  int64_t workspace_bytes;
+} sgl_prefix_plan_t;
+#define SGL_PREFIX_MAX_QO 64
+int sgl_prefix_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len,
+                    int num_qo_heads, int num_kv_heads, int head_dim, sgl_prefix_plan_t* plan);
+int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q, int64_t q_stride_token,
+                         int64_t q_stride_head, const void* k_cache, const void* v_cache,
+                         int64_t kv_stride_slot, int64_t kv_stride_head,
+                         const int32_t* prefix_indices, const int32_t* indices,
+                         const int32_t* kv_indptr, const int32_t* qo_indptr, int batch_size,
+                         int max_tokens, int num_qo_heads, int num_kv_heads, int head_dim,
+                         float sm_scale, void* o, int64_t o_stride_token, int64_t o_stride_head,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ */
 /* Residual path: RMSNorm, fused add + RMSNorm, gated activations      */
 /* ------------------------------------------------------------------ */
@@ -644,6 +777,47 @@ typedef struct {
 } sgl_sampling_args_t;
 int64_t sgl_sampling_workspace_bytes(int batch_size, int d);
 int sgl_sampling_rows(const sgl_sampling_args_t* args, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/*
+ * Verification of drafted tokens (speculative sampling), from given random numbers.
+ * Request r's drafts are draft_tokens[i] for i in [draft_indptr[r], draft_indptr[r + 1]);
+ * its target rows, one more than its drafts, are rows draft_indptr[r] + r on of
+ * target_probs (fp32 [num_drafts + batch_size, vocab]; row i of a request: the
+ * probabilities of the token after i drafts, as sgl_softmax_temperature writes them for a
+ * batch whose q rows are the request's last token and its drafts). draft_probs: the
+ * probabilities each draft was drawn from (fp32 [num_drafts, vocab]), or NULL for drafts
+ * without any (n-gram lookup, greedy drafts: point masses). Drafts are accepted in order
+ * while accept_uniform[i] * q(x) < p(x); the next token is the first j whose running sum
+ * of max(p_j - q_j, 0) at the first rejected draft, or of p_j behind the last one, exceeds
+ * sample_uniform[r] times the sum (the last j with any weight if rounding leaves none; p
+ * where p <= q everywhere; vocab - 1 where p has no positive value). Products, differences
+ * and sums in 64 bits; NaN weighs nothing and rejects. Uniforms are in [0, 1).
+ * tokens: int32 [num_drafts + batch_size], request r's part starting at draft_indptr[r] + r:
+ * the accepted drafts, the drawn token, then -1. accepted: int32 [batch_size], accepted
+ * drafts, or -1 (and its tokens left as they were) for a request whose offsets decrease or
+ * leave [0, num_drafts]. A draft outside [0, vocab) is rejected. workspace:
+ * sgl_verify_workspace_bytes, 16-byte aligned, written before it is read; calls that share
+ * one must be stream-ordered. Up to 65,535 requests and 2^24 tokens.
+ * Replaces: no counterpart in the reference, whose Sampler draws one token per row
+ *           (src/engine/engine.cc:300-345).
+ */
+typedef struct {
+  const float* target_probs;
+  const float* draft_probs;
+  const int32_t* draft_tokens;
+  const int32_t* draft_indptr; /* [batch_size + 1] */
+  const float* accept_uniform; /* [num_drafts] */
+  const float* sample_uniform; /* [batch_size] */
+  int32_t* tokens;
+  int32_t* accepted;
+  int64_t target_stride_row, draft_stride_row; /* elements, >= vocab */
+  int64_t num_drafts;
+  int32_t batch_size;
+  int32_t vocab;
+} sgl_verify_args_t;
+int64_t sgl_verify_workspace_bytes(int batch_size, int vocab);
+int sgl_verify_drafts(const sgl_verify_args_t* args, void* workspace, int64_t workspace_bytes,
                       void* stream);
 
 #ifdef __cplusplus

@@ -27,7 +27,7 @@ SGL_INDEX_I64 = 1
 SGL_DTYPE_BF16 = 0
 SGL_DTYPE_F16 = 1
 SGL_DTYPE_F32 = 2
-ABI_VERSION = 16
+ABI_VERSION = 17
 FUSED_NO_K_WRITEBACK = 1  # SGL_FUSED_NO_K_WRITEBACK
 
 
@@ -92,6 +92,55 @@ class SamplingArgs(ctypes.Structure):
         ("d", ctypes.c_int32),
         ("max_rounds", ctypes.c_int32),
     ]
+
+
+class RopeScaling(ctypes.Structure):
+    """sgl_rope_scaling_t; kind: a key of ROPE_SCALING."""
+    _fields_ = [("kind", ctypes.c_int32), ("original_max_position", ctypes.c_int32),
+                *[(n, ctypes.c_double) for n in ("factor", "beta_fast", "beta_slow",
+                                                 "low_freq_factor", "high_freq_factor",
+                                                 "attention_factor")]]
+
+
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+ROPE_INTERLEAVED = 1  # SGL_ROPE_INTERLEAVED
+
+
+class RopeAppendArgs(ctypes.Structure):
+    """sgl_rope_append_t."""
+    _fields_ = [*[(n, ctypes.c_void_p) for n in ("q", "q_out", "k", "v", "k_cache", "v_cache",
+                                                 "cos", "sin", "positions", "out_loc")],
+                *[(n, ctypes.c_int64) for n in ("tokens", "num_slots", "max_pos",
+                                                "q_stride_token", "q_stride_head",
+                                                "q_out_stride_token", "q_out_stride_head",
+                                                "k_stride_token", "k_stride_head",
+                                                "v_stride_token", "v_stride_head",
+                                                "kv_stride_slot", "kv_stride_head")],
+                *[(n, ctypes.c_int32) for n in ("num_qo_heads", "num_kv_heads", "head_dim",
+                                                "rotary_dim", "dtype", "index_dtype", "flags",
+                                                "reserved")]]
+
+
+class PrefixPlan(ctypes.Structure):
+    """sgl_prefix_plan_t."""
+    _fields_ = [*[(n, ctypes.c_int32) for n in ("prefix_len", "batch_size", "max_tokens",
+                                                "max_qo_len", "num_qo_heads", "num_kv_heads",
+                                                "head_dim", "num_units", "tile_rows", "num_tiles",
+                                                "num_shares", "reserved")],
+                ("workspace_bytes", ctypes.c_int64)]
+
+
+PREFIX_MAX_QO = 64
+
+
+class VerifyArgs(ctypes.Structure):
+    """sgl_verify_args_t."""
+    _fields_ = [*[(n, ctypes.c_void_p) for n in ("target_probs", "draft_probs", "draft_tokens",
+                                                 "draft_indptr", "accept_uniform",
+                                                 "sample_uniform", "tokens", "accepted")],
+                *[(n, ctypes.c_int64) for n in ("target_stride_row", "draft_stride_row",
+                                                "num_drafts")],
+                ("batch_size", ctypes.c_int32), ("vocab", ctypes.c_int32)]
 
 
 class I32Copy(ctypes.Structure):
@@ -160,6 +209,16 @@ _SIGNATURES = {
     "sgl_paged_prefill_planned": ([ctypes.POINTER(PrefillPlan), _vp, _vp, _i64, _i64, _vp, _vp,
                                    _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _vp,
                                    _i64, _i64, _vp, _i64, _vp], _i32),
+    "sgl_rope_scaled_cache": ([_vp, _vp, _i64, _i32, ctypes.c_double,
+                               ctypes.POINTER(RopeScaling), _vp], _i32),
+    "sgl_rope_append": ([ctypes.POINTER(RopeAppendArgs), _vp], _i32),
+    "sgl_prefix_plan": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(PrefixPlan)],
+                        _i32),
+    "sgl_prefix_attention": ([ctypes.POINTER(PrefixPlan), _vp, _i64, _i64, _vp, _vp, _i64, _i64,
+                              _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _i64,
+                              _i64, _vp, _i64, _vp], _i32),
+    "sgl_verify_workspace_bytes": ([_i32, _i32], _i64),
+    "sgl_verify_drafts": ([ctypes.POINTER(VerifyArgs), _vp, _i64, _vp], _i32),
     "sgl_mixed_decode_cus": ([_i64, _i32, _i32, ctypes.c_double], _i32),
     "sgl_decode_plan_cus": ([_vp, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(DecodePlan)], _i32),
     "sgl_paged_mixed": ([ctypes.POINTER(DecodePlan), _vp, _i64, _i64, _vp, _vp, _i64, _i64,
@@ -484,7 +543,122 @@ def fused_qknorm_rope_store(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         "sgl_fused_qknorm_rope_store")
 
 
+def rope_scaling(kind: str, factor: float = 1.0, original_max_position: int = 0,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, low_freq_factor: float = 1.0,
+                 high_freq_factor: float = 4.0, attention_factor: float = 0.0) -> RopeScaling:
+    """sgl_rope_scaling_t; kind: none, linear, ntk, yarn or bands."""
+    if kind not in ROPE_SCALING:
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    return RopeScaling(ROPE_SCALING[kind], original_max_position, factor, beta_fast, beta_slow,
+                       low_freq_factor, high_freq_factor, attention_factor)
+
+
+def rope_scaled_cache(max_pos: int, rotary_dim: int, base: float, device: torch.device,
+                      scaling: Optional[RopeScaling] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin) of a scaled rotary embedding, float32 [max_pos, rotary_dim / 2]."""
+    cos = torch.empty((max_pos, rotary_dim // 2), dtype=torch.float32, device=device)
+    sin = torch.empty_like(cos)
+    with torch.cuda.device(cos.device):
+        _check(lib().sgl_rope_scaled_cache(_p(cos), _p(sin), max_pos, rotary_dim, base,
+                                           None if scaling is None else ctypes.byref(scaling),
+                                           _stream(cos.device)), "sgl_rope_scaled_cache")
+    return cos, sin
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor],
+                k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], cos: torch.Tensor,
+                sin: torch.Tensor, positions: torch.Tensor, out_loc: Optional[torch.Tensor],
+                interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates q [T, Hq, D] (returned, or into q_out, which may be q) and k [T, Hkv, D] and
+    appends k and v to the pool at out_loc (int32 or int64 [T]; None: slot t). The caches are
+    [slots, Hkv, D]; cos and sin [max_pos, rotary_dim / 2]; v and v_cache None: k alone."""
+    if (v is None) != (v_cache is None):
+        raise ValueError("v and v_cache go together")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    dev = _need_gpu(q, k, v, k_cache, v_cache, cos, sin, positions, out_loc, q_out)
+    T, hq, d = q.shape
+    hkv = k.shape[1]
+    dt = _dtype_code(*[t for t in (q, k, v, k_cache, v_cache, q_out) if t is not None])
+    for t, shape in ((k, (T, hkv, d)), (v, (T, hkv, d)), (q_out, (T, hq, d)),
+                     (k_cache, (k_cache.shape[0], hkv, d)), (v_cache, (k_cache.shape[0], hkv, d))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError("q, k, v, q_out and the caches must agree in tokens, heads and head_dim")
+    if any(t is not None and t.stride(2) != 1 for t in (q, k, v, q_out, k_cache, v_cache)):
+        raise ValueError("the last dimensions must be contiguous")
+    if v_cache is not None and v_cache.stride() != k_cache.stride():
+        raise ValueError("K and V caches must share strides")
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2
+            or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous())):
+        raise ValueError("cos and sin must be contiguous float32 [max_pos, rotary_dim / 2]")
+    if positions.dtype != torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 [T]")
+    if out_loc is not None and (out_loc.dtype not in (torch.int32, torch.int64)
+                                or out_loc.shape != (T,) or not out_loc.is_contiguous()):
+        raise ValueError("out_loc must be contiguous int32 or int64 [T]")
+    vs = (0, 0) if v is None else (v.stride(0), v.stride(1))
+    args = RopeAppendArgs(
+        q.data_ptr(), q_out.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(),
+        k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), cos.data_ptr(),
+        sin.data_ptr(), positions.data_ptr(), 0 if out_loc is None else out_loc.data_ptr(), T,
+        k_cache.shape[0], cos.shape[0], q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1),
+        k.stride(0), k.stride(1), vs[0], vs[1], k_cache.stride(0), k_cache.stride(1), hq, hkv, d,
+        2 * cos.shape[1], dt,
+        SGL_INDEX_I64 if out_loc is not None and out_loc.dtype == torch.int64 else SGL_INDEX_I32,
+        ROPE_INTERLEAVED if interleaved else 0, 0)
+    with torch.cuda.device(dev):
+        _check(lib().sgl_rope_append(ctypes.byref(args), _stream(dev)), "sgl_rope_append")
+    return q_out
+
+
 # ---------------------------------------------------------------- attention
+
+def prefix_plan(prefix_len: int, batch_size: int, max_tokens: int, max_qo_len: int,
+                num_qo_heads: int, num_kv_heads: int, head_dim: int) -> PrefixPlan:
+    """sgl_prefix_plan: for up to batch_size requests of up to max_qo_len query tokens
+    (max_tokens together) behind a shared prefix."""
+    plan = PrefixPlan()
+    _check(lib().sgl_prefix_plan(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads,
+                                 num_kv_heads, head_dim, ctypes.byref(plan)), "sgl_prefix_plan")
+    return plan
+
+
+def prefix_workspace(plan: PrefixPlan, device: torch.device) -> torch.Tensor:
+    return torch.empty(int(plan.workspace_bytes), dtype=torch.uint8, device=device)
+
+
+def prefix_attention(plan: PrefixPlan, q: torch.Tensor, k_cache: torch.Tensor,
+                     v_cache: torch.Tensor, prefix_indices: torch.Tensor, indices: torch.Tensor,
+                     kv_indptr: torch.Tensor, qo_indptr: torch.Tensor, o: torch.Tensor,
+                     workspace: torch.Tensor, sm_scale: Optional[float] = None) -> None:
+    """sgl_prefix_attention: o [T, Hq, D] for q [T, Hq, D], each request's kv the shared
+    prefix_indices, then its own part of indices."""
+    dev = _need_gpu(q, k_cache, v_cache, prefix_indices, indices, kv_indptr, qo_indptr, o, workspace)
+    if any(t.dtype != torch.bfloat16 for t in (q, k_cache, v_cache, o)):
+        raise ValueError("attention supports bf16 q / KV / o only")
+    if any(t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()
+           for t in (prefix_indices, indices, kv_indptr, qo_indptr)):
+        raise ValueError("the indices and offsets must be contiguous int32")
+    if q.dim() != 3 or o.shape != q.shape or q.stride(2) != 1 or o.stride(2) != 1:
+        raise ValueError("q and o must be [T, Hq, D] with a contiguous last dim")
+    if prefix_indices.numel() != plan.prefix_len:
+        raise ValueError("the plan is for another prefix length")
+    if kv_indptr.numel() != qo_indptr.numel() or kv_indptr.numel() < 1:
+        raise ValueError("kv_indptr and qo_indptr must be [batch + 1]")
+    ss, sh = _kv_strides(k_cache)
+    if v_cache.stride() != k_cache.stride() or v_cache.shape != k_cache.shape:
+        raise ValueError("K and V caches must share shape and strides")
+    hq, D = q.shape[1], q.shape[2]
+    if k_cache.shape[2] != D:
+        raise ValueError("q and the caches must share the head size")
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else sm_scale
+    with torch.cuda.device(dev):
+        _check(lib().sgl_prefix_attention(
+            ctypes.byref(plan), _p(q), q.stride(0), q.stride(1), _p(k_cache), _p(v_cache), ss, sh,
+            _p(prefix_indices), _p(indices), _p(kv_indptr), _p(qo_indptr), kv_indptr.numel() - 1,
+            q.shape[0], hq, k_cache.shape[1], D, scale, _p(o), o.stride(0), o.stride(1),
+            _p(workspace), workspace.numel() * workspace.element_size(), _stream(dev)),
+            "sgl_prefix_attention")
+
 
 def decode_plan(kv_indptr_host: Sequence[int], num_qo_heads: int, num_kv_heads: int,
                 head_dim: int) -> DecodePlan:
@@ -903,3 +1077,47 @@ def top_k_top_p_sampling_from_probs(probs, uniform_samples, top_k: Optional[torc
         int(top_k_value), float(top_p_value), probs.shape[1], uniform_samples.shape[0],
         int(deterministic), _stream(dev)), "sgl_top_k_top_p_sampling_from_probs")
     return out, ok
+
+
+def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor],
+                  draft_tokens: torch.Tensor, draft_indptr: torch.Tensor,
+                  accept_uniform: torch.Tensor, sample_uniform: torch.Tensor,
+                  workspace: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(tokens int32 [drafts + batch], accepted int32 [batch]) of sgl_verify_drafts:
+    target_probs float32 [drafts + batch, vocab], draft_probs float32 [drafts, vocab] or
+    None (point masses), draft_tokens int32 [drafts], draft_indptr int32 [batch + 1]."""
+    dev = _need_gpu(target_probs, draft_probs, draft_tokens, draft_indptr, accept_uniform,
+                    sample_uniform, workspace)
+    if draft_indptr.dim() != 1 or draft_indptr.numel() < 1:
+        raise ValueError("draft_indptr must be [batch + 1]")
+    n, b = draft_tokens.numel(), draft_indptr.numel() - 1
+    if any(t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()
+           for t in (draft_tokens, draft_indptr)):
+        raise ValueError("draft_tokens and draft_indptr must be contiguous int32")
+    if any(t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous()
+           for t in (accept_uniform, sample_uniform)):
+        raise ValueError("the uniforms must be contiguous float32")
+    if accept_uniform.numel() != n or sample_uniform.numel() != b:
+        raise ValueError("accept_uniform must be [drafts] and sample_uniform [batch]")
+    if target_probs.dim() != 2:
+        raise ValueError("target_probs must be [drafts + batch, vocab]")
+    v = target_probs.shape[1]
+    for t, rows, what in ((target_probs, n + b, "target_probs"), (draft_probs, n, "draft_probs")):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (rows, v)
+                              or (t.numel() > 0 and v > 1 and t.stride(1) != 1)):
+            raise ValueError(f"{what} must be float32 [{rows}, vocab] with contiguous rows")
+    tokens = torch.empty(n + b, dtype=torch.int32, device=dev)
+    accepted = torch.empty(b, dtype=torch.int32, device=dev)
+    if workspace is None:
+        workspace = torch.empty(lib().sgl_verify_workspace_bytes(b, v), dtype=torch.uint8, device=dev)
+    stride = lambda t: max(t.stride(0), v) if t.shape[0] <= 1 else t.stride(0)
+    args = VerifyArgs(
+        target_probs.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(),
+        draft_tokens.data_ptr(), draft_indptr.data_ptr(), accept_uniform.data_ptr(),
+        sample_uniform.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), stride(target_probs),
+        v if draft_probs is None else stride(draft_probs), n, b, v)
+    with torch.cuda.device(dev):
+        _check(lib().sgl_verify_drafts(ctypes.byref(args), _p(workspace),
+                                       workspace.numel() * workspace.element_size(), _stream(dev)),
+               "sgl_verify_drafts")
+    return tokens, accepted

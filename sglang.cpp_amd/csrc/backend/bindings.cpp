@@ -207,6 +207,62 @@ PYBIND11_MODULE(sgl_backend, m) {
       .def("cos_cache", &RotaryEmbedding::cos_cache)
       .def("sin_cache", &RotaryEmbedding::sin_cache);
 
+  py::class_<RopeScaling>(m, "RopeScaling")
+      .def(py::init([](const std::string& kind, double factor, int original, double beta_fast,
+                       double beta_slow, double low, double high, double attention) {
+             return RopeScaling{kind, factor, original, beta_fast, beta_slow, low, high, attention};
+           }),
+           py::arg("kind") = "none", py::arg("factor") = 1.0, py::arg("original_max_position") = 0,
+           py::arg("beta_fast") = 32.0, py::arg("beta_slow") = 1.0,
+           py::arg("low_freq_factor") = 1.0, py::arg("high_freq_factor") = 4.0,
+           py::arg("attention_factor") = 0.0);
+  m.def("rope_scaled_cache",
+        [](int64_t max_pos, int rotary_dim, double base, const RopeScaling& scaling, int device) {
+          return rope_scaled_cache(max_pos, rotary_dim, base, scaling, cuda(device));
+        },
+        py::arg("max_pos"), py::arg("rotary_dim"), py::arg("base"),
+        py::arg("scaling") = RopeScaling(), py::arg("device") = 0);
+  m.def("rope_append",
+        [](const torch::Tensor& q, const torch::Tensor& k, c10::optional<torch::Tensor> v,
+           const torch::Tensor& kc, c10::optional<torch::Tensor> vc, const torch::Tensor& cos,
+           const torch::Tensor& sin, const torch::Tensor& positions,
+           c10::optional<torch::Tensor> out_loc, bool interleaved,
+           c10::optional<torch::Tensor> q_out) {
+          return rope_append(q, k, v.value_or(torch::Tensor()), kc, vc.value_or(torch::Tensor()), cos,
+                             sin, positions, out_loc.value_or(torch::Tensor()), interleaved,
+                             q_out.value_or(torch::Tensor()));
+        },
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("out_loc"),
+        py::arg("interleaved") = false, py::arg("q_out") = py::none());
+  py::class_<PrefixAttention, std::shared_ptr<PrefixAttention>>(m, "PrefixAttention")
+      .def(py::init([](int prefix_len, int batch, int tokens, int qo, int hq, int hkv, int d, int device) {
+             return std::make_shared<PrefixAttention>(prefix_len, batch, tokens, qo, hq, hkv, d,
+                                                      cuda(device));
+           }),
+           py::arg("prefix_len"), py::arg("batch_size"), py::arg("max_tokens"),
+           py::arg("max_qo_len"), py::arg("num_qo_heads"), py::arg("num_kv_heads"),
+           py::arg("head_dim"), py::arg("device") = 0)
+      .def("forward",
+           [](const PrefixAttention& p, const torch::Tensor& q, const torch::Tensor& kc,
+              const torch::Tensor& vc, const torch::Tensor& prefix_indices,
+              const torch::Tensor& indices, const torch::Tensor& kv_indptr,
+              const torch::Tensor& qo_indptr, c10::optional<double> scale,
+              c10::optional<torch::Tensor> out) {
+             return p.forward(q, kc, vc, prefix_indices, indices, kv_indptr, qo_indptr, scale,
+                              out.value_or(torch::Tensor()));
+           },
+           py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("prefix_indices"),
+           py::arg("indices"), py::arg("kv_indptr"), py::arg("qo_indptr"),
+           py::arg("sm_scale") = py::none(), py::arg("out") = py::none());
+  m.def("verify_drafts",
+        [](const torch::Tensor& target, c10::optional<torch::Tensor> draft, const torch::Tensor& tokens,
+           const torch::Tensor& indptr, const torch::Tensor& accept, const torch::Tensor& sample) {
+          return verify_drafts(target, draft.value_or(torch::Tensor()), tokens, indptr, accept, sample);
+        },
+        py::arg("target_probs"), py::arg("draft_probs"), py::arg("draft_tokens"),
+        py::arg("draft_indptr"), py::arg("accept_uniform"), py::arg("sample_uniform"));
+
   py::class_<AttentionLayer, std::shared_ptr<AttentionLayer>>(m, "AttentionLayer")
       .def(py::init<int, int, int, int, std::shared_ptr<HipAttnBackend>,
                     std::shared_ptr<RotaryEmbedding>, std::shared_ptr<RMSNorm>,

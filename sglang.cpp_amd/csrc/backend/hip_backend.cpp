@@ -2,6 +2,7 @@
 #include "hip_backend.h"
 
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <hip/hip_runtime.h>
 
@@ -1229,6 +1230,224 @@ void RotaryEmbedding::forward_inplace(const torch::Tensor& positions, torch::Ten
                      cos_cache_.size(1), query.stride(0), query.stride(1), key.stride(0),
                      key.stride(1), dt, current_stream(query.device())),
             "sgl_rope");
+}
+
+namespace {
+void check_i32(const torch::Tensor& t, const torch::Device& dev, const char* what) {
+  TORCH_CHECK(t.defined() && t.device() == dev && t.scalar_type() == torch::kInt32 && t.dim() == 1 &&
+                  t.is_contiguous(),
+              what, " must be a contiguous int32 vector on the inputs' device");
+}
+
+void check_heads(const torch::Tensor& t, const torch::Tensor& like, const char* what) {
+  TORCH_CHECK(t.defined() && t.device() == like.device() && t.scalar_type() == like.scalar_type() &&
+                  t.dim() == 3 && t.stride(2) == 1,
+              what, " must be rank 3 with a contiguous last dim, on q's device and of its dtype");
+}
+
+int scaling_kind(const std::string& kind) {
+  if (kind == "none") return SGL_ROPE_SCALING_NONE;
+  if (kind == "linear") return SGL_ROPE_SCALING_LINEAR;
+  if (kind == "ntk") return SGL_ROPE_SCALING_NTK;
+  if (kind == "yarn") return SGL_ROPE_SCALING_YARN;
+  TORCH_CHECK(kind == "bands", "unknown rotary scaling: ", kind);
+  return SGL_ROPE_SCALING_BANDS;
+}
+}  // namespace
+
+std::pair<torch::Tensor, torch::Tensor> rope_scaled_cache(int64_t max_pos, int rotary_dim,
+                                                          double base, const RopeScaling& scaling,
+                                                          torch::Device device) {
+  TORCH_CHECK(max_pos >= 0 && rotary_dim > 0 && rotary_dim % 2 == 0,
+              "max_pos must not be negative and rotary_dim even and positive");
+  TORCH_CHECK(device.is_cuda(), "the tables are built on a HIP device");
+  const sgl_rope_scaling_t sc{scaling_kind(scaling.kind), scaling.original_max_position,
+                              scaling.factor, scaling.beta_fast, scaling.beta_slow,
+                              scaling.low_freq_factor, scaling.high_freq_factor,
+                              scaling.attention_factor};
+  const c10::DeviceGuard guard(device);
+  auto opts = torch::TensorOptions().dtype(torch::kFloat32).device(device);
+  auto cos = torch::empty({max_pos, rotary_dim / 2}, opts);
+  auto sin = torch::empty_like(cos);
+  check_sgl(sgl_rope_scaled_cache(cos.data_ptr<float>(), sin.data_ptr<float>(), max_pos, rotary_dim,
+                                  base, &sc, current_stream(cos.device())),
+            "sgl_rope_scaled_cache");
+  return {cos, sin};
+}
+
+torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                          const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                          const torch::Tensor& cos, const torch::Tensor& sin,
+                          const torch::Tensor& positions, const torch::Tensor& out_loc,
+                          bool interleaved, const torch::Tensor& q_out) {
+  TORCH_CHECK(q.is_cuda(), "rope_append takes HIP device tensors");
+  const c10::DeviceGuard guard(q.device());
+  sgl_rope_append_t a{};
+  a.dtype = half_dtype(q, "q");
+  check_heads(q, q, "q");
+  check_heads(k, q, "k");
+  check_heads(k_cache, q, "k_cache");
+  const int64_t T = q.size(0), hq = q.size(1), d = q.size(2), hkv = k.size(1);
+  TORCH_CHECK(k.size(0) == T && k.size(2) == d && k_cache.size(1) == hkv && k_cache.size(2) == d,
+              "q, k and k_cache must agree in tokens, kv heads and head_dim");
+  TORCH_CHECK(v.defined() == v_cache.defined(), "v and v_cache go together");
+  if (v.defined()) {
+    check_heads(v, q, "v");
+    check_heads(v_cache, q, "v_cache");
+    TORCH_CHECK(v.sizes() == k.sizes() && v_cache.sizes() == k_cache.sizes() &&
+                    v_cache.strides() == k_cache.strides(),
+                "v must match k, and v_cache k_cache");
+  }
+  for (const torch::Tensor* t : {&cos, &sin})
+    TORCH_CHECK(t->defined() && t->device() == q.device() && t->scalar_type() == torch::kFloat32 &&
+                    t->dim() == 2 && t->is_contiguous() && t->sizes() == cos.sizes(),
+                "cos and sin must be contiguous float32 [max_pos, rotary_dim / 2]");
+  check_i32(positions, q.device(), "positions");
+  TORCH_CHECK(positions.size(0) == T, "positions needs one entry per token");
+  if (out_loc.defined()) {
+    TORCH_CHECK(out_loc.device() == q.device() && out_loc.dim() == 1 && out_loc.is_contiguous() &&
+                    out_loc.size(0) == T &&
+                    (out_loc.scalar_type() == torch::kInt32 || out_loc.scalar_type() == torch::kInt64),
+                "out_loc must be a contiguous int32 or int64 vector with one entry per token");
+    a.out_loc = out_loc.data_ptr();
+    a.index_dtype = out_loc.scalar_type() == torch::kInt64 ? SGL_INDEX_I64 : SGL_INDEX_I32;
+  }
+  if (q_out.defined()) check_heads(q_out, q, "q_out");
+  TORCH_CHECK(!q_out.defined() || q_out.sizes() == q.sizes(), "q_out must have q's shape");
+  auto out = q_out.defined() ? q_out : torch::empty({T, hq, d}, q.options());
+  a.q = q.data_ptr();
+  a.q_out = out.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.defined() ? v.data_ptr() : nullptr;
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v.defined() ? v_cache.data_ptr() : nullptr;
+  a.cos = cos.data_ptr<float>();
+  a.sin = sin.data_ptr<float>();
+  a.positions = positions.data_ptr<int32_t>();
+  a.tokens = T;
+  a.num_slots = k_cache.size(0);
+  a.max_pos = cos.size(0);
+  a.q_stride_token = q.stride(0);
+  a.q_stride_head = q.stride(1);
+  a.q_out_stride_token = out.stride(0);
+  a.q_out_stride_head = out.stride(1);
+  a.k_stride_token = k.stride(0);
+  a.k_stride_head = k.stride(1);
+  a.v_stride_token = v.defined() ? v.stride(0) : 0;
+  a.v_stride_head = v.defined() ? v.stride(1) : 0;
+  a.kv_stride_slot = k_cache.stride(0);
+  a.kv_stride_head = k_cache.stride(1);
+  a.num_qo_heads = narrow_dim(hq, "q heads");
+  a.num_kv_heads = narrow_dim(hkv, "kv heads");
+  a.head_dim = narrow_dim(d, "head_dim");
+  a.rotary_dim = narrow_dim(2 * cos.size(1), "rotary_dim");
+  a.flags = interleaved ? SGL_ROPE_INTERLEAVED : 0;
+  check_sgl(sgl_rope_append(&a, current_stream(q.device())), "sgl_rope_append");
+  return out;
+}
+
+PrefixAttention::PrefixAttention(int prefix_len, int batch_size, int max_tokens, int max_qo_len,
+                                 int num_qo_heads, int num_kv_heads, int head_dim,
+                                 torch::Device device) {
+  TORCH_CHECK(device.is_cuda(), "PrefixAttention runs on a HIP device");
+  const c10::DeviceGuard guard(device);
+  check_sgl(sgl_prefix_plan(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads,
+                            num_kv_heads, head_dim, &plan_),
+            "sgl_prefix_plan");
+  workspace_ = torch::empty({plan_.workspace_bytes},
+                            torch::TensorOptions().dtype(torch::kUInt8).device(device));
+}
+
+torch::Tensor PrefixAttention::forward(const torch::Tensor& q, const torch::Tensor& k_cache,
+                                       const torch::Tensor& v_cache,
+                                       const torch::Tensor& prefix_indices,
+                                       const torch::Tensor& indices, const torch::Tensor& kv_indptr,
+                                       const torch::Tensor& qo_indptr,
+                                       c10::optional<double> sm_scale,
+                                       const torch::Tensor& out) const {
+  TORCH_CHECK(q.is_cuda() && q.device() == workspace_.device(), "q must be on the plan's device");
+  const c10::DeviceGuard guard(q.device());
+  check_bf16(q, "q");
+  check_heads(q, q, "q");
+  check_heads(k_cache, q, "k_cache");
+  check_heads(v_cache, q, "v_cache");
+  TORCH_CHECK(v_cache.sizes() == k_cache.sizes() && v_cache.strides() == k_cache.strides(),
+              "K and V caches must share shape and strides");
+  TORCH_CHECK(k_cache.size(1) == plan_.num_kv_heads && k_cache.size(2) == plan_.head_dim &&
+                  q.size(1) == plan_.num_qo_heads && q.size(2) == plan_.head_dim,
+              "q and the caches must have the plan's heads");
+  check_i32(prefix_indices, q.device(), "prefix_indices");
+  check_i32(indices, q.device(), "indices");
+  check_i32(kv_indptr, q.device(), "kv_indptr");
+  check_i32(qo_indptr, q.device(), "qo_indptr");
+  TORCH_CHECK(prefix_indices.size(0) == plan_.prefix_len, "the plan is for another prefix length");
+  TORCH_CHECK(kv_indptr.size(0) == qo_indptr.size(0) && kv_indptr.size(0) >= 1,
+              "kv_indptr and qo_indptr must be [batch + 1]");
+  if (out.defined()) check_heads(out, q, "out");
+  TORCH_CHECK(!out.defined() || out.sizes() == q.sizes(), "out must have q's shape");
+  auto o = out.defined() ? out : torch::empty(q.sizes(), q.options());
+  const double scale = sm_scale.value_or(1.0 / std::sqrt(static_cast<double>(q.size(2))));
+  check_sgl(sgl_prefix_attention(
+                &plan_, q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+                k_cache.stride(0), k_cache.stride(1), prefix_indices.data_ptr<int32_t>(),
+                indices.data_ptr<int32_t>(), kv_indptr.data_ptr<int32_t>(),
+                qo_indptr.data_ptr<int32_t>(), narrow_dim(kv_indptr.size(0) - 1, "batch"),
+                narrow_dim(q.size(0), "tokens"), plan_.num_qo_heads, plan_.num_kv_heads,
+                plan_.head_dim, static_cast<float>(scale), o.data_ptr(), o.stride(0), o.stride(1),
+                workspace_.data_ptr(), workspace_.numel(), current_stream(q.device())),
+            "sgl_prefix_attention");
+  return o;
+}
+
+std::pair<torch::Tensor, torch::Tensor> verify_drafts(
+    const torch::Tensor& target_probs, const torch::Tensor& draft_probs,
+    const torch::Tensor& draft_tokens, const torch::Tensor& draft_indptr,
+    const torch::Tensor& accept_uniform, const torch::Tensor& sample_uniform) {
+  TORCH_CHECK(target_probs.defined() && target_probs.is_cuda() && target_probs.dim() == 2,
+              "target_probs must be a [drafts + batch, vocab] device tensor");
+  const auto dev = target_probs.device();
+  const c10::DeviceGuard guard(dev);
+  check_i32(draft_tokens, dev, "draft_tokens");
+  check_i32(draft_indptr, dev, "draft_indptr");
+  TORCH_CHECK(draft_indptr.size(0) >= 1, "draft_indptr must be [batch + 1]");
+  const int64_t n = draft_tokens.size(0), b = draft_indptr.size(0) - 1, vocab = target_probs.size(1);
+  auto check_uniforms = [&](const torch::Tensor& t, int64_t size, const char* what) {
+    TORCH_CHECK(t.defined() && t.device() == dev && t.scalar_type() == torch::kFloat32 && t.dim() == 1 &&
+                    t.is_contiguous() && t.size(0) == size,
+                what, " must be contiguous float32 [", size, "] on the probabilities' device");
+  };
+  check_uniforms(accept_uniform, n, "accept_uniform");
+  check_uniforms(sample_uniform, b, "sample_uniform");
+  auto stride_of = [&](const torch::Tensor& t, int64_t rows, const char* what) {
+    TORCH_CHECK(t.device() == dev && t.scalar_type() == torch::kFloat32 && t.dim() == 2 &&
+                    t.size(0) == rows && t.size(1) == vocab &&
+                    (rows == 0 || vocab <= 1 || t.stride(1) == 1),
+                what, " must be float32 [", rows, ", vocab] with contiguous rows");
+    return rows <= 1 ? std::max<int64_t>(t.stride(0), vocab) : t.stride(0);
+  };
+  sgl_verify_args_t a{};
+  a.target_stride_row = stride_of(target_probs, n + b, "target_probs");
+  a.target_probs = target_probs.data_ptr<float>();
+  if (draft_probs.defined()) {
+    a.draft_stride_row = stride_of(draft_probs, n, "draft_probs");
+    a.draft_probs = draft_probs.data_ptr<float>();
+  }
+  auto opts = target_probs.options().dtype(torch::kInt32);
+  auto tokens = torch::empty({n + b}, opts);
+  auto accepted = torch::empty({b}, opts);
+  a.draft_tokens = draft_tokens.data_ptr<int32_t>();
+  a.draft_indptr = draft_indptr.data_ptr<int32_t>();
+  a.accept_uniform = accept_uniform.data_ptr<float>();
+  a.sample_uniform = sample_uniform.data_ptr<float>();
+  a.tokens = tokens.data_ptr<int32_t>();
+  a.accepted = accepted.data_ptr<int32_t>();
+  a.num_drafts = n;
+  a.batch_size = narrow_dim(b, "batch");
+  a.vocab = narrow_dim(vocab, "vocab");
+  const int64_t bytes = sgl_verify_workspace_bytes(a.batch_size, a.vocab);
+  auto ws = torch::empty({bytes}, opts.dtype(torch::kUInt8));
+  check_sgl(sgl_verify_drafts(&a, ws.data_ptr(), bytes, current_stream(dev)), "sgl_verify_drafts");
+  return {tokens, accepted};
 }
 
 AttentionLayer::AttentionLayer(int layer_id, int num_qo_heads, int num_kv_heads, int head_dim,

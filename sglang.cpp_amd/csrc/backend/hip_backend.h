@@ -15,8 +15,10 @@
 #include <torch/torch.h>
 
 #include <map>
-#include <tuple>
 #include <memory>
+#include <string>
+#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "../../../include/sgl_attn.h"
@@ -299,6 +301,61 @@ class RotaryEmbedding {
   int head_size_, rotary_dim_;
   torch::Tensor cos_cache_, sin_cache_;
 };
+
+// A rotary embedding scaled for long contexts (sgl_rope_scaling_t): kind is
+// "none", "linear", "ntk", "yarn" or "bands".
+struct RopeScaling {
+  std::string kind = "none";
+  double factor = 1.0;
+  int original_max_position = 0;
+  double beta_fast = 32.0, beta_slow = 1.0;
+  double low_freq_factor = 1.0, high_freq_factor = 4.0;
+  double attention_factor = 0.0;
+};
+
+// (cos, sin) tables of a scaled rotary embedding, fp32 [max_pos, rotary_dim / 2],
+// angles in 64 bits.
+std::pair<torch::Tensor, torch::Tensor> rope_scaled_cache(int64_t max_pos, int rotary_dim,
+                                                          double base, const RopeScaling& scaling,
+                                                          torch::Device device);
+
+// q [T, Hq, D] and k [T, Hkv, D] rotated (rotary_dim = twice the tables' width), k
+// and v appended to one layer's caches [slots, Hkv, D] at out_loc (int32 or int64
+// [T]); bf16 or fp16. Returns the rotated q: q_out when defined (it may be q), else
+// a new contiguous tensor. Undefined v and v_cache: k alone.
+torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                          const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                          const torch::Tensor& cos, const torch::Tensor& sin,
+                          const torch::Tensor& positions, const torch::Tensor& out_loc,
+                          bool interleaved, const torch::Tensor& q_out);
+
+// Attention of a batch behind a shared prefix (sgl_prefix_attention): the plan and
+// its workspace, which the calls of one object share (they must be stream-ordered,
+// graphs captured from it among them).
+class PrefixAttention {
+ public:
+  PrefixAttention(int prefix_len, int batch_size, int max_tokens, int max_qo_len, int num_qo_heads,
+                  int num_kv_heads, int head_dim, torch::Device device);
+  // q [T, Hq, D], caches [slots, Hkv, D], int32 slots and offsets; returns [T, Hq, D],
+  // rows of no request undefined (into `out`, where it is defined: left as they were).
+  torch::Tensor forward(const torch::Tensor& q, const torch::Tensor& k_cache,
+                        const torch::Tensor& v_cache, const torch::Tensor& prefix_indices,
+                        const torch::Tensor& indices, const torch::Tensor& kv_indptr,
+                        const torch::Tensor& qo_indptr, c10::optional<double> sm_scale,
+                        const torch::Tensor& out) const;
+  const sgl_prefix_plan_t& plan() const { return plan_; }
+
+ private:
+  sgl_prefix_plan_t plan_{};
+  torch::Tensor workspace_;
+};
+
+// Verification of drafted tokens (sgl_verify_drafts): (tokens [drafts + batch],
+// accepted [batch]), int32. draft_probs undefined: drafts without probabilities.
+std::pair<torch::Tensor, torch::Tensor> verify_drafts(
+    const torch::Tensor& target_probs, const torch::Tensor& draft_probs,
+    const torch::Tensor& draft_tokens, const torch::Tensor& draft_indptr,
+    const torch::Tensor& accept_uniform, const torch::Tensor& sample_uniform);
 
 // qkv [T, (Hq + 2 Hkv) D] -> o [T, Hq D]: qk-norm, RoPE and the KV store in
 // one fused pass, then paged attention (attention_layer.cc:17-51).

@@ -1,0 +1,551 @@
+// Attention of a batch that shares a prefix: row (token t, head) of request r is
+//   o = softmax_j(q . k_j scale) . v_j  over the prefix's tokens, then the request's own,
+// j <= i + kv_len - qo_len for its i-th query token. A softmax over a joined
+// sequence folds from its parts: with each part's sum l, reference point m and
+// output o (normalised), weights 2^(lse - max lse), lse = m + log2 l. So the prefix's
+// K/V are walked once with the rows of every request as columns of one product,
+// each request's own tokens with its rows alone, and a second launch folds.
+//
+// Units: the prefix (once per tile of up to 64 packed rows) and then the
+// requests' own tokens form one stream, cut into units of equal length, one
+// workgroup each; a wave has one kv head, so a workgroup reads whole token rows.
+// A wave walks its piece 16 tokens a step on the matrix cores: S^T = K Q^T, then
+// O^T += V^T P^T, whose operand P^T is S^T's accumulator layout, for up to four
+// column blocks of 16 rows per K/V read. Both put the row on the lane's column, so
+// the running maximum and sum are lane-local but for one exchange across four lane
+// groups. K and V of the next step are in flight during a step.
+#include <math.h>
+
+#include "common.h"
+
+namespace sgl {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kStep = 16;                 // tokens a step
+constexpr int kMinUnit = 64;              // shortest unit
+constexpr int kQPitch = kD + 8;           // LDS row pitch (bf16) of the Q^T copy
+constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
+constexpr int kMaxTileRows = 64;
+
+struct PrefixArgs {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const uint16_t* kc;
+  const uint16_t* vc;
+  int64_t kv_ss, kv_sh;
+  const int32_t* pidx;
+  const int32_t* indices;
+  const int32_t* kv_indptr;
+  const int32_t* qo_indptr;
+  int batch, tokens, hq, hkv, group;
+  int prefix, tile_rows, tiles, units, max_qo;
+  float scale_log2;
+  uint16_t* o;
+  int64_t o_st, o_sh;
+  // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix pieces: piece u + tile,
+  // [piece][kv head][row of the tile]. Own pieces: [token slot][q head], the piece a
+  // request starts with at its rows' own tokens, the one running into unit u from
+  // before it at tokens + u max_qo + i.
+  float* p_o;
+  float* p_lse;
+  float* s_o;
+  float* s_lse;
+};
+
+// Tokens of a unit, from the requests' lengths as they are now.
+__device__ __forceinline__ int64_t unit_tokens(const PrefixArgs& a, int64_t all) {
+  int64_t w = (all + a.units - 1) / a.units;
+  w = (w + kStep - 1) / kStep * kStep;
+  return w < kMinUnit ? kMinUnit : w;
+}
+
+__device__ __forceinline__ int64_t own_tokens(const PrefixArgs& a) {
+  const int64_t n = static_cast<int64_t>(a.kv_indptr[a.batch]) - a.kv_indptr[0];
+  return n < 0 ? 0 : n;
+}
+
+struct Request {
+  int q0, qo, kv0, kv;  // first query token, query tokens, first own index, own tokens
+  bool ok;
+};
+
+__device__ __forceinline__ Request request_of(const PrefixArgs& a, int r) {
+  Request x;
+  x.q0 = a.qo_indptr[r];
+  const int64_t q1 = a.qo_indptr[r + 1];
+  x.kv0 = a.kv_indptr[r];
+  const int64_t k1 = a.kv_indptr[r + 1];
+  x.qo = static_cast<int>(q1 - x.q0);
+  x.kv = static_cast<int>(k1 - x.kv0);
+  // Rows and pieces of anything else have no place in the outputs and the workspace.
+  x.ok = x.q0 >= max(a.qo_indptr[0], 0) && q1 >= x.q0 && q1 <= min(a.qo_indptr[a.batch], a.tokens) &&
+         q1 - x.q0 <= a.max_qo && x.kv0 >= a.kv_indptr[0] && k1 >= x.kv0 && k1 <= a.kv_indptr[a.batch];
+  return x;
+}
+
+__device__ __forceinline__ bf16x8_t as_bf16x8(const u32x4_t& v) {
+  return __builtin_bit_cast(bf16x8_t, v);
+}
+
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ const char* slot_row(const char* base, int slot, uint32_t ss_bytes) {
+  return base + static_cast<uint64_t>(static_cast<uint32_t>(slot)) * ss_bytes;
+}
+
+// A operand of O^T product nb: V^T[d = 8 n + nb][token 4 j + e], e < 4, from four rows.
+template <int nb>
+__device__ __forceinline__ bf16x4_t v_operand(const u32x4_t (&vr)[4]) {
+  constexpr int w = nb / 2;
+  constexpr uint32_t sel = (nb & 1) ? 0x07060302u : 0x05040100u;
+  u32x2_t out;
+  out[0] = __builtin_amdgcn_perm(vr[1][w], vr[0][w], sel);
+  out[1] = __builtin_amdgcn_perm(vr[3][w], vr[2][w], sel);
+  return __builtin_bit_cast(bf16x4_t, out);
+}
+
+// One wave: kv head h over the len tokens of slots idx[0, len), for the packed
+// rows [row0, row_end) (at most 16 RB; row p: token tok0 + p / G, head h G + p % G).
+// Row of token i sees the tokens below sees0 + i (all of them: sees0 >= len).
+// Its output and lse go to row out0 + (p - row0) of o/lse, or, with by_token, to
+// row (out0 + i) hq + head. lq: the wave's Q copy, 16 RB rows.
+// Lane (n, j), n = lane % 16: token n (K), chunk n of tokens 4 j + e (V), row n
+// (S, O).
+template <int RB>
+__device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const int32_t* idx, int len,
+                                     int h, int tok0, int row0, int row_end, int sees0, float* o,
+                                     float* lse, int64_t out0, bool by_token, int lane) {
+  const int n = lane & 15, j = lane >> 4;
+  const int G = a.group;
+  const uint32_t ss_bytes = static_cast<uint32_t>(a.kv_ss * 2);
+  const char* klane = reinterpret_cast<const char*>(a.kc + h * a.kv_sh + 8 * j);
+  const char* vlane = reinterpret_cast<const char*>(a.vc + h * a.kv_sh + 8 * n);
+
+  auto load_k = [&](int slot, u32x4_t (&kr)[4]) {
+    const char* row = slot_row(klane, slot, ss_bytes);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) kr[s] = ldg128(row + 64 * s);
+  };
+  auto load_v = [&](int slot, u32x4_t (&vr)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      vr[e] = ldg128(slot_row(vlane, __shfl(slot, 4 * j + e, kWave), ss_bytes));
+  };
+
+  int slot = idx[min(n, len - 1)];
+  int slot_next = idx[min(kStep + n, len - 1)];
+  u32x4_t kr[4], vr[4];
+  load_k(slot, kr);
+  load_v(slot, vr);
+  // Q rows, four of a block at a time (chunk n), to LDS.
+#pragma unroll
+  for (int u = 0; u < 4 * RB; ++u) {
+    const int p = row0 + 4 * u + j;
+    u32x4_t qv = {0, 0, 0, 0};
+    if (p < row_end) {
+      const int i = p / G;
+      qv = ldg128(a.q + (tok0 + i) * a.q_st + (h * G + p - i * G) * a.q_sh + 8 * n);
+    }
+    *reinterpret_cast<u32x4_t*>(lq + (4 * u + j) * kQPitch + 8 * n) = qv;
+  }
+  wave_lds_sync();
+  int sees[RB];
+  float m[RB], l[RB];
+  f32x4_t acc[RB][8];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int p = row0 + 16 * b + n;
+    sees[b] = p < row_end ? min(sees0 + p / G, len) : 0;
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) acc[b][nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int t = 0; t < len; t += kStep) {
+    // The workgroup's waves (its kv heads) keep in step: together they read
+    // whole token rows.
+    __builtin_amdgcn_s_barrier();
+    const int slot_after = idx[min(t + 2 * kStep + n, len - 1)];
+    f32x4_t sacc[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      sacc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const bf16x8_t qop =
+            *reinterpret_cast<const bf16x8_t*>(lq + (16 * b + n) * kQPitch + 32 * s + 8 * j);
+        sacc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[s]), qop, sacc[b], 0, 0, 0);
+      }
+    }
+    load_k(slot_next, kr);
+    bf16x4_t pop[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      float sc[4];
+      float mt = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[i] = t + 4 * j + i < sees[b] ? sacc[b][i] : -INFINITY;
+        mt = fmaxf(mt, sc[i]);
+      }
+      // The reference point moves only where a row's maximum exceeds it by
+      // more than kRescaleSlack; p and l always use the same one, so the result
+      // is exact and most steps leave O as it is.
+      mt = max_xor32(max_xor16(mt)) * a.scale_log2;
+      const bool move = mt > m[b] + kRescaleSlack;
+      if (__builtin_amdgcn_ballot_w64(move) != 0) {
+        const float mn = move ? mt : m[b];
+        const float alpha = move ? __builtin_amdgcn_exp2f(m[b] - mn) : 1.f;
+        l[b] *= alpha;
+        m[b] = mn;
+#pragma unroll
+        for (int nb = 0; nb < 8; ++nb) acc[b][nb] *= alpha;
+      }
+      const float neg_m = m[b] == -INFINITY ? 0.f : -m[b];  // nothing seen yet
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], a.scale_log2, neg_m));
+      l[b] += (p[0] + p[1]) + (p[2] + p[3]);
+      // P in bf16, the product's operand type: a weight is off by at most 2^-9 of
+      // itself, below what rounding the output to bf16 takes.
+      const u32x2_t pw = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+      pop[b] = __builtin_bit_cast(bf16x4_t, pw);
+    }
+    static_for<0, 8>([&](auto NB) {
+      constexpr int nb = decltype(NB)::value;
+      const bf16x4_t vop = v_operand<nb>(vr);
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+        acc[b][nb] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vop, pop[b], acc[b][nb], 0, 0, 0);
+    });
+    load_v(slot_next, vr);
+    slot_next = slot_after;
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const float sum = sum_xor32(sum_xor16(l[b]));
+    const int p = row0 + 16 * b + n;
+    if (p >= row_end) continue;
+    const int i = p / G;
+    const int64_t row = by_token ? (out0 + i) * a.hq + (h * G + p - i * G) : out0 + (p - row0);
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // a NaN sum stays one
+    // acc[nb][c] holds d = 32 j + 8 c + nb.
+    float* op = o + row * kD + 32 * j;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      f32x4_t lo, hi;
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) lo[nb] = acc[b][nb][c] * inv, hi[nb] = acc[b][nb + 4][c] * inv;
+      *reinterpret_cast<f32x4_t*>(op + 8 * c) = lo;
+      *reinterpret_cast<f32x4_t*>(op + 8 * c + 4) = hi;
+    }
+    if (j == 0) lse[row] = sum == 0.f ? -INFINITY : m[b] + log2f(sum);
+  }
+}
+
+template <int RB>
+__global__ void __launch_bounds__(512) prefix_units_kernel(PrefixArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds_q[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.y * (blockDim.x >> 6) + wave;
+  const int u = blockIdx.x;
+  uint16_t* lq = lds_q + wave * 16 * RB * kQPitch;
+  const int64_t P = a.prefix, shared = P * a.tiles;
+  const int64_t all = shared + own_tokens(a);
+  const int64_t W = unit_tokens(a, all);
+  const int64_t t0 = u * W, t1 = min(all, t0 + W);
+  if (t0 >= t1) return;
+  // The shared prefix's part.
+  if (t0 < shared) {
+    const int first = max(a.qo_indptr[0], 0);
+    const int last = min(a.qo_indptr[a.batch], a.tokens);
+    const int64_t rows = static_cast<int64_t>(max(last - first, 0)) * a.group;
+    for (int tile = static_cast<int>(t0 / P); tile < a.tiles && tile * P < t1; ++tile) {
+      const int row0 = tile * a.tile_rows;
+      if (row0 >= rows) break;
+      const int s0 = static_cast<int>(max(t0 - tile * P, int64_t{0}));
+      const int s1 = static_cast<int>(min(t1 - tile * P, P));
+      const int64_t out0 = (static_cast<int64_t>(u + tile) * a.hkv + h) * a.tile_rows;
+      walk<RB>(a, lq, a.pidx + s0, s1 - s0, h, first, row0,
+               static_cast<int>(min(rows, static_cast<int64_t>(row0) + a.tile_rows)), s1 - s0, a.p_o,
+               a.p_lse, out0, false, lane);
+    }
+  }
+  if (t1 <= shared) return;
+  // The requests' own tokens [b0, b1) of the joined list.
+  const int kv_first = a.kv_indptr[0];
+  const int64_t b0 = max(t0 - shared, int64_t{0}), b1 = t1 - shared;
+  int r = 0;  // requests that end at or before b0, 64 at a time
+  for (int at = 0; at < a.batch; at += kWave) {
+    const int e = at + lane;
+    const bool before = e < a.batch && static_cast<int64_t>(a.kv_indptr[e + 1]) - kv_first <= b0;
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(before);
+    r += __builtin_popcountll(mask);
+    if (mask != ~0ull) break;
+  }
+  for (; r < a.batch; ++r) {
+    const Request x = request_of(a, r);
+    const int64_t rb = static_cast<int64_t>(x.kv0) - kv_first;
+    if (rb >= b1) break;
+    if (!x.ok || x.qo == 0 || x.kv == 0) continue;
+    const int s0 = static_cast<int>(max(b0 - rb, int64_t{0}));
+    const int s1 = static_cast<int>(min(b1 - rb, static_cast<int64_t>(x.kv)));
+    if (s1 <= s0) continue;
+    const int64_t out0 = s0 == 0 ? x.q0 : a.tokens + static_cast<int64_t>(u) * a.max_qo;
+    for (int row0 = 0; row0 < x.qo * a.group; row0 += 16 * RB)
+      walk<RB>(a, lq, a.indices + x.kv0 + s0, s1 - s0, h, x.q0, row0,
+               min(x.qo * a.group, row0 + 16 * RB), max(x.kv - x.qo + 1 - s0, -x.qo), a.s_o, a.s_lse,
+               out0, true, lane);
+  }
+}
+
+// Sum over the 32 lanes of a half wave, the same in each.
+__device__ __forceinline__ float half_sum(float x) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor(x, off, kWave);
+  return x;
+}
+
+// The row again, token by token over those it sees, by 32 lanes (4 values each):
+// for rows that do not see the whole prefix, and for those whose products brought in
+// a V value that is not finite from a token they do not see (0 x inf).
+__device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request& x, int tok, int head,
+                                             int64_t sees, int c) {
+  const int h = head / a.group;
+  const u32x2_t qw = *reinterpret_cast<const u32x2_t*>(a.q + tok * a.q_st + head * a.q_sh + 4 * c);
+  const float q[4] = {bf16_lo(qw[0]), bf16_hi(qw[0]), bf16_lo(qw[1]), bf16_hi(qw[1])};
+  float m = -INFINITY, l = 0.f;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t t = 0; t < sees; ++t) {
+    const int64_t slot = static_cast<uint32_t>(t < a.prefix ? a.pidx[t] : a.indices[x.kv0 + (t - a.prefix)]);
+    const u32x2_t kw = *reinterpret_cast<const u32x2_t*>(a.kc + slot * a.kv_ss + h * a.kv_sh + 4 * c);
+    const u32x2_t vw = *reinterpret_cast<const u32x2_t*>(a.vc + slot * a.kv_ss + h * a.kv_sh + 4 * c);
+    float s = q[0] * bf16_lo(kw[0]) + q[1] * bf16_hi(kw[0]) + q[2] * bf16_lo(kw[1]) + q[3] * bf16_hi(kw[1]);
+    s = half_sum(s) * a.scale_log2;
+    const float mn = fmaxf(m, s);
+    const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
+    const float p = s == -INFINITY ? 0.f : exp2f(s - mn);  // NaN stays NaN
+    l = l * alpha + p;
+    const f32x4_t v = {bf16_lo(vw[0]), bf16_hi(vw[0]), bf16_lo(vw[1]), bf16_hi(vw[1])};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * alpha + p * v[i];
+    m = mn;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  return acc * inv;
+}
+
+// Folds the pieces of each row: a workgroup per token, 32 lanes a row.
+__global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a) {
+  __shared__ int before[4];
+  const int t = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  // The token's request: those that end at or before it are counted.
+  int n = 0;
+  for (int e = threadIdx.x; e < a.batch; e += 256) n += a.qo_indptr[e + 1] <= t;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, kWave);
+  if (lane == 0) before[threadIdx.x >> 6] = n;
+  __syncthreads();
+  const int r = before[0] + before[1] + before[2] + before[3];
+  if (r >= a.batch || t < a.qo_indptr[0]) return;  // no request's row: left as it was
+  const Request x = request_of(a, r);
+  const int first = max(a.qo_indptr[0], 0);
+  const int64_t P = a.prefix, shared = P * a.tiles;
+  const int64_t W = unit_tokens(a, shared + own_tokens(a));
+  const int c = threadIdx.x & 31;
+  const int i = t - x.q0;
+  const int64_t own0 = shared + x.kv0 - a.kv_indptr[0];
+  // Tokens this row sees, prefix first.
+  const int64_t sees = P + x.kv - x.qo + i + 1;
+  for (int head = threadIdx.x >> 5; head < a.hq; head += 8) {
+    uint16_t* op = a.o + t * a.o_st + head * a.o_sh + 4 * c;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    if (!x.ok) {
+      acc = f32x4_t{NAN, NAN, NAN, NAN};
+    } else if (sees < P) {
+      acc = plain_row(a, x, t, head, sees, c);
+    } else {
+      const int h = head / a.group;
+      const int prow = (t - first) * a.group + head - h * a.group;
+      float m = -INFINITY, l = 0.f;
+      auto add = [&](const float* o, const float* lse, int64_t row) {
+        const float s = lse[row];
+        if (s == -INFINITY) return;  // nothing seen there: its values do not count
+        const float mn = fmaxf(m, s);
+        const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
+        const float w = exp2f(s - mn);
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(o + row * kD + 4 * c);
+        l = l * alpha + w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = acc[k] * alpha + v[k] * w;
+        m = mn;
+      };
+      if (P > 0) {
+        const int tile = prow / a.tile_rows;
+        for (int64_t u = tile * P / W; u <= (tile * P + P - 1) / W; ++u)
+          add(a.p_o, a.p_lse, ((u + tile) * a.hkv + h) * a.tile_rows + prow - tile * a.tile_rows);
+      }
+      if (x.kv > 0) {
+        const int64_t u0 = own0 / W, u1 = (own0 + x.kv - 1) / W;
+        add(a.s_o, a.s_lse, static_cast<int64_t>(t) * a.hq + head);
+        for (int64_t u = u0 + 1; u <= u1; ++u)
+          add(a.s_o, a.s_lse, (a.tokens + u * a.max_qo + i) * a.hq + head);
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] *= inv;
+      // Tokens of the request behind this row's last one may have brought in
+      // values that are not finite.
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) bad = bad || !(fabsf(acc[k]) < INFINITY);
+      const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
+      if (i + 1 < x.qo && ((any >> (lane & 32)) & 0xffffffffull) != 0)
+        acc = plain_row(a, x, t, head, sees, c);
+    }
+    *reinterpret_cast<u32x2_t*>(op) = u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+  }
+}
+
+int device_cus() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) == hipSuccess &&
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && cus > 0)
+    return cus;
+  return 256;
+}
+
+// kv heads of a workgroup: the largest divisor of theirs up to 8.
+int heads_per_group(int hkv) {
+  for (int n = 8; n > 1; --n)
+    if (hkv % n == 0) return n;
+  return 1;
+}
+
+struct Layout {
+  int64_t p_o, p_lse, s_o, s_lse, total;
+};
+
+Layout workspace_layout(const sgl_prefix_plan_t& p) {
+  auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
+  const int64_t prefix_rows = p.num_tiles > 0
+      ? (static_cast<int64_t>(p.num_units) + p.num_tiles) * p.num_kv_heads * p.tile_rows : 0;
+  const int64_t own_rows =
+      (p.max_tokens + static_cast<int64_t>(p.num_units) * p.max_qo_len) * p.num_qo_heads;
+  Layout l;
+  l.p_o = 0;
+  l.p_lse = l.p_o + align(prefix_rows * kD * 4);
+  l.s_o = l.p_lse + align(prefix_rows * 4);
+  l.s_lse = l.s_o + align(own_rows * kD * 4);
+  l.total = l.s_lse + align(own_rows * 4);
+  return l;
+}
+
+}  // namespace
+}  // namespace sgl
+
+using namespace sgl;
+
+extern "C" int sgl_prefix_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len,
+                               int num_qo_heads, int num_kv_heads, int head_dim,
+                               sgl_prefix_plan_t* plan) {
+  if (!plan || prefix_len < 0 || batch_size < 0 || max_tokens < 0 || max_qo_len < 0 ||
+      num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0)
+    return SGL_ERR_INVALID_ARG;
+  const int group = num_qo_heads / num_kv_heads;
+  if (head_dim != kD || group > kMaxTileRows || max_qo_len > SGL_PREFIX_MAX_QO ||
+      num_kv_heads > 65535)
+    return SGL_ERR_UNSUPPORTED;
+  // Packed rows and their tiles are counted in 32 bits.
+  if (static_cast<int64_t>(max_tokens) * group > (1 << 30)) return SGL_ERR_UNSUPPORTED;
+  *plan = sgl_prefix_plan_t{};
+  plan->prefix_len = prefix_len;
+  plan->batch_size = batch_size;
+  plan->max_tokens = max_tokens;
+  plan->max_qo_len = max_qo_len;
+  plan->num_qo_heads = num_qo_heads;
+  plan->num_kv_heads = num_kv_heads;
+  plan->head_dim = head_dim;
+  const int64_t units = static_cast<int64_t>(device_cus()) * 8 / num_kv_heads;
+  plan->num_units = static_cast<int32_t>(units < 1 ? 1 : units);
+  const int64_t rows = static_cast<int64_t>(max_tokens) * group;
+  plan->tile_rows = static_cast<int32_t>(rows < kMaxTileRows ? (rows + 15) / 16 * 16 : kMaxTileRows);
+  plan->num_tiles = prefix_len > 0 && rows > 0
+                        ? static_cast<int32_t>((rows + plan->tile_rows - 1) / plan->tile_rows) : 0;
+  plan->workspace_bytes = workspace_layout(*plan).total;
+  return SGL_OK;
+}
+
+extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q,
+                                    int64_t q_stride_token, int64_t q_stride_head,
+                                    const void* k_cache, const void* v_cache,
+                                    int64_t kv_stride_slot, int64_t kv_stride_head,
+                                    const int32_t* prefix_indices, const int32_t* indices,
+                                    const int32_t* kv_indptr, const int32_t* qo_indptr,
+                                    int batch_size, int max_tokens, int num_qo_heads,
+                                    int num_kv_heads, int head_dim, float sm_scale, void* o,
+                                    int64_t o_stride_token, int64_t o_stride_head, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  if (!plan || batch_size < 0 || max_tokens < 0) return SGL_ERR_INVALID_ARG;
+  if (num_qo_heads != plan->num_qo_heads || num_kv_heads != plan->num_kv_heads ||
+      head_dim != plan->head_dim)
+    return SGL_ERR_INVALID_ARG;
+  // A plan as sgl_prefix_plan makes it.
+  sgl_prefix_plan_t p;
+  int st = sgl_prefix_plan(plan->prefix_len, plan->batch_size, plan->max_tokens, plan->max_qo_len,
+                           num_qo_heads, num_kv_heads, head_dim, &p);
+  if (st != SGL_OK) return st;
+  p.num_units = plan->num_units;
+  if (p.num_units <= 0 || p.num_units > (1 << 20) || plan->tile_rows != p.tile_rows ||
+      plan->num_tiles != p.num_tiles)
+    return SGL_ERR_INVALID_ARG;
+  if (batch_size > p.batch_size || max_tokens > p.max_tokens) return SGL_ERR_CAPACITY;
+  if (batch_size == 0 || max_tokens == 0) return SGL_OK;
+  if (!q || !k_cache || !v_cache || !kv_indptr || !qo_indptr || !o ||
+      (p.prefix_len > 0 && !prefix_indices))
+    return SGL_ERR_INVALID_ARG;
+  // Slot addresses use 32-bit byte strides.
+  if (kv_stride_slot <= 0 || kv_stride_slot > 0x3fffffff) return SGL_ERR_UNSUPPORTED;
+  if (q_stride_head % 8 || q_stride_token % 8 || kv_stride_slot % 8 || kv_stride_head % 8 ||
+      o_stride_token % 8 || o_stride_head % 8 || !aligned16(q) || !aligned16(k_cache) ||
+      !aligned16(v_cache) || !aligned16(o) || !aligned16(workspace))
+    return SGL_ERR_ALIGNMENT;
+  const Layout l = workspace_layout(p);
+  if (!workspace || workspace_bytes < l.total) return SGL_ERR_CAPACITY;
+  char* ws = static_cast<char*>(workspace);
+  PrefixArgs a{};
+  a.q = static_cast<const uint16_t*>(q), a.q_st = q_stride_token, a.q_sh = q_stride_head;
+  a.kc = static_cast<const uint16_t*>(k_cache), a.vc = static_cast<const uint16_t*>(v_cache);
+  a.kv_ss = kv_stride_slot, a.kv_sh = kv_stride_head;
+  a.pidx = prefix_indices, a.indices = indices, a.kv_indptr = kv_indptr, a.qo_indptr = qo_indptr;
+  a.batch = batch_size, a.tokens = max_tokens;
+  a.hq = num_qo_heads, a.hkv = num_kv_heads, a.group = num_qo_heads / num_kv_heads;
+  a.prefix = p.prefix_len, a.tile_rows = p.tile_rows, a.units = p.num_units, a.max_qo = p.max_qo_len;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.o = static_cast<uint16_t*>(o), a.o_st = o_stride_token, a.o_sh = o_stride_head;
+  a.p_o = reinterpret_cast<float*>(ws + l.p_o), a.p_lse = reinterpret_cast<float*>(ws + l.p_lse);
+  a.s_o = reinterpret_cast<float*>(ws + l.s_o), a.s_lse = reinterpret_cast<float*>(ws + l.s_lse);
+  const int64_t rows = static_cast<int64_t>(max_tokens) * a.group;
+  a.tiles = p.num_tiles > 0 ? static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows) : 0;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int waves = heads_per_group(num_kv_heads);
+  const dim3 grid(p.num_units, num_kv_heads / waves), block(64 * waves);
+  const int need = p.max_qo_len * a.group > a.tile_rows ? p.max_qo_len * a.group : a.tile_rows;
+  const int rb = need <= 16 ? 1 : need <= 32 ? 2 : 4;
+  const size_t lds = static_cast<size_t>(waves) * 16 * rb * kQPitch * 2;
+  if (rb == 1) hipLaunchKernelGGL(prefix_units_kernel<1>, grid, block, lds, s, a);
+  else if (rb == 2) hipLaunchKernelGGL(prefix_units_kernel<2>, grid, block, lds, s, a);
+  else hipLaunchKernelGGL(prefix_units_kernel<4>, grid, block, lds, s, a);
+  st = launch_status();
+  if (st != SGL_OK) return st;
+  hipLaunchKernelGGL(prefix_fold_kernel, dim3(max_tokens), dim3(256), 0, s, a);
+  return launch_status();
+}

@@ -1,0 +1,305 @@
+// Verification of drafted tokens (speculative sampling): request r's drafts
+// x_i, i < n, each drawn from q_i, are accepted in order while
+//   u_i q_i(x_i) < p_i(x_i)            (probability min(1, p / q)),
+// p_i the target's probabilities after i drafts. The token that follows the
+// accepted ones is drawn from w(j) = max(p_a(j) - q_a(j), 0) at the first
+// rejected draft a, or from p_n when all were accepted: the first j whose running
+// sum of w exceeds u * sum(w). The tokens are then distributed as the target's
+// own draws. Drafts without probabilities are point masses: q_i(x_i) = 1.
+//
+// The product u q and the difference p - q of fp32 values and all sums are in
+// 64 bits, where products are exact and the order of a sum moves the drawn
+// token only for a u within about 1e-13 of a border.
+//
+// Two launches. verify_sums_kernel: a workgroup per (request, slice of the
+// vocabulary) finds the request's first rejected draft by itself (a few
+// dependent loads) and sums its slice of w and of p. verify_draw_kernel: a
+// workgroup per request picks the slice the draw falls into from the slices'
+// sums and walks that slice alone. Bound by reading one target row and, where a
+// draft was rejected, one draft row per request.
+#include "common.h"
+
+namespace sgl {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kPer = 16;                    // elements of a thread
+constexpr int kSlice = kThreads * kPer;     // elements of a slice
+constexpr int kLines = kPer / 4;            // groups of 4 consecutive elements of a thread
+
+struct VerifyArgs {
+  const float* target;
+  int64_t target_st;
+  const float* draft;  // null: point masses
+  int64_t draft_st;
+  const int32_t* draft_tokens;
+  const int32_t* indptr;
+  const float* accept_u;
+  const float* sample_u;
+  int64_t num_drafts;
+  int vocab, slices;
+  int32_t* tokens;
+  int32_t* accepted;
+  double* sums;  // [batch, slices, 2]: of w and of p
+};
+
+struct Request {
+  int64_t d0;   // first draft
+  int n;        // drafts; -1: the offsets are not valid
+  int a;        // accepted
+};
+
+// Accepted drafts of request r, the same in every thread of the calling wave.
+__device__ __forceinline__ Request judge(const VerifyArgs& v, int r, int lane) {
+  Request q;
+  const int64_t d0 = v.indptr[r], d1 = v.indptr[r + 1];
+  q.d0 = d0;
+  q.n = d0 >= 0 && d1 >= d0 && d1 <= v.num_drafts ? static_cast<int>(d1 - d0) : -1;
+  q.a = q.n < 0 ? -1 : q.n;
+  for (int i0 = 0; i0 < q.n; i0 += kWave) {
+    const int i = i0 + lane;
+    bool reject = false;
+    if (i < q.n) {
+      const int x = v.draft_tokens[d0 + i];
+      reject = true;
+      if (x >= 0 && x < v.vocab) {
+        const double p = v.target[(d0 + i + r) * v.target_st + x];
+        const double qx = v.draft ? static_cast<double>(v.draft[(d0 + i) * v.draft_st + x]) : 1.0;
+        reject = !(static_cast<double>(v.accept_u[d0 + i]) * qx < p);
+      }
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(reject);
+    if (m != 0) {
+      q.a = i0 + __builtin_ctzll(m);
+      break;
+    }
+  }
+  return q;
+}
+
+// The rows the draw of a request reads: p, and q where a draft was rejected.
+struct Rows {
+  const float* p;
+  const float* q;  // null: none
+  int point;       // the rejected draft as a point mass, or -1
+};
+
+__device__ __forceinline__ Rows rows_of(const VerifyArgs& v, const Request& q, int r) {
+  Rows w;
+  w.p = v.target + (q.d0 + q.a + r) * v.target_st;
+  w.q = nullptr;
+  w.point = -1;
+  if (q.a < q.n) {
+    if (v.draft) w.q = v.draft + (q.d0 + q.a) * v.draft_st;
+    else w.point = v.draft_tokens[q.d0 + q.a];
+  }
+  return w;
+}
+
+__device__ __forceinline__ float at_or_zero(const float* row, int e, int n) { return e < n ? row[e] : 0.f; }
+
+// A thread's 16 elements of slice s: group g holds elements
+// [1024 g + 4 t, ... + 4) of the slice, so a wave reads whole lines.
+__device__ __forceinline__ void load_slice(const float* row, int s, int vocab, int t,
+                                           float (&x)[kPer]) {
+#pragma unroll
+  for (int g = 0; g < kLines; ++g) {
+    const int e = s * kSlice + g * 4 * kThreads + 4 * t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[4 * g + i] = at_or_zero(row, e + i, vocab);
+  }
+}
+
+// What an element weighs: its p, and its w.
+__device__ __forceinline__ double positive(double x) { return x > 0 ? x : 0; }  // NaN weighs nothing
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, kWave);
+  return x;
+}
+
+__global__ void __launch_bounds__(kThreads) verify_sums_kernel(VerifyArgs v) {
+  __shared__ double part[2][kWaves];
+  const int s = blockIdx.x, r = blockIdx.y;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const Request q = judge(v, r, lane);
+  if (s == 0) {
+    // The accepted drafts, and -1 behind the place of the drawn token.
+    for (int i = t; i < q.n; i += kThreads) {
+      if (i < q.a) v.tokens[q.d0 + r + i] = v.draft_tokens[q.d0 + i];
+      else v.tokens[q.d0 + r + i + 1] = -1;
+    }
+    if (t == 0) v.accepted[r] = q.a;
+  }
+  if (q.n < 0) return;
+  const Rows w = rows_of(v, q, r);
+  float p[kPer], d[kPer];
+  load_slice(w.p, s, v.vocab, t, p);
+  if (w.q) load_slice(w.q, s, v.vocab, t, d);
+  double sp = 0, sw = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = s * kSlice + (i >> 2) * 4 * kThreads + 4 * t + (i & 3);
+    sp += positive(p[i]);
+    double x = p[i];
+    if (w.q) x -= static_cast<double>(d[i]);
+    if (e == w.point) x = 0;
+    sw += positive(x);
+  }
+  sp = wave_sum(sp);
+  sw = wave_sum(sw);
+  if (lane == 0) part[0][wave] = sw, part[1][wave] = sp;
+  __syncthreads();
+  if (t < 2) {
+    double x = 0;
+    for (int k = 0; k < kWaves; ++k) x += part[t][k];
+    v.sums[(static_cast<int64_t>(r) * v.slices + s) * 2 + t] = x;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs v) {
+  __shared__ double part[kLines][kWaves];
+  __shared__ int hit[kLines * kWaves], last[kLines * kWaves];
+  const int r = blockIdx.x;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int a = v.accepted[r];
+  if (a < 0) return;
+  Request q;
+  q.d0 = v.indptr[r];
+  q.n = static_cast<int>(v.indptr[r + 1] - q.d0);
+  q.a = a;
+  const double u = v.sample_u[r];
+  const double* sums = v.sums + static_cast<int64_t>(r) * v.slices * 2;
+  // Every thread walks the slices' sums (a few tens, from L2).
+  double total = 0;
+  for (int k = 0; k < v.slices; ++k) total += sums[2 * k];
+  const bool residual = total > 0;  // p <= q everywhere: the draw is from p
+  const int col = residual ? 0 : 1;
+  if (!residual)
+    for (int k = 0; k < v.slices; ++k) total += sums[2 * k + 1];
+  int32_t* out = v.tokens + q.d0 + r + a;
+  if (!(total > 0)) {
+    if (t == 0) *out = v.vocab - 1;
+    return;
+  }
+  const double goal = u * total;
+  double before = 0, base = 0;
+  int s = -1;
+  bool found = false;
+  for (int k = 0; k < v.slices && !found; ++k) {
+    const double x = sums[2 * k + col];
+    if (x > 0) {
+      s = k;  // the last one with any weight, should rounding leave none past the goal
+      base = before;
+    }
+    before += x;
+    found = before > goal;
+  }
+  Rows w = rows_of(v, q, r);
+  if (!residual) w.q = nullptr, w.point = -1;
+  float p[kPer], d[kPer];
+  load_slice(w.p, s, v.vocab, t, p);
+  if (w.q) load_slice(w.q, s, v.vocab, t, d);
+  double x[kPer];
+  double lines[kLines];
+#pragma unroll
+  for (int g = 0; g < kLines; ++g) {
+    double sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = s * kSlice + g * 4 * kThreads + 4 * t + i;
+      double y = p[4 * g + i];
+      if (w.q) y -= static_cast<double>(d[4 * g + i]);
+      if (e == w.point) y = 0;
+      x[4 * g + i] = positive(y);
+      sum += x[4 * g + i];
+    }
+    lines[g] = sum;
+    const double all = wave_sum(sum);
+    if (lane == 0) part[g][wave] = all;
+  }
+  __syncthreads();
+  // First element past the goal, wave by wave: each (group, wave) starts from
+  // the sums before it and looks among its own 256 elements.
+#pragma unroll
+  for (int g = 0; g < kLines; ++g) {
+    double start = base;
+    for (int k = 0; k < g * kWaves + wave; ++k) start += part[k / kWaves][k % kWaves];
+    double incl = lines[g];
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      const double y = __shfl_up(incl, off, kWave);
+      if (lane >= off) incl += y;
+    }
+    double run = start + (incl - lines[g]);
+    int first = -1, final = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      run += x[4 * g + i];
+      if (x[4 * g + i] > 0) {
+        final = s * kSlice + g * 4 * kThreads + 4 * t + i;
+        if (first < 0 && run > goal) first = final;
+      }
+    }
+    const uint64_t mf = __builtin_amdgcn_ballot_w64(first >= 0);
+    const uint64_t ml = __builtin_amdgcn_ballot_w64(final >= 0);
+    const int f = mf ? __shfl(first, __builtin_ctzll(mf), kWave) : -1;
+    const int l = ml ? __shfl(final, 63 - __builtin_clzll(ml), kWave) : -1;
+    if (lane == 0) hit[g * kWaves + wave] = f, last[g * kWaves + wave] = l;
+  }
+  __syncthreads();
+  if (t == 0) {
+    int token = -1, end = v.vocab - 1;
+    for (int k = 0; k < kLines * kWaves; ++k) {
+      if (token < 0) token = hit[k];
+      if (last[k] >= 0) end = last[k];
+    }
+    *out = token >= 0 ? token : end;
+  }
+}
+
+inline int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
+
+}  // namespace
+}  // namespace sgl
+
+using namespace sgl;
+
+extern "C" int64_t sgl_verify_workspace_bytes(int batch_size, int vocab) {
+  if (batch_size <= 0 || vocab <= 0) return 0;
+  return static_cast<int64_t>(batch_size) * slices_of(vocab) * 2 * 8;
+}
+
+extern "C" int sgl_verify_drafts(const sgl_verify_args_t* args, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  if (!args) return SGL_ERR_INVALID_ARG;
+  const sgl_verify_args_t& x = *args;
+  if (x.batch_size < 0 || x.num_drafts < 0 || x.vocab <= 0) return SGL_ERR_INVALID_ARG;
+  if (x.batch_size == 0) return x.num_drafts == 0 ? SGL_OK : SGL_ERR_INVALID_ARG;
+  if (!x.target_probs || !x.draft_indptr || !x.sample_uniform || !x.tokens || !x.accepted)
+    return SGL_ERR_INVALID_ARG;
+  if (x.num_drafts > 0 && (!x.draft_tokens || !x.accept_uniform)) return SGL_ERR_INVALID_ARG;
+  if (x.target_stride_row < x.vocab || (x.draft_probs && x.draft_stride_row < x.vocab))
+    return SGL_ERR_INVALID_ARG;
+  if (x.batch_size > 65535 || x.num_drafts > 0x7fffffff - x.batch_size || x.vocab > (1 << 24))
+    return SGL_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < sgl_verify_workspace_bytes(x.batch_size, x.vocab))
+    return SGL_ERR_CAPACITY;
+  if (!aligned16(workspace)) return SGL_ERR_ALIGNMENT;
+  VerifyArgs v{};
+  v.target = x.target_probs, v.target_st = x.target_stride_row;
+  v.draft = x.draft_probs, v.draft_st = x.draft_stride_row;
+  v.draft_tokens = x.draft_tokens, v.indptr = x.draft_indptr;
+  v.accept_u = x.accept_uniform, v.sample_u = x.sample_uniform;
+  v.num_drafts = x.num_drafts, v.vocab = x.vocab, v.slices = slices_of(x.vocab);
+  v.tokens = x.tokens, v.accepted = x.accepted;
+  v.sums = static_cast<double*>(workspace);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(verify_sums_kernel, dim3(v.slices, x.batch_size), dim3(kThreads), 0, s, v);
+  const int st = launch_status();
+  if (st != SGL_OK) return st;
+  hipLaunchKernelGGL(verify_draw_kernel, dim3(x.batch_size), dim3(kThreads), 0, s, v);
+  return launch_status();
+}
