@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
-constexpr int kMinUnit = 64;              // shortest unit
+constexpr int kMinUnit = 16;              // shortest unit
 constexpr int kQPitch = kD + 8;           // LDS row pitch (bf16) of the Q^T copy
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
 constexpr int kMaxTileRows = 64;
@@ -137,30 +137,45 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const in
       vr[e] = ldg128(slot_row(vlane, __shfl(slot, 4 * j + e, kWave), ss_bytes));
   };
 
-  int slot = idx[min(n, len - 1)];
+  // Token i and head of packed row p = row0 + x, x < 64: i0 + (rem + x) / G, the
+  // division (of a number below 128 by G <= 64) as a product.
+  const int i0 = row0 / G, rem = row0 - i0 * G;
+  const uint32_t inv_g = (65536u + G - 1) / G;
+  auto token_of = [&](int x, int& head) {
+    const int y = rem + x;
+    const int d = static_cast<int>(static_cast<uint32_t>(y) * inv_g >> 16);
+    head = h * G + (y - d * G);
+    return i0 + d;
+  };
+  const int nrows = row_end - row0;
+
+  const int slot = idx[min(n, len - 1)];
   int slot_next = idx[min(kStep + n, len - 1)];
+  // Q rows, four of a block at a time (chunk n); rows past the last one read it again
+  // and are cleared, so that every load is in flight at once.
+  u32x4_t qv[4 * RB];
+#pragma unroll
+  for (int u = 0; u < 4 * RB; ++u) {
+    int head;
+    const int i = token_of(min(4 * u + j, nrows - 1), head);
+    qv[u] = ldg128(a.q + (tok0 + i) * a.q_st + head * a.q_sh + 8 * n);
+  }
   u32x4_t kr[4], vr[4];
   load_k(slot, kr);
   load_v(slot, vr);
-  // Q rows, four of a block at a time (chunk n), to LDS.
 #pragma unroll
-  for (int u = 0; u < 4 * RB; ++u) {
-    const int p = row0 + 4 * u + j;
-    u32x4_t qv = {0, 0, 0, 0};
-    if (p < row_end) {
-      const int i = p / G;
-      qv = ldg128(a.q + (tok0 + i) * a.q_st + (h * G + p - i * G) * a.q_sh + 8 * n);
-    }
-    *reinterpret_cast<u32x4_t*>(lq + (4 * u + j) * kQPitch + 8 * n) = qv;
-  }
+  for (int u = 0; u < 4 * RB; ++u)
+    *reinterpret_cast<u32x4_t*>(lq + (4 * u + j) * kQPitch + 8 * n) =
+        4 * u + j < nrows ? qv[u] : u32x4_t{0, 0, 0, 0};
   wave_lds_sync();
   int sees[RB];
   float m[RB], l[RB];
   f32x4_t acc[RB][8];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    const int p = row0 + 16 * b + n;
-    sees[b] = p < row_end ? min(sees0 + p / G, len) : 0;
+    int head;
+    const int i = token_of(16 * b + n, head);
+    sees[b] = 16 * b + n < nrows ? min(sees0 + i, len) : 0;
     m[b] = -INFINITY;
     l[b] = 0.f;
 #pragma unroll
@@ -230,10 +245,10 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const in
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const float sum = sum_xor32(sum_xor16(l[b]));
-    const int p = row0 + 16 * b + n;
-    if (p >= row_end) continue;
-    const int i = p / G;
-    const int64_t row = by_token ? (out0 + i) * a.hq + (h * G + p - i * G) : out0 + (p - row0);
+    if (16 * b + n >= nrows) continue;
+    int head;
+    const int i = token_of(16 * b + n, head);
+    const int64_t row = by_token ? (out0 + i) * a.hq + head : out0 + 16 * b + n;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // a NaN sum stays one
     // acc[nb][c] holds d = 32 j + 8 c + nb.
     float* op = o + row * kD + 32 * j;
@@ -342,10 +357,15 @@ __device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request&
   return acc * inv;
 }
 
-// Folds the pieces of each row: a workgroup per token, 32 lanes a row.
-__global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a) {
+// Folds the pieces of each row: kSets groups of 32 lanes take them in turn, four
+// pieces' loads in flight, and are folded through LDS; 8 / kSets heads of one token a
+// workgroup.
+template <int kSets>
+__global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head_groups) {
+  constexpr int kRows = 8 / kSets;
   __shared__ int before[4];
-  const int t = blockIdx.x;
+  __shared__ float xch[6][8][32];
+  const int t = blockIdx.x / static_cast<uint32_t>(head_groups);
   const int lane = threadIdx.x & 63;
   // The token's request: those that end at or before it are counted.
   int n = 0;
@@ -360,59 +380,102 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a) {
   const int first = max(a.qo_indptr[0], 0);
   const int64_t P = a.prefix, shared = P * a.tiles;
   const int64_t W = unit_tokens(a, shared + own_tokens(a));
-  const int c = threadIdx.x & 31;
+  const int c = threadIdx.x & 31, group = threadIdx.x >> 5;
+  const int set = group % kSets;
+  const int head = (blockIdx.x - t * head_groups) * kRows + group / kSets;
+  const bool head_ok = head < a.hq;
+  const int hh = head_ok ? head : a.hq - 1;
+  const int h = hh / a.group;
   const int i = t - x.q0;
-  const int64_t own0 = shared + x.kv0 - a.kv_indptr[0];
-  // Tokens this row sees, prefix first.
-  const int64_t sees = P + x.kv - x.qo + i + 1;
-  for (int head = threadIdx.x >> 5; head < a.hq; head += 8) {
-    uint16_t* op = a.o + t * a.o_st + head * a.o_sh + 4 * c;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    if (!x.ok) {
-      acc = f32x4_t{NAN, NAN, NAN, NAN};
-    } else if (sees < P) {
-      acc = plain_row(a, x, t, head, sees, c);
-    } else {
-      const int h = head / a.group;
-      const int prow = (t - first) * a.group + head - h * a.group;
-      float m = -INFINITY, l = 0.f;
-      auto add = [&](const float* o, const float* lse, int64_t row) {
-        const float s = lse[row];
-        if (s == -INFINITY) return;  // nothing seen there: its values do not count
-        const float mn = fmaxf(m, s);
-        const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
-        const float w = exp2f(s - mn);
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(o + row * kD + 4 * c);
-        l = l * alpha + w;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] = acc[k] * alpha + v[k] * w;
-        m = mn;
-      };
-      if (P > 0) {
-        const int tile = prow / a.tile_rows;
-        for (int64_t u = tile * P / W; u <= (tile * P + P - 1) / W; ++u)
-          add(a.p_o, a.p_lse, ((u + tile) * a.hkv + h) * a.tile_rows + prow - tile * a.tile_rows);
-      }
-      if (x.kv > 0) {
-        const int64_t u0 = own0 / W, u1 = (own0 + x.kv - 1) / W;
-        add(a.s_o, a.s_lse, static_cast<int64_t>(t) * a.hq + head);
-        for (int64_t u = u0 + 1; u <= u1; ++u)
-          add(a.s_o, a.s_lse, (a.tokens + u * a.max_qo + i) * a.hq + head);
-      }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] *= inv;
-      // Tokens of the request behind this row's last one may have brought in
-      // values that are not finite.
-      bool bad = false;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) bad = bad || !(fabsf(acc[k]) < INFINITY);
-      const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
-      if (i + 1 < x.qo && ((any >> (lane & 32)) & 0xffffffffull) != 0)
-        acc = plain_row(a, x, t, head, sees, c);
+  const int64_t sees = P + x.kv - x.qo + i + 1;  // tokens this row sees, prefix first
+  float m = -INFINITY, l = 0.f;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  const bool folded = x.ok && sees >= P;
+  if (folded) {
+    // Prefix pieces [0, np) at p0 + k p_step, then the request's own.
+    int np = 0, ns = 0;
+    int64_t p0 = 0, s1 = 0;
+    const int64_t p_step = static_cast<int64_t>(a.hkv) * a.tile_rows;
+    if (P > 0) {
+      const int prow = (t - first) * a.group + hh - h * a.group;
+      const int tile = prow / a.tile_rows;
+      const int64_t u0 = tile * P / W;
+      np = static_cast<int>((tile * P + P - 1) / W - u0) + 1;
+      p0 = ((u0 + tile) * a.hkv + h) * a.tile_rows + prow - tile * a.tile_rows;
     }
-    *reinterpret_cast<u32x2_t*>(op) = u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+    if (x.kv > 0) {
+      const int64_t own0 = shared + x.kv0 - a.kv_indptr[0], u0 = own0 / W;
+      ns = static_cast<int>((own0 + x.kv - 1) / W - u0) + 1;
+      s1 = (a.tokens + u0 * a.max_qo + i) * a.hq + hh;
+    }
+    const int64_t s0 = static_cast<int64_t>(t) * a.hq + hh, s_step = static_cast<int64_t>(a.max_qo) * a.hq;
+    for (int k0 = set; k0 < np + ns; k0 += 4 * kSets) {
+      f32x4_t v[4];
+      float lse[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = min(k0 + e * kSets, np + ns - 1);
+        const int64_t row = k < np ? p0 + k * p_step : k == np ? s0 : s1 + (k - np) * s_step;
+        v[e] = *reinterpret_cast<const f32x4_t*>((k < np ? a.p_o : a.s_o) + row * kD + 4 * c);
+        lse[e] = (k < np ? a.p_lse : a.s_lse)[row];
+        if (k0 + e * kSets >= np + ns) lse[e] = -INFINITY;
+      }
+      float mn = m;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mn = fmaxf(mn, lse[e]);
+      const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] *= alpha;
+      m = mn;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (lse[e] == -INFINITY) continue;  // nothing seen there: its values do not count
+        const float w = exp2f(lse[e] - mn);
+        l += w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += v[e][k] * w;
+      }
+    }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) xch[k][group][c] = acc[k];
+  xch[4][group][c] = m;
+  xch[5][group][c] = l;
+  __syncthreads();
+  if (set != 0 || !head_ok) return;
+  if (!x.ok) {
+    acc = f32x4_t{NAN, NAN, NAN, NAN};
+  } else if (!folded) {
+    acc = plain_row(a, x, t, head, sees, c);
+  } else {
+#pragma unroll
+    for (int e = 1; e < kSets; ++e) m = fmaxf(m, xch[4][group + e][c]);
+    l = 0.f;
+    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < kSets; ++e) {
+      const float me = xch[4][group + e][c], le = xch[5][group + e][c];
+      if (le == 0.f) continue;  // no piece with a weight
+      const float w = exp2f(me - m);
+      l += le * w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += xch[k][group + e][c] * w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] *= inv;
+    // Tokens of the request behind this row's last one may have brought in
+    // values that are not finite.
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) bad = bad || !(fabsf(acc[k]) < INFINITY);
+    const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
+    if (i + 1 < x.qo && ((any >> (lane & 32)) & 0xffffffffull) != 0)
+      acc = plain_row(a, x, t, head, sees, c);
+  }
+  *reinterpret_cast<u32x2_t*>(a.o + t * a.o_st + head * a.o_sh + 4 * c) =
+      u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
 }
 
 int device_cus() {
@@ -536,6 +599,8 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   const int64_t rows = static_cast<int64_t>(max_tokens) * a.group;
   a.tiles = p.num_tiles > 0 ? static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows) : 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  // The fold's grid is at most a workgroup per row.
+  if (static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff) return SGL_ERR_UNSUPPORTED;
   const int waves = heads_per_group(num_kv_heads);
   const dim3 grid(p.num_units, num_kv_heads / waves), block(64 * waves);
   const int need = p.max_qo_len * a.group > a.tile_rows ? p.max_qo_len * a.group : a.tile_rows;
@@ -546,6 +611,12 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   else hipLaunchKernelGGL(prefix_units_kernel<4>, grid, block, lds, s, a);
   st = launch_status();
   if (st != SGL_OK) return st;
-  hipLaunchKernelGGL(prefix_fold_kernel, dim3(max_tokens), dim3(256), 0, s, a);
+  // Many pieces a row: a workgroup for each. Few: two groups of lanes a row.
+  const int64_t pieces = a.tiles > 0 ? p.num_units / a.tiles + 2 : 2;
+  const int rows_per = pieces > 8 ? 1 : 4;
+  const int head_groups = (num_qo_heads + rows_per - 1) / rows_per;
+  const dim3 fold(static_cast<uint32_t>(max_tokens) * head_groups);
+  if (rows_per == 1) hipLaunchKernelGGL(prefix_fold_kernel<8>, fold, dim3(256), 0, s, a, head_groups);
+  else hipLaunchKernelGGL(prefix_fold_kernel<2>, fold, dim3(256), 0, s, a, head_groups);
   return launch_status();
 }

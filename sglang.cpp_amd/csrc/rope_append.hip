@@ -170,6 +170,141 @@ __global__ void __launch_bounds__(256) rope_append_elements_kernel(AppendArgs a)
   }
 }
 
+// Rows in 16-byte chunks: a job takes two chunks of a row, so that a rotated pair
+// of the half layout is in one thread (chunks j and j + R / 16) and nothing is
+// exchanged; interleaved pairs and copied elements lie inside a chunk, and there the
+// two are half a row apart, so that the lanes of a row read and write whole lines.
+// The token is the same for a whole workgroup (scalar slot and position loads); its
+// rows' jobs take blocks_per_token workgroups of a width that leaves few threads
+// without a job. kTokens tokens a thread, their loads in flight together. Bound by
+// the bytes of the rows, read once and written once: non-temporal.
+constexpr int kTokens = 2;
+
+template <int DT>
+__device__ __forceinline__ void rotate_half(u32x4_t& x, u32x4_t& y, const float* c, const float* s) {
+  float a[8], b[8], u[8], v[8];
+  unpack8_t<DT>(x, a);
+  unpack8_t<DT>(y, b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    u[i] = rope_one(a[i], -b[i], c[i], s[i]);
+    v[i] = rope_one(b[i], a[i], c[i], s[i]);
+  }
+  x = pack8_t<DT>(u);
+  y = pack8_t<DT>(v);
+}
+
+template <int DT>
+__device__ __forceinline__ void rotate_pairs(u32x4_t& x, const f32x4_t& c, const f32x4_t& s) {
+  float a[8], u[8];
+  unpack8_t<DT>(x, a);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u[2 * i] = rope_one(a[2 * i], -a[2 * i + 1], c[i], s[i]);
+    u[2 * i + 1] = rope_one(a[2 * i + 1], a[2 * i], c[i], s[i]);
+  }
+  x = pack8_t<DT>(u);
+}
+
+// J: jobs of a row (head_dim / 16), 0: read from the arguments.
+template <int DT, bool kInterleaved, int J>
+__global__ void __launch_bounds__(512) rope_append_kernel(AppendArgs a, int blocks_per_token) {
+  const int jobs = J ? J : a.d / 16;
+  const uint32_t group = blockIdx.x / static_cast<uint32_t>(blocks_per_token);
+  const int item = static_cast<int>(blockIdx.x - group * blocks_per_token) * blockDim.x + threadIdx.x;
+  const int r = item / jobs, j = item - r * jobs;
+  if (r >= a.hq + a.hk + a.hv) return;
+  const bool is_v = r >= a.hq + a.hk;
+  const int pairs = a.rotary / 16;  // half layout: jobs that rotate
+  int c0, c1;                       // the job's chunks
+  bool turn0, turn1;
+  if (kInterleaved || is_v) {
+    c0 = j, c1 = j + jobs;
+    turn0 = !is_v && 8 * c0 < a.rotary, turn1 = !is_v && 8 * c1 < a.rotary;
+  } else {
+    turn0 = turn1 = j < pairs;
+    c0 = turn0 ? j : 2 * pairs + (j - pairs);
+    c1 = turn0 ? j + pairs : c0 + (jobs - pairs);
+  }
+  u32x4_t x[kTokens], y[kTokens];
+  uint16_t* dst[kTokens];
+  int64_t pos[kTokens];
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k) {
+    const int64_t t = min(static_cast<int64_t>(group) * kTokens + k, a.tokens - 1);
+    const uint16_t* src;
+    append_row(a, t, r, slot_of(a, t), src, dst[k]);
+    if (static_cast<int64_t>(group) * kTokens + k >= a.tokens) dst[k] = nullptr;
+    x[k] = ldg128_nt<true>(src + 8 * c0);
+    y[k] = ldg128_nt<true>(src + 8 * c1);
+    pos[k] = a.positions[t];
+  }
+  const int half = a.rotary / 2;
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k) {
+    if (dst[k] == nullptr) continue;
+    const bool far = pos[k] < 0 || pos[k] >= a.max_pos;  // never rotated by a guess: NaN
+    const float* cr = a.cos + (far ? 0 : pos[k]) * half;
+    const float* sr = a.sin + (far ? 0 : pos[k]) * half;
+    if (kInterleaved) {
+      const f32x4_t nan = {NAN, NAN, NAN, NAN};
+      if (turn0) {
+        f32x4_t c = nan, s = nan;
+        if (!far) {
+          c = *reinterpret_cast<const f32x4_t*>(cr + 4 * c0);
+          s = *reinterpret_cast<const f32x4_t*>(sr + 4 * c0);
+        }
+        rotate_pairs<DT>(x[k], c, s);
+      }
+      if (turn1) {
+        f32x4_t c = nan, s = nan;
+        if (!far) {
+          c = *reinterpret_cast<const f32x4_t*>(cr + 4 * c1);
+          s = *reinterpret_cast<const f32x4_t*>(sr + 4 * c1);
+        }
+        rotate_pairs<DT>(y[k], c, s);
+      }
+    } else if (turn0) {
+      float c[8], s[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        f32x4_t cv = {NAN, NAN, NAN, NAN}, sv = cv;
+        if (!far) {
+          cv = *reinterpret_cast<const f32x4_t*>(cr + 8 * j + i);
+          sv = *reinterpret_cast<const f32x4_t*>(sr + 8 * j + i);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[i + e] = cv[e], s[i + e] = sv[e];
+      }
+      rotate_half<DT>(x[k], y[k], c, s);
+    }
+    stg128_nt<true>(dst[k] + 8 * c0, x[k]);
+    stg128_nt<true>(dst[k] + 8 * c1, y[k]);
+  }
+}
+
+template <int DT, bool kInterleaved>
+void launch_chunks(const AppendArgs& a, hipStream_t s) {
+  const int jobs = a.d / 16;
+  const int64_t items = (static_cast<int64_t>(a.hq) + a.hk + a.hv) * jobs;
+  // The workgroup width, in waves, that leaves the fewest threads without a job.
+  int waves = 4;
+  int64_t best = -1;
+  for (int w = 8; w >= 2; --w) {
+    const int64_t idle = (items + 64 * w - 1) / (64 * w) * (64 * w) - items;
+    if (best < 0 || idle < best) best = idle, waves = w;
+  }
+  const int64_t per_token = (items + 64 * waves - 1) / (64 * waves);
+  const dim3 grid(static_cast<uint32_t>((a.tokens + kTokens - 1) / kTokens * per_token));
+  const dim3 block(64 * waves);
+  const int bpt = static_cast<int>(per_token);
+  switch (jobs) {
+    case 4: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 4>), grid, block, 0, s, a, bpt); break;
+    case 8: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 8>), grid, block, 0, s, a, bpt); break;
+    default: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 0>), grid, block, 0, s, a, bpt);
+  }
+}
+
 inline int64_t blocks_for(int64_t jobs, int64_t per_block) { return (jobs + per_block - 1) / per_block; }
 
 // f_i of each pair and the factor of cos and sin, from the scaling's published
@@ -306,9 +441,25 @@ extern "C" int sgl_rope_append(const sgl_rope_append_t* args, void* stream) {
   const int64_t rows = static_cast<int64_t>(a.hq) + a.hk + a.hv;
   const int64_t per_token = rows * (a.d - a.rotary / 2);
   if (per_token > 0x7fffffff) return SGL_ERR_UNSUPPORTED;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  auto chunked = [](const void* p, int64_t st, int64_t sh) {
+    return p == nullptr || (aligned16(p) && st % 8 == 0 && sh % 8 == 0);
+  };
+  // Whole chunks everywhere; the grid (at most rows * d / 16 threads a token) in 31 bits.
+  if (a.d % 16 == 0 && a.rotary % 16 == 0 && chunked(a.q, a.q_st, a.q_sh) &&
+      chunked(a.q_out, a.qo_st, a.qo_sh) && chunked(a.k, a.k_st, a.k_sh) &&
+      chunked(a.v, a.v_st, a.v_sh) && chunked(a.k_cache, a.kv_ss, a.kv_sh) &&
+      chunked(a.v_cache, a.kv_ss, a.kv_sh) && aligned16(a.cos) && aligned16(a.sin) &&
+      (a.tokens / kTokens + 1) * (rows * (a.d / 16) / 128 + 1) < 0x7fffffff) {
+    if (x.dtype == SGL_DTYPE_BF16) {
+      if (il) launch_chunks<SGL_DTYPE_BF16, true>(a, s); else launch_chunks<SGL_DTYPE_BF16, false>(a, s);
+    } else {
+      if (il) launch_chunks<SGL_DTYPE_F16, true>(a, s); else launch_chunks<SGL_DTYPE_F16, false>(a, s);
+    }
+    return launch_status();
+  }
   const int64_t blocks = blocks_for(a.tokens * per_token, 256);
   const dim3 grid(static_cast<uint32_t>(blocks < 65536 ? blocks : 65536));
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   if (x.dtype == SGL_DTYPE_BF16) {
     if (il) hipLaunchKernelGGL((rope_append_elements_kernel<SGL_DTYPE_BF16, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((rope_append_elements_kernel<SGL_DTYPE_BF16, false>), grid, dim3(256), 0, s, a);

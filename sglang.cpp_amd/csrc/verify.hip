@@ -97,18 +97,30 @@ __device__ __forceinline__ Rows rows_of(const VerifyArgs& v, const Request& q, i
   return w;
 }
 
-__device__ __forceinline__ float at_or_zero(const float* row, int e, int n) { return e < n ? row[e] : 0.f; }
+// Four consecutive elements of a row, whose address is a multiple of 4 bytes.
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // A thread's 16 elements of slice s: group g holds elements
 // [1024 g + 4 t, ... + 4) of the slice, so a wave reads whole lines.
 __device__ __forceinline__ void load_slice(const float* row, int s, int vocab, int t,
                                            float (&x)[kPer]) {
+  const int e0 = s * kSlice + 4 * t;
+  if ((s + 1) * kSlice <= vocab) {  // a whole slice
 #pragma unroll
-  for (int g = 0; g < kLines; ++g) {
-    const int e = s * kSlice + g * 4 * kThreads + 4 * t;
+    for (int g = 0; g < kLines; ++g) {
+      const f32x4_any_t v = *reinterpret_cast<const f32x4_any_t*>(row + e0 + g * 4 * kThreads);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[4 * g + i] = at_or_zero(row, e + i, vocab);
+      for (int i = 0; i < 4; ++i) x[4 * g + i] = v[i];
+    }
+    return;
   }
+#pragma unroll
+  for (int g = 0; g < kLines; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = e0 + g * 4 * kThreads + i;
+      x[4 * g + i] = e < vocab ? row[e] : 0.f;
+    }
 }
 
 // What an element weighs: its p, and its w.
@@ -117,6 +129,16 @@ __device__ __forceinline__ double positive(double x) { return x > 0 ? x : 0; }  
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, kWave);
+  return x;
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ double wave_scan(double x, int lane) {
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const double y = __shfl_up(x, off, kWave);
+    if (lane >= off) x += y;
+  }
   return x;
 }
 
@@ -172,30 +194,38 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs v) {
   q.a = a;
   const double u = v.sample_u[r];
   const double* sums = v.sums + static_cast<int64_t>(r) * v.slices * 2;
-  // Every thread walks the slices' sums (a few tens, from L2).
-  double total = 0;
-  for (int k = 0; k < v.slices; ++k) total += sums[2 * k];
+  // Every wave looks through the slices' sums, 64 at a time.
+  double total = 0, total_p = 0;
+  for (int k0 = 0; k0 < v.slices; k0 += kWave) {
+    const int k = k0 + lane;
+    total += wave_sum(k < v.slices ? sums[2 * k] : 0);
+    total_p += wave_sum(k < v.slices ? sums[2 * k + 1] : 0);
+  }
   const bool residual = total > 0;  // p <= q everywhere: the draw is from p
   const int col = residual ? 0 : 1;
-  if (!residual)
-    for (int k = 0; k < v.slices; ++k) total += sums[2 * k + 1];
+  if (!residual) total = total_p;
   int32_t* out = v.tokens + q.d0 + r + a;
   if (!(total > 0)) {
     if (t == 0) *out = v.vocab - 1;
     return;
   }
   const double goal = u * total;
+  // The slice whose running sum passes the goal, or the last one with any weight,
+  // should rounding leave none.
   double before = 0, base = 0;
-  int s = -1;
-  bool found = false;
-  for (int k = 0; k < v.slices && !found; ++k) {
-    const double x = sums[2 * k + col];
-    if (x > 0) {
-      s = k;  // the last one with any weight, should rounding leave none past the goal
-      base = before;
-    }
-    before += x;
-    found = before > goal;
+  int s = 0;
+  for (int k0 = 0; k0 < v.slices; k0 += kWave) {
+    const int k = k0 + lane;
+    const double x = k < v.slices ? sums[2 * k + col] : 0;
+    const double incl = wave_scan(x, lane);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > goal && x > 0);
+    const uint64_t any = __builtin_amdgcn_ballot_w64(x > 0);
+    if (any == 0) continue;
+    const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
+    s = k0 + at;
+    base = before + __shfl(incl - x, at, kWave);
+    if (past) break;
+    before += __shfl(incl, 63, kWave);
   }
   Rows w = rows_of(v, q, r);
   if (!residual) w.q = nullptr, w.point = -1;
@@ -227,12 +257,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs v) {
   for (int g = 0; g < kLines; ++g) {
     double start = base;
     for (int k = 0; k < g * kWaves + wave; ++k) start += part[k / kWaves][k % kWaves];
-    double incl = lines[g];
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const double y = __shfl_up(incl, off, kWave);
-      if (lane >= off) incl += y;
-    }
+    const double incl = wave_scan(lines[g], lane);
     double run = start + (incl - lines[g]);
     int first = -1, final = -1;
 #pragma unroll
