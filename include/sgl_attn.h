@@ -578,9 +578,9 @@ typedef struct {
   int32_t num_kv_heads;
   int32_t head_dim;
   int32_t num_units;    /* workgroups that walk equal shares of the tokens */
-  int32_t tile_rows;    /* packed query rows of a walk over the prefix */
-  int32_t num_tiles;    /* such walks of the units (0: the prefix has launches of its own) */
-  int32_t num_shares;   /* shares of the prefix's own launch */
+  int32_t tile_rows;    /* packed query rows (tokens x heads of a kv head) of a walk over the prefix */
+  int32_t num_tiles;    /* 1: the units walk the prefix too, 0: it has a launch of its own */
+  int32_t num_shares;   /* shares of the prefix in that launch */
   int32_t reserved;
   int64_t workspace_bytes;
 } sgl_prefix_plan_t;

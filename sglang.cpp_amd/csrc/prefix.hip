@@ -17,6 +17,7 @@
 #include <math.h>
 
 #include "common.h"
+#include "prefill_impl.h"
 
 namespace sgl {
 namespace {
@@ -40,11 +41,12 @@ struct PrefixArgs {
   const int32_t* qo_indptr;
   int batch, tokens, hq, hkv, group;
   int prefix, tile_rows, tiles, units, max_qo;
+  int shares, row_tiles;  // of the prefix's own launch: item = row tile, then kv head, then share
   float scale_log2;
   uint16_t* o;
   int64_t o_st, o_sh;
   // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix pieces: piece u + tile,
-  // [piece][kv head][row of the tile]. Own pieces: [token slot][q head], the piece a
+  // [piece][kv head][row of the tile], or [share][kv head][packed row]. Own pieces: [token slot][q head], the piece a
   // request starts with at its rows' own tokens, the one running into unit u from
   // before it at tokens + u max_qo + i.
   float* p_o;
@@ -321,6 +323,147 @@ __global__ void __launch_bounds__(512) prefix_units_kernel(PrefixArgs a) {
   }
 }
 
+// The prefix for many rows: W waves with 32 packed rows each share the 64-token K/V
+// tiles that they gather into LDS (two buffers, K one tile ahead of V), and tile t + 1's
+// scores are on the matrix cores while tile t's become weights; the prefill kernel's
+// tile steps without a causal bound. Item: (row tile, kv head, share of the prefix's
+// tiles). Bound by the matrix cores: 4 x 64 x 128 flops a row and tile.
+template <int W>
+__device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* lds_raw, int item) {
+  using namespace pf;
+  const int per_tile = a.hkv * a.shares;
+  const int rt = item / per_tile;
+  const int hs = item - rt * per_tile;
+  const int h = hs % a.hkv, share = hs / a.hkv;
+  const int first = max(a.qo_indptr[0], 0);
+  const int last = min(a.qo_indptr[a.batch], a.tokens);
+  const int rows = max(last - first, 0) * a.group;
+  const int row0 = rt * 32 * W;
+  if (row0 >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = threadIdx.x;
+  const int c = lane & 31, hl = lane >> 5;
+  const int prow = row0 + 32 * wave + c;
+  const bool row_ok = prow < rows;
+  const bool works = row0 + 32 * wave < rows;  // the others only gather
+  const int safe = row_ok ? prow : row0;
+  const int qtok = safe / a.group;
+  const int qhead = h * a.group + (safe - qtok * a.group);
+  const int nt = (a.prefix + kBN - 1) / kBN;
+  const int per = (nt + a.shares - 1) / a.shares;
+  const int tb = share * per, te = min(nt, tb + per);
+  if (tb >= te) return;
+  const int kv_len = a.prefix;
+
+  Tile* tiles = reinterpret_cast<Tile*>(lds_raw);
+  const uint16_t* kbase = a.kc + h * a.kv_sh;
+  const uint16_t* vbase = a.vc + h * a.kv_sh;
+  const uint32_t ss_bytes = static_cast<uint32_t>(a.kv_ss * 2);
+  const int lch0 = (lane & 15) ^ swz(4 * wave + (lane >> 4));
+  const int lch1 = (lane & 15) ^ swz((4 * wave + (lane >> 4) + 8) & 15);
+  const char* const klane[2] = {reinterpret_cast<const char*>(kbase) + lch0 * 16,
+                                reinterpret_cast<const char*>(kbase) + lch1 * 16};
+  const char* const vlane[2] = {reinterpret_cast<const char*>(vbase) + lch0 * 16,
+                                reinterpret_cast<const char*>(vbase) + lch1 * 16};
+  LaneAddr la;
+  {
+    const uint32_t base = lds_addr(tiles);
+    const int sw = swz(c);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) la.k[s] = base + c * pf::kD * 2 + ((2 * s + hl) ^ sw) * 16;
+    const int vrow = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int g = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        const int row = vrow + 8 * hi;
+        la.v[2 * db + hi] = base + kVOffset + row * pf::kD * 2 + ((4 * db + g) ^ swz(row)) * 16 + 8 * (lane & 1);
+      }
+  }
+  PrefillArgs pa{};
+  pa.scale_log2 = a.scale_log2;
+  RowState rs;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) rs.acc[db][v] = 0.f;
+  rs.m = -INFINITY;
+  rs.l = 0.f;
+
+  int32_t sl_k[16 / W], sl_v[16 / W];
+  load_slots<W>(a.pidx, tb * kBN, kv_len, tid, sl_k);
+  load_slots<W>(a.pidx, (tb + 1) * kBN, kv_len, tid, sl_v);
+  wait_gathers();
+  issue_half<W>(klane, ss_bytes, sl_k, tiles[0].k, wave);
+  issue_half<W>(vlane, ss_bytes, sl_k, tiles[0].v, wave);
+  if (tb + 1 < te) issue_half<W>(klane, ss_bytes, sl_v, tiles[1].k, wave);
+  load_slots<W>(a.pidx, (tb + 2) * kBN, kv_len, tid, sl_k);
+  bf16x8_t qop[8];
+  {
+    const uint16_t* qp = a.q + static_cast<int64_t>(first + qtok) * a.q_st + static_cast<int64_t>(qhead) * a.q_sh;
+    u32x4_t qv[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) qv[s] = ldg128(qp + 16 * s + 8 * hl);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) qop[s] = pf::as_bf16x8(row_ok ? qv[s] : u32x4_t{0, 0, 0, 0});
+  }
+  wait_gathers();
+  __syncthreads();
+  f32x16_t s_a[2], s_b[2];
+  bf16x8_t pop[4];
+  qk_tile<0>(la, qop, s_a);
+  __syncthreads();  // every wave has read K(0) before K(2) overwrites it
+  auto step = [&](auto B, int t, f32x16_t(&s_cur)[2], f32x16_t(&s_next)[2]) {
+    constexpr int buf = decltype(B)::value;  // (t - tb) % 2
+    if (t + 2 < te) issue_half<W>(klane, ss_bytes, sl_k, tiles[buf].k, wave);
+    if (t + 1 < te) issue_half<W>(vlane, ss_bytes, sl_v, tiles[buf ^ 1].v, wave);
+#pragma unroll
+    for (int u = 0; u < 16 / W; ++u) sl_v[u] = sl_k[u];
+    load_slots<W>(a.pidx, (t + 3) * kBN, kv_len, tid, sl_k);
+    if (works) {
+      u32x4_t kb[16];
+      qk_tile_prefetch<buf ^ 1>(la, kb);
+      softmax_head(pa, s_cur, rs, t * kBN, kv_len, kv_len - 1, kv_len, hl);
+      lgkm_wait<0>(kb[kKAhead - 1]);
+      u32x2_t vr[4][8];
+      qk_tile_run<buf ^ 1>(la, qop, s_next, kb);  // S(t + 1); unused after the last tile
+      softmax_exp_half<0>(pa, s_cur, rs, pop);
+      pv_reads<buf, 0>(la, vr[0]);
+      pv_steps<buf, 0, 2>(la, pop, vr, rs);
+      softmax_exp_half<1>(pa, s_cur, rs, pop);
+      pv_steps<buf, 2, 4>(la, pop, vr, rs);
+    }
+    wait_gathers();
+    __syncthreads();
+  };
+  for (int t = tb; t < te; t += 2) {
+    step(std::integral_constant<int, 0>{}, t, s_a, s_b);
+    if (t + 1 >= te) break;
+    step(std::integral_constant<int, 1>{}, t + 1, s_b, s_a);
+  }
+  const float l = sum_xor32(rs.l);
+  if (!row_ok) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const int64_t row = (static_cast<int64_t>(share) * a.hkv + h) * (static_cast<int64_t>(a.tokens) * a.group) + prow;
+  float* op = a.p_o + row * sgl::kD;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4_t*>(op + 32 * db + 8 * g + 4 * hl) =
+          f32x4_t{rs.acc[db][4 * g] * inv, rs.acc[db][4 * g + 1] * inv, rs.acc[db][4 * g + 2] * inv,
+                  rs.acc[db][4 * g + 3] * inv};
+  if (hl == 0) a.p_lse[row] = l == 0.f ? -INFINITY : rs.m + log2f(l);
+}
+
+template <int W>
+__global__ void __launch_bounds__(64 * W, 8 / W) prefix_rows_kernel(PrefixArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds_raw[2 * pf::kTileBytes];
+  prefix_item<W>(a, lds_raw, blockIdx.x);
+}
+
 // Sum over the 32 lanes of a half wave, the same in each.
 __device__ __forceinline__ float half_sum(float x) {
 #pragma unroll
@@ -395,9 +538,13 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
     // Prefix pieces [0, np) at p0 + k p_step, then the request's own.
     int np = 0, ns = 0;
     int64_t p0 = 0, s1 = 0;
-    const int64_t p_step = static_cast<int64_t>(a.hkv) * a.tile_rows;
-    if (P > 0) {
-      const int prow = (t - first) * a.group + hh - h * a.group;
+    int64_t p_step = static_cast<int64_t>(a.hkv) * a.tile_rows;
+    const int prow = (t - first) * a.group + hh - h * a.group;
+    if (P > 0 && a.shares > 0) {
+      np = a.shares;
+      p_step = static_cast<int64_t>(a.hkv) * a.tokens * a.group;
+      p0 = static_cast<int64_t>(h) * a.tokens * a.group + prow;
+    } else if (P > 0) {
       const int tile = prow / a.tile_rows;
       const int64_t u0 = tile * P / W;
       np = static_cast<int>((tile * P + P - 1) / W - u0) + 1;
@@ -500,7 +647,8 @@ struct Layout {
 Layout workspace_layout(const sgl_prefix_plan_t& p) {
   auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
   const int64_t prefix_rows = p.num_tiles > 0
-      ? (static_cast<int64_t>(p.num_units) + p.num_tiles) * p.num_kv_heads * p.tile_rows : 0;
+      ? (static_cast<int64_t>(p.num_units) + p.num_tiles) * p.num_kv_heads * p.tile_rows
+      : static_cast<int64_t>(p.num_shares) * p.max_tokens * p.num_qo_heads;
   const int64_t own_rows =
       (p.max_tokens + static_cast<int64_t>(p.num_units) * p.max_qo_len) * p.num_qo_heads;
   Layout l;
@@ -540,9 +688,27 @@ extern "C" int sgl_prefix_plan(int prefix_len, int batch_size, int max_tokens, i
   const int64_t units = static_cast<int64_t>(device_cus()) * 8 / num_kv_heads;
   plan->num_units = static_cast<int32_t>(units < 1 ? 1 : units);
   const int64_t rows = static_cast<int64_t>(max_tokens) * group;
-  plan->tile_rows = static_cast<int32_t>(rows < kMaxTileRows ? (rows + 15) / 16 * 16 : kMaxTileRows);
-  plan->num_tiles = prefix_len > 0 && rows > 0
-                        ? static_cast<int32_t>((rows + plan->tile_rows - 1) / plan->tile_rows) : 0;
+  if (prefix_len > 0 && rows > 0) {
+    if (rows <= kMaxTileRows) {  // the units walk the prefix
+      plan->tile_rows = static_cast<int32_t>((rows + 15) / 16 * 16);
+      plan->num_tiles = 1;
+    } else {
+      // A launch of its own: the shares whose items, all rounds together, walk the
+      // fewest tiles one after the other (two for an item's start and its states).
+      plan->tile_rows = rows <= 128 ? 128 : 256;
+      const int64_t slots = device_cus() * (256 / plan->tile_rows);
+      const int64_t per_share = (rows + plan->tile_rows - 1) / plan->tile_rows * num_kv_heads;
+      const int64_t nt = (prefix_len + pf::kBN - 1) / pf::kBN;
+      int64_t best = 0, shares = 1;
+      for (int64_t n = 1; n <= nt && (n == 1 || (n - 1) * per_share < 4 * slots); ++n) {
+        const int64_t per = (nt + n - 1) / n, used = (nt + per - 1) / per;
+        if (used != n) continue;
+        const int64_t cost = (n * per_share + slots - 1) / slots * (per + 2);
+        if (best == 0 || cost < best) best = cost, shares = n;
+      }
+      plan->num_shares = static_cast<int32_t>(shares);
+    }
+  }
   plan->workspace_bytes = workspace_layout(*plan).total;
   return SGL_OK;
 }
@@ -568,7 +734,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   if (st != SGL_OK) return st;
   p.num_units = plan->num_units;
   if (p.num_units <= 0 || p.num_units > (1 << 20) || plan->tile_rows != p.tile_rows ||
-      plan->num_tiles != p.num_tiles)
+      plan->num_tiles != p.num_tiles || plan->num_shares != p.num_shares)
     return SGL_ERR_INVALID_ARG;
   if (batch_size > p.batch_size || max_tokens > p.max_tokens) return SGL_ERR_CAPACITY;
   if (batch_size == 0 || max_tokens == 0) return SGL_OK;
@@ -597,13 +763,25 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   a.p_o = reinterpret_cast<float*>(ws + l.p_o), a.p_lse = reinterpret_cast<float*>(ws + l.p_lse);
   a.s_o = reinterpret_cast<float*>(ws + l.s_o), a.s_lse = reinterpret_cast<float*>(ws + l.s_lse);
   const int64_t rows = static_cast<int64_t>(max_tokens) * a.group;
-  a.tiles = p.num_tiles > 0 ? static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows) : 0;
+  a.tiles = p.num_tiles;
+  a.shares = p.num_shares;
+  a.row_tiles = a.shares > 0 ? static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows) : 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t items = static_cast<int64_t>(a.row_tiles) * num_kv_heads * a.shares;
+  if (items > 0x7fffffff) return SGL_ERR_UNSUPPORTED;
   // The fold's grid is at most a workgroup per row.
   if (static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff) return SGL_ERR_UNSUPPORTED;
   const int waves = heads_per_group(num_kv_heads);
   const dim3 grid(p.num_units, num_kv_heads / waves), block(64 * waves);
-  const int need = p.max_qo_len * a.group > a.tile_rows ? p.max_qo_len * a.group : a.tile_rows;
+  if (items > 0) {
+    const dim3 own(static_cast<uint32_t>(items));
+    if (p.tile_rows == 128) hipLaunchKernelGGL(prefix_rows_kernel<4>, own, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(prefix_rows_kernel<8>, own, dim3(512), 0, s, a);
+    st = launch_status();
+    if (st != SGL_OK) return st;
+  }
+  const int own_rows = p.max_qo_len * a.group;
+  const int need = a.tiles > 0 && own_rows < a.tile_rows ? a.tile_rows : own_rows;
   const int rb = need <= 16 ? 1 : need <= 32 ? 2 : 4;
   const size_t lds = static_cast<size_t>(waves) * 16 * rb * kQPitch * 2;
   if (rb == 1) hipLaunchKernelGGL(prefix_units_kernel<1>, grid, block, lds, s, a);
@@ -612,7 +790,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   st = launch_status();
   if (st != SGL_OK) return st;
   // Many pieces a row: a workgroup for each. Few: two groups of lanes a row.
-  const int64_t pieces = a.tiles > 0 ? p.num_units / a.tiles + 2 : 2;
+  const int64_t pieces = a.tiles > 0 ? p.num_units : a.shares + 1;
   const int rows_per = pieces > 8 ? 1 : 4;
   const int head_groups = (num_qo_heads + rows_per - 1) / rows_per;
   const dim3 fold(static_cast<uint32_t>(max_tokens) * head_groups);

@@ -27,6 +27,7 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kPer = 16;                    // elements of a thread
 constexpr int kSlice = kThreads * kPer;     // elements of a slice
 constexpr int kLines = kPer / 4;            // groups of 4 consecutive elements of a thread
+constexpr int64_t kSingles = 1024;          // slices of a launch up to which each is a workgroup
 
 struct VerifyArgs {
   const float* target;
@@ -104,7 +105,7 @@ typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 // [1024 g + 4 t, ... + 4) of the slice, so a wave reads whole lines.
 __device__ __forceinline__ void load_slice(const float* row, int s, int vocab, int t,
                                            float (&x)[kPer]) {
-  const int e0 = s * kSlice + 4 * t;
+  const int e0 = s * kSlice + 4 * t;  // at most 2^24 and a few slices
   if ((s + 1) * kSlice <= vocab) {  // a whole slice
 #pragma unroll
     for (int g = 0; g < kLines; ++g) {
@@ -126,28 +127,45 @@ __device__ __forceinline__ void load_slice(const float* row, int s, int vocab, i
 // What an element weighs: its p, and its w.
 __device__ __forceinline__ double positive(double x) { return x > 0 ? x : 0; }  // NaN weighs nothing
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, kWave);
+// Lane exchange inside the vector registers (a shuffle is an LDS round trip, twice for
+// 64 bits): lanes that a shift brings nothing to, and rows outside the mask, get 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double x) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(w), CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(w >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Sum over the lanes up to this one: shifts by 1, 2, 4 and 8 in each row of 16, then
+// the last lane of a row to the next row, of the first half to the second.
+__device__ __forceinline__ double wave_scan(double x) {
+  x += dpp_or_zero<0x111, 0xF>(x);
+  x += dpp_or_zero<0x112, 0xF>(x);
+  x += dpp_or_zero<0x114, 0xF>(x);
+  x += dpp_or_zero<0x118, 0xF>(x);
+  x += dpp_or_zero<0x142, 0xA>(x);
+  x += dpp_or_zero<0x143, 0xC>(x);
   return x;
 }
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ double wave_scan(double x, int lane) {
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const double y = __shfl_up(x, off, kWave);
-    if (lane >= off) x += y;
-  }
-  return x;
+// Lane `at`'s value (the same `at` in every lane).
+__device__ __forceinline__ double lane_value(double x, int at) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(w), at);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(w >> 32), at);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
+// kRun consecutive slices a workgroup, the next one's loads in flight while one is
+// summed: the dependent loads of judge() come before 16 KB or before 64.
+template <int kRun>
 __global__ void __launch_bounds__(kThreads) verify_sums_kernel(VerifyArgs v) {
-  __shared__ double part[2][kWaves];
-  const int s = blockIdx.x, r = blockIdx.y;
+  __shared__ double part[kRun][2][kWaves];
+  const int s0 = blockIdx.x * kRun, r = blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const Request q = judge(v, r, lane);
-  if (s == 0) {
+  if (s0 == 0) {
     // The accepted drafts, and -1 behind the place of the drawn token.
     for (int i = t; i < q.n; i += kThreads) {
       if (i < q.a) v.tokens[q.d0 + r + i] = v.draft_tokens[q.d0 + i];
@@ -157,54 +175,61 @@ __global__ void __launch_bounds__(kThreads) verify_sums_kernel(VerifyArgs v) {
   }
   if (q.n < 0) return;
   const Rows w = rows_of(v, q, r);
-  float p[kPer], d[kPer];
-  load_slice(w.p, s, v.vocab, t, p);
-  if (w.q) load_slice(w.q, s, v.vocab, t, d);
-  double sp = 0, sw = 0;
+  float p[2][kPer], d[2][kPer];
+  load_slice(w.p, s0, v.vocab, t, p[0]);
+  if (w.q) load_slice(w.q, s0, v.vocab, t, d[0]);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int e = s * kSlice + (i >> 2) * 4 * kThreads + 4 * t + (i & 3);
-    sp += positive(p[i]);
-    double x = p[i];
-    if (w.q) x -= static_cast<double>(d[i]);
-    if (e == w.point) x = 0;
-    sw += positive(x);
+  for (int k = 0; k < kRun; ++k) {
+    const int s = s0 + k, b = k & 1;
+    if (k + 1 < kRun) {  // past the last slice: all zero, not read
+      load_slice(w.p, s + 1, v.vocab, t, p[b ^ 1]);
+      if (w.q) load_slice(w.q, s + 1, v.vocab, t, d[b ^ 1]);
+    }
+    double sp = 0, sw = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = s * kSlice + (i >> 2) * 4 * kThreads + 4 * t + (i & 3);
+      sp += positive(p[b][i]);
+      double x = p[b][i];
+      if (w.q) x -= static_cast<double>(d[b][i]);
+      if (e == w.point) x = 0;
+      sw += positive(x);
+    }
+    sp = wave_scan(sp);
+    sw = wave_scan(sw);
+    if (lane == 63) part[k][0][wave] = sw, part[k][1][wave] = sp;
   }
-  sp = wave_sum(sp);
-  sw = wave_sum(sw);
-  if (lane == 0) part[0][wave] = sw, part[1][wave] = sp;
   __syncthreads();
-  if (t < 2) {
+  if (t < 2 * kRun && s0 + t / 2 < v.slices) {
     double x = 0;
-    for (int k = 0; k < kWaves; ++k) x += part[t][k];
-    v.sums[(static_cast<int64_t>(r) * v.slices + s) * 2 + t] = x;
+    for (int k = 0; k < kWaves; ++k) x += part[t / 2][t & 1][k];
+    v.sums[(static_cast<int64_t>(r) * v.slices + s0) * 2 + t] = x;
   }
 }
 
 __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs v) {
-  __shared__ double part[kLines][kWaves];
-  __shared__ int hit[kLines * kWaves], last[kLines * kWaves];
+  __shared__ double part[kWaves];
+  __shared__ int hit[kWaves], last[kWaves];
   const int r = blockIdx.x;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int a = v.accepted[r];
-  if (a < 0) return;
+  const double* sums = v.sums + static_cast<int64_t>(r) * v.slices * 2;
   Request q;
+  q.a = v.accepted[r];
   q.d0 = v.indptr[r];
   q.n = static_cast<int>(v.indptr[r + 1] - q.d0);
-  q.a = a;
   const double u = v.sample_u[r];
-  const double* sums = v.sums + static_cast<int64_t>(r) * v.slices * 2;
   // Every wave looks through the slices' sums, 64 at a time.
   double total = 0, total_p = 0;
   for (int k0 = 0; k0 < v.slices; k0 += kWave) {
     const int k = k0 + lane;
-    total += wave_sum(k < v.slices ? sums[2 * k] : 0);
-    total_p += wave_sum(k < v.slices ? sums[2 * k + 1] : 0);
+    total += lane_value(wave_scan(k < v.slices ? sums[2 * k] : 0), 63);
+    total_p += lane_value(wave_scan(k < v.slices ? sums[2 * k + 1] : 0), 63);
   }
+  if (q.a < 0) return;
   const bool residual = total > 0;  // p <= q everywhere: the draw is from p
   const int col = residual ? 0 : 1;
   if (!residual) total = total_p;
-  int32_t* out = v.tokens + q.d0 + r + a;
+  int32_t* out = v.tokens + q.d0 + r + q.a;
   if (!(total > 0)) {
     if (t == 0) *out = v.vocab - 1;
     return;
@@ -217,67 +242,69 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs v) {
   for (int k0 = 0; k0 < v.slices; k0 += kWave) {
     const int k = k0 + lane;
     const double x = k < v.slices ? sums[2 * k + col] : 0;
-    const double incl = wave_scan(x, lane);
+    const double incl = wave_scan(x);
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > goal && x > 0);
     const uint64_t any = __builtin_amdgcn_ballot_w64(x > 0);
     if (any == 0) continue;
     const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
     s = k0 + at;
-    base = before + __shfl(incl - x, at, kWave);
+    base = before + lane_value(incl - x, at);
     if (past) break;
-    before += __shfl(incl, 63, kWave);
+    before += lane_value(incl, 63);
   }
+  // The slice in order: thread t has its elements [16 t, 16 t + 16).
   Rows w = rows_of(v, q, r);
   if (!residual) w.q = nullptr, w.point = -1;
-  float p[kPer], d[kPer];
-  load_slice(w.p, s, v.vocab, t, p);
-  if (w.q) load_slice(w.q, s, v.vocab, t, d);
+  const int e0 = s * kSlice + kPer * t;
   double x[kPer];
-  double lines[kLines];
+  if (e0 + kPer <= v.vocab) {
+    f32x4_any_t p[kLines], d[kLines];
 #pragma unroll
-  for (int g = 0; g < kLines; ++g) {
-    double sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = s * kSlice + g * 4 * kThreads + 4 * t + i;
-      double y = p[4 * g + i];
-      if (w.q) y -= static_cast<double>(d[4 * g + i]);
-      if (e == w.point) y = 0;
-      x[4 * g + i] = positive(y);
-      sum += x[4 * g + i];
+    for (int g = 0; g < kLines; ++g) {
+      p[g] = *reinterpret_cast<const f32x4_any_t*>(w.p + e0 + 4 * g);
+      if (w.q) d[g] = *reinterpret_cast<const f32x4_any_t*>(w.q + e0 + 4 * g);
     }
-    lines[g] = sum;
-    const double all = wave_sum(sum);
-    if (lane == 0) part[g][wave] = all;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      x[i] = p[i >> 2][i & 3];
+      if (w.q) x[i] -= static_cast<double>(d[i >> 2][i & 3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      x[i] = e0 + i < v.vocab ? w.p[e0 + i] : 0.f;
+      if (w.q && e0 + i < v.vocab) x[i] -= static_cast<double>(w.q[e0 + i]);
+    }
   }
+  double sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    x[i] = e0 + i == w.point ? 0 : positive(x[i]);
+    sum += x[i];
+  }
+  const double incl = wave_scan(sum);
+  if (lane == 63) part[wave] = incl;
   __syncthreads();
-  // First element past the goal, wave by wave: each (group, wave) starts from
-  // the sums before it and looks among its own 256 elements.
+  double run = base + (incl - sum);
+  for (int k = 0; k < wave; ++k) run += part[k];
+  int first = -1, final = -1;
 #pragma unroll
-  for (int g = 0; g < kLines; ++g) {
-    double start = base;
-    for (int k = 0; k < g * kWaves + wave; ++k) start += part[k / kWaves][k % kWaves];
-    const double incl = wave_scan(lines[g], lane);
-    double run = start + (incl - lines[g]);
-    int first = -1, final = -1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      run += x[4 * g + i];
-      if (x[4 * g + i] > 0) {
-        final = s * kSlice + g * 4 * kThreads + 4 * t + i;
-        if (first < 0 && run > goal) first = final;
-      }
+  for (int i = 0; i < kPer; ++i) {
+    run += x[i];
+    if (x[i] > 0) {
+      final = e0 + i;
+      if (first < 0 && run > goal) first = final;
     }
-    const uint64_t mf = __builtin_amdgcn_ballot_w64(first >= 0);
-    const uint64_t ml = __builtin_amdgcn_ballot_w64(final >= 0);
-    const int f = mf ? __shfl(first, __builtin_ctzll(mf), kWave) : -1;
-    const int l = ml ? __shfl(final, 63 - __builtin_clzll(ml), kWave) : -1;
-    if (lane == 0) hit[g * kWaves + wave] = f, last[g * kWaves + wave] = l;
   }
+  const uint64_t mf = __builtin_amdgcn_ballot_w64(first >= 0);
+  const uint64_t ml = __builtin_amdgcn_ballot_w64(final >= 0);
+  const int f = mf ? __builtin_amdgcn_readlane(first, __builtin_ctzll(mf)) : -1;
+  const int l = ml ? __builtin_amdgcn_readlane(final, 63 - __builtin_clzll(ml)) : -1;
+  if (lane == 0) hit[wave] = f, last[wave] = l;
   __syncthreads();
   if (t == 0) {
     int token = -1, end = v.vocab - 1;
-    for (int k = 0; k < kLines * kWaves; ++k) {
+    for (int k = 0; k < kWaves; ++k) {
       if (token < 0) token = hit[k];
       if (last[k] >= 0) end = last[k];
     }
@@ -322,7 +349,11 @@ extern "C" int sgl_verify_drafts(const sgl_verify_args_t* args, void* workspace,
   v.tokens = x.tokens, v.accepted = x.accepted;
   v.sums = static_cast<double*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(verify_sums_kernel, dim3(v.slices, x.batch_size), dim3(kThreads), 0, s, v);
+  // Few slices in all: each its own workgroup. Many: runs of four.
+  if (static_cast<int64_t>(v.slices) * x.batch_size <= kSingles)
+    hipLaunchKernelGGL(verify_sums_kernel<1>, dim3(v.slices, x.batch_size), dim3(kThreads), 0, s, v);
+  else
+    hipLaunchKernelGGL(verify_sums_kernel<4>, dim3((v.slices + 3) / 4, x.batch_size), dim3(kThreads), 0, s, v);
   const int st = launch_status();
   if (st != SGL_OK) return st;
   hipLaunchKernelGGL(verify_draw_kernel, dim3(x.batch_size), dim3(kThreads), 0, s, v);

@@ -75,8 +75,11 @@ def test_prefix_plan():
     st, p = plan()
     assert st == 0 and p.num_units >= 1 and p.workspace_bytes > 0
     assert plan(P=0)[0] == plan(B=0, T=0, qo=0)[0] == 0
-    # Longer batches need no less room.
-    assert plan(T=64)[1].workspace_bytes >= p.workspace_bytes
+    # Room for every row's own piece (128 fp32 values), whichever way the prefix goes.
+    for T in (1, 8, 16, 17, 64, 700):
+        st, p = plan(T=T)
+        assert p.num_tiles + (p.num_shares > 0) == 1 and p.workspace_bytes >= T * 8 * 512
+        assert (p.num_shares > 0) == (4 * T > 64)
 
 
 def attend(p, **kw):
