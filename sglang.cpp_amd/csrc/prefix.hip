@@ -6,8 +6,8 @@
 // K/V are walked once with the rows of every request as columns of one product,
 // each request's own tokens with its rows alone, and a second launch folds.
 //
-// Units: the prefix (once per tile of up to 64 packed rows) and then the
-// requests' own tokens form one stream, cut into units of equal length, one
+// Units: the prefix (where the batch has at most 64 packed rows a kv head) and then
+// the requests' own tokens form one stream, cut into units of equal length, one
 // workgroup each; a wave has one kv head, so a workgroup reads whole token rows.
 // A wave walks its piece 16 tokens a step on the matrix cores: S^T = K Q^T, then
 // O^T += V^T P^T, whose operand P^T is S^T's accumulator layout, for up to four
@@ -45,8 +45,8 @@ struct PrefixArgs {
   float scale_log2;
   uint16_t* o;
   int64_t o_st, o_sh;
-  // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix pieces: piece u + tile,
-  // [piece][kv head][row of the tile], or [share][kv head][packed row]. Own pieces: [token slot][q head], the piece a
+  // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix pieces: unit u's,
+  // [u][kv head][packed row], or [share][kv head][packed row]. Own pieces: [token slot][q head], the piece a
   // request starts with at its rows' own tokens, the one running into unit u from
   // before it at tokens + u max_qo + i.
   float* p_o;
@@ -55,16 +55,16 @@ struct PrefixArgs {
   float* s_lse;
 };
 
+// The stream's places are below 2^30 (prefix) + 2^31 (the offsets are int32): 32 bits
+// without a sign.
 // Tokens of a unit, from the requests' lengths as they are now.
-__device__ __forceinline__ int64_t unit_tokens(const PrefixArgs& a, int64_t all) {
-  int64_t w = (all + a.units - 1) / a.units;
-  w = (w + kStep - 1) / kStep * kStep;
-  return w < kMinUnit ? kMinUnit : w;
+__device__ __forceinline__ uint32_t unit_tokens(const PrefixArgs& a, uint32_t all) {
+  const uint32_t w = all / static_cast<uint32_t>(a.units) + 1;  // one more where it divides
+  return max((w + kStep - 1) / kStep * kStep, static_cast<uint32_t>(kMinUnit));
 }
 
-__device__ __forceinline__ int64_t own_tokens(const PrefixArgs& a) {
-  const int64_t n = static_cast<int64_t>(a.kv_indptr[a.batch]) - a.kv_indptr[0];
-  return n < 0 ? 0 : n;
+__device__ __forceinline__ uint32_t own_tokens(const PrefixArgs& a) {
+  return static_cast<uint32_t>(max(a.kv_indptr[a.batch] - max(a.kv_indptr[0], 0), 0));
 }
 
 struct Request {
@@ -81,7 +81,7 @@ __device__ __forceinline__ Request request_of(const PrefixArgs& a, int r) {
   x.qo = static_cast<int>(q1 - x.q0);
   x.kv = static_cast<int>(k1 - x.kv0);
   // Rows and pieces of anything else have no place in the outputs and the workspace.
-  x.ok = x.q0 >= max(a.qo_indptr[0], 0) && q1 >= x.q0 && q1 <= min(a.qo_indptr[a.batch], a.tokens) &&
+  x.ok = x.kv0 >= 0 && x.q0 >= max(a.qo_indptr[0], 0) && q1 >= x.q0 && q1 <= min(a.qo_indptr[a.batch], a.tokens) &&
          q1 - x.q0 <= a.max_qo && x.kv0 >= a.kv_indptr[0] && k1 >= x.kv0 && k1 <= a.kv_indptr[a.batch];
   return x;
 }
@@ -136,7 +136,7 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const in
   auto load_v = [&](int slot, u32x4_t (&vr)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      vr[e] = ldg128(slot_row(vlane, __shfl(slot, 4 * j + e, kWave), ss_bytes));
+      vr[e] = ldg128_nt<true>(slot_row(vlane, __shfl(slot, 4 * j + e, kWave), ss_bytes));
   };
 
   // Token i and head of packed row p = row0 + x, x < 64: i0 + (rem + x) / G, the
@@ -266,43 +266,51 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const in
   }
 }
 
+// The walk with as many column blocks as the rows need.
+template <int RB>
+__device__ __forceinline__ void walk_rows(const PrefixArgs& a, uint16_t* lq, const int32_t* idx, int len,
+                                          int h, int tok0, int row0, int row_end, int sees0, float* o,
+                                          float* lse, int64_t out0, bool by_token, int lane) {
+  if constexpr (RB > 1) {
+    if (row_end - row0 <= 8 * RB) {
+      walk_rows<RB / 2>(a, lq, idx, len, h, tok0, row0, row_end, sees0, o, lse, out0, by_token, lane);
+      return;
+    }
+  }
+  walk<RB>(a, lq, idx, len, h, tok0, row0, row_end, sees0, o, lse, out0, by_token, lane);
+}
+
 template <int RB>
 __global__ void __launch_bounds__(512) prefix_units_kernel(PrefixArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t lds_q[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.y * (blockDim.x >> 6) + wave;
-  const int u = blockIdx.x;
+  const uint32_t u = blockIdx.x;
   uint16_t* lq = lds_q + wave * 16 * RB * kQPitch;
-  const int64_t P = a.prefix, shared = P * a.tiles;
-  const int64_t all = shared + own_tokens(a);
-  const int64_t W = unit_tokens(a, all);
-  const int64_t t0 = u * W, t1 = min(all, t0 + W);
-  if (t0 >= t1) return;
+  const uint32_t shared = a.tiles > 0 ? a.prefix : 0;
+  const uint32_t all = shared + own_tokens(a);
+  const uint32_t W = unit_tokens(a, all);
+  if (static_cast<uint64_t>(u) * W >= all) return;
+  const uint32_t t0 = u * W, t1 = min(all, t0 + W);
   // The shared prefix's part.
   if (t0 < shared) {
     const int first = max(a.qo_indptr[0], 0);
     const int last = min(a.qo_indptr[a.batch], a.tokens);
-    const int64_t rows = static_cast<int64_t>(max(last - first, 0)) * a.group;
-    for (int tile = static_cast<int>(t0 / P); tile < a.tiles && tile * P < t1; ++tile) {
-      const int row0 = tile * a.tile_rows;
-      if (row0 >= rows) break;
-      const int s0 = static_cast<int>(max(t0 - tile * P, int64_t{0}));
-      const int s1 = static_cast<int>(min(t1 - tile * P, P));
-      const int64_t out0 = (static_cast<int64_t>(u + tile) * a.hkv + h) * a.tile_rows;
-      walk<RB>(a, lq, a.pidx + s0, s1 - s0, h, first, row0,
-               static_cast<int>(min(rows, static_cast<int64_t>(row0) + a.tile_rows)), s1 - s0, a.p_o,
-               a.p_lse, out0, false, lane);
-    }
+    const int rows = min(max(last - first, 0) * a.group, a.tile_rows);
+    const int len = static_cast<int>(min(t1, shared) - t0);
+    if (rows > 0)
+      walk_rows<RB>(a, lq, a.pidx + t0, len, h, first, 0, rows, len, a.p_o, a.p_lse,
+                    (static_cast<int64_t>(u) * a.hkv + h) * a.tile_rows, false, lane);
   }
   if (t1 <= shared) return;
   // The requests' own tokens [b0, b1) of the joined list.
-  const int kv_first = a.kv_indptr[0];
-  const int64_t b0 = max(t0 - shared, int64_t{0}), b1 = t1 - shared;
+  const int kv_first = max(a.kv_indptr[0], 0);
+  const uint32_t b0 = max(t0, shared) - shared, b1 = t1 - shared;
   int r = 0;  // requests that end at or before b0, 64 at a time
   for (int at = 0; at < a.batch; at += kWave) {
     const int e = at + lane;
-    const bool before = e < a.batch && static_cast<int64_t>(a.kv_indptr[e + 1]) - kv_first <= b0;
+    const bool before = e < a.batch && a.kv_indptr[e + 1] - kv_first <= static_cast<int64_t>(b0);
     const uint64_t mask = __builtin_amdgcn_ballot_w64(before);
     r += __builtin_popcountll(mask);
     if (mask != ~0ull) break;
@@ -317,9 +325,9 @@ __global__ void __launch_bounds__(512) prefix_units_kernel(PrefixArgs a) {
     if (s1 <= s0) continue;
     const int64_t out0 = s0 == 0 ? x.q0 : a.tokens + static_cast<int64_t>(u) * a.max_qo;
     for (int row0 = 0; row0 < x.qo * a.group; row0 += 16 * RB)
-      walk<RB>(a, lq, a.indices + x.kv0 + s0, s1 - s0, h, x.q0, row0,
-               min(x.qo * a.group, row0 + 16 * RB), max(x.kv - x.qo + 1 - s0, -x.qo), a.s_o, a.s_lse,
-               out0, true, lane);
+      walk_rows<RB>(a, lq, a.indices + x.kv0 + s0, s1 - s0, h, x.q0, row0,
+                    min(x.qo * a.group, row0 + 16 * RB), max(x.kv - x.qo + 1 - s0, -x.qo), a.s_o,
+                    a.s_lse, out0, true, lane);
   }
 }
 
@@ -521,8 +529,9 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   if (r >= a.batch || t < a.qo_indptr[0]) return;  // no request's row: left as it was
   const Request x = request_of(a, r);
   const int first = max(a.qo_indptr[0], 0);
-  const int64_t P = a.prefix, shared = P * a.tiles;
-  const int64_t W = unit_tokens(a, shared + own_tokens(a));
+  const int P = a.prefix;
+  const uint32_t shared = a.tiles > 0 ? P : 0;
+  const uint32_t W = unit_tokens(a, shared + own_tokens(a));
   const int c = threadIdx.x & 31, group = threadIdx.x >> 5;
   const int set = group % kSets;
   const int head = (blockIdx.x - t * head_groups) * kRows + group / kSets;
@@ -530,7 +539,7 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   const int hh = head_ok ? head : a.hq - 1;
   const int h = hh / a.group;
   const int i = t - x.q0;
-  const int64_t sees = P + x.kv - x.qo + i + 1;  // tokens this row sees, prefix first
+  const int64_t sees = static_cast<int64_t>(P) + x.kv - x.qo + i + 1;  // tokens this row sees, prefix first
   float m = -INFINITY, l = 0.f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   const bool folded = x.ok && sees >= P;
@@ -545,15 +554,13 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
       p_step = static_cast<int64_t>(a.hkv) * a.tokens * a.group;
       p0 = static_cast<int64_t>(h) * a.tokens * a.group + prow;
     } else if (P > 0) {
-      const int tile = prow / a.tile_rows;
-      const int64_t u0 = tile * P / W;
-      np = static_cast<int>((tile * P + P - 1) / W - u0) + 1;
-      p0 = ((u0 + tile) * a.hkv + h) * a.tile_rows + prow - tile * a.tile_rows;
+      np = static_cast<int>((P - 1) / W) + 1;
+      p0 = static_cast<int64_t>(h) * a.tile_rows + prow;
     }
     if (x.kv > 0) {
-      const int64_t own0 = shared + x.kv0 - a.kv_indptr[0], u0 = own0 / W;
+      const uint32_t own0 = shared + (x.kv0 - max(a.kv_indptr[0], 0)), u0 = own0 / W;
       ns = static_cast<int>((own0 + x.kv - 1) / W - u0) + 1;
-      s1 = (a.tokens + u0 * a.max_qo + i) * a.hq + hh;
+      s1 = (a.tokens + static_cast<int64_t>(u0) * a.max_qo + i) * a.hq + hh;
     }
     const int64_t s0 = static_cast<int64_t>(t) * a.hq + hh, s_step = static_cast<int64_t>(a.max_qo) * a.hq;
     for (int k0 = set; k0 < np + ns; k0 += 4 * kSets) {
@@ -647,7 +654,7 @@ struct Layout {
 Layout workspace_layout(const sgl_prefix_plan_t& p) {
   auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
   const int64_t prefix_rows = p.num_tiles > 0
-      ? (static_cast<int64_t>(p.num_units) + p.num_tiles) * p.num_kv_heads * p.tile_rows
+      ? static_cast<int64_t>(p.num_units) * p.num_kv_heads * p.tile_rows
       : static_cast<int64_t>(p.num_shares) * p.max_tokens * p.num_qo_heads;
   const int64_t own_rows =
       (p.max_tokens + static_cast<int64_t>(p.num_units) * p.max_qo_len) * p.num_qo_heads;
@@ -676,7 +683,8 @@ extern "C" int sgl_prefix_plan(int prefix_len, int batch_size, int max_tokens, i
       num_kv_heads > 65535)
     return SGL_ERR_UNSUPPORTED;
   // Packed rows and their tiles are counted in 32 bits.
-  if (static_cast<int64_t>(max_tokens) * group > (1 << 30)) return SGL_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(max_tokens) * group > (1 << 30) || prefix_len > (1 << 30))
+    return SGL_ERR_UNSUPPORTED;
   *plan = sgl_prefix_plan_t{};
   plan->prefix_len = prefix_len;
   plan->batch_size = batch_size;
@@ -791,7 +799,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   if (st != SGL_OK) return st;
   // Many pieces a row: a workgroup for each. Few: two groups of lanes a row.
   const int64_t pieces = a.tiles > 0 ? p.num_units : a.shares + 1;
-  const int rows_per = pieces > 8 ? 1 : 4;
+  const int rows_per = pieces > 16 ? 1 : 4;
   const int head_groups = (num_qo_heads + rows_per - 1) / rows_per;
   const dim3 fold(static_cast<uint32_t>(max_tokens) * head_groups);
   if (rows_per == 1) hipLaunchKernelGGL(prefix_fold_kernel<8>, fold, dim3(256), 0, s, a, head_groups);
