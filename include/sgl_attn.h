@@ -577,11 +577,12 @@ typedef struct {
   int32_t num_qo_heads;
   int32_t num_kv_heads;
   int32_t head_dim;
-  int32_t num_units;    /* workgroups that walk equal shares of the tokens */
-  int32_t tile_rows;    /* packed query rows (tokens x heads of a kv head) of a walk over the prefix */
-  int32_t num_tiles;    /* 1: the units walk the prefix too, 0: it has a launch of its own */
-  int32_t num_shares;   /* shares of the prefix in that launch */
+  int32_t num_blocks;   /* workgroups of the launch (one per CU) */
+  int32_t max_units;    /* parts the requests' own tokens are cut into at most */
+  int32_t walk_rows;    /* packed rows (tokens x heads of a kv head) up to which those parts
+                           take the prefix too; 0: it has workgroups of its own */
   int32_t reserved;
+  int64_t prefix_rows;  /* partial rows of the prefix in the workspace */
   int64_t workspace_bytes;
 } sgl_prefix_plan_t;
 #define SGL_PREFIX_MAX_QO 64

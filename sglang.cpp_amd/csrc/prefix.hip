@@ -6,15 +6,17 @@
 // K/V are walked once with the rows of every request as columns of one product,
 // each request's own tokens with its rows alone, and a second launch folds.
 //
-// Units: the prefix (where the batch has at most 64 packed rows a kv head) and then
-// the requests' own tokens form one stream, cut into units of equal length, one
-// workgroup each; a wave has one kv head, so a workgroup reads whole token rows.
+// Two ways over tokens in one launch (split_of). Units: the requests' own tokens, behind
+// the prefix where the batch has at most 32 packed rows a kv head, form one stream, cut
+// into units of equal length, one workgroup each as a rule; a wave has one kv head, so a workgroup reads whole token rows.
 // A wave walks its piece 16 tokens a step on the matrix cores: S^T = K Q^T, then
-// O^T += V^T P^T, whose operand P^T is S^T's accumulator layout, for up to four
+// O^T += V^T P^T, whose operand P^T is S^T's accumulator layout, for one or two
 // column blocks of 16 rows per K/V read. Both put the row on the lane's column, so
 // the running maximum and sum are lane-local but for one exchange across four lane
 // groups. K and V of the next step are in flight during a step.
 #include <math.h>
+
+#include <algorithm>
 
 #include "common.h"
 #include "prefill_impl.h"
@@ -25,9 +27,9 @@ namespace {
 constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
 constexpr int kMinUnit = 16;              // shortest unit
-constexpr int kQPitch = kD + 8;           // LDS row pitch (bf16) of the Q^T copy
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
-constexpr int kMaxTileRows = 64;
+constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
+constexpr int kMaxWalkRows = 32;         // packed rows up to which the units walk the prefix
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -40,31 +42,79 @@ struct PrefixArgs {
   const int32_t* kv_indptr;
   const int32_t* qo_indptr;
   int batch, tokens, hq, hkv, group;
-  int prefix, tile_rows, tiles, units, max_qo;
-  int shares, row_tiles;  // of the prefix's own launch: item = row tile, then kv head, then share
+  int prefix, max_qo;
+  int walk_rows;         // packed rows whose prefix the units walk (0: the tiles' workgroups do)
+  int blocks;            // workgroups of the launch
+  int heads, side, rest; // kv heads of a unit, units side by side in a workgroup, head groups
   float scale_log2;
   uint16_t* o;
   int64_t o_st, o_sh;
-  // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix pieces: unit u's,
-  // [u][kv head][packed row], or [share][kv head][packed row]. Own pieces: [token slot][q head], the piece a
-  // request starts with at its rows' own tokens, the one running into unit u from
-  // before it at tokens + u max_qo + i.
+  // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix: [unit][kv head][packed
+  // row] or [piece of the item][kv head][packed row]. Own tokens: [token slot][q head],
+  // the piece a request starts with at its rows' own tokens, the one running into unit
+  // u from before it at tokens + u max_qo + i.
   float* p_o;
   float* p_lse;
   float* s_o;
   float* s_lse;
 };
 
-// The stream's places are below 2^30 (prefix) + 2^31 (the offsets are int32): 32 bits
-// without a sign.
-// Tokens of a unit, from the requests' lengths as they are now.
-__device__ __forceinline__ uint32_t unit_tokens(const PrefixArgs& a, uint32_t all) {
-  const uint32_t w = all / static_cast<uint32_t>(a.units) + 1;  // one more where it divides
-  return max((w + kStep - 1) / kStep * kStep, static_cast<uint32_t>(kMinUnit));
-}
+// How a launch is shared out, from the lengths as they are now (so a captured launch
+// follows them): the main and the fold kernel work it out alike, in whole numbers.
+// Prefix tiles: workgroups [0, tile_blocks) take tile_run consecutive ones each of the
+// list (row tile, kv head, 64-token tile of the prefix), the tiles varying fastest; the
+// others' units walk the stream of `all` tokens, `shared` of them the prefix's, W a unit.
+struct Split {
+  int first, rows;        // first query token, packed rows of a kv head
+  int row_tiles, row_step;  // row tiles and their rows (32 a wave, spread evenly)
+  int tiles;              // 64-token tiles of the prefix
+  uint32_t list, tile_run;
+  int tile_blocks;
+  uint32_t shared, all, W;
+  int units;
+};
 
-__device__ __forceinline__ uint32_t own_tokens(const PrefixArgs& a) {
-  return static_cast<uint32_t>(max(a.kv_indptr[a.batch] - max(a.kv_indptr[0], 0), 0));
+// What a tile of a row tile takes by its waves of rows, ns, and a token of a kv head
+// on one workgroup.
+__device__ constexpr uint16_t kTileNs[9] = {0, 1400, 1400, 1500, 1500, 2000, 2200, 2400, 2700};
+constexpr uint32_t kTokenNs = 11;
+// A request counts as this many tokens more in the units' stream: the loads that lead
+// to its first step, about 3.4 us (a unit that took eight requests of one token each was
+// 28 us behind the others).
+constexpr uint32_t kRequestTokens = 24;
+
+__device__ __forceinline__ Split split_of(const PrefixArgs& a) {
+  Split s;
+  s.first = max(a.qo_indptr[0], 0);
+  s.rows = max(min(a.qo_indptr[a.batch], a.tokens) - s.first, 0) * a.group;
+  const uint32_t own = static_cast<uint32_t>(max(a.kv_indptr[a.batch] - max(a.kv_indptr[0], 0), 0)) +
+                       a.batch * kRequestTokens;
+  s.tiles = (a.prefix + pf::kBN - 1) / pf::kBN;
+  s.row_tiles = s.row_step = s.tile_blocks = 0;
+  s.list = 0, s.tile_run = 1;
+  s.shared = 0;
+  if (a.walk_rows > 0) {
+    s.shared = a.prefix;
+  } else if (s.rows > 0 && s.tiles > 0) {
+    const int waves = (s.rows + 31) / 32;
+    s.row_tiles = (waves + 7) / 8;
+    const int each = (waves + s.row_tiles - 1) / s.row_tiles;
+    s.row_step = 32 * each;
+    s.row_tiles = (waves + each - 1) / each;
+    s.list = static_cast<uint32_t>(s.row_tiles) * a.hkv * s.tiles;
+    const uint64_t t = static_cast<uint64_t>(s.list) * kTileNs[each];
+    const uint64_t sum = t + static_cast<uint64_t>(own) * a.hkv * kTokenNs;
+    const int shift = max(0, 42 - __builtin_clzll(sum));  // to 22 bits
+    const uint32_t ts = static_cast<uint32_t>(t >> shift), ss = static_cast<uint32_t>(sum >> shift);
+    s.tile_blocks = static_cast<int>((a.blocks * ts + ss / 2) / ss);
+    s.tile_blocks = max(1, min(s.tile_blocks, a.blocks - 1));
+    s.tile_run = (s.list + s.tile_blocks - 1) / s.tile_blocks;
+  }
+  s.all = s.shared + own;
+  s.units = max(1, (a.blocks - s.tile_blocks) * a.side / a.rest);
+  const uint32_t w = s.all / static_cast<uint32_t>(s.units) + 1;  // one more where it divides
+  s.W = max((w + kStep - 1) / kStep * kStep, static_cast<uint32_t>(kMinUnit));
+  return s;
 }
 
 struct Request {
@@ -90,6 +140,8 @@ __device__ __forceinline__ bf16x8_t as_bf16x8(const u32x4_t& v) {
   return __builtin_bit_cast(bf16x8_t, v);
 }
 
+// Orders LDS traffic between the lanes of one wave (it runs in order; this only keeps
+// the compiler from moving it).
 __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -111,19 +163,30 @@ __device__ __forceinline__ bf16x4_t v_operand(const u32x4_t (&vr)[4]) {
   return __builtin_bit_cast(bf16x4_t, out);
 }
 
-// One wave: kv head h over the len tokens of slots idx[0, len), for the packed
-// rows [row0, row_end) (at most 16 RB; row p: token tok0 + p / G, head h G + p % G).
-// Row of token i sees the tokens below sees0 + i (all of them: sees0 >= len).
-// Its output and lse go to row out0 + (p - row0) of o/lse, or, with by_token, to
-// row (out0 + i) hq + head. lq: the wave's Q copy, 16 RB rows.
-// Lane (n, j), n = lane % 16: token n (K), chunk n of tokens 4 j + e (V), row n
-// (S, O).
-template <int RB>
-__device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const int32_t* idx, int len,
-                                     int h, int tok0, int row0, int row_end, int sees0, float* o,
-                                     float* lse, int64_t out0, bool by_token, int lane) {
+// A piece: the len tokens of slots idx[0, len) for the packed rows [row0, row0 + rows)
+// (row p: token tok0 + p / G, head h G + p % G of kv head h). A row of token i sees the
+// tokens below sees0 + i. Row x's output and lse go to row out0 + x of o / lse, or, with
+// by_token, to row (out0 + i) hq + head.
+struct Piece {
+  const int32_t* idx;
+  int len;
+  int tok0, row0, rows, sees0;
+  float* o;
+  float* lse;
+  int64_t out0;
+  bool by_token;
+};
+
+// One wave over a piece of at most 16 RB rows. Lane (n, j), n = lane % 16: token n (K),
+// chunk n of tokens 4 j + e (V), row n of each block (Q, S, O). Q stays in registers. The
+// code is kept short (one call, addresses once a row): a piece of a step or two runs most
+// of it once, and what it does not find in the instruction cache costs more than the
+// arithmetic (with Q in LDS and four row blocks 64 requests of 6 query tokens and 16 of
+// their own took 36 us, 16 of one query token).
+template <int RB, bool kSync>
+__device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* xch, int h, int lane) {
   const int n = lane & 15, j = lane >> 4;
-  const int G = a.group;
+  const int G = a.group, len = w.len;
   const uint32_t ss_bytes = static_cast<uint32_t>(a.kv_ss * 2);
   const char* klane = reinterpret_cast<const char*>(a.kc + h * a.kv_sh + 8 * j);
   const char* vlane = reinterpret_cast<const char*>(a.vc + h * a.kv_sh + 8 * n);
@@ -138,67 +201,51 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const in
     for (int e = 0; e < 4; ++e)
       vr[e] = ldg128_nt<true>(slot_row(vlane, __shfl(slot, 4 * j + e, kWave), ss_bytes));
   };
-
-  // Token i and head of packed row p = row0 + x, x < 64: i0 + (rem + x) / G, the
-  // division (of a number below 128 by G <= 64) as a product.
-  const int i0 = row0 / G, rem = row0 - i0 * G;
-  const uint32_t inv_g = (65536u + G - 1) / G;
-  auto token_of = [&](int x, int& head) {
-    const int y = rem + x;
-    const int d = static_cast<int>(static_cast<uint32_t>(y) * inv_g >> 16);
-    head = h * G + (y - d * G);
-    return i0 + d;
-  };
-  const int nrows = row_end - row0;
-
-  const int slot = idx[min(n, len - 1)];
-  int slot_next = idx[min(kStep + n, len - 1)];
-  // Q rows, four of a block at a time (chunk n); rows past the last one read it again
-  // and are cleared, so that every load is in flight at once.
-  u32x4_t qv[4 * RB];
+  const int slot = w.idx[min(n, len - 1)];
+  int slot_next = w.idx[min(kStep + n, len - 1)];
+  // Token and head of this lane's row of each block; rows past the last one read
+  // its Q again and see nothing.
+  const int i0 = w.row0 / G, rem = w.row0 - i0 * G;
+  const uint32_t inv_g = (65536u + G - 1) / G;  // (rem + x) / G as a product, both below 128
+  int tok[RB], head[RB], sees[RB];
+  u32x4_t q[RB][4];
 #pragma unroll
-  for (int u = 0; u < 4 * RB; ++u) {
-    int head;
-    const int i = token_of(min(4 * u + j, nrows - 1), head);
-    qv[u] = ldg128(a.q + (tok0 + i) * a.q_st + head * a.q_sh + 8 * n);
+  for (int b = 0; b < RB; ++b) {
+    const int x = min(16 * b + n, w.rows - 1) + rem;
+    const int d = static_cast<int>(static_cast<uint32_t>(x) * inv_g >> 16);
+    tok[b] = i0 + d;
+    head[b] = h * G + (x - d * G);
+    sees[b] = 16 * b + n < w.rows ? min(w.sees0 + tok[b], len) : 0;
+    const uint16_t* qp = a.q + (w.tok0 + tok[b]) * a.q_st + head[b] * a.q_sh + 8 * j;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) q[b][s] = ldg128(qp + 32 * s);
   }
   u32x4_t kr[4], vr[4];
   load_k(slot, kr);
   load_v(slot, vr);
-#pragma unroll
-  for (int u = 0; u < 4 * RB; ++u)
-    *reinterpret_cast<u32x4_t*>(lq + (4 * u + j) * kQPitch + 8 * n) =
-        4 * u + j < nrows ? qv[u] : u32x4_t{0, 0, 0, 0};
-  wave_lds_sync();
-  int sees[RB];
   float m[RB], l[RB];
   f32x4_t acc[RB][8];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    int head;
-    const int i = token_of(16 * b + n, head);
-    sees[b] = 16 * b + n < nrows ? min(sees0 + i, len) : 0;
     m[b] = -INFINITY;
     l[b] = 0.f;
 #pragma unroll
     for (int nb = 0; nb < 8; ++nb) acc[b][nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
+#pragma unroll 1
   for (int t = 0; t < len; t += kStep) {
-    // The workgroup's waves (its kv heads) keep in step: together they read
-    // whole token rows.
-    __builtin_amdgcn_s_barrier();
-    const int slot_after = idx[min(t + 2 * kStep + n, len - 1)];
+    // Where the workgroup's waves are one unit's kv heads they keep in step:
+    // together they read whole token rows.
+    if constexpr (kSync) __builtin_amdgcn_s_barrier();
+    const int slot_after = w.idx[min(t + 2 * kStep + n, len - 1)];
     f32x4_t sacc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       sacc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const bf16x8_t qop =
-            *reinterpret_cast<const bf16x8_t*>(lq + (16 * b + n) * kQPitch + 32 * s + 8 * j);
-        sacc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[s]), qop, sacc[b], 0, 0, 0);
-      }
+      for (int s = 0; s < 4; ++s)
+        sacc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[s]), as_bf16x8(q[b][s]), sacc[b], 0, 0, 0);
     }
     load_k(slot_next, kr);
     bf16x4_t pop[RB];
@@ -229,8 +276,8 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const in
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], a.scale_log2, neg_m));
       l[b] += (p[0] + p[1]) + (p[2] + p[3]);
-      // P in bf16, the product's operand type: a weight is off by at most 2^-9 of
-      // itself, below what rounding the output to bf16 takes.
+      // P in bf16, the product's operand type: a weight is off by at most 2^-8 of
+      // itself, as the rounding of the output.
       const u32x2_t pw = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
       pop[b] = __builtin_bit_cast(bf16x4_t, pw);
     }
@@ -244,124 +291,135 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, uint16_t* lq, const in
     load_v(slot_next, vr);
     slot_next = slot_after;
   }
+  // The block's output through LDS (16 rows of 32 16-byte chunks, chunk c of row n at
+  // c ^ n: no bank conflicts either way), so that whole rows are stored: as they lie in
+  // the accumulators a store would touch 64 lines for 1 KB (128 units of 32 rows, 8 kv
+  // heads: 39.8 us, 9.7 of them without the rows).
+  f32x4_t* xr = reinterpret_cast<f32x4_t*>(xch);
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
+    if (16 * b >= w.rows) break;
     const float sum = sum_xor32(sum_xor16(l[b]));
-    if (16 * b + n >= nrows) continue;
-    int head;
-    const int i = token_of(16 * b + n, head);
-    const int64_t row = by_token ? (out0 + i) * a.hq + head : out0 + 16 * b + n;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // a NaN sum stays one
     // acc[nb][c] holds d = 32 j + 8 c + nb.
-    float* op = o + row * kD + 32 * j;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       f32x4_t lo, hi;
 #pragma unroll
       for (int nb = 0; nb < 4; ++nb) lo[nb] = acc[b][nb][c] * inv, hi[nb] = acc[b][nb + 4][c] * inv;
-      *reinterpret_cast<f32x4_t*>(op + 8 * c) = lo;
-      *reinterpret_cast<f32x4_t*>(op + 8 * c + 4) = hi;
+      xr[32 * n + ((8 * j + 2 * c) ^ n)] = lo;
+      xr[32 * n + ((8 * j + 2 * c + 1) ^ n)] = hi;
     }
-    if (j == 0) lse[row] = sum == 0.f ? -INFINITY : m[b] + log2f(sum);
+    wave_lds_sync();
+    if (j == 0 && 16 * b + n < w.rows)
+      w.lse[w.by_token ? (w.out0 + tok[b]) * a.hq + head[b] : w.out0 + 16 * b + n] =
+          sum == 0.f ? -INFINITY : m[b] + log2f(sum);
+    const int c = lane & 31;
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      const int x = 2 * it + (lane >> 5), y = 16 * b + x + rem;
+      if (16 * b + x >= w.rows) break;
+      const int d = static_cast<int>(static_cast<uint32_t>(y) * inv_g >> 16);
+      const int64_t row = w.by_token ? (w.out0 + i0 + d) * a.hq + (h * G + y - d * G) : w.out0 + 16 * b + x;
+      __builtin_nontemporal_store(xr[32 * x + (c ^ x)], reinterpret_cast<f32x4_t*>(w.o + row * kD + 4 * c));
+    }
+    wave_lds_sync();
   }
 }
 
-// The walk with as many column blocks as the rows need.
-template <int RB>
-__device__ __forceinline__ void walk_rows(const PrefixArgs& a, uint16_t* lq, const int32_t* idx, int len,
-                                          int h, int tok0, int row0, int row_end, int sees0, float* o,
-                                          float* lse, int64_t out0, bool by_token, int lane) {
-  if constexpr (RB > 1) {
-    if (row_end - row0 <= 8 * RB) {
-      walk_rows<RB / 2>(a, lq, idx, len, h, tok0, row0, row_end, sees0, o, lse, out0, by_token, lane);
-      return;
-    }
-  }
-  walk<RB>(a, lq, idx, len, h, tok0, row0, row_end, sees0, o, lse, out0, by_token, lane);
+// Where request r begins among the requests in the stream.
+__device__ __forceinline__ int64_t place_of(const PrefixArgs& a, int r, int kv_first) {
+  return static_cast<int64_t>(a.kv_indptr[r]) - kv_first + static_cast<int64_t>(r) * kRequestTokens;
 }
 
-template <int RB>
-__global__ void __launch_bounds__(512) prefix_units_kernel(PrefixArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t lds_q[];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y * (blockDim.x >> 6) + wave;
-  const uint32_t u = blockIdx.x;
-  uint16_t* lq = lds_q + wave * 16 * RB * kQPitch;
-  const uint32_t shared = a.tiles > 0 ? a.prefix : 0;
-  const uint32_t all = shared + own_tokens(a);
-  const uint32_t W = unit_tokens(a, all);
-  if (static_cast<uint64_t>(u) * W >= all) return;
-  const uint32_t t0 = u * W, t1 = min(all, t0 + W);
-  // The shared prefix's part.
-  if (t0 < shared) {
-    const int first = max(a.qo_indptr[0], 0);
-    const int last = min(a.qo_indptr[a.batch], a.tokens);
-    const int rows = min(max(last - first, 0) * a.group, a.tile_rows);
-    const int len = static_cast<int>(min(t1, shared) - t0);
-    if (rows > 0)
-      walk_rows<RB>(a, lq, a.pidx + t0, len, h, first, 0, rows, len, a.p_o, a.p_lse,
-                    (static_cast<int64_t>(u) * a.hkv + h) * a.tile_rows, false, lane);
-  }
-  if (t1 <= shared) return;
-  // The requests' own tokens [b0, b1) of the joined list.
+// Unit u's pieces of the stream for kv head h: places below 2^29 (prefix) + 2^31 (the
+// offsets are int32) + 2^30 (2^25 requests), 32 bits without a sign.
+template <int RB, bool kSync>
+__device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s, char* xch, uint32_t u, int h,
+                                            int lane) {
+  if (static_cast<uint64_t>(u) * s.W >= s.all) return;
+  const uint32_t t0 = u * s.W, t1 = min(s.all, t0 + s.W);
+  // The requests' own tokens [b0, b1) of the joined list, from request r on.
   const int kv_first = max(a.kv_indptr[0], 0);
-  const uint32_t b0 = max(t0, shared) - shared, b1 = t1 - shared;
-  int r = 0;  // requests that end at or before b0, 64 at a time
-  for (int at = 0; at < a.batch; at += kWave) {
-    const int e = at + lane;
-    const bool before = e < a.batch && a.kv_indptr[e + 1] - kv_first <= static_cast<int64_t>(b0);
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(before);
-    r += __builtin_popcountll(mask);
-    if (mask != ~0ull) break;
+  const uint32_t b0 = max(t0, s.shared) - s.shared, b1 = max(t1, s.shared) - s.shared;
+  int r = -1;  // the prefix's part
+  int left = 0;  // rows of the current request not walked yet
+  Piece w;
+  if (t0 < s.shared) {
+    w.idx = a.pidx + t0;
+    w.len = w.sees0 = static_cast<int>(min(t1, s.shared) - t0);
+    w.tok0 = s.first;
+    w.row0 = 0;
+    left = min(s.rows, a.walk_rows);
+    w.o = a.p_o, w.lse = a.p_lse;
+    w.out0 = (static_cast<int64_t>(u) * a.hkv + h) * a.walk_rows;
+    w.by_token = false;
   }
-  for (; r < a.batch; ++r) {
-    const Request x = request_of(a, r);
-    const int64_t rb = static_cast<int64_t>(x.kv0) - kv_first;
-    if (rb >= b1) break;
-    if (!x.ok || x.qo == 0 || x.kv == 0) continue;
-    const int s0 = static_cast<int>(max(b0 - rb, int64_t{0}));
-    const int s1 = static_cast<int>(min(b1 - rb, static_cast<int64_t>(x.kv)));
-    if (s1 <= s0) continue;
-    const int64_t out0 = s0 == 0 ? x.q0 : a.tokens + static_cast<int64_t>(u) * a.max_qo;
-    for (int row0 = 0; row0 < x.qo * a.group; row0 += 16 * RB)
-      walk_rows<RB>(a, lq, a.indices + x.kv0 + s0, s1 - s0, h, x.q0, row0,
-                    min(x.qo * a.group, row0 + 16 * RB), max(x.kv - x.qo + 1 - s0, -x.qo), a.s_o,
-                    a.s_lse, out0, true, lane);
+  while (true) {
+    while (left <= 0) {  // the next request
+      if (b1 == 0) return;
+      if (r < 0) {  // those that end at or before b0 are passed over, 64 at a time
+        r = 0;
+        for (int at = 0; at < a.batch; at += kWave) {
+          const int e = at + lane;
+          const bool before = e < a.batch && place_of(a, e + 1, kv_first) <= static_cast<int64_t>(b0);
+          const uint64_t mask = __builtin_amdgcn_ballot_w64(before);
+          r += __builtin_popcountll(mask);
+          if (mask != ~0ull) break;
+        }
+      } else {
+        ++r;
+      }
+      if (r >= a.batch) return;
+      const Request x = request_of(a, r);
+      const int64_t rb = place_of(a, r, kv_first);  // then its kRequestTokens, then its tokens
+      if (rb >= b1) return;
+      if (!x.ok) continue;
+      const int64_t at = rb + kRequestTokens;
+      const int s0 = static_cast<int>(max(b0 - at, int64_t{0}));
+      w.len = static_cast<int>(min(b1 - at, static_cast<int64_t>(x.kv))) - s0;
+      if (w.len <= 0) continue;
+      w.idx = a.indices + x.kv0 + s0;
+      w.tok0 = x.q0;
+      w.row0 = 0;
+      left = x.qo * a.group;
+      w.sees0 = max(x.kv - x.qo + 1 - s0, -x.qo);
+      w.o = a.s_o, w.lse = a.s_lse;
+      w.out0 = s0 == 0 ? x.q0 : a.tokens + static_cast<int64_t>(u) * a.max_qo;
+      w.by_token = true;
+    }
+    w.rows = min(left, 16 * RB);
+    walk<RB, kSync>(a, w, xch, h, lane);
+    left -= w.rows;
+    w.row0 += w.rows;
+    if (!w.by_token) w.out0 += w.rows;
   }
 }
 
 // The prefix for many rows: W waves with 32 packed rows each share the 64-token K/V
 // tiles that they gather into LDS (two buffers, K one tile ahead of V), and tile t + 1's
 // scores are on the matrix cores while tile t's become weights; the prefill kernel's
-// tile steps without a causal bound. Item: (row tile, kv head, share of the prefix's
-// tiles). Bound by the matrix cores: 4 x 64 x 128 flops a row and tile.
-template <int W>
-__device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* lds_raw, int item) {
+// tile steps without a causal bound. Tiles [tb, te) of the prefix for row tile rt of kv
+// head h, the item's piece number `piece`. Bound by the matrix cores: 4 x 64 x 128 flops
+// a row and tile.
+constexpr int kTileWaves = 8;
+
+__device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& sp, char* lds_raw, int rt,
+                                             int h, int tb, int te, int piece) {
   using namespace pf;
-  const int per_tile = a.hkv * a.shares;
-  const int rt = item / per_tile;
-  const int hs = item - rt * per_tile;
-  const int h = hs % a.hkv, share = hs / a.hkv;
-  const int first = max(a.qo_indptr[0], 0);
-  const int last = min(a.qo_indptr[a.batch], a.tokens);
-  const int rows = max(last - first, 0) * a.group;
-  const int row0 = rt * 32 * W;
-  if (row0 >= rows) return;
+  constexpr int W = kTileWaves;
+  const int rows = sp.rows, first = sp.first;
+  const int row0 = rt * sp.row_step, row_end = min(rows, row0 + sp.row_step);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x;
   const int c = lane & 31, hl = lane >> 5;
   const int prow = row0 + 32 * wave + c;
-  const bool row_ok = prow < rows;
-  const bool works = row0 + 32 * wave < rows;  // the others only gather
+  const bool row_ok = prow < row_end;
+  const bool works = row0 + 32 * wave < row_end;  // the others only gather
   const int safe = row_ok ? prow : row0;
   const int qtok = safe / a.group;
   const int qhead = h * a.group + (safe - qtok * a.group);
-  const int nt = (a.prefix + kBN - 1) / kBN;
-  const int per = (nt + a.shares - 1) / a.shares;
-  const int tb = share * per, te = min(nt, tb + per);
-  if (tb >= te) return;
   const int kv_len = a.prefix;
 
   Tile* tiles = reinterpret_cast<Tile*>(lds_raw);
@@ -452,24 +510,69 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, char* lds_raw, 
     step(std::integral_constant<int, 1>{}, t + 1, s_b, s_a);
   }
   const float l = sum_xor32(rs.l);
-  if (!row_ok) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const int64_t row = (static_cast<int64_t>(share) * a.hkv + h) * (static_cast<int64_t>(a.tokens) * a.group) + prow;
-  float* op = a.p_o + row * sgl::kD;
+  const int64_t row_first = (static_cast<int64_t>(piece) * a.hkv + h) * rows + row0 + 32 * wave;
+  if (row_ok && hl == 0) a.p_lse[row_first + c] = l == 0.f ? -INFINITY : rs.m + log2f(l);
+  // Whole rows to memory through the wave's 8 KB of LDS (free behind the last step's
+  // barrier), half a row (64 values, 16 chunks; chunk k of row c at k ^ c) at a time.
+  f32x4_t* xr = reinterpret_cast<f32x4_t*>(lds_raw + wave * kWaveLds);
+  const int left = row_end - (row0 + 32 * wave);
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<f32x4_t*>(op + 32 * db + 8 * g + 4 * hl) =
-          f32x4_t{rs.acc[db][4 * g] * inv, rs.acc[db][4 * g + 1] * inv, rs.acc[db][4 * g + 2] * inv,
-                  rs.acc[db][4 * g + 3] * inv};
-  if (hl == 0) a.p_lse[row] = l == 0.f ? -INFINITY : rs.m + log2f(l);
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x16_t& x = rs.acc[2 * half + e];
+        xr[16 * c + ((8 * e + 2 * g + hl) ^ (c & 15))] =
+            f32x4_t{x[4 * g] * inv, x[4 * g + 1] * inv, x[4 * g + 2] * inv, x[4 * g + 3] * inv};
+      }
+    wave_lds_sync();
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      const int x = 4 * it + (lane >> 4), k = lane & 15;
+      if (x < left)
+        __builtin_nontemporal_store(
+            xr[16 * x + (k ^ (x & 15))],
+            reinterpret_cast<f32x4_t*>(a.p_o + (row_first + x) * sgl::kD + 64 * half + 4 * k));
+    }
+    wave_lds_sync();
+  }
+  __syncthreads();  // before the next item's tiles
 }
 
-template <int W>
-__global__ void __launch_bounds__(64 * W, 8 / W) prefix_rows_kernel(PrefixArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds_raw[2 * pf::kTileBytes];
-  prefix_item<W>(a, lds_raw, blockIdx.x);
+// One workgroup per CU (eight waves with all its registers): the first tile_blocks walk
+// their run of the prefix's tiles, bound by the matrix cores, beside the others' units,
+// bound by memory.
+template <int RB, bool kSync>
+__global__ void __launch_bounds__(512, 1) prefix_attention_kernel(PrefixArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Split s = split_of(a);
+  const int b = blockIdx.x;
+  if (b < s.tile_blocks) {
+    uint32_t at = b * s.tile_run;
+    const uint32_t end = min(s.list, at + s.tile_run);
+    while (at < end) {
+      const uint32_t item = at / static_cast<uint32_t>(s.tiles);
+      const int tb = static_cast<int>(at - item * s.tiles);
+      const int te = static_cast<int>(min(static_cast<uint32_t>(s.tiles), tb + (end - at)));
+      // The item's first tile is in workgroup item tiles / tile_run.
+      const int piece = b - static_cast<int>(item * s.tiles / s.tile_run);
+      const int rt = static_cast<int>(item / static_cast<uint32_t>(a.hkv));
+      prefix_tiles(a, s, smem, rt, static_cast<int>(item - rt * a.hkv), tb, te, piece);
+      at += te - tb;
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = wave / a.heads;
+  if (g >= a.side) return;  // kSync: none
+  const int n = a.blocks - s.tile_blocks;
+  for (int v = (b - s.tile_blocks) * a.side + g; v < s.units * a.rest; v += n * a.side) {
+    const int u = v / a.rest;
+    unit_pieces<RB, kSync>(a, s, smem + wave * kWaveLds, u, (v - u * a.rest) * a.heads + wave - g * a.heads, lane);
+  }
 }
 
 // Sum over the 32 lanes of a half wave, the same in each.
@@ -508,7 +611,7 @@ __device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request&
   return acc * inv;
 }
 
-// Folds the pieces of each row: kSets groups of 32 lanes take them in turn, four
+// Folds the pieces of each row: kSets groups of 32 lanes take them in turn, eight
 // pieces' loads in flight, and are folded through LDS; 8 / kSets heads of one token a
 // workgroup.
 template <int kSets>
@@ -528,10 +631,8 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   const int r = before[0] + before[1] + before[2] + before[3];
   if (r >= a.batch || t < a.qo_indptr[0]) return;  // no request's row: left as it was
   const Request x = request_of(a, r);
-  const int first = max(a.qo_indptr[0], 0);
+  const Split sp = split_of(a);
   const int P = a.prefix;
-  const uint32_t shared = a.tiles > 0 ? P : 0;
-  const uint32_t W = unit_tokens(a, shared + own_tokens(a));
   const int c = threadIdx.x & 31, group = threadIdx.x >> 5;
   const int set = group % kSets;
   const int head = (blockIdx.x - t * head_groups) * kRows + group / kSets;
@@ -547,27 +648,30 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
     // Prefix pieces [0, np) at p0 + k p_step, then the request's own.
     int np = 0, ns = 0;
     int64_t p0 = 0, s1 = 0;
-    int64_t p_step = static_cast<int64_t>(a.hkv) * a.tile_rows;
-    const int prow = (t - first) * a.group + hh - h * a.group;
-    if (P > 0 && a.shares > 0) {
-      np = a.shares;
-      p_step = static_cast<int64_t>(a.hkv) * a.tokens * a.group;
-      p0 = static_cast<int64_t>(h) * a.tokens * a.group + prow;
+    int64_t p_step = static_cast<int64_t>(a.hkv) * a.walk_rows;
+    const int prow = (t - sp.first) * a.group + hh - h * a.group;
+    if (sp.tile_blocks > 0) {
+      const uint32_t item = static_cast<uint32_t>(prow / sp.row_step * a.hkv + h) * sp.tiles;
+      np = static_cast<int>((item + sp.tiles - 1) / sp.tile_run - item / sp.tile_run) + 1;
+      p_step = static_cast<int64_t>(a.hkv) * sp.rows;
+      p0 = static_cast<int64_t>(h) * sp.rows + prow;
     } else if (P > 0) {
-      np = static_cast<int>((P - 1) / W) + 1;
-      p0 = static_cast<int64_t>(h) * a.tile_rows + prow;
+      np = static_cast<int>((P - 1) / sp.W) + 1;
+      p0 = static_cast<int64_t>(h) * a.walk_rows + prow;
     }
     if (x.kv > 0) {
-      const uint32_t own0 = shared + (x.kv0 - max(a.kv_indptr[0], 0)), u0 = own0 / W;
-      ns = static_cast<int>((own0 + x.kv - 1) / W - u0) + 1;
+      const uint32_t own0 = sp.shared + (x.kv0 - max(a.kv_indptr[0], 0)) + (r + 1) * kRequestTokens;
+      const uint32_t u0 = own0 / sp.W;
+      ns = static_cast<int>((own0 + x.kv - 1) / sp.W - u0) + 1;
       s1 = (a.tokens + static_cast<int64_t>(u0) * a.max_qo + i) * a.hq + hh;
     }
     const int64_t s0 = static_cast<int64_t>(t) * a.hq + hh, s_step = static_cast<int64_t>(a.max_qo) * a.hq;
-    for (int k0 = set; k0 < np + ns; k0 += 4 * kSets) {
-      f32x4_t v[4];
-      float lse[4];
+    constexpr int kLoads = kSets == 2 ? 4 : 8;
+    for (int k0 = set; k0 < np + ns; k0 += kLoads * kSets) {
+      f32x4_t v[kLoads];
+      float lse[kLoads];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < kLoads; ++e) {
         const int k = min(k0 + e * kSets, np + ns - 1);
         const int64_t row = k < np ? p0 + k * p_step : k == np ? s0 : s1 + (k - np) * s_step;
         v[e] = *reinterpret_cast<const f32x4_t*>((k < np ? a.p_o : a.s_o) + row * kD + 4 * c);
@@ -576,14 +680,14 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
       }
       float mn = m;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mn = fmaxf(mn, lse[e]);
+      for (int e = 0; e < kLoads; ++e) mn = fmaxf(mn, lse[e]);
       const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
       l *= alpha;
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[k] *= alpha;
       m = mn;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < kLoads; ++e) {
         if (lse[e] == -INFINITY) continue;  // nothing seen there: its values do not count
         const float w = exp2f(lse[e] - mn);
         l += w;
@@ -598,11 +702,10 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   xch[5][group][c] = l;
   __syncthreads();
   if (set != 0 || !head_ok) return;
+  bool again = x.ok && !folded;
   if (!x.ok) {
     acc = f32x4_t{NAN, NAN, NAN, NAN};
-  } else if (!folded) {
-    acc = plain_row(a, x, t, head, sees, c);
-  } else {
+  } else if (folded) {
 #pragma unroll
     for (int e = 1; e < kSets; ++e) m = fmaxf(m, xch[4][group + e][c]);
     l = 0.f;
@@ -625,9 +728,9 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
 #pragma unroll
     for (int k = 0; k < 4; ++k) bad = bad || !(fabsf(acc[k]) < INFINITY);
     const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
-    if (i + 1 < x.qo && ((any >> (lane & 32)) & 0xffffffffull) != 0)
-      acc = plain_row(a, x, t, head, sees, c);
+    again = i + 1 < x.qo && ((any >> (lane & 32)) & 0xffffffffull) != 0;
   }
+  if (again) acc = plain_row(a, x, t, head, sees, c);
   *reinterpret_cast<u32x2_t*>(a.o + t * a.o_st + head * a.o_sh + 4 * c) =
       u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
 }
@@ -653,18 +756,60 @@ struct Layout {
 
 Layout workspace_layout(const sgl_prefix_plan_t& p) {
   auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
-  const int64_t prefix_rows = p.num_tiles > 0
-      ? static_cast<int64_t>(p.num_units) * p.num_kv_heads * p.tile_rows
-      : static_cast<int64_t>(p.num_shares) * p.max_tokens * p.num_qo_heads;
   const int64_t own_rows =
-      (p.max_tokens + static_cast<int64_t>(p.num_units) * p.max_qo_len) * p.num_qo_heads;
+      (p.max_tokens + static_cast<int64_t>(p.max_units) * p.max_qo_len) * p.num_qo_heads;
   Layout l;
   l.p_o = 0;
-  l.p_lse = l.p_o + align(prefix_rows * kD * 4);
-  l.s_o = l.p_lse + align(prefix_rows * 4);
+  l.p_lse = l.p_o + align(p.prefix_rows * kD * 4);
+  l.s_o = l.p_lse + align(p.prefix_rows * 4);
   l.s_lse = l.s_o + align(own_rows * kD * 4);
   l.total = l.s_lse + align(own_rows * 4);
   return l;
+}
+
+// The plan for workgroups `blocks`; everything else follows from the sizes.
+int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, int num_qo_heads,
+              int num_kv_heads, int head_dim, int blocks, sgl_prefix_plan_t& p) {
+  if (prefix_len < 0 || batch_size < 0 || max_tokens < 0 || max_qo_len < 0 || num_qo_heads <= 0 ||
+      num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0 || blocks < 2 || blocks > 512)
+    return SGL_ERR_INVALID_ARG;
+  const int group = num_qo_heads / num_kv_heads;
+  if (head_dim != kD || group > 64 || max_qo_len > SGL_PREFIX_MAX_QO ||
+      num_kv_heads > 65535 || prefix_len > (1 << 29) || batch_size > (1 << 25))
+    return SGL_ERR_UNSUPPORTED;
+  // Packed rows, and the list of tiles, are counted in 32 bits, and the fold's grid is a
+  // workgroup per row at most.
+  const int64_t rows = static_cast<int64_t>(max_tokens) * group;
+  const int64_t row_tiles = (rows + 255) / 256, tiles = (prefix_len + pf::kBN - 1) / pf::kBN;
+  if (rows > (1 << 30) || static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff ||
+      row_tiles * num_kv_heads > 0x7fffffff / (tiles > 0 ? tiles : 1))
+    return SGL_ERR_UNSUPPORTED;
+  p = sgl_prefix_plan_t{};
+  p.prefix_len = prefix_len, p.batch_size = batch_size, p.max_tokens = max_tokens, p.max_qo_len = max_qo_len;
+  p.num_qo_heads = num_qo_heads, p.num_kv_heads = num_kv_heads, p.head_dim = head_dim;
+  p.num_blocks = blocks;
+  const int heads = heads_per_group(num_kv_heads);
+  const int64_t units = static_cast<int64_t>(blocks) * (8 / heads) / (num_kv_heads / heads);
+  p.max_units = static_cast<int32_t>(units < 1 ? 1 : units);
+  if (prefix_len > 0 && rows > 0) {
+    if (rows <= kMaxWalkRows) {  // the units walk the prefix
+      p.walk_rows = static_cast<int32_t>((rows + 15) / 16 * 16);
+      p.prefix_rows = static_cast<int64_t>(p.max_units) * num_kv_heads * p.walk_rows;
+    } else {
+      // Pieces of an item: at most blocks / (items) + 2, of at most 256 rows an item.
+      p.prefix_rows = (blocks + 2 * row_tiles * num_kv_heads) * 256;
+    }
+  }
+  p.workspace_bytes = workspace_layout(p).total;
+  return SGL_OK;
+}
+
+template <int RB>
+void launch_attention(const PrefixArgs& a, bool sync, hipStream_t s) {
+  static_assert(2 * pf::kTileBytes >= 8 * kWaveLds, "the waves' output rows take the tiles' place");
+  const size_t lds = 2 * pf::kTileBytes;
+  if (sync) hipLaunchKernelGGL((prefix_attention_kernel<RB, true>), dim3(a.blocks), dim3(512), lds, s, a);
+  else hipLaunchKernelGGL((prefix_attention_kernel<RB, false>), dim3(a.blocks), dim3(512), lds, s, a);
 }
 
 }  // namespace
@@ -675,50 +820,9 @@ using namespace sgl;
 extern "C" int sgl_prefix_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len,
                                int num_qo_heads, int num_kv_heads, int head_dim,
                                sgl_prefix_plan_t* plan) {
-  if (!plan || prefix_len < 0 || batch_size < 0 || max_tokens < 0 || max_qo_len < 0 ||
-      num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0)
-    return SGL_ERR_INVALID_ARG;
-  const int group = num_qo_heads / num_kv_heads;
-  if (head_dim != kD || group > kMaxTileRows || max_qo_len > SGL_PREFIX_MAX_QO ||
-      num_kv_heads > 65535)
-    return SGL_ERR_UNSUPPORTED;
-  // Packed rows and their tiles are counted in 32 bits.
-  if (static_cast<int64_t>(max_tokens) * group > (1 << 30) || prefix_len > (1 << 30))
-    return SGL_ERR_UNSUPPORTED;
-  *plan = sgl_prefix_plan_t{};
-  plan->prefix_len = prefix_len;
-  plan->batch_size = batch_size;
-  plan->max_tokens = max_tokens;
-  plan->max_qo_len = max_qo_len;
-  plan->num_qo_heads = num_qo_heads;
-  plan->num_kv_heads = num_kv_heads;
-  plan->head_dim = head_dim;
-  const int64_t units = static_cast<int64_t>(device_cus()) * 8 / num_kv_heads;
-  plan->num_units = static_cast<int32_t>(units < 1 ? 1 : units);
-  const int64_t rows = static_cast<int64_t>(max_tokens) * group;
-  if (prefix_len > 0 && rows > 0) {
-    if (rows <= kMaxTileRows) {  // the units walk the prefix
-      plan->tile_rows = static_cast<int32_t>((rows + 15) / 16 * 16);
-      plan->num_tiles = 1;
-    } else {
-      // A launch of its own: the shares whose items, all rounds together, walk the
-      // fewest tiles one after the other (two for an item's start and its states).
-      plan->tile_rows = rows <= 128 ? 128 : 256;
-      const int64_t slots = device_cus() * (256 / plan->tile_rows);
-      const int64_t per_share = (rows + plan->tile_rows - 1) / plan->tile_rows * num_kv_heads;
-      const int64_t nt = (prefix_len + pf::kBN - 1) / pf::kBN;
-      int64_t best = 0, shares = 1;
-      for (int64_t n = 1; n <= nt && (n == 1 || (n - 1) * per_share < 4 * slots); ++n) {
-        const int64_t per = (nt + n - 1) / n, used = (nt + per - 1) / per;
-        if (used != n) continue;
-        const int64_t cost = (n * per_share + slots - 1) / slots * (per + 2);
-        if (best == 0 || cost < best) best = cost, shares = n;
-      }
-      plan->num_shares = static_cast<int32_t>(shares);
-    }
-  }
-  plan->workspace_bytes = workspace_layout(*plan).total;
-  return SGL_OK;
+  if (!plan) return SGL_ERR_INVALID_ARG;
+  return make_plan(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads, num_kv_heads, head_dim,
+                   std::min(std::max(device_cus(), 2), 512), *plan);
 }
 
 extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q,
@@ -737,12 +841,11 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
     return SGL_ERR_INVALID_ARG;
   // A plan as sgl_prefix_plan makes it.
   sgl_prefix_plan_t p;
-  int st = sgl_prefix_plan(plan->prefix_len, plan->batch_size, plan->max_tokens, plan->max_qo_len,
-                           num_qo_heads, num_kv_heads, head_dim, &p);
+  int st = make_plan(plan->prefix_len, plan->batch_size, plan->max_tokens, plan->max_qo_len,
+                     num_qo_heads, num_kv_heads, head_dim, plan->num_blocks, p);
   if (st != SGL_OK) return st;
-  p.num_units = plan->num_units;
-  if (p.num_units <= 0 || p.num_units > (1 << 20) || plan->tile_rows != p.tile_rows ||
-      plan->num_tiles != p.num_tiles || plan->num_shares != p.num_shares)
+  if (plan->max_units != p.max_units || plan->walk_rows != p.walk_rows ||
+      plan->prefix_rows != p.prefix_rows)
     return SGL_ERR_INVALID_ARG;
   if (batch_size > p.batch_size || max_tokens > p.max_tokens) return SGL_ERR_CAPACITY;
   if (batch_size == 0 || max_tokens == 0) return SGL_OK;
@@ -765,40 +868,22 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   a.pidx = prefix_indices, a.indices = indices, a.kv_indptr = kv_indptr, a.qo_indptr = qo_indptr;
   a.batch = batch_size, a.tokens = max_tokens;
   a.hq = num_qo_heads, a.hkv = num_kv_heads, a.group = num_qo_heads / num_kv_heads;
-  a.prefix = p.prefix_len, a.tile_rows = p.tile_rows, a.units = p.num_units, a.max_qo = p.max_qo_len;
+  a.prefix = p.prefix_len, a.max_qo = p.max_qo_len, a.walk_rows = p.walk_rows, a.blocks = p.num_blocks;
+  a.heads = heads_per_group(num_kv_heads), a.side = 8 / a.heads, a.rest = num_kv_heads / a.heads;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.o = static_cast<uint16_t*>(o), a.o_st = o_stride_token, a.o_sh = o_stride_head;
   a.p_o = reinterpret_cast<float*>(ws + l.p_o), a.p_lse = reinterpret_cast<float*>(ws + l.p_lse);
   a.s_o = reinterpret_cast<float*>(ws + l.s_o), a.s_lse = reinterpret_cast<float*>(ws + l.s_lse);
-  const int64_t rows = static_cast<int64_t>(max_tokens) * a.group;
-  a.tiles = p.num_tiles;
-  a.shares = p.num_shares;
-  a.row_tiles = a.shares > 0 ? static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows) : 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t items = static_cast<int64_t>(a.row_tiles) * num_kv_heads * a.shares;
-  if (items > 0x7fffffff) return SGL_ERR_UNSUPPORTED;
-  // The fold's grid is at most a workgroup per row.
-  if (static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff) return SGL_ERR_UNSUPPORTED;
-  const int waves = heads_per_group(num_kv_heads);
-  const dim3 grid(p.num_units, num_kv_heads / waves), block(64 * waves);
-  if (items > 0) {
-    const dim3 own(static_cast<uint32_t>(items));
-    if (p.tile_rows == 128) hipLaunchKernelGGL(prefix_rows_kernel<4>, own, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(prefix_rows_kernel<8>, own, dim3(512), 0, s, a);
-    st = launch_status();
-    if (st != SGL_OK) return st;
-  }
   const int own_rows = p.max_qo_len * a.group;
-  const int need = a.tiles > 0 && own_rows < a.tile_rows ? a.tile_rows : own_rows;
-  const int rb = need <= 16 ? 1 : need <= 32 ? 2 : 4;
-  const size_t lds = static_cast<size_t>(waves) * 16 * rb * kQPitch * 2;
-  if (rb == 1) hipLaunchKernelGGL(prefix_units_kernel<1>, grid, block, lds, s, a);
-  else if (rb == 2) hipLaunchKernelGGL(prefix_units_kernel<2>, grid, block, lds, s, a);
-  else hipLaunchKernelGGL(prefix_units_kernel<4>, grid, block, lds, s, a);
+  const int need = own_rows < a.walk_rows ? a.walk_rows : own_rows;
+  if (need <= 16) launch_attention<1>(a, a.heads == 8, s);
+  else launch_attention<2>(a, a.heads == 8, s);
   st = launch_status();
   if (st != SGL_OK) return st;
   // Many pieces a row: a workgroup for each. Few: two groups of lanes a row.
-  const int64_t pieces = a.tiles > 0 ? p.num_units : a.shares + 1;
+  const int64_t pieces = a.walk_rows > 0 ? p.max_units
+      : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 255) / 256 * num_kv_heads) + 2;
   const int rows_per = pieces > 16 ? 1 : 4;
   const int head_groups = (num_qo_heads + rows_per - 1) / rows_per;
   const dim3 fold(static_cast<uint32_t>(max_tokens) * head_groups);

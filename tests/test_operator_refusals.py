@@ -73,13 +73,13 @@ def test_prefix_plan():
     for kw in (dict(d=64), dict(qo=capi.PREFIX_MAX_QO + 1), dict(hq=65, hkv=1), dict(T=1 << 29)):
         assert plan(**kw)[0] == -2, kw
     st, p = plan()
-    assert st == 0 and p.num_units >= 1 and p.workspace_bytes > 0
+    assert st == 0 and p.num_blocks >= 1 and p.max_units >= 1 and p.workspace_bytes > 0
     assert plan(P=0)[0] == plan(B=0, T=0, qo=0)[0] == 0
     # Room for every row's own piece (128 fp32 values), whichever way the prefix goes.
     for T in (1, 8, 16, 17, 64, 700):
         st, p = plan(T=T)
-        assert p.num_tiles + (p.num_shares > 0) == 1 and p.workspace_bytes >= T * 8 * 512
-        assert (p.num_shares > 0) == (4 * T > 64)
+        assert p.workspace_bytes >= T * 8 * 512 and p.prefix_rows > 0
+        assert p.walk_rows == (-(-4 * T // 16) * 16 if 4 * T <= 32 else 0)
 
 
 def attend(p, **kw):
@@ -107,10 +107,10 @@ def test_prefix_attention_refusals():
     assert attend(p, ks=0) == -2
     # A plan that was not made by sgl_prefix_plan.
     q = capi.PrefixPlan.from_buffer_copy(p)
-    q.num_units = 0
+    q.num_blocks = 0
     assert attend(q) == -1
     q = capi.PrefixPlan.from_buffer_copy(p)
-    q.num_tiles += 1
+    q.prefix_rows += 1
     assert attend(q) == -1
 
 
