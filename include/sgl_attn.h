@@ -577,7 +577,7 @@ typedef struct {
   int32_t num_qo_heads;
   int32_t num_kv_heads;
   int32_t head_dim;
-  int32_t num_blocks;   /* workgroups of the launch (one per CU) */
+  int32_t num_blocks;   /* workgroups of the launch (two per CU) */
   int32_t max_units;    /* parts the requests' own tokens are cut into at most */
   int32_t walk_rows;    /* packed rows (tokens x heads of a kv head) up to which those parts
                            take the prefix too; 0: it has workgroups of its own */

@@ -28,6 +28,7 @@ constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
 constexpr int kMinUnit = 16;              // shortest unit
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
+constexpr int kWaves = 4;                 // waves of a workgroup, two workgroups per CU
 constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
 constexpr int kMaxWalkRows = 32;         // packed rows up to which the units walk the prefix
 
@@ -61,59 +62,81 @@ struct PrefixArgs {
 
 // How a launch is shared out, from the lengths as they are now (so a captured launch
 // follows them): the main and the fold kernel work it out alike, in whole numbers.
-// Prefix tiles: workgroups [0, tile_blocks) take tile_run consecutive ones each of the
-// list (row tile, kv head, 64-token tile of the prefix), the tiles varying fastest; the
-// others' units walk the stream of `all` tokens, `shared` of them the prefix's, W a unit.
+// Workgroups [0, tile_blocks) walk the prefix's 64-token tiles for one kv head and row
+// tile at a time, per_head of them for a head: with `shares` each row tile's tiles are
+// cut into that many runs (all row tiles alike, so that the workgroups of a head, on the
+// same XCD where there are eight heads, read the same K/V at the same time), else the
+// list (row tile, tile) into per_head runs. The others' units walk the stream of `all`
+// tokens, `shared` of them the prefix's, W a unit.
 struct Split {
-  int first, rows;        // first query token, packed rows of a kv head
+  int first, rows;          // first query token, packed rows of a kv head
   int row_tiles, row_step;  // row tiles and their rows (32 a wave, spread evenly)
-  int tiles;              // 64-token tiles of the prefix
-  uint32_t list, tile_run;
-  int tile_blocks;
+  int tiles;                // 64-token tiles of the prefix
+  int tile_blocks, per_head, shares;
+  uint32_t run;
   uint32_t shared, all, W;
   int units;
 };
 
-// What a tile of a row tile takes by its waves of rows, ns, and a token of a kv head
-// on one workgroup.
-__device__ constexpr uint16_t kTileNs[9] = {0, 1400, 1400, 1500, 1500, 2000, 2200, 2400, 2700};
-constexpr uint32_t kTokenNs = 11;
+// What a tile takes on one workgroup, and a token of a kv head, ns.
+constexpr uint32_t kTileNs = 1400;
+constexpr uint32_t kTokenNs = 24;
 // A request counts as this many tokens more in the units' stream: the loads that lead
 // to its first step, about 3.4 us (a unit that took eight requests of one token each was
 // 28 us behind the others).
 constexpr uint32_t kRequestTokens = 24;
 
+// A loaded value that is the same in every lane, in a scalar register (the compiler
+// keeps it in a vector one, as the kernel's stores might change the memory).
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 __device__ __forceinline__ Split split_of(const PrefixArgs& a) {
   Split s;
-  s.first = max(a.qo_indptr[0], 0);
-  s.rows = max(min(a.qo_indptr[a.batch], a.tokens) - s.first, 0) * a.group;
-  const uint32_t own = static_cast<uint32_t>(max(a.kv_indptr[a.batch] - max(a.kv_indptr[0], 0), 0)) +
-                       a.batch * kRequestTokens;
+  const int q_end = uniform(a.qo_indptr[a.batch]), kv_begin = uniform(a.kv_indptr[0]);
+  const int kv_end = uniform(a.kv_indptr[a.batch]);
+  s.first = max(uniform(a.qo_indptr[0]), 0);
+  s.rows = max(min(q_end, a.tokens) - s.first, 0) * a.group;
+  const uint32_t own = static_cast<uint32_t>(max(kv_end - max(kv_begin, 0), 0)) + a.batch * kRequestTokens;
   s.tiles = (a.prefix + pf::kBN - 1) / pf::kBN;
-  s.row_tiles = s.row_step = s.tile_blocks = 0;
-  s.list = 0, s.tile_run = 1;
+  s.row_tiles = s.row_step = s.tile_blocks = s.per_head = s.shares = 0;
+  s.run = 1;
   s.shared = 0;
   if (a.walk_rows > 0) {
     s.shared = a.prefix;
   } else if (s.rows > 0 && s.tiles > 0) {
     const int waves = (s.rows + 31) / 32;
-    s.row_tiles = (waves + 7) / 8;
+    s.row_tiles = (waves + kWaves - 1) / kWaves;
     const int each = (waves + s.row_tiles - 1) / s.row_tiles;
     s.row_step = 32 * each;
     s.row_tiles = (waves + each - 1) / each;
-    s.list = static_cast<uint32_t>(s.row_tiles) * a.hkv * s.tiles;
-    const uint64_t t = static_cast<uint64_t>(s.list) * kTileNs[each];
+    const uint32_t list = static_cast<uint32_t>(s.row_tiles) * s.tiles;  // of a head
+    const uint64_t t = static_cast<uint64_t>(list) * a.hkv * kTileNs;
     const uint64_t sum = t + static_cast<uint64_t>(own) * a.hkv * kTokenNs;
     const int shift = max(0, 42 - __builtin_clzll(sum));  // to 22 bits
     const uint32_t ts = static_cast<uint32_t>(t >> shift), ss = static_cast<uint32_t>(sum >> shift);
-    s.tile_blocks = static_cast<int>((a.blocks * ts + ss / 2) / ss);
-    s.tile_blocks = max(1, min(s.tile_blocks, a.blocks - 1));
-    s.tile_run = (s.list + s.tile_blocks - 1) / s.tile_blocks;
+    // A second workgroup of tiles on a CU brings nothing (1.4 us a tile alone, 2.7 for
+    // each of two).
+    s.tile_blocks = max(1, min(static_cast<int>((a.blocks * ts + ss / 2) / ss), a.blocks / 2));
+    s.per_head = max(1, s.tile_blocks / a.hkv);
+    if (s.per_head >= s.row_tiles) {
+      int n = (s.per_head + s.row_tiles / 2) / s.row_tiles;
+      if (n > 1 && n * s.row_tiles * a.hkv > a.blocks / 2) --n;
+      s.run = (s.tiles + n - 1) / n;
+      s.shares = static_cast<int>((s.tiles + s.run - 1) / s.run);
+      s.per_head = s.shares * s.row_tiles;
+    } else {
+      s.run = (list + s.per_head - 1) / s.per_head;
+    }
+    s.tile_blocks = min(s.per_head * a.hkv, a.blocks - 1);
   }
   s.all = s.shared + own;
   s.units = max(1, (a.blocks - s.tile_blocks) * a.side / a.rest);
   const uint32_t w = s.all / static_cast<uint32_t>(s.units) + 1;  // one more where it divides
   s.W = max((w + kStep - 1) / kStep * kStep, static_cast<uint32_t>(kMinUnit));
+  // Quotients come from the vector unit.
+  s.row_tiles = uniform(s.row_tiles), s.row_step = uniform(s.row_step), s.tile_blocks = uniform(s.tile_blocks);
+  s.per_head = uniform(s.per_head), s.shares = uniform(s.shares), s.run = uniform(s.run);
+  s.W = uniform(s.W), s.units = uniform(s.units);
   return s;
 }
 
@@ -124,15 +147,16 @@ struct Request {
 
 __device__ __forceinline__ Request request_of(const PrefixArgs& a, int r) {
   Request x;
-  x.q0 = a.qo_indptr[r];
-  const int64_t q1 = a.qo_indptr[r + 1];
-  x.kv0 = a.kv_indptr[r];
-  const int64_t k1 = a.kv_indptr[r + 1];
+  x.q0 = uniform(a.qo_indptr[r]);
+  const int64_t q1 = uniform(a.qo_indptr[r + 1]);
+  x.kv0 = uniform(a.kv_indptr[r]);
+  const int64_t k1 = uniform(a.kv_indptr[r + 1]);
   x.qo = static_cast<int>(q1 - x.q0);
   x.kv = static_cast<int>(k1 - x.kv0);
   // Rows and pieces of anything else have no place in the outputs and the workspace.
-  x.ok = x.kv0 >= 0 && x.q0 >= max(a.qo_indptr[0], 0) && q1 >= x.q0 && q1 <= min(a.qo_indptr[a.batch], a.tokens) &&
-         q1 - x.q0 <= a.max_qo && x.kv0 >= a.kv_indptr[0] && k1 >= x.kv0 && k1 <= a.kv_indptr[a.batch];
+  x.ok = x.q0 >= max(uniform(a.qo_indptr[0]), 0) && q1 >= x.q0 &&
+         q1 <= min(uniform(a.qo_indptr[a.batch]), a.tokens) && q1 - x.q0 <= a.max_qo &&
+         x.kv0 >= max(uniform(a.kv_indptr[0]), 0) && k1 >= x.kv0 && k1 <= uniform(a.kv_indptr[a.batch]);
   return x;
 }
 
@@ -183,7 +207,7 @@ struct Piece {
 // of it once, and what it does not find in the instruction cache costs more than the
 // arithmetic (with Q in LDS and four row blocks 64 requests of 6 query tokens and 16 of
 // their own took 36 us, 16 of one query token).
-template <int RB, bool kSync>
+template <int RB>
 __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* xch, int h, int lane) {
   const int n = lane & 15, j = lane >> 4;
   const int G = a.group, len = w.len;
@@ -201,8 +225,11 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
     for (int e = 0; e < 4; ++e)
       vr[e] = ldg128_nt<true>(slot_row(vlane, __shfl(slot, 4 * j + e, kWave), ss_bytes));
   };
-  const int slot = w.idx[min(n, len - 1)];
-  int slot_next = w.idx[min(kStep + n, len - 1)];
+  // Slots of this lane's token, and K and V, of the step at hand, the next and the one
+  // behind it.
+  const int slot0 = w.idx[min(n, len - 1)];
+  const int slot1 = w.idx[min(kStep + n, len - 1)];
+  int slot_next = slot1;
   // Token and head of this lane's row of each block; rows past the last one read
   // its Q again and see nothing.
   const int i0 = w.row0 / G, rem = w.row0 - i0 * G;
@@ -220,9 +247,9 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
 #pragma unroll
     for (int s = 0; s < 4; ++s) q[b][s] = ldg128(qp + 32 * s);
   }
-  u32x4_t kr[4], vr[4];
-  load_k(slot, kr);
-  load_v(slot, vr);
+  u32x4_t kr1[4], vr1[4];
+  load_k(slot0, kr1);
+  load_v(slot0, vr1);
   float m[RB], l[RB];
   f32x4_t acc[RB][8];
 #pragma unroll
@@ -233,11 +260,7 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
     for (int nb = 0; nb < 8; ++nb) acc[b][nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-#pragma unroll 1
-  for (int t = 0; t < len; t += kStep) {
-    // Where the workgroup's waves are one unit's kv heads they keep in step:
-    // together they read whole token rows.
-    if constexpr (kSync) __builtin_amdgcn_s_barrier();
+  auto step = [&](int t, u32x4_t (&kr)[4], u32x4_t (&vr)[4]) {
     const int slot_after = w.idx[min(t + 2 * kStep + n, len - 1)];
     f32x4_t sacc[RB];
 #pragma unroll
@@ -290,7 +313,9 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
     });
     load_v(slot_next, vr);
     slot_next = slot_after;
-  }
+  };
+#pragma unroll 1
+  for (int t = 0; t < len; t += kStep) step(t, kr1, vr1);
   // The block's output through LDS (16 rows of 32 16-byte chunks, chunk c of row n at
   // c ^ n: no bank conflicts either way), so that whole rows are stored: as they lie in
   // the accumulators a store would touch 64 lines for 1 KB (128 units of 32 rows, 8 kv
@@ -334,13 +359,13 @@ __device__ __forceinline__ int64_t place_of(const PrefixArgs& a, int r, int kv_f
 
 // Unit u's pieces of the stream for kv head h: places below 2^29 (prefix) + 2^31 (the
 // offsets are int32) + 2^30 (2^25 requests), 32 bits without a sign.
-template <int RB, bool kSync>
+template <int RB>
 __device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s, char* xch, uint32_t u, int h,
                                             int lane) {
   if (static_cast<uint64_t>(u) * s.W >= s.all) return;
   const uint32_t t0 = u * s.W, t1 = min(s.all, t0 + s.W);
   // The requests' own tokens [b0, b1) of the joined list, from request r on.
-  const int kv_first = max(a.kv_indptr[0], 0);
+  const int kv_first = max(uniform(a.kv_indptr[0]), 0);
   const uint32_t b0 = max(t0, s.shared) - s.shared, b1 = max(t1, s.shared) - s.shared;
   int r = -1;  // the prefix's part
   int left = 0;  // rows of the current request not walked yet
@@ -372,7 +397,7 @@ __device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s,
       }
       if (r >= a.batch) return;
       const Request x = request_of(a, r);
-      const int64_t rb = place_of(a, r, kv_first);  // then its kRequestTokens, then its tokens
+      const int64_t rb = static_cast<int64_t>(x.kv0) - kv_first + static_cast<int64_t>(r) * kRequestTokens;  // then its kRequestTokens, then its tokens
       if (rb >= b1) return;
       if (!x.ok) continue;
       const int64_t at = rb + kRequestTokens;
@@ -389,7 +414,7 @@ __device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s,
       w.by_token = true;
     }
     w.rows = min(left, 16 * RB);
-    walk<RB, kSync>(a, w, xch, h, lane);
+    walk<RB>(a, w, xch, h, lane);
     left -= w.rows;
     w.row0 += w.rows;
     if (!w.by_token) w.out0 += w.rows;
@@ -402,12 +427,10 @@ __device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s,
 // tile steps without a causal bound. Tiles [tb, te) of the prefix for row tile rt of kv
 // head h, the item's piece number `piece`. Bound by the matrix cores: 4 x 64 x 128 flops
 // a row and tile.
-constexpr int kTileWaves = 8;
-
 __device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& sp, char* lds_raw, int rt,
                                              int h, int tb, int te, int piece) {
   using namespace pf;
-  constexpr int W = kTileWaves;
+  constexpr int W = kWaves;
   const int rows = sp.rows, first = sp.first;
   const int row0 = rt * sp.row_step, row_end = min(rows, row0 + sp.row_step);
   const int lane = threadIdx.x & 63;
@@ -516,6 +539,10 @@ __device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& s
   // Whole rows to memory through the wave's 8 KB of LDS (free behind the last step's
   // barrier), half a row (64 values, 16 chunks; chunk k of row c at k ^ c) at a time.
   f32x4_t* xr = reinterpret_cast<f32x4_t*>(lds_raw + wave * kWaveLds);
+  // The lane's places are worked out here, not ahead of the tiles, where they would
+  // take registers that the tiles need.
+  int ln = lane;
+  asm volatile("" : "+v"(ln));
   const int left = row_end - (row0 + 32 * wave);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -524,13 +551,13 @@ __device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& s
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x16_t& x = rs.acc[2 * half + e];
-        xr[16 * c + ((8 * e + 2 * g + hl) ^ (c & 15))] =
+        xr[16 * (ln & 31) + ((8 * e + 2 * g + (ln >> 5)) ^ (ln & 15))] =
             f32x4_t{x[4 * g] * inv, x[4 * g + 1] * inv, x[4 * g + 2] * inv, x[4 * g + 3] * inv};
       }
     wave_lds_sync();
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
-      const int x = 4 * it + (lane >> 4), k = lane & 15;
+      const int x = 4 * it + (ln >> 4), k = ln & 15;
       if (x < left)
         __builtin_nontemporal_store(
             xr[16 * x + (k ^ (x & 15))],
@@ -541,37 +568,51 @@ __device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& s
   __syncthreads();  // before the next item's tiles
 }
 
-// One workgroup per CU (eight waves with all its registers): the first tile_blocks walk
-// their run of the prefix's tiles, bound by the matrix cores, beside the others' units,
-// bound by memory.
-template <int RB, bool kSync>
-__global__ void __launch_bounds__(512, 1) prefix_attention_kernel(PrefixArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+// Two workgroups of four waves per CU: those that walk the prefix's tiles, bound by
+// the matrix cores, lie beside the others' units, bound by memory (a CU takes in about
+// 25 GB/s whatever it has in flight, so the units need every CU).
+template <int RB>
+__global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(PrefixArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * pf::kTileBytes];
+  static_assert(sizeof(smem) >= kWaves * kWaveLds, "the waves' output rows take the tiles' place");
   const Split s = split_of(a);
   const int b = blockIdx.x;
   if (b < s.tile_blocks) {
-    uint32_t at = b * s.tile_run;
-    const uint32_t end = min(s.list, at + s.tile_run);
-    while (at < end) {
-      const uint32_t item = at / static_cast<uint32_t>(s.tiles);
-      const int tb = static_cast<int>(at - item * s.tiles);
-      const int te = static_cast<int>(min(static_cast<uint32_t>(s.tiles), tb + (end - at)));
-      // The item's first tile is in workgroup item tiles / tile_run.
-      const int piece = b - static_cast<int>(item * s.tiles / s.tile_run);
-      const int rt = static_cast<int>(item / static_cast<uint32_t>(a.hkv));
-      prefix_tiles(a, s, smem, rt, static_cast<int>(item - rt * a.hkv), tb, te, piece);
-      at += te - tb;
+    for (int v = b; v < s.per_head * a.hkv; v += s.tile_blocks) {
+      const int j = v / a.hkv, h = v - j * a.hkv;
+      const int run = static_cast<int>(s.run);
+      int rt, tb, left, piece;
+      if (s.shares > 0) {
+        rt = j / s.shares;
+        piece = j - rt * s.shares;
+        tb = piece * run;
+        left = min(s.tiles - tb, run);
+      } else {
+        const uint32_t at = j * s.run, end = min(static_cast<uint32_t>(s.row_tiles) * s.tiles, at + s.run);
+        rt = static_cast<int>(at / static_cast<uint32_t>(s.tiles));
+        piece = j - static_cast<int>(rt * static_cast<uint32_t>(s.tiles) / s.run);
+        tb = static_cast<int>(at - rt * s.tiles);
+        left = end > at ? static_cast<int>(end - at) : 0;
+      }
+      while (left > 0) {
+        const int te = min(s.tiles, tb + left);
+        prefix_tiles(a, s, smem, uniform(rt), uniform(h), uniform(tb), uniform(te), uniform(piece));
+        left -= te - tb;
+        ++rt;  // its first run is number rt tiles / run
+        piece = j - static_cast<int>(rt * static_cast<uint32_t>(s.tiles) / s.run);
+        tb = 0;
+      }
     }
     return;
   }
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = wave / a.heads;
-  if (g >= a.side) return;  // kSync: none
+  if (g >= a.side) return;
   const int n = a.blocks - s.tile_blocks;
   for (int v = (b - s.tile_blocks) * a.side + g; v < s.units * a.rest; v += n * a.side) {
     const int u = v / a.rest;
-    unit_pieces<RB, kSync>(a, s, smem + wave * kWaveLds, u, (v - u * a.rest) * a.heads + wave - g * a.heads, lane);
+    unit_pieces<RB>(a, s, smem + wave * kWaveLds, u, (v - u * a.rest) * a.heads + wave - g * a.heads, lane);
   }
 }
 
@@ -651,8 +692,8 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
     int64_t p_step = static_cast<int64_t>(a.hkv) * a.walk_rows;
     const int prow = (t - sp.first) * a.group + hh - h * a.group;
     if (sp.tile_blocks > 0) {
-      const uint32_t item = static_cast<uint32_t>(prow / sp.row_step * a.hkv + h) * sp.tiles;
-      np = static_cast<int>((item + sp.tiles - 1) / sp.tile_run - item / sp.tile_run) + 1;
+      const uint32_t at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
+      np = sp.shares > 0 ? sp.shares : static_cast<int>((at + sp.tiles - 1) / sp.run - at / sp.run) + 1;
       p_step = static_cast<int64_t>(a.hkv) * sp.rows;
       p0 = static_cast<int64_t>(h) * sp.rows + prow;
     } else if (P > 0) {
@@ -743,9 +784,9 @@ int device_cus() {
   return 256;
 }
 
-// kv heads of a workgroup: the largest divisor of theirs up to 8.
+// kv heads of a unit: the largest divisor of theirs up to a workgroup's waves.
 int heads_per_group(int hkv) {
-  for (int n = 8; n > 1; --n)
+  for (int n = kWaves; n > 1; --n)
     if (hkv % n == 0) return n;
   return 1;
 }
@@ -771,7 +812,7 @@ Layout workspace_layout(const sgl_prefix_plan_t& p) {
 int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, int num_qo_heads,
               int num_kv_heads, int head_dim, int blocks, sgl_prefix_plan_t& p) {
   if (prefix_len < 0 || batch_size < 0 || max_tokens < 0 || max_qo_len < 0 || num_qo_heads <= 0 ||
-      num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0 || blocks < 2 || blocks > 512)
+      num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0 || blocks < 2 || blocks > 1022)
     return SGL_ERR_INVALID_ARG;
   const int group = num_qo_heads / num_kv_heads;
   if (head_dim != kD || group > 64 || max_qo_len > SGL_PREFIX_MAX_QO ||
@@ -780,7 +821,7 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
   // Packed rows, and the list of tiles, are counted in 32 bits, and the fold's grid is a
   // workgroup per row at most.
   const int64_t rows = static_cast<int64_t>(max_tokens) * group;
-  const int64_t row_tiles = (rows + 255) / 256, tiles = (prefix_len + pf::kBN - 1) / pf::kBN;
+  const int64_t row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves), tiles = (prefix_len + pf::kBN - 1) / pf::kBN;
   if (rows > (1 << 30) || static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff ||
       row_tiles * num_kv_heads > 0x7fffffff / (tiles > 0 ? tiles : 1))
     return SGL_ERR_UNSUPPORTED;
@@ -789,15 +830,16 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
   p.num_qo_heads = num_qo_heads, p.num_kv_heads = num_kv_heads, p.head_dim = head_dim;
   p.num_blocks = blocks;
   const int heads = heads_per_group(num_kv_heads);
-  const int64_t units = static_cast<int64_t>(blocks) * (8 / heads) / (num_kv_heads / heads);
+  const int64_t units = static_cast<int64_t>(blocks) * (kWaves / heads) / (num_kv_heads / heads);
   p.max_units = static_cast<int32_t>(units < 1 ? 1 : units);
   if (prefix_len > 0 && rows > 0) {
     if (rows <= kMaxWalkRows) {  // the units walk the prefix
       p.walk_rows = static_cast<int32_t>((rows + 15) / 16 * 16);
       p.prefix_rows = static_cast<int64_t>(p.max_units) * num_kv_heads * p.walk_rows;
     } else {
-      // Pieces of an item: at most blocks / (items) + 2, of at most 256 rows an item.
-      p.prefix_rows = (blocks + 2 * row_tiles * num_kv_heads) * 256;
+      // At most `blocks` shares of a row tile and head, or two runs that each of them
+      // lies in, of 128 rows.
+      p.prefix_rows = (blocks + 2 * row_tiles * num_kv_heads) * 32 * kWaves;
     }
   }
   p.workspace_bytes = workspace_layout(p).total;
@@ -805,11 +847,8 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
 }
 
 template <int RB>
-void launch_attention(const PrefixArgs& a, bool sync, hipStream_t s) {
-  static_assert(2 * pf::kTileBytes >= 8 * kWaveLds, "the waves' output rows take the tiles' place");
-  const size_t lds = 2 * pf::kTileBytes;
-  if (sync) hipLaunchKernelGGL((prefix_attention_kernel<RB, true>), dim3(a.blocks), dim3(512), lds, s, a);
-  else hipLaunchKernelGGL((prefix_attention_kernel<RB, false>), dim3(a.blocks), dim3(512), lds, s, a);
+void launch_attention(const PrefixArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(prefix_attention_kernel<RB>, dim3(a.blocks), dim3(64 * kWaves), 0, s, a);
 }
 
 }  // namespace
@@ -822,7 +861,7 @@ extern "C" int sgl_prefix_plan(int prefix_len, int batch_size, int max_tokens, i
                                sgl_prefix_plan_t* plan) {
   if (!plan) return SGL_ERR_INVALID_ARG;
   return make_plan(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads, num_kv_heads, head_dim,
-                   std::min(std::max(device_cus(), 2), 512), *plan);
+                   std::min(2 * device_cus(), 1022), *plan);
 }
 
 extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q,
@@ -869,7 +908,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   a.batch = batch_size, a.tokens = max_tokens;
   a.hq = num_qo_heads, a.hkv = num_kv_heads, a.group = num_qo_heads / num_kv_heads;
   a.prefix = p.prefix_len, a.max_qo = p.max_qo_len, a.walk_rows = p.walk_rows, a.blocks = p.num_blocks;
-  a.heads = heads_per_group(num_kv_heads), a.side = 8 / a.heads, a.rest = num_kv_heads / a.heads;
+  a.heads = heads_per_group(num_kv_heads), a.side = kWaves / a.heads, a.rest = num_kv_heads / a.heads;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.o = static_cast<uint16_t*>(o), a.o_st = o_stride_token, a.o_sh = o_stride_head;
   a.p_o = reinterpret_cast<float*>(ws + l.p_o), a.p_lse = reinterpret_cast<float*>(ws + l.p_lse);
@@ -877,13 +916,13 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int own_rows = p.max_qo_len * a.group;
   const int need = own_rows < a.walk_rows ? a.walk_rows : own_rows;
-  if (need <= 16) launch_attention<1>(a, a.heads == 8, s);
-  else launch_attention<2>(a, a.heads == 8, s);
+  if (need <= 16) launch_attention<1>(a, s);
+  else launch_attention<2>(a, s);
   st = launch_status();
   if (st != SGL_OK) return st;
   // Many pieces a row: a workgroup for each. Few: two groups of lanes a row.
   const int64_t pieces = a.walk_rows > 0 ? p.max_units
-      : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 255) / 256 * num_kv_heads) + 2;
+      : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 127) / 128 * num_kv_heads) + 2;
   const int rows_per = pieces > 16 ? 1 : 4;
   const int head_groups = (num_qo_heads + rows_per - 1) / rows_per;
   const dim3 fold(static_cast<uint32_t>(max_tokens) * head_groups);
