@@ -28,6 +28,7 @@ constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
 constexpr int kMinUnit = 16;              // shortest unit
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
+constexpr int kDepth = 1;                 // steps whose K/V rows are in flight
 constexpr int kWaves = 4;                 // waves of a workgroup, two workgroups per CU
 constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
 constexpr int kMaxWalkRows = 32;         // packed rows up to which the units walk the prefix
@@ -225,11 +226,13 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
     for (int e = 0; e < 4; ++e)
       vr[e] = ldg128_nt<true>(slot_row(vlane, __shfl(slot, 4 * j + e, kWave), ss_bytes));
   };
-  // Slots of this lane's token, and K and V, of the step at hand, the next and the one
-  // behind it.
-  const int slot0 = w.idx[min(n, len - 1)];
-  const int slot1 = w.idx[min(kStep + n, len - 1)];
-  int slot_next = slot1;
+  // Slots of this lane's token, kDepth steps' for the first K/V rows, then two steps' for
+  // the next ones.
+  int slot0[kDepth], slot[2];
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) slot0[i] = w.idx[min(i * kStep + n, len - 1)];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) slot[i] = w.idx[min((kDepth + i) * kStep + n, len - 1)];
   // Token and head of this lane's row of each block; rows past the last one read
   // its Q again and see nothing.
   const int i0 = w.row0 / G, rem = w.row0 - i0 * G;
@@ -247,9 +250,17 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
 #pragma unroll
     for (int s = 0; s < 4; ++s) q[b][s] = ldg128(qp + 32 * s);
   }
-  u32x4_t kr1[4], vr1[4];
-  load_k(slot0, kr1);
-  load_v(slot0, vr1);
+  // K before V, as in the loop, whose waits count the loads in flight: the compiler
+  // merges the two orders, and waited for V with K where they differed.
+  u32x4_t kr[kDepth][4], vr[kDepth][4];
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(slot0[i], kr[i]);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(slot0[i], vr[i]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   float m[RB], l[RB];
   f32x4_t acc[RB][8];
 #pragma unroll
@@ -260,8 +271,7 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
     for (int nb = 0; nb < 8; ++nb) acc[b][nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto step = [&](int t, u32x4_t (&kr)[4], u32x4_t (&vr)[4]) {
-    const int slot_after = w.idx[min(t + 2 * kStep + n, len - 1)];
+  auto step = [&](int t, int& slot, u32x4_t (&kr)[4], u32x4_t (&vr)[4]) {
     f32x4_t sacc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
@@ -270,7 +280,9 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
       for (int s = 0; s < 4; ++s)
         sacc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[s]), as_bf16x8(q[b][s]), sacc[b], 0, 0, 0);
     }
-    load_k(slot_next, kr);
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(slot, kr);
+    __builtin_amdgcn_sched_barrier(0);
     bf16x4_t pop[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
@@ -311,11 +323,17 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
       for (int b = 0; b < RB; ++b)
         acc[b][nb] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vop, pop[b], acc[b][nb], 0, 0, 0);
     });
-    load_v(slot_next, vr);
-    slot_next = slot_after;
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(slot, vr);
+    slot = w.idx[min(t + (kDepth + 2) * kStep + n, len - 1)];
+    __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll 1
-  for (int t = 0; t < len; t += kStep) step(t, kr1, vr1);
+  for (int t = 0; t < len; t += 2 * kStep) {
+    step(t, slot[0], kr[0], vr[0]);
+    if (t + kStep >= len) break;
+    step(t + kStep, slot[1], kr[kDepth - 1], vr[kDepth - 1]);
+  }
   // The block's output through LDS (16 rows of 32 16-byte chunks, chunk c of row n at
   // c ^ n: no bank conflicts either way), so that whole rows are stored: as they lie in
   // the accumulators a store would touch 64 lines for 1 KB (128 units of 32 rows, 8 kv
