@@ -28,6 +28,7 @@ constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
 constexpr int kMinUnit = 16;              // shortest unit
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
+constexpr int kFoldGroups = 1024;          // workgroups of the fold up to which a row has lanes of its own
 constexpr int kDepth = 1;                 // steps whose K/V rows are in flight
 constexpr int kWaves = 4;                 // waves of a workgroup, two workgroups per CU
 constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
@@ -203,11 +204,7 @@ struct Piece {
 };
 
 // One wave over a piece of at most 16 RB rows. Lane (n, j), n = lane % 16: token n (K),
-// chunk n of tokens 4 j + e (V), row n of each block (Q, S, O). Q stays in registers. The
-// code is kept short (one call, addresses once a row): a piece of a step or two runs most
-// of it once, and what it does not find in the instruction cache costs more than the
-// arithmetic (with Q in LDS and four row blocks 64 requests of 6 query tokens and 16 of
-// their own took 36 us, 16 of one query token).
+// chunk n of tokens 4 j + e (V), row n of each block (Q, S, O). Q stays in registers.
 template <int RB>
 __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* xch, int h, int lane) {
   const int n = lane & 15, j = lane >> 4;
@@ -670,128 +667,137 @@ __device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request&
   return acc * inv;
 }
 
-// Folds the pieces of each row: kSets groups of 32 lanes take them in turn, eight
-// pieces' loads in flight, and are folded through LDS; 8 / kSets heads of one token a
-// workgroup.
+// Folds the pieces of each row: kSets groups of 32 lanes take them in turn and are
+// folded through LDS; a workgroup has `iters` times 8 / kSets heads of one token. Bound by
+// instructions and the chain of dependent loads (request, its offsets, its pieces), so
+// what is a token's is worked out once for its heads, in scalar registers, with every
+// load that does not wait for another sent first.
 template <int kSets>
-__global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head_groups) {
-  constexpr int kRows = 8 / kSets;
+__global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head_groups, int iters) {
+  constexpr int kRows = 8 / kSets, kLoads = kSets == 1 ? 4 : 8;
   __shared__ int before[4];
-  __shared__ float xch[6][8][32];
-  const int t = blockIdx.x / static_cast<uint32_t>(head_groups);
-  const int lane = threadIdx.x & 63;
+  __shared__ float xch[kSets > 1 ? 6 : 1][8][32];
+  const int t = uniform(blockIdx.x / static_cast<uint32_t>(head_groups));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // The token's request: those that end at or before it are counted.
   int n = 0;
-  for (int e = threadIdx.x; e < a.batch; e += 256) n += a.qo_indptr[e + 1] <= t;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, kWave);
-  if (lane == 0) before[threadIdx.x >> 6] = n;
+  for (int at = 64 * wave; at < a.batch; at += 256) {
+    const bool done = at + lane < a.batch && a.qo_indptr[at + lane + 1] <= t;
+    n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(done));
+  }
+  const Split sp = split_of(a);
+  if (lane == 0) before[wave] = n;
   __syncthreads();
-  const int r = before[0] + before[1] + before[2] + before[3];
+  const int r = uniform(before[0] + before[1] + before[2] + before[3]);
   if (r >= a.batch || t < a.qo_indptr[0]) return;  // no request's row: left as it was
   const Request x = request_of(a, r);
-  const Split sp = split_of(a);
-  const int P = a.prefix;
-  const int c = threadIdx.x & 31, group = threadIdx.x >> 5;
-  const int set = group % kSets;
-  const int head = (blockIdx.x - t * head_groups) * kRows + group / kSets;
-  const bool head_ok = head < a.hq;
-  const int hh = head_ok ? head : a.hq - 1;
-  const int h = hh / a.group;
-  const int i = t - x.q0;
+  const int P = a.prefix, i = t - x.q0;
   const int64_t sees = static_cast<int64_t>(P) + x.kv - x.qo + i + 1;  // tokens this row sees, prefix first
-  float m = -INFINITY, l = 0.f;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   const bool folded = x.ok && sees >= P;
-  if (folded) {
-    // Prefix pieces [0, np) at p0 + k p_step, then the request's own.
-    int np = 0, ns = 0;
-    int64_t p0 = 0, s1 = 0;
-    int64_t p_step = static_cast<int64_t>(a.hkv) * a.walk_rows;
-    const int prow = (t - sp.first) * a.group + hh - h * a.group;
-    if (sp.tile_blocks > 0) {
-      const uint32_t at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
-      np = sp.shares > 0 ? sp.shares : static_cast<int>((at + sp.tiles - 1) / sp.run - at / sp.run) + 1;
-      p_step = static_cast<int64_t>(a.hkv) * sp.rows;
-      p0 = static_cast<int64_t>(h) * sp.rows + prow;
-    } else if (P > 0) {
-      np = static_cast<int>((P - 1) / sp.W) + 1;
-      p0 = static_cast<int64_t>(h) * a.walk_rows + prow;
-    }
-    if (x.kv > 0) {
-      const uint32_t own0 = sp.shared + (x.kv0 - max(a.kv_indptr[0], 0)) + (r + 1) * kRequestTokens;
-      const uint32_t u0 = own0 / sp.W;
-      ns = static_cast<int>((own0 + x.kv - 1) / sp.W - u0) + 1;
-      s1 = (a.tokens + static_cast<int64_t>(u0) * a.max_qo + i) * a.hq + hh;
-    }
-    const int64_t s0 = static_cast<int64_t>(t) * a.hq + hh, s_step = static_cast<int64_t>(a.max_qo) * a.hq;
-    constexpr int kLoads = kSets == 2 ? 4 : 8;
-    for (int k0 = set; k0 < np + ns; k0 += kLoads * kSets) {
-      f32x4_t v[kLoads];
-      float lse[kLoads];
-#pragma unroll
-      for (int e = 0; e < kLoads; ++e) {
-        const int k = min(k0 + e * kSets, np + ns - 1);
-        const int64_t row = k < np ? p0 + k * p_step : k == np ? s0 : s1 + (k - np) * s_step;
-        v[e] = *reinterpret_cast<const f32x4_t*>((k < np ? a.p_o : a.s_o) + row * kD + 4 * c);
-        lse[e] = (k < np ? a.p_lse : a.s_lse)[row];
-        if (k0 + e * kSets >= np + ns) lse[e] = -INFINITY;
-      }
-      float mn = m;
-#pragma unroll
-      for (int e = 0; e < kLoads; ++e) mn = fmaxf(mn, lse[e]);
-      const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
-      l *= alpha;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] *= alpha;
-      m = mn;
-#pragma unroll
-      for (int e = 0; e < kLoads; ++e) {
-        if (lse[e] == -INFINITY) continue;  // nothing seen there: its values do not count
-        const float w = exp2f(lse[e] - mn);
-        l += w;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += v[e][k] * w;
-      }
-    }
+  // The request's own pieces: ns of them, the first at s0 + head, the k-th behind it at s1 + k s_step + head.
+  int ns = 0;
+  int64_t s1 = 0;
+  if (x.kv > 0 && x.ok) {
+    const uint32_t own0 = sp.shared + (x.kv0 - max(uniform(a.kv_indptr[0]), 0)) + (r + 1) * kRequestTokens;
+    const uint32_t u0 = uniform(own0 / sp.W);
+    ns = uniform((own0 + x.kv - 1) / sp.W) - u0 + 1;
+    s1 = (a.tokens + static_cast<int64_t>(u0) * a.max_qo + i) * a.hq;
   }
+  const int64_t s0 = static_cast<int64_t>(t) * a.hq, s_step = static_cast<int64_t>(a.max_qo) * a.hq;
+  const int row_of_head = (t - sp.first) * a.group;
+  const int c = threadIdx.x & 31, group = threadIdx.x >> 5, set = group % kSets;
+  for (int it = 0; it < iters; ++it) {
+    const int head = ((blockIdx.x - t * head_groups) * iters + it) * kRows + group / kSets;
+    const int hh = min(head, a.hq - 1);
+    const int h = hh / a.group;
+    float m = -INFINITY, l = 0.f;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    if (folded) {
+      // Prefix pieces: np of them, p_step rows apart.
+      const int prow = row_of_head + hh - h * a.group;
+      int np = 0;
+      int64_t p0 = 0, p_step = static_cast<int64_t>(a.hkv) * a.walk_rows;
+      if (sp.tile_blocks > 0) {
+        np = sp.shares;
+        if (np == 0) {
+          const uint32_t at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
+          np = static_cast<int>((at + sp.tiles - 1) / sp.run - at / sp.run) + 1;
+        }
+        p_step = static_cast<int64_t>(a.hkv) * sp.rows;
+        p0 = static_cast<int64_t>(h) * sp.rows + prow;
+      } else if (P > 0) {
+        np = static_cast<int>((P - 1) / sp.W) + 1;
+        p0 = static_cast<int64_t>(h) * a.walk_rows + prow;
+      }
+      for (int k0 = set; k0 < np + ns; k0 += kLoads * kSets) {
+        f32x4_t v[kLoads];
+        float lse[kLoads];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) xch[k][group][c] = acc[k];
-  xch[4][group][c] = m;
-  xch[5][group][c] = l;
-  __syncthreads();
-  if (set != 0 || !head_ok) return;
-  bool again = x.ok && !folded;
-  if (!x.ok) {
-    acc = f32x4_t{NAN, NAN, NAN, NAN};
-  } else if (folded) {
+        for (int e = 0; e < kLoads; ++e) {
+          const int k = min(k0 + e * kSets, np + ns - 1);
+          const int64_t row = k < np ? p0 + k * p_step : hh + (k == np ? s0 : s1 + (k - np) * s_step);
+          v[e] = *reinterpret_cast<const f32x4_t*>((k < np ? a.p_o : a.s_o) + row * kD + 4 * c);
+          lse[e] = (k < np ? a.p_lse : a.s_lse)[row];
+          if (k0 + e * kSets >= np + ns) lse[e] = -INFINITY;
+        }
+        float mn = m;
 #pragma unroll
-    for (int e = 1; e < kSets; ++e) m = fmaxf(m, xch[4][group + e][c]);
-    l = 0.f;
-    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < kLoads; ++e) mn = fmaxf(mn, lse[e]);
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= alpha;
 #pragma unroll
-    for (int e = 0; e < kSets; ++e) {
-      const float me = xch[4][group + e][c], le = xch[5][group + e][c];
-      if (le == 0.f) continue;  // no piece with a weight
-      const float w = exp2f(me - m);
-      l += le * w;
+        for (int k = 0; k < 4; ++k) acc[k] *= alpha;
+        m = mn;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += xch[k][group + e][c] * w;
+        for (int e = 0; e < kLoads; ++e) {
+          if (lse[e] == -INFINITY) continue;  // nothing seen there: its values do not count
+          const float w = __builtin_amdgcn_exp2f(lse[e] - mn);
+          l += w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] += v[e][k] * w;
+        }
+      }
+    }
+    if constexpr (kSets > 1) {
+      if (it > 0) __syncthreads();  // the last row's values have been read
+#pragma unroll
+      for (int k = 0; k < 4; ++k) xch[k][group][c] = acc[k];
+      xch[4][group][c] = m;
+      xch[5][group][c] = l;
+      __syncthreads();
+      if (set == 0) {
+#pragma unroll
+        for (int e = 1; e < kSets; ++e) m = fmaxf(m, xch[4][group + e][c]);
+        l = 0.f;
+        acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < kSets; ++e) {
+          const float me = xch[4][group + e][c], le = xch[5][group + e][c];
+          if (le == 0.f) continue;  // no piece with a weight
+          const float w = __builtin_amdgcn_exp2f(me - m);
+          l += le * w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] += xch[k][group + e][c] * w;
+        }
+      }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] *= inv;
-    // Tokens of the request behind this row's last one may have brought in
-    // values that are not finite.
+    if (!x.ok) acc = f32x4_t{NAN, NAN, NAN, NAN};
+    // Tokens of the request behind this row's last one may have brought in values
+    // that are not finite.
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < 4; ++k) bad = bad || !(fabsf(acc[k]) < INFINITY);
     const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
-    again = i + 1 < x.qo && ((any >> (lane & 32)) & 0xffffffffull) != 0;
+    const bool again = x.ok && (!folded || (i + 1 < x.qo && ((any >> (lane & 32)) & 0xffffffffull) != 0));
+    if (set == 0 && head < a.hq) {
+      if (again) acc = plain_row(a, x, t, head, sees, c);
+      *reinterpret_cast<u32x2_t*>(a.o + t * a.o_st + head * a.o_sh + 4 * c) =
+          u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+    }
   }
-  if (again) acc = plain_row(a, x, t, head, sees, c);
-  *reinterpret_cast<u32x2_t*>(a.o + t * a.o_st + head * a.o_sh + 4 * c) =
-      u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
 }
 
 int device_cus() {
@@ -938,13 +944,18 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   else launch_attention<2>(a, s);
   st = launch_status();
   if (st != SGL_OK) return st;
-  // Many pieces a row: a workgroup for each. Few: two groups of lanes a row.
+  // Many pieces a row: a workgroup for each. Few: 32 lanes a row, and of many rows
+  // several a lane group (2,048 workgroups of four heads each took 12.5 us for 256 tokens
+  // of 32 heads).
   const int64_t pieces = a.walk_rows > 0 ? p.max_units
-      : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 127) / 128 * num_kv_heads) + 2;
-  const int rows_per = pieces > 16 ? 1 : 4;
-  const int head_groups = (num_qo_heads + rows_per - 1) / rows_per;
+      : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 127) / 128 * num_kv_heads) / 2 + 2;
+  const int rows_per = pieces > 16 ? 1 : 8;
+  const int all_iters = (num_qo_heads + rows_per - 1) / rows_per;
+  int iters = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(max_tokens) * all_iters + kFoldGroups - 1) / kFoldGroups, all_iters));
+  iters = std::max(iters, 1);
+  const int head_groups = (all_iters + iters - 1) / iters;
   const dim3 fold(static_cast<uint32_t>(max_tokens) * head_groups);
-  if (rows_per == 1) hipLaunchKernelGGL(prefix_fold_kernel<8>, fold, dim3(256), 0, s, a, head_groups);
-  else hipLaunchKernelGGL(prefix_fold_kernel<2>, fold, dim3(256), 0, s, a, head_groups);
+  if (rows_per == 1) hipLaunchKernelGGL(prefix_fold_kernel<8>, fold, dim3(256), 0, s, a, head_groups, iters);
+  else hipLaunchKernelGGL(prefix_fold_kernel<1>, fold, dim3(256), 0, s, a, head_groups, iters);
   return launch_status();
 }
