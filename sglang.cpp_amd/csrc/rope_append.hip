@@ -177,8 +177,10 @@ __global__ void __launch_bounds__(256) rope_append_elements_kernel(AppendArgs a)
 // The token is the same for a whole workgroup (scalar slot and position loads); its
 // rows' jobs take blocks_per_token workgroups of a width that leaves few threads
 // without a job. kTokens tokens a thread, their loads in flight together. Bound by
-// the bytes of the rows, read once and written once: non-temporal.
-constexpr int kTokens = 2;
+// the bytes of the rows, read once and written once: non-temporal. 32q/8kv, head_dim
+// 128, us with two tokens a thread and with one: 2,047 tokens (50 MB, from and to the
+// last-level cache) 9.8 and 10.6, 4,096 20.3 and 18.4, 16,384 (403 MB) 72 and 67.
+constexpr int64_t kOneTokenBytes = 64ll << 20;  // rows read and written, from which a thread has one token
 
 template <int DT>
 __device__ __forceinline__ void rotate_half(u32x4_t& x, u32x4_t& y, const float* c, const float* s) {
@@ -207,7 +209,7 @@ __device__ __forceinline__ void rotate_pairs(u32x4_t& x, const f32x4_t& c, const
 }
 
 // J: jobs of a row (head_dim / 16), 0: read from the arguments.
-template <int DT, bool kInterleaved, int J>
+template <int DT, bool kInterleaved, int J, int kTokens>
 __global__ void __launch_bounds__(512) rope_append_kernel(AppendArgs a, int blocks_per_token) {
   const int jobs = J ? J : a.d / 16;
   const uint32_t group = blockIdx.x / static_cast<uint32_t>(blocks_per_token);
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(512) rope_append_kernel(AppendArgs a, int bloc
   }
 }
 
-template <int DT, bool kInterleaved>
+template <int DT, bool kInterleaved, int kTokens>
 void launch_chunks(const AppendArgs& a, hipStream_t s) {
   const int jobs = a.d / 16;
   const int64_t items = (static_cast<int64_t>(a.hq) + a.hk + a.hv) * jobs;
@@ -299,9 +301,19 @@ void launch_chunks(const AppendArgs& a, hipStream_t s) {
   const dim3 block(64 * waves);
   const int bpt = static_cast<int>(per_token);
   switch (jobs) {
-    case 4: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 4>), grid, block, 0, s, a, bpt); break;
-    case 8: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 8>), grid, block, 0, s, a, bpt); break;
-    default: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 0>), grid, block, 0, s, a, bpt);
+    case 4: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 4, kTokens>), grid, block, 0, s, a, bpt); break;
+    case 8: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 8, kTokens>), grid, block, 0, s, a, bpt); break;
+    default: hipLaunchKernelGGL((rope_append_kernel<DT, kInterleaved, 0, kTokens>), grid, block, 0, s, a, bpt);
+  }
+}
+
+template <int DT>
+void launch_chunks(const AppendArgs& a, bool interleaved, hipStream_t s) {
+  const int64_t bytes = a.tokens * (static_cast<int64_t>(a.hq) + a.hk + a.hv) * a.d * 4;
+  if (bytes >= kOneTokenBytes) {
+    if (interleaved) launch_chunks<DT, true, 1>(a, s); else launch_chunks<DT, false, 1>(a, s);
+  } else {
+    if (interleaved) launch_chunks<DT, true, 2>(a, s); else launch_chunks<DT, false, 2>(a, s);
   }
 }
 
@@ -450,12 +462,9 @@ extern "C" int sgl_rope_append(const sgl_rope_append_t* args, void* stream) {
       chunked(a.q_out, a.qo_st, a.qo_sh) && chunked(a.k, a.k_st, a.k_sh) &&
       chunked(a.v, a.v_st, a.v_sh) && chunked(a.k_cache, a.kv_ss, a.kv_sh) &&
       chunked(a.v_cache, a.kv_ss, a.kv_sh) && aligned16(a.cos) && aligned16(a.sin) &&
-      (a.tokens / kTokens + 1) * (rows * (a.d / 16) / 128 + 1) < 0x7fffffff) {
-    if (x.dtype == SGL_DTYPE_BF16) {
-      if (il) launch_chunks<SGL_DTYPE_BF16, true>(a, s); else launch_chunks<SGL_DTYPE_BF16, false>(a, s);
-    } else {
-      if (il) launch_chunks<SGL_DTYPE_F16, true>(a, s); else launch_chunks<SGL_DTYPE_F16, false>(a, s);
-    }
+      a.tokens * (rows * (a.d / 16) / 128 + 1) < 0x7fffffff) {
+    if (x.dtype == SGL_DTYPE_BF16) launch_chunks<SGL_DTYPE_BF16>(a, il, s);
+    else launch_chunks<SGL_DTYPE_F16>(a, il, s);
     return launch_status();
   }
   const int64_t blocks = blocks_for(a.tokens * per_token, 256);

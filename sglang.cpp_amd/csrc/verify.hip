@@ -27,7 +27,7 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kPer = 16;                    // elements of a thread
 constexpr int kSlice = kThreads * kPer;     // elements of a slice
 constexpr int kLines = kPer / 4;            // groups of 4 consecutive elements of a thread
-constexpr int64_t kSingles = 1024;          // slices of a launch up to which each is a workgroup
+constexpr int64_t kSingles = 4096;          // slices of a launch up to which each is a workgroup
 
 struct VerifyArgs {
   const float* target;
@@ -109,7 +109,8 @@ __device__ __forceinline__ void load_slice(const float* row, int s, int vocab, i
   if ((s + 1) * kSlice <= vocab) {  // a whole slice
 #pragma unroll
     for (int g = 0; g < kLines; ++g) {
-      const f32x4_any_t v = *reinterpret_cast<const f32x4_any_t*>(row + e0 + g * 4 * kThreads);
+      const f32x4_any_t v =
+          __builtin_nontemporal_load(reinterpret_cast<const f32x4_any_t*>(row + e0 + g * 4 * kThreads));
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[4 * g + i] = v[i];
     }

@@ -224,3 +224,19 @@ def test_append_far_slots_on_a_side_stream_and_in_a_graph(dev):
                                  x["pos"], x["loc"])
         assert torch.equal(out, eager) and torch.equal(vc[rows], x["v"])
         assert torch.equal(kc[rows], x["kc"][x["loc"].long()])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_many_tokens(dev, interleaved):
+    """A batch whose rows pass the size from which a thread has one token: the bits of the
+    same call on its parts."""
+    T = 4099
+    x = make(dev, T, 32, 8, 128, 128, "bf16", 6)
+    kc, vc = x["kc"].clone(), x["vc"].clone()
+    q = capi.rope_append(x["q"], x["k"], x["v"], x["kc"], x["vc"], x["cos"], x["sin"], x["pos"],
+                         x["loc"], interleaved)
+    for a, b in ((0, 1000), (1000, 1001), (1001, T)):
+        part = capi.rope_append(*(x[k][a:b] for k in ("q", "k", "v")), kc, vc, x["cos"], x["sin"],
+                                x["pos"][a:b], x["loc"][a:b], interleaved)
+        assert torch.equal(part, q[a:b])
+    assert torch.equal(kc, x["kc"]) and torch.equal(vc, x["vc"])
