@@ -194,19 +194,6 @@ PYBIND11_MODULE(sgl_backend, m) {
           fused_qk_rmsnorm_inplace_3d_strided(q, k, qn, kn);
         });
 
-  py::class_<RotaryEmbedding, std::shared_ptr<RotaryEmbedding>>(m, "RotaryEmbedding")
-      .def(py::init([](int head_size, int rotary_dim, int max_pos, float base, int device) {
-             return std::make_shared<RotaryEmbedding>(head_size, rotary_dim, max_pos, base,
-                                                      cuda(device));
-           }),
-           py::arg("head_size"), py::arg("rotary_dim"), py::arg("max_position_embeddings"),
-           py::arg("base"), py::arg("device") = 0)
-      .def("forward_inplace",
-           [](const RotaryEmbedding& r, const torch::Tensor& pos, torch::Tensor q,
-              torch::Tensor k) { r.forward_inplace(pos, q, k); })
-      .def("cos_cache", &RotaryEmbedding::cos_cache)
-      .def("sin_cache", &RotaryEmbedding::sin_cache);
-
   py::class_<RopeScaling>(m, "RopeScaling")
       .def(py::init([](const std::string& kind, double factor, int original, double beta_fast,
                        double beta_slow, double low, double high, double attention) {
@@ -216,6 +203,27 @@ PYBIND11_MODULE(sgl_backend, m) {
            py::arg("beta_fast") = 32.0, py::arg("beta_slow") = 1.0,
            py::arg("low_freq_factor") = 1.0, py::arg("high_freq_factor") = 4.0,
            py::arg("attention_factor") = 0.0);
+  py::class_<RotaryEmbedding, std::shared_ptr<RotaryEmbedding>>(m, "RotaryEmbedding")
+      .def(py::init([](int head_size, int rotary_dim, int max_pos, float base, int device) {
+             return std::make_shared<RotaryEmbedding>(head_size, rotary_dim, max_pos, base,
+                                                      cuda(device));
+           }),
+           py::arg("head_size"), py::arg("rotary_dim"), py::arg("max_position_embeddings"),
+           py::arg("base"), py::arg("device") = 0)
+      .def(py::init([](int head_size, int rotary_dim, int max_pos, double base,
+                       const RopeScaling& scaling, bool interleaved, int device) {
+             return std::make_shared<RotaryEmbedding>(head_size, rotary_dim, max_pos, base,
+                                                      cuda(device), scaling, interleaved);
+           }),
+           py::arg("head_size"), py::arg("rotary_dim"), py::arg("max_position_embeddings"),
+           py::arg("base"), py::arg("scaling"), py::arg("interleaved") = false,
+           py::arg("device") = 0)
+      .def("forward_inplace",
+           [](const RotaryEmbedding& r, const torch::Tensor& pos, torch::Tensor q,
+              torch::Tensor k) { r.forward_inplace(pos, q, k); })
+      .def("cos_cache", &RotaryEmbedding::cos_cache)
+      .def("sin_cache", &RotaryEmbedding::sin_cache);
+
   m.def("rope_scaled_cache",
         [](int64_t max_pos, int rotary_dim, double base, const RopeScaling& scaling, int device) {
           return rope_scaled_cache(max_pos, rotary_dim, base, scaling, cuda(device));

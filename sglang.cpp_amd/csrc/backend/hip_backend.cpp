@@ -1203,35 +1203,6 @@ void fused_qk_rmsnorm_inplace_3d_strided(torch::Tensor& q, torch::Tensor& k, con
             "sgl_qk_rmsnorm");
 }
 
-RotaryEmbedding::RotaryEmbedding(int head_size, int rotary_dim, int max_position_embeddings,
-                                 float base, torch::Device device)
-    : head_size_(head_size), rotary_dim_(rotary_dim) {
-  TORCH_CHECK(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= head_size,
-              "rotary_dim must be even and <= head_size");
-  auto opts = torch::TensorOptions().dtype(torch::kFloat32).device(device);
-  cos_cache_ = torch::empty({max_position_embeddings, rotary_dim / 2}, opts);
-  sin_cache_ = torch::empty_like(cos_cache_);
-  check_sgl(sgl_rope_cos_sin_cache(cos_cache_.data_ptr<float>(), sin_cache_.data_ptr<float>(),
-                                   max_position_embeddings, rotary_dim, base,
-                                   current_stream(device)),
-            "sgl_rope_cos_sin_cache");
-}
-
-void RotaryEmbedding::forward_inplace(const torch::Tensor& positions, torch::Tensor& query,
-                                      torch::Tensor& key) const {
-  TORCH_CHECK(query.is_cuda() && key.is_cuda() && positions.is_cuda(),
-              "Inputs must be device tensors");
-  TORCH_CHECK(positions.scalar_type() == torch::kInt32, "positions must be int32");
-  const int dt = half_dtype(query, "query");
-  check_same_dtype(query, key, "query and key");
-  check_sgl(sgl_rope(query.data_ptr(), key.data_ptr(), cos_cache_.data_ptr<float>(),
-                     sin_cache_.data_ptr<float>(), positions.data_ptr<int32_t>(),
-                     positions.size(0), query.size(1), key.size(1), rotary_dim_, query.size(2),
-                     cos_cache_.size(1), query.stride(0), query.stride(1), key.stride(0),
-                     key.stride(1), dt, current_stream(query.device())),
-            "sgl_rope");
-}
-
 namespace {
 void check_i32(const torch::Tensor& t, const torch::Device& dev, const char* what) {
   TORCH_CHECK(t.defined() && t.device() == dev && t.scalar_type() == torch::kInt32 && t.dim() == 1 &&
@@ -1346,9 +1317,54 @@ torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const 
   return out;
 }
 
+RotaryEmbedding::RotaryEmbedding(int head_size, int rotary_dim, int max_position_embeddings,
+                                 float base, torch::Device device)
+    : head_size_(head_size), rotary_dim_(rotary_dim) {
+  TORCH_CHECK(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= head_size,
+              "rotary_dim must be even and <= head_size");
+  auto opts = torch::TensorOptions().dtype(torch::kFloat32).device(device);
+  cos_cache_ = torch::empty({max_position_embeddings, rotary_dim / 2}, opts);
+  sin_cache_ = torch::empty_like(cos_cache_);
+  check_sgl(sgl_rope_cos_sin_cache(cos_cache_.data_ptr<float>(), sin_cache_.data_ptr<float>(),
+                                   max_position_embeddings, rotary_dim, base,
+                                   current_stream(device)),
+            "sgl_rope_cos_sin_cache");
+}
+
+RotaryEmbedding::RotaryEmbedding(int head_size, int rotary_dim, int max_position_embeddings,
+                                 double base, torch::Device device, const RopeScaling& scaling,
+                                 bool interleaved)
+    : head_size_(head_size), rotary_dim_(rotary_dim), interleaved_(interleaved) {
+  TORCH_CHECK(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= head_size,
+              "rotary_dim must be even and <= head_size");
+  std::tie(cos_cache_, sin_cache_) =
+      rope_scaled_cache(max_position_embeddings, rotary_dim, base, scaling, device);
+}
+
+void RotaryEmbedding::forward_inplace(const torch::Tensor& positions, torch::Tensor& query,
+                                      torch::Tensor& key) const {
+  TORCH_CHECK(query.is_cuda() && key.is_cuda() && positions.is_cuda(),
+              "Inputs must be device tensors");
+  TORCH_CHECK(positions.scalar_type() == torch::kInt32, "positions must be int32");
+  const int dt = half_dtype(query, "query");
+  check_same_dtype(query, key, "query and key");
+  if (interleaved_) {
+    rope_append(query, key, torch::Tensor(), key, torch::Tensor(), cos_cache_, sin_cache_, positions,
+                torch::Tensor(), true, query);
+    return;
+  }
+  check_sgl(sgl_rope(query.data_ptr(), key.data_ptr(), cos_cache_.data_ptr<float>(),
+                     sin_cache_.data_ptr<float>(), positions.data_ptr<int32_t>(),
+                     positions.size(0), query.size(1), key.size(1), rotary_dim_, query.size(2),
+                     cos_cache_.size(1), query.stride(0), query.stride(1), key.stride(0),
+                     key.stride(1), dt, current_stream(query.device())),
+            "sgl_rope");
+}
+
 PrefixAttention::PrefixAttention(int prefix_len, int batch_size, int max_tokens, int max_qo_len,
                                  int num_qo_heads, int num_kv_heads, int head_dim,
-                                 torch::Device device) {
+                                 torch::Device device)
+    : made_on_(at::hip::getCurrentHIPStream(device.index()).unwrap()) {
   TORCH_CHECK(device.is_cuda(), "PrefixAttention runs on a HIP device");
   const c10::DeviceGuard guard(device);
   check_sgl(sgl_prefix_plan(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads,
@@ -1386,6 +1402,11 @@ torch::Tensor PrefixAttention::forward(const torch::Tensor& q, const torch::Tens
   if (out.defined()) check_heads(out, q, "out");
   TORCH_CHECK(!out.defined() || out.sizes() == q.sizes(), "out must have q's shape");
   auto o = out.defined() ? out : torch::empty(q.sizes(), q.options());
+  const auto stream = at::hip::getCurrentHIPStream(q.device().index());
+  // Freed only once the work queued here is done, also where that is not the stream
+  // it was allocated on.
+  if (stream.unwrap() != made_on_ && workspace_.numel() > 0)
+    c10::hip::HIPCachingAllocator::recordStream(workspace_.storage().data_ptr(), stream);
   const double scale = sm_scale.value_or(1.0 / std::sqrt(static_cast<double>(q.size(2))));
   check_sgl(sgl_prefix_attention(
                 &plan_, q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -1465,7 +1486,6 @@ AttentionLayer::AttentionLayer(int layer_id, int num_qo_heads, int num_kv_heads,
   TORCH_CHECK(backend_ && rotary_, "AttentionLayer needs a backend and a rotary embedding");
   TORCH_CHECK(static_cast<bool>(q_norm_) == static_cast<bool>(k_norm_),
               "the fused pass needs both q and k norms or neither");
-  TORCH_CHECK(rotary_->rotary_dim() == head_dim, "the fused pass uses full-width rotary");
 }
 
 torch::Tensor AttentionLayer::forward(const torch::Tensor& qkv, const torch::Tensor& positions,
@@ -1482,14 +1502,25 @@ torch::Tensor AttentionLayer::forward(const torch::Tensor& qkv, const torch::Ten
               "positions and out_loc must be int32 for the fused pass");
   TORCH_CHECK(batch.out_loc.size(0) == qkv.size(0) && positions.size(0) == qkv.size(0),
               "positions and out_loc need one entry per token");
+  auto kc = backend_->kv_cache()->k_cache(layer_id_);
+  auto vc = backend_->kv_cache()->v_cache(layer_id_);
+  if (rotary_->interleaved() || rotary_->rotary_dim() != head_dim_) {
+    auto heads = [&](int first, int count) {
+      return qkv.narrow(1, first * head_dim_, count * head_dim_).view({-1, count, head_dim_});
+    };
+    auto q = heads(0, num_qo_heads_), k = heads(num_qo_heads_, num_kv_heads_);
+    if (q_norm_) fused_qk_rmsnorm_inplace_3d_strided(q, k, *q_norm_, *k_norm_);
+    rope_append(q, k, heads(num_qo_heads_ + num_kv_heads_, num_kv_heads_), kc, vc,
+                rotary_->cos_cache(), rotary_->sin_cache(), positions, batch.out_loc,
+                rotary_->interleaved(), q);
+    return backend_->attend(q, layer_id_, batch);
+  }
   if (num_qo_heads_ == backend_->num_qo_heads() && num_kv_heads_ == backend_->num_kv_heads() &&
       head_dim_ == backend_->head_dim() && backend_->decode_layer_fits(qkv, batch))
     return backend_->decode_layer(qkv, positions, q_norm_ ? q_norm_->weight.data_ptr() : nullptr,
                                   k_norm_ ? k_norm_->weight.data_ptr() : nullptr,
                                   q_norm_ ? q_norm_->eps() : 0.f, rotary_->cos_cache(),
                                   rotary_->sin_cache(), layer_id_, batch);
-  auto kc = backend_->kv_cache()->k_cache(layer_id_);
-  auto vc = backend_->kv_cache()->v_cache(layer_id_);
   check_sgl(sgl_fused_qknorm_rope_store(
                 qkv.data_ptr(), qkv.stride(0), kc.data_ptr(), vc.data_ptr(),
                 q_norm_ ? q_norm_->weight.data_ptr() : nullptr,

@@ -285,23 +285,6 @@ FlashInferSamplingResult sample_from_logits(const torch::Tensor& logits,
                                             const torch::Tensor& uniform_samples,
                                             const torch::Tensor& top_k, const torch::Tensor& top_p);
 
-// NeoX RoPE with a half-width fp32 cos/sin cache built on the device
-// (rotary_embedding.cu:75-94 builds the same table with LibTorch-CPU ops).
-class RotaryEmbedding {
- public:
-  RotaryEmbedding(int head_size, int rotary_dim, int max_position_embeddings, float base,
-                  torch::Device device);
-  void forward_inplace(const torch::Tensor& positions, torch::Tensor& query,
-                       torch::Tensor& key) const;
-  const torch::Tensor& cos_cache() const { return cos_cache_; }
-  const torch::Tensor& sin_cache() const { return sin_cache_; }
-  int rotary_dim() const { return rotary_dim_; }
-
- private:
-  int head_size_, rotary_dim_;
-  torch::Tensor cos_cache_, sin_cache_;
-};
-
 // A rotary embedding scaled for long contexts (sgl_rope_scaling_t): kind is
 // "none", "linear", "ntk", "yarn" or "bands".
 struct RopeScaling {
@@ -311,6 +294,29 @@ struct RopeScaling {
   double beta_fast = 32.0, beta_slow = 1.0;
   double low_freq_factor = 1.0, high_freq_factor = 4.0;
   double attention_factor = 0.0;
+};
+
+// RoPE with a half-width fp32 cos/sin cache built on the device
+// (rotary_embedding.cu:75-94 builds the same table with LibTorch-CPU ops).
+class RotaryEmbedding {
+ public:
+  RotaryEmbedding(int head_size, int rotary_dim, int max_position_embeddings, float base,
+                  torch::Device device);
+  // Scaled for long contexts (rope_scaled_cache), and with interleaved the pairs
+  // (x[2 i], x[2 i + 1]) instead of (x[i], x[i + rotary_dim / 2]).
+  RotaryEmbedding(int head_size, int rotary_dim, int max_position_embeddings, double base,
+                  torch::Device device, const RopeScaling& scaling, bool interleaved);
+  void forward_inplace(const torch::Tensor& positions, torch::Tensor& query,
+                       torch::Tensor& key) const;
+  const torch::Tensor& cos_cache() const { return cos_cache_; }
+  const torch::Tensor& sin_cache() const { return sin_cache_; }
+  int rotary_dim() const { return rotary_dim_; }
+  bool interleaved() const { return interleaved_; }
+
+ private:
+  int head_size_, rotary_dim_;
+  bool interleaved_ = false;
+  torch::Tensor cos_cache_, sin_cache_;
 };
 
 // (cos, sin) tables of a scaled rotary embedding, fp32 [max_pos, rotary_dim / 2],
@@ -330,8 +336,8 @@ torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const 
                           bool interleaved, const torch::Tensor& q_out);
 
 // Attention of a batch behind a shared prefix (sgl_prefix_attention): the plan and
-// its workspace, which the calls of one object share (they must be stream-ordered,
-// graphs captured from it among them).
+// its workspace, which the calls of one object share (they must be stream-ordered, the
+// replays of graphs captured from it among them, and it lives as long as those).
 class PrefixAttention {
  public:
   PrefixAttention(int prefix_len, int batch_size, int max_tokens, int max_qo_len, int num_qo_heads,
@@ -348,6 +354,7 @@ class PrefixAttention {
  private:
   sgl_prefix_plan_t plan_{};
   torch::Tensor workspace_;
+  c10::Stream made_on_;  // the stream the workspace was allocated on
 };
 
 // Verification of drafted tokens (sgl_verify_drafts): (tokens [drafts + batch],
@@ -358,7 +365,8 @@ std::pair<torch::Tensor, torch::Tensor> verify_drafts(
     const torch::Tensor& accept_uniform, const torch::Tensor& sample_uniform);
 
 // qkv [T, (Hq + 2 Hkv) D] -> o [T, Hq D]: qk-norm, RoPE and the KV store in
-// one fused pass, then paged attention (attention_layer.cc:17-51).
+// one fused pass, then paged attention (attention_layer.cc:17-51). A rotary embedding
+// of part of the head or of interleaved pairs takes the norm in place, then rope_append.
 class AttentionLayer {
  public:
   AttentionLayer(int layer_id, int num_qo_heads, int num_kv_heads, int head_dim,

@@ -29,7 +29,6 @@ constexpr int kStep = 16;                 // tokens a step
 constexpr int kMinUnit = 16;              // shortest unit
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
 constexpr int kFoldGroups = 1024;          // workgroups of the fold up to which a row has lanes of its own
-constexpr int kDepth = 1;                 // steps whose K/V rows are in flight
 constexpr int kWaves = 4;                 // waves of a workgroup, two workgroups per CU
 constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
 constexpr int kMaxWalkRows = 32;         // packed rows up to which the units walk the prefix
@@ -82,7 +81,7 @@ struct Split {
 
 // What a tile takes on one workgroup, and a token of a kv head, ns.
 constexpr uint32_t kTileNs = 1400;
-constexpr uint32_t kTokenNs = 24;
+constexpr uint32_t kTokenNs = 16;
 // A request counts as this many tokens more in the units' stream: the loads that lead
 // to its first step, about 3.4 us (a unit that took eight requests of one token each was
 // 28 us behind the others).
@@ -207,8 +206,10 @@ struct Piece {
 // chunk n of tokens 4 j + e (V), row n of each block (Q, S, O). Q stays in registers.
 template <int RB>
 __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* xch, int h, int lane) {
+  // Steps whose K/V rows are in flight: two where the registers hold them.
+  constexpr int kDepth = RB == 1 ? 2 : 1;
   const int n = lane & 15, j = lane >> 4;
-  const int G = a.group, len = w.len;
+  const int G = a.group, len = uniform(w.len), rows = uniform(w.rows);
   const uint32_t ss_bytes = static_cast<uint32_t>(a.kv_ss * 2);
   const char* klane = reinterpret_cast<const char*>(a.kc + h * a.kv_sh + 8 * j);
   const char* vlane = reinterpret_cast<const char*>(a.vc + h * a.kv_sh + 8 * n);
@@ -238,11 +239,11 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
   u32x4_t q[RB][4];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    const int x = min(16 * b + n, w.rows - 1) + rem;
+    const int x = min(16 * b + n, rows - 1) + rem;
     const int d = static_cast<int>(static_cast<uint32_t>(x) * inv_g >> 16);
     tok[b] = i0 + d;
     head[b] = h * G + (x - d * G);
-    sees[b] = 16 * b + n < w.rows ? min(w.sees0 + tok[b], len) : 0;
+    sees[b] = 16 * b + n < rows ? min(w.sees0 + tok[b], len) : 0;
     const uint16_t* qp = a.q + (w.tok0 + tok[b]) * a.q_st + head[b] * a.q_sh + 8 * j;
 #pragma unroll
     for (int s = 0; s < 4; ++s) q[b][s] = ldg128(qp + 32 * s);
@@ -325,12 +326,15 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
     slot = w.idx[min(t + (kDepth + 2) * kStep + n, len - 1)];
     __builtin_amdgcn_sched_barrier(0);
   };
+  // Pairs of steps and one alone: with a way out between the two of a pair the compiler
+  // takes the next pair to follow the first directly and waits for every load.
+  int t = 0;
 #pragma unroll 1
-  for (int t = 0; t < len; t += 2 * kStep) {
+  for (; t + kStep < len; t += 2 * kStep) {
     step(t, slot[0], kr[0], vr[0]);
-    if (t + kStep >= len) break;
     step(t + kStep, slot[1], kr[kDepth - 1], vr[kDepth - 1]);
   }
+  if (t < len) step(t, slot[0], kr[0], vr[0]);
   // The block's output through LDS (16 rows of 32 16-byte chunks, chunk c of row n at
   // c ^ n: no bank conflicts either way), so that whole rows are stored: as they lie in
   // the accumulators a store would touch 64 lines for 1 KB (128 units of 32 rows, 8 kv
@@ -338,7 +342,7 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
   f32x4_t* xr = reinterpret_cast<f32x4_t*>(xch);
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    if (16 * b >= w.rows) break;
+    if (16 * b >= rows) break;
     const float sum = sum_xor32(sum_xor16(l[b]));
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // a NaN sum stays one
     // acc[nb][c] holds d = 32 j + 8 c + nb.
@@ -351,14 +355,14 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
       xr[32 * n + ((8 * j + 2 * c + 1) ^ n)] = hi;
     }
     wave_lds_sync();
-    if (j == 0 && 16 * b + n < w.rows)
+    if (j == 0 && 16 * b + n < rows)
       w.lse[w.by_token ? (w.out0 + tok[b]) * a.hq + head[b] : w.out0 + 16 * b + n] =
           sum == 0.f ? -INFINITY : m[b] + log2f(sum);
     const int c = lane & 31;
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
       const int x = 2 * it + (lane >> 5), y = 16 * b + x + rem;
-      if (16 * b + x >= w.rows) break;
+      if (16 * b + x >= rows) break;
       const int d = static_cast<int>(static_cast<uint32_t>(y) * inv_g >> 16);
       const int64_t row = w.by_token ? (w.out0 + i0 + d) * a.hq + (h * G + y - d * G) : w.out0 + 16 * b + x;
       __builtin_nontemporal_store(xr[32 * x + (c ^ x)], reinterpret_cast<f32x4_t*>(w.o + row * kD + 4 * c));
