@@ -1505,6 +1505,10 @@ torch::Tensor AttentionLayer::forward(const torch::Tensor& qkv, const torch::Ten
   auto kc = backend_->kv_cache()->k_cache(layer_id_);
   auto vc = backend_->kv_cache()->v_cache(layer_id_);
   if (rotary_->interleaved() || rotary_->rotary_dim() != head_dim_) {
+    // Refused before the pool is written, as attend would behind it.
+    TORCH_CHECK(num_qo_heads_ == backend_->num_qo_heads() && num_kv_heads_ == backend_->num_kv_heads() &&
+                    head_dim_ == backend_->head_dim(),
+                "AttentionLayer: num_qo_heads, num_kv_heads and head_dim must be the backend's");
     auto heads = [&](int first, int count) {
       return qkv.narrow(1, first * head_dim_, count * head_dim_).view({-1, count, head_dim_});
     };

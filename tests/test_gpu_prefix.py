@@ -236,3 +236,30 @@ def test_captured_steps_share_a_workspace(dev):
             assert torch.equal(o, want)
             check(other, run(other))
         check(x, outs[0])
+
+
+@pytest.mark.parametrize("B,qo,hq,hkv,P,own", [
+    (9, 1, 32, 8, 65, 3),        # 36 rows: the smallest batch whose prefix has workgroups of its own
+    (33, 1, 32, 8, 640, 1),      # one row more than a row tile holds
+    (65, 1, 32, 8, 63, 20),
+    (257, 1, 16, 4, 1025, 2),
+    (100, 8, 16, 2, 129, 9),     # 6,400 rows a kv head
+    (300, 4, 64, 1, 130, 4),     # 76,800: more row tiles than workgroups
+    (40, 1, 600, 600, 70, 2),    # more kv heads than workgroups for the prefix
+    (45, 1, 39, 13, 200, 5),
+])
+def test_many_rows(dev, B, qo, hq, hkv, P, own):
+    x = make(dev, P, [own + r % 3 for r in range(B)], [qo - r % qo for r in range(B)], hq, hkv, B)
+    check(x, run(x))
+    check(x, run(x, plan_of(x, B=B + 7, T=x["T"] + 300, max_qo=qo + 3)))  # a plan for more of everything
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_drawn_shapes(dev, seed):
+    rng = np.random.default_rng(seed)
+    hq, hkv = [(16, 8), (32, 8), (32, 4), (8, 8), (24, 3), (20, 5)][seed % 6]
+    B = int(rng.integers(1, 60))
+    qo = rng.integers(0, int(rng.choice([2, 5, 12])), B)
+    kv = rng.integers(0, int(rng.choice([4, 80, 700])), B) + qo
+    x = make(dev, int(rng.integers(0, 3000)), kv, qo, hq, hkv, 500 + seed)
+    check(x, run(x))

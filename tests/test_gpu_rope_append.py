@@ -32,8 +32,8 @@ def be():
 @pytest.mark.parametrize("max_pos,rotary", [(1, 2), (7, 6), (1000, 64), (513, 96), (2049, 128),
                                             (33, 512), (5, 508)])
 def test_scaled_table(dev, kind, extra, max_pos, rotary):
-    if kind == "ntk" and rotary == 2:
-        pytest.skip("refused: its exponent has no value")
+    if kind == "ntk":
+        rotary += 2 * (rotary == 2)  # two pairs at least: of one the exponent has no value
     factor, original = 4.0, 500
     sc = capi.rope_scaling(kind, factor, original, **extra)
     cos, sin = capi.rope_scaled_cache(max_pos, rotary, 10000.0, dev, sc)
