@@ -951,7 +951,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   // Many pieces a row: a workgroup for each. Few: 32 lanes a row, and of many rows
   // several a lane group (2,048 workgroups of four heads each took 12.5 us for 256 tokens
   // of 32 heads).
-  const int64_t pieces = a.walk_rows > 0 ? p.max_units
+  const int64_t pieces = a.prefix == 0 ? 2 : a.walk_rows > 0 ? p.max_units
       : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 127) / 128 * num_kv_heads) / 2 + 2;
   const int rows_per = pieces > 16 ? 1 : 8;
   const int all_iters = (num_qo_heads + rows_per - 1) / rows_per;
