@@ -261,7 +261,7 @@ int sgl_rope_scaled_cache(float* cos_cache, float* sin_cache, int64_t max_pos, i
  * q_out may be q (same strides) and the cache rows k's own (rotation in place); other
  * overlaps are the caller's error. A token whose slot is outside [0, num_slots) (padding)
  * is not appended; one whose position is outside [0, max_pos) gets NaN in the rotated
- * elements. Tokens with the same slot: which of them it then holds is open. out_loc NULL:
+ * elements. A slot listed for several tokens then holds parts of any of them. out_loc NULL:
  * token t goes to slot t. v and v_cache both NULL: no v. No q with num_qo_heads 0, no k
  * and v with num_kv_heads 0.
  * Replaces: RotaryEmbedding::forward_inplace, then MHAKVCache::store_kv
@@ -552,16 +552,22 @@ int sgl_paged_mixed(const sgl_decode_plan_t* plan, const void* q,
  * i sees kv j with j <= i + kv_len - qo_len, kv_len = prefix_len + own length: the
  * result of sgl_paged_prefill over the joined sequences (of sgl_paged_decode for one
  * query token). A row that sees nothing is zero. K and V of tokens a row does not see
- * never reach it, whatever they hold.
+ * never reach it, whatever they hold. Rows that see less than the prefix (a request with
+ * fewer own tokens than query tokens) are computed one by one: right, not fast.
  *   sgl_prefix_plan: host plan for up to batch_size requests with up to max_tokens query
  *     tokens together (max_qo_len of one request at most SGL_PREFIX_MAX_QO). It does not
  *     depend on the requests' own lengths, so it serves every step of a batch (graph
- *     capture and replay) behind a prefix of prefix_len.
+ *     capture and replay) behind a prefix of prefix_len. Up to 2^29 tokens of prefix,
+ *     2^25 requests, 2^24 - 1 query tokens, 2^30 of them times the heads of a kv head, 2^31
+ *     times num_qo_heads; and the 64-token tiles of the prefix times the 128-row tiles of
+ *     the query tokens times num_kv_heads below 2^31.
  *   sgl_prefix_attention: q and o have max_tokens rows here (at most the plan's);
  *     rows outside [qo_indptr[0], qo_indptr[batch_size]) are left as they were. The
  *     offsets may start past 0 (a part of a larger batch); they must not decrease. A
  *     request whose own do, or leave the batch's or [0, max_tokens], or whose qo_len
- *     exceeds the plan's, gets NaN rows. workspace: plan->workspace_bytes, 16-byte aligned, written before it is
+ *     exceeds the plan's, gets NaN rows; where offsets decrease, the rows of the other
+ *     requests are open. Slots are the caller's to keep inside the caches. sm_scale is
+ *     positive. workspace: plan->workspace_bytes, 16-byte aligned, written before it is
  *     read; calls that share one must be stream-ordered.
  * q, o: bf16 [max_tokens, num_qo_heads, 128], caches one layer's bf16 [slots,
  * num_kv_heads, 128]; strides multiples of 8 elements; 1 to 64 query heads per kv head.
@@ -579,8 +585,6 @@ typedef struct {
   int32_t head_dim;
   int32_t num_blocks;   /* workgroups of the launch (two per CU) */
   int32_t max_units;    /* parts the requests' own tokens are cut into at most */
-  int32_t walk_rows;    /* packed rows (tokens x heads of a kv head) up to which those parts
-                           take the prefix too; 0: it has workgroups of its own */
   int32_t reserved;
   int64_t prefix_rows;  /* partial rows of the prefix in the workspace */
   int64_t workspace_bytes;

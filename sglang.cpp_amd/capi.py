@@ -125,8 +125,7 @@ class PrefixPlan(ctypes.Structure):
     """sgl_prefix_plan_t."""
     _fields_ = [*[(n, ctypes.c_int32) for n in ("prefix_len", "batch_size", "max_tokens",
                                                 "max_qo_len", "num_qo_heads", "num_kv_heads",
-                                                "head_dim", "num_blocks", "max_units", "walk_rows",
-                                                "reserved")],
+                                                "head_dim", "num_blocks", "max_units", "reserved")],
                 ("prefix_rows", ctypes.c_int64), ("workspace_bytes", ctypes.c_int64)]
 
 

@@ -6,14 +6,19 @@
 // K/V are walked once with the rows of every request as columns of one product,
 // each request's own tokens with its rows alone, and a second launch folds.
 //
-// Two ways over tokens in one launch (split_of). Units: the requests' own tokens, behind
-// the prefix where the batch has at most 32 packed rows a kv head, form one stream, cut
-// into units of equal length, one workgroup each as a rule; a wave has one kv head, so a workgroup reads whole token rows.
-// A wave walks its piece 16 tokens a step on the matrix cores: S^T = K Q^T, then
-// O^T += V^T P^T, whose operand P^T is S^T's accumulator layout, for one or two
-// column blocks of 16 rows per K/V read. Both put the row on the lane's column, so
-// the running maximum and sum are lane-local but for one exchange across four lane
-// groups. K and V of the next step are in flight during a step.
+// Two ways over tokens in one launch (split_of). Tiles: the prefix, 64 tokens at a time
+// through LDS, for up to 128 packed rows of a kv head. Units: the requests' own tokens
+// form one stream, cut into units of equal length, one workgroup each as a rule; a wave
+// has one kv head, so a workgroup reads whole token rows. A wave walks its piece 16
+// tokens a step on the matrix cores: S^T = K Q^T, then O^T += V^T P^T, whose operand P^T
+// is S^T's accumulator layout, for one or two column blocks of 16 rows per K/V read. Both
+// put the row on the lane's column, so the running maximum and sum are lane-local but for
+// one exchange across four lane groups. K and V of the next steps are in flight during one.
+//
+// The units could walk the prefix too where rows are few (32 at most, 16 tokens a step in
+// registers, no LDS): 32q/8kv, 64 own tokens, 8 requests behind 1,024 / 4,096 / 16,384 /
+// 65,536 tokens took 15.9 / 24.4 / 32.0 / 59.6 us so, 12.8 / 14.4 / 22.8 / 53.9 with tiles;
+// one request 11.8 / 15.9 / 23.4 / 50.2, with tiles 12.1 / 13.0 / 21.8 / 51.4.
 #include <math.h>
 
 #include <algorithm>
@@ -28,10 +33,9 @@ constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
 constexpr int kMinUnit = 16;              // shortest unit
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
-constexpr int kFoldGroups = 1024;          // workgroups of the fold up to which a row has lanes of its own
+constexpr int kFoldGroups = 1024;         // workgroups of the fold up to which a row has lanes of its own
 constexpr int kWaves = 4;                 // waves of a workgroup, two workgroups per CU
 constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
-constexpr int kMaxWalkRows = 32;         // packed rows up to which the units walk the prefix
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -45,14 +49,13 @@ struct PrefixArgs {
   const int32_t* qo_indptr;
   int batch, tokens, hq, hkv, group;
   int prefix, max_qo;
-  int walk_rows;         // packed rows whose prefix the units walk (0: the tiles' workgroups do)
   int blocks;            // workgroups of the launch
   int heads, side, rest; // kv heads of a unit, units side by side in a workgroup, head groups
   float scale_log2;
   uint16_t* o;
   int64_t o_st, o_sh;
-  // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix: [unit][kv head][packed
-  // row] or [piece of the item][kv head][packed row]. Own tokens: [token slot][q head],
+  // Partial outputs (fp32 [.., 128]) and log2-sum-exp. Prefix: [piece of the
+  // item][kv head][packed row]. Own tokens: [token slot][q head],
   // the piece a request starts with at its rows' own tokens, the one running into unit
   // u from before it at tokens + u max_qo + i.
   float* p_o;
@@ -68,24 +71,27 @@ struct PrefixArgs {
 // cut into that many runs (all row tiles alike, so that the workgroups of a head, on the
 // same XCD where there are eight heads, read the same K/V at the same time), else the
 // list (row tile, tile) into per_head runs. The others' units walk the stream of `all`
-// tokens, `shared` of them the prefix's, W a unit.
+// tokens, W a unit.
 struct Split {
   int first, rows;          // first query token, packed rows of a kv head
   int row_tiles, row_step;  // row tiles and their rows (32 a wave, spread evenly)
   int tiles;                // 64-token tiles of the prefix
   int tile_blocks, per_head, shares;
   uint32_t run;
-  uint32_t shared, all, W;
+  uint32_t all, W;
   int units;
 };
 
-// What a tile takes on one workgroup, and a token of a kv head, ns.
+// What a tile takes on one workgroup, and a token of a kv head, ns. Half and twice of the
+// first: 256 requests of 200 own tokens behind 16,384 tokens 121 and 121 us (123 so), 128
+// of 2,000 behind 1,024 183 and 177 (183), 32 of 300 behind 4,096 26.5 and 27.9 (26.2).
 constexpr uint32_t kTileNs = 1400;
 constexpr uint32_t kTokenNs = 16;
 // A request counts as this many tokens more in the units' stream: the loads that lead
-// to its first step, about 3.4 us (a unit that took eight requests of one token each was
-// 28 us behind the others).
-constexpr uint32_t kRequestTokens = 24;
+// to its first step, about 3.4 us. 0, 24, 48 and 96 measured: 64 requests of 5 own tokens
+// 16.7, 11.2, 10.3, 11.2 us; 64 of 16 behind 1,024 tokens 25.2, 25.6, 22.7, 22.8; 256 of
+// 200 behind 16,384 121 to 125 with any.
+constexpr uint32_t kRequestTokens = 48;
 
 // A loaded value that is the same in every lane, in a scalar register (the compiler
 // keeps it in a vector one, as the kernel's stores might change the memory).
@@ -97,14 +103,11 @@ __device__ __forceinline__ Split split_of(const PrefixArgs& a) {
   const int kv_end = uniform(a.kv_indptr[a.batch]);
   s.first = max(uniform(a.qo_indptr[0]), 0);
   s.rows = max(min(q_end, a.tokens) - s.first, 0) * a.group;
-  const uint32_t own = static_cast<uint32_t>(max(kv_end - max(kv_begin, 0), 0)) + a.batch * kRequestTokens;
+  s.all = static_cast<uint32_t>(max(kv_end - max(kv_begin, 0), 0)) + a.batch * kRequestTokens;
   s.tiles = (a.prefix + pf::kBN - 1) / pf::kBN;
   s.row_tiles = s.row_step = s.tile_blocks = s.per_head = s.shares = 0;
   s.run = 1;
-  s.shared = 0;
-  if (a.walk_rows > 0) {
-    s.shared = a.prefix;
-  } else if (s.rows > 0 && s.tiles > 0) {
+  if (s.rows > 0 && s.tiles > 0) {
     const int waves = (s.rows + 31) / 32;
     s.row_tiles = (waves + kWaves - 1) / kWaves;
     const int each = (waves + s.row_tiles - 1) / s.row_tiles;
@@ -112,7 +115,7 @@ __device__ __forceinline__ Split split_of(const PrefixArgs& a) {
     s.row_tiles = (waves + each - 1) / each;
     const uint32_t list = static_cast<uint32_t>(s.row_tiles) * s.tiles;  // of a head
     const uint64_t t = static_cast<uint64_t>(list) * a.hkv * kTileNs;
-    const uint64_t sum = t + static_cast<uint64_t>(own) * a.hkv * kTokenNs;
+    const uint64_t sum = t + static_cast<uint64_t>(s.all) * a.hkv * kTokenNs;
     const int shift = max(0, 42 - __builtin_clzll(sum));  // to 22 bits
     const uint32_t ts = static_cast<uint32_t>(t >> shift), ss = static_cast<uint32_t>(sum >> shift);
     // A second workgroup of tiles on a CU brings nothing (1.4 us a tile alone, 2.7 for
@@ -130,7 +133,6 @@ __device__ __forceinline__ Split split_of(const PrefixArgs& a) {
     }
     s.tile_blocks = min(s.per_head * a.hkv, a.blocks - 1);
   }
-  s.all = s.shared + own;
   s.units = max(1, (a.blocks - s.tile_blocks) * a.side / a.rest);
   const uint32_t w = s.all / static_cast<uint32_t>(s.units) + 1;  // one more where it divides
   s.W = max((w + kStep - 1) / kStep * kStep, static_cast<uint32_t>(kMinUnit));
@@ -190,16 +192,12 @@ __device__ __forceinline__ bf16x4_t v_operand(const u32x4_t (&vr)[4]) {
 
 // A piece: the len tokens of slots idx[0, len) for the packed rows [row0, row0 + rows)
 // (row p: token tok0 + p / G, head h G + p % G of kv head h). A row of token i sees the
-// tokens below sees0 + i. Row x's output and lse go to row out0 + x of o / lse, or, with
-// by_token, to row (out0 + i) hq + head.
+// tokens below sees0 + i. Its output and lse go to row (out0 + i) hq + head.
 struct Piece {
   const int32_t* idx;
   int len;
   int tok0, row0, rows, sees0;
-  float* o;
-  float* lse;
   int64_t out0;
-  bool by_token;
 };
 
 // One wave over a piece of at most 16 RB rows. Lane (n, j), n = lane % 16: token n (K),
@@ -337,8 +335,8 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
   if (t < len) step(t, slot[0], kr[0], vr[0]);
   // The block's output through LDS (16 rows of 32 16-byte chunks, chunk c of row n at
   // c ^ n: no bank conflicts either way), so that whole rows are stored: as they lie in
-  // the accumulators a store would touch 64 lines for 1 KB (128 units of 32 rows, 8 kv
-  // heads: 39.8 us, 9.7 of them without the rows).
+  // the accumulators a store would touch 64 lines for 1 KB (64 requests of 6 query and
+  // 256 own tokens, 32q/4kv: 42.4 us so, 32.2 through LDS).
   f32x4_t* xr = reinterpret_cast<f32x4_t*>(xch);
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -356,16 +354,15 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
     }
     wave_lds_sync();
     if (j == 0 && 16 * b + n < rows)
-      w.lse[w.by_token ? (w.out0 + tok[b]) * a.hq + head[b] : w.out0 + 16 * b + n] =
-          sum == 0.f ? -INFINITY : m[b] + log2f(sum);
+      a.s_lse[(w.out0 + tok[b]) * a.hq + head[b]] = sum == 0.f ? -INFINITY : m[b] + log2f(sum);
     const int c = lane & 31;
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
       const int x = 2 * it + (lane >> 5), y = 16 * b + x + rem;
       if (16 * b + x >= rows) break;
       const int d = static_cast<int>(static_cast<uint32_t>(y) * inv_g >> 16);
-      const int64_t row = w.by_token ? (w.out0 + i0 + d) * a.hq + (h * G + y - d * G) : w.out0 + 16 * b + x;
-      __builtin_nontemporal_store(xr[32 * x + (c ^ x)], reinterpret_cast<f32x4_t*>(w.o + row * kD + 4 * c));
+      const int64_t row = (w.out0 + i0 + d) * a.hq + (h * G + y - d * G);
+      __builtin_nontemporal_store(xr[32 * x + (c ^ x)], reinterpret_cast<f32x4_t*>(a.s_o + row * kD + 4 * c));
     }
     wave_lds_sync();
   }
@@ -376,71 +373,48 @@ __device__ __forceinline__ int64_t place_of(const PrefixArgs& a, int r, int kv_f
   return static_cast<int64_t>(a.kv_indptr[r]) - kv_first + static_cast<int64_t>(r) * kRequestTokens;
 }
 
-// Unit u's pieces of the stream for kv head h: places below 2^29 (prefix) + 2^31 (the
-// offsets are int32) + 2^30 (2^25 requests), 32 bits without a sign.
+// Unit u's pieces of the stream for kv head h: places below 2^31 (the offsets are int32)
+// + 2^25 requests' kRequestTokens, 32 bits without a sign.
 template <int RB>
 __device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s, char* xch, uint32_t u, int h,
                                             int lane) {
   if (static_cast<uint64_t>(u) * s.W >= s.all) return;
-  const uint32_t t0 = u * s.W, t1 = min(s.all, t0 + s.W);
-  // The requests' own tokens [b0, b1) of the joined list, from request r on.
+  // The places [b0, b1), from request r on: those that end at or before b0 are passed
+  // over, 64 at a time.
+  const uint32_t b0 = u * s.W, b1 = min(s.all, b0 + s.W);
   const int kv_first = max(uniform(a.kv_indptr[0]), 0);
-  const uint32_t b0 = max(t0, s.shared) - s.shared, b1 = max(t1, s.shared) - s.shared;
-  int r = -1;  // the prefix's part
-  int left = 0;  // rows of the current request not walked yet
-  Piece w;
-  if (t0 < s.shared) {
-    w.idx = a.pidx + t0;
-    w.len = w.sees0 = static_cast<int>(min(t1, s.shared) - t0);
-    w.tok0 = s.first;
-    w.row0 = 0;
-    left = min(s.rows, a.walk_rows);
-    w.o = a.p_o, w.lse = a.p_lse;
-    w.out0 = (static_cast<int64_t>(u) * a.hkv + h) * a.walk_rows;
-    w.by_token = false;
+  int r = 0;
+  for (int at = 0; at < a.batch; at += kWave) {
+    const int e = at + lane;
+    const bool before = e < a.batch && place_of(a, e + 1, kv_first) <= static_cast<int64_t>(b0);
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(before);
+    r += __builtin_popcountll(mask);
+    if (mask != ~0ull) break;
   }
-  while (true) {
-    while (left <= 0) {  // the next request
-      if (b1 == 0) return;
-      if (r < 0) {  // those that end at or before b0 are passed over, 64 at a time
-        r = 0;
-        for (int at = 0; at < a.batch; at += kWave) {
-          const int e = at + lane;
-          const bool before = e < a.batch && place_of(a, e + 1, kv_first) <= static_cast<int64_t>(b0);
-          const uint64_t mask = __builtin_amdgcn_ballot_w64(before);
-          r += __builtin_popcountll(mask);
-          if (mask != ~0ull) break;
-        }
-      } else {
-        ++r;
-      }
-      if (r >= a.batch) return;
-      const Request x = request_of(a, r);
-      const int64_t rb = static_cast<int64_t>(x.kv0) - kv_first + static_cast<int64_t>(r) * kRequestTokens;  // then its kRequestTokens, then its tokens
-      if (rb >= b1) return;
-      if (!x.ok) continue;
-      const int64_t at = rb + kRequestTokens;
-      const int s0 = static_cast<int>(max(b0 - at, int64_t{0}));
-      w.len = static_cast<int>(min(b1 - at, static_cast<int64_t>(x.kv))) - s0;
-      if (w.len <= 0) continue;
-      w.idx = a.indices + x.kv0 + s0;
-      w.tok0 = x.q0;
-      w.row0 = 0;
-      left = x.qo * a.group;
-      w.sees0 = max(x.kv - x.qo + 1 - s0, -x.qo);
-      w.o = a.s_o, w.lse = a.s_lse;
-      w.out0 = s0 == 0 ? x.q0 : a.tokens + static_cast<int64_t>(u) * a.max_qo;
-      w.by_token = true;
+  for (; r < a.batch; ++r) {
+    const Request x = request_of(a, r);
+    // Its kRequestTokens places, then its tokens'.
+    const int64_t rb = static_cast<int64_t>(x.kv0) - kv_first + static_cast<int64_t>(r) * kRequestTokens;
+    if (rb >= b1) return;
+    if (!x.ok) continue;
+    const int64_t at = rb + kRequestTokens;
+    const int s0 = static_cast<int>(max(b0 - at, int64_t{0}));
+    Piece w;
+    w.len = static_cast<int>(min(b1 - at, static_cast<int64_t>(x.kv))) - s0;
+    if (w.len <= 0) continue;
+    w.idx = a.indices + x.kv0 + s0;
+    w.tok0 = x.q0;
+    w.sees0 = max(x.kv - x.qo + 1 - s0, -x.qo);
+    w.out0 = s0 == 0 ? x.q0 : a.tokens + static_cast<int64_t>(u) * a.max_qo;
+    const int rows = x.qo * a.group;
+    for (w.row0 = 0; w.row0 < rows; w.row0 += 16 * RB) {
+      w.rows = min(rows - w.row0, 16 * RB);
+      walk<RB>(a, w, xch, h, lane);
     }
-    w.rows = min(left, 16 * RB);
-    walk<RB>(a, w, xch, h, lane);
-    left -= w.rows;
-    w.row0 += w.rows;
-    if (!w.by_token) w.out0 += w.rows;
   }
 }
 
-// The prefix for many rows: W waves with 32 packed rows each share the 64-token K/V
+// The prefix: W waves with 32 packed rows each share the 64-token K/V
 // tiles that they gather into LDS (two buffers, K one tile ahead of V), and tile t + 1's
 // scores are on the matrix cores while tile t's become weights; the prefill kernel's
 // tile steps without a causal bound. Tiles [tb, te) of the prefix for row tile rt of kv
@@ -694,7 +668,8 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   __syncthreads();
   const int r = uniform(before[0] + before[1] + before[2] + before[3]);
   if (r >= a.batch || t < a.qo_indptr[0]) return;  // no request's row: left as it was
-  const Request x = request_of(a, r);
+  Request x = request_of(a, r);
+  x.ok = x.ok && t >= x.q0 && t - x.q0 < x.qo;  // not so where other requests' offsets decrease
   const int P = a.prefix, i = t - x.q0;
   const int64_t sees = static_cast<int64_t>(P) + x.kv - x.qo + i + 1;  // tokens this row sees, prefix first
   const bool folded = x.ok && sees >= P;
@@ -702,7 +677,7 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   int ns = 0;
   int64_t s1 = 0;
   if (x.kv > 0 && x.ok) {
-    const uint32_t own0 = sp.shared + (x.kv0 - max(uniform(a.kv_indptr[0]), 0)) + (r + 1) * kRequestTokens;
+    const uint32_t own0 = (x.kv0 - max(uniform(a.kv_indptr[0]), 0)) + (r + 1) * kRequestTokens;
     const uint32_t u0 = uniform(own0 / sp.W);
     ns = uniform((own0 + x.kv - 1) / sp.W) - u0 + 1;
     s1 = (a.tokens + static_cast<int64_t>(u0) * a.max_qo + i) * a.hq;
@@ -719,20 +694,12 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
     if (folded) {
       // Prefix pieces: np of them, p_step rows apart.
       const int prow = row_of_head + hh - h * a.group;
-      int np = 0;
-      int64_t p0 = 0, p_step = static_cast<int64_t>(a.hkv) * a.walk_rows;
-      if (sp.tile_blocks > 0) {
-        np = sp.shares;
-        if (np == 0) {
-          const uint32_t at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
-          np = static_cast<int>((at + sp.tiles - 1) / sp.run - at / sp.run) + 1;
-        }
-        p_step = static_cast<int64_t>(a.hkv) * sp.rows;
-        p0 = static_cast<int64_t>(h) * sp.rows + prow;
-      } else if (P > 0) {
-        np = static_cast<int>((P - 1) / sp.W) + 1;
-        p0 = static_cast<int64_t>(h) * a.walk_rows + prow;
+      int np = sp.shares;
+      if (sp.tile_blocks > 0 && np == 0) {
+        const uint32_t at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
+        np = static_cast<int>((at + sp.tiles - 1) / sp.run - at / sp.run) + 1;
       }
+      const int64_t p_step = static_cast<int64_t>(a.hkv) * sp.rows, p0 = static_cast<int64_t>(h) * sp.rows + prow;
       for (int k0 = set; k0 < np + ns; k0 += kLoads * kSets) {
         f32x4_t v[kLoads];
         float lse[kLoads];
@@ -846,11 +813,11 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
   if (head_dim != kD || group > 64 || max_qo_len > SGL_PREFIX_MAX_QO ||
       num_kv_heads > 65535 || prefix_len > (1 << 29) || batch_size > (1 << 25))
     return SGL_ERR_UNSUPPORTED;
-  // Packed rows, and the list of tiles, are counted in 32 bits, and the fold's grid is a
-  // workgroup per row at most.
+  // Packed rows, and the list of tiles, are counted in 32 bits, and so are the threads of
+  // the fold's launch, a workgroup of 256 a token from kFoldGroups tokens on.
   const int64_t rows = static_cast<int64_t>(max_tokens) * group;
   const int64_t row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves), tiles = (prefix_len + pf::kBN - 1) / pf::kBN;
-  if (rows > (1 << 30) || static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff ||
+  if (rows > (1 << 30) || max_tokens >= 1 << 24 || static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff ||
       row_tiles * num_kv_heads > 0x7fffffff / (tiles > 0 ? tiles : 1))
     return SGL_ERR_UNSUPPORTED;
   p = sgl_prefix_plan_t{};
@@ -860,16 +827,9 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
   const int heads = heads_per_group(num_kv_heads);
   const int64_t units = static_cast<int64_t>(blocks) * (kWaves / heads) / (num_kv_heads / heads);
   p.max_units = static_cast<int32_t>(units < 1 ? 1 : units);
-  if (prefix_len > 0 && rows > 0) {
-    if (rows <= kMaxWalkRows) {  // the units walk the prefix
-      p.walk_rows = static_cast<int32_t>((rows + 15) / 16 * 16);
-      p.prefix_rows = static_cast<int64_t>(p.max_units) * num_kv_heads * p.walk_rows;
-    } else {
-      // At most `blocks` shares of a row tile and head, or two runs that each of them
-      // lies in, of 128 rows.
-      p.prefix_rows = (blocks + 2 * row_tiles * num_kv_heads) * 32 * kWaves;
-    }
-  }
+  // At most `blocks` shares of a row tile and head, or two runs that each of them lies in,
+  // of up to 128 rows.
+  if (prefix_len > 0) p.prefix_rows = (blocks + 2 * row_tiles * num_kv_heads) * std::min<int64_t>(rows, 32 * kWaves);
   p.workspace_bytes = workspace_layout(p).total;
   return SGL_OK;
 }
@@ -903,6 +863,8 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
                                     int64_t o_stride_token, int64_t o_stride_head, void* workspace,
                                     int64_t workspace_bytes, void* stream) {
   if (!plan || batch_size < 0 || max_tokens < 0) return SGL_ERR_INVALID_ARG;
+  // The maximum of the scores is taken before the scale.
+  if (!(sm_scale > 0.f) || !isfinite(sm_scale)) return SGL_ERR_INVALID_ARG;
   if (num_qo_heads != plan->num_qo_heads || num_kv_heads != plan->num_kv_heads ||
       head_dim != plan->head_dim)
     return SGL_ERR_INVALID_ARG;
@@ -911,9 +873,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   int st = make_plan(plan->prefix_len, plan->batch_size, plan->max_tokens, plan->max_qo_len,
                      num_qo_heads, num_kv_heads, head_dim, plan->num_blocks, p);
   if (st != SGL_OK) return st;
-  if (plan->max_units != p.max_units || plan->walk_rows != p.walk_rows ||
-      plan->prefix_rows != p.prefix_rows)
-    return SGL_ERR_INVALID_ARG;
+  if (plan->max_units != p.max_units || plan->prefix_rows != p.prefix_rows) return SGL_ERR_INVALID_ARG;
   if (batch_size > p.batch_size || max_tokens > p.max_tokens) return SGL_ERR_CAPACITY;
   if (batch_size == 0 || max_tokens == 0) return SGL_OK;
   if (!q || !k_cache || !v_cache || !kv_indptr || !qo_indptr || !o ||
@@ -935,23 +895,21 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   a.pidx = prefix_indices, a.indices = indices, a.kv_indptr = kv_indptr, a.qo_indptr = qo_indptr;
   a.batch = batch_size, a.tokens = max_tokens;
   a.hq = num_qo_heads, a.hkv = num_kv_heads, a.group = num_qo_heads / num_kv_heads;
-  a.prefix = p.prefix_len, a.max_qo = p.max_qo_len, a.walk_rows = p.walk_rows, a.blocks = p.num_blocks;
+  a.prefix = p.prefix_len, a.max_qo = p.max_qo_len, a.blocks = p.num_blocks;
   a.heads = heads_per_group(num_kv_heads), a.side = kWaves / a.heads, a.rest = num_kv_heads / a.heads;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.o = static_cast<uint16_t*>(o), a.o_st = o_stride_token, a.o_sh = o_stride_head;
   a.p_o = reinterpret_cast<float*>(ws + l.p_o), a.p_lse = reinterpret_cast<float*>(ws + l.p_lse);
   a.s_o = reinterpret_cast<float*>(ws + l.s_o), a.s_lse = reinterpret_cast<float*>(ws + l.s_lse);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int own_rows = p.max_qo_len * a.group;
-  const int need = own_rows < a.walk_rows ? a.walk_rows : own_rows;
-  if (need <= 16) launch_attention<1>(a, s);
+  if (p.max_qo_len * a.group <= 16) launch_attention<1>(a, s);
   else launch_attention<2>(a, s);
   st = launch_status();
   if (st != SGL_OK) return st;
   // Many pieces a row: a workgroup for each. Few: 32 lanes a row, and of many rows
   // several a lane group (2,048 workgroups of four heads each took 12.5 us for 256 tokens
   // of 32 heads).
-  const int64_t pieces = a.prefix == 0 ? 2 : a.walk_rows > 0 ? p.max_units
+  const int64_t pieces = a.prefix == 0 ? 2
       : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 127) / 128 * num_kv_heads) / 2 + 2;
   const int rows_per = pieces > 16 ? 1 : 8;
   const int all_iters = (num_qo_heads + rows_per - 1) / rows_per;

@@ -457,12 +457,13 @@ extern "C" int sgl_rope_append(const sgl_rope_append_t* args, void* stream) {
   auto chunked = [](const void* p, int64_t st, int64_t sh) {
     return p == nullptr || (aligned16(p) && st % 8 == 0 && sh % 8 == 0);
   };
-  // Whole chunks everywhere; the grid (at most rows * d / 16 threads a token) in 31 bits.
+  // Whole chunks everywhere; the launch's threads (rows d / 16 a token and up to a
+  // workgroup more) in 32 bits.
   if (a.d % 16 == 0 && a.rotary % 16 == 0 && chunked(a.q, a.q_st, a.q_sh) &&
       chunked(a.q_out, a.qo_st, a.qo_sh) && chunked(a.k, a.k_st, a.k_sh) &&
       chunked(a.v, a.v_st, a.v_sh) && chunked(a.k_cache, a.kv_ss, a.kv_sh) &&
       chunked(a.v_cache, a.kv_ss, a.kv_sh) && aligned16(a.cos) && aligned16(a.sin) &&
-      a.tokens * (rows * (a.d / 16) / 128 + 1) < 0x7fffffff) {
+      a.tokens < 0xffffffffll / (rows * (a.d / 16) + 512)) {
     if (x.dtype == SGL_DTYPE_BF16) launch_chunks<SGL_DTYPE_BF16>(a, il, s);
     else launch_chunks<SGL_DTYPE_F16>(a, il, s);
     return launch_status();

@@ -177,6 +177,12 @@ def test_invalid_requests_get_nan_rows(dev):
     y = make(dev, 64, [9, 9], [2, 5], 16, 8, 18)
     o = run(y, plan_of(y, max_qo=4))
     assert o[2:].isnan().all() and not o[:2].isnan().any()
+    # q offsets that decrease: rows 4 to 9 belong to no request (the third one, whose own
+    # offsets hold, is the one that their place in the list points to).
+    z = make(dev, 64, [40, 9, 9, 9], [4, 2, 2, 4], 16, 8, 20)
+    z["qop"] = torch.tensor([0, 10, 2, 4, 12], device=dev, dtype=torch.int32)
+    o = run(z, plan_of(z, max_qo=8))
+    assert o[4:10].isnan().all()
 
 
 def test_strided_rows_far_slots_and_a_side_stream(dev):

@@ -70,7 +70,8 @@ def test_prefix_plan():
     assert capi.lib().sgl_prefix_plan(1, 1, 1, 1, 1, 1, 128, None) == -1
     for kw in (dict(P=-1), dict(B=-1), dict(T=-1), dict(qo=-1), dict(hq=0), dict(hkv=0), dict(hkv=3)):
         assert plan(**kw)[0] == -1, kw
-    for kw in (dict(d=64), dict(qo=capi.PREFIX_MAX_QO + 1), dict(hq=65, hkv=1), dict(T=1 << 29)):
+    for kw in (dict(d=64), dict(qo=capi.PREFIX_MAX_QO + 1), dict(hq=65, hkv=1), dict(T=1 << 29),
+               dict(T=1 << 24, hq=1, hkv=1), dict(P=(1 << 29) + 1), dict(B=(1 << 25) + 1)):
         assert plan(**kw)[0] == -2, kw
     st, p = plan()
     assert st == 0 and p.num_blocks >= 1 and p.max_units >= 1 and p.workspace_bytes > 0
@@ -79,17 +80,16 @@ def test_prefix_plan():
     for T in (1, 8, 16, 17, 64, 700):
         st, p = plan(T=T)
         assert p.workspace_bytes >= T * 8 * 512 and p.prefix_rows > 0
-        assert p.walk_rows == (-(-4 * T // 16) * 16 if 4 * T <= 32 else 0)
 
 
 def attend(p, **kw):
     a = dict(q=16, qs=1024, qh=128, k=32, v=48, ks=256, kh=128, pidx=64, idx=64, kvp=80, qop=96, B=4,
-             T=8, hq=8, hkv=2, d=128, o=112, os=1024, oh=128, ws=256, wsb=p.workspace_bytes)
+             T=8, hq=8, hkv=2, d=128, o=112, os=1024, oh=128, ws=256, wsb=p.workspace_bytes, scale=0.1)
     a.update(kw)
     return capi.lib().sgl_prefix_attention(
         ctypes.byref(p), a["q"], a["qs"], a["qh"], a["k"], a["v"], a["ks"], a["kh"], a["pidx"],
-        a["idx"], a["kvp"], a["qop"], a["B"], a["T"], a["hq"], a["hkv"], a["d"], 0.1, a["o"], a["os"],
-        a["oh"], a["ws"], a["wsb"], None)
+        a["idx"], a["kvp"], a["qop"], a["B"], a["T"], a["hq"], a["hkv"], a["d"], a["scale"], a["o"],
+        a["os"], a["oh"], a["ws"], a["wsb"], None)
 
 
 def test_prefix_attention_refusals():
@@ -105,6 +105,8 @@ def test_prefix_attention_refusals():
     assert attend(p, q=18) == attend(p, o=24) == attend(p, k=40) == attend(p, qs=1020) == -4
     assert attend(p, kh=100) == attend(p, oh=129) == attend(p, ws=264) == -4
     assert attend(p, ks=0) == -2
+    for scale in (0.0, -0.1, float("inf"), float("nan")):
+        assert attend(p, scale=scale) == -1, scale
     # A plan that was not made by sgl_prefix_plan.
     q = capi.PrefixPlan.from_buffer_copy(p)
     q.num_blocks = 0
