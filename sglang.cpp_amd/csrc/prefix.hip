@@ -37,6 +37,11 @@ constexpr int kFoldGroups = 1024;         // workgroups of the fold up to which 
 constexpr int kWaves = 4;                 // waves of a workgroup, two workgroups per CU
 constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
 
+// What the fold needs of a launch's Split.
+struct alignas(16) FoldSplit {
+  int first, rows, row_step, tiles, shares, run, W, pad;
+};
+
 struct PrefixArgs {
   const uint16_t* q;
   int64_t q_st, q_sh;
@@ -62,10 +67,12 @@ struct PrefixArgs {
   float* p_lse;
   float* s_o;
   float* s_lse;
+  FoldSplit* split;
 };
 
 // How a launch is shared out, from the lengths as they are now (so a captured launch
-// follows them): the main and the fold kernel work it out alike, in whole numbers.
+// follows them): every workgroup works it out alike, in whole numbers, and one leaves the
+// fold what it needs of it.
 // Workgroups [0, tile_blocks) walk the prefix's 64-token tiles for one kv head and row
 // tile at a time, per_head of them for a head: with `shares` each row tile's tiles are
 // cut into that many runs (all row tiles alike, so that the workgroups of a head, on the
@@ -148,19 +155,23 @@ struct Request {
   bool ok;
 };
 
-__device__ __forceinline__ Request request_of(const PrefixArgs& a, int r) {
+// From its own offsets and the batch's.
+__device__ __forceinline__ Request request_from(const PrefixArgs& a, int q0, int64_t q1, int kv0, int64_t k1,
+                                                int q_first, int q_end, int kv_first, int kv_end) {
   Request x;
-  x.q0 = uniform(a.qo_indptr[r]);
-  const int64_t q1 = uniform(a.qo_indptr[r + 1]);
-  x.kv0 = uniform(a.kv_indptr[r]);
-  const int64_t k1 = uniform(a.kv_indptr[r + 1]);
-  x.qo = static_cast<int>(q1 - x.q0);
-  x.kv = static_cast<int>(k1 - x.kv0);
+  x.q0 = q0, x.kv0 = kv0;
+  x.qo = static_cast<int>(q1 - q0);
+  x.kv = static_cast<int>(k1 - kv0);
   // Rows and pieces of anything else have no place in the outputs and the workspace.
-  x.ok = x.q0 >= max(uniform(a.qo_indptr[0]), 0) && q1 >= x.q0 &&
-         q1 <= min(uniform(a.qo_indptr[a.batch]), a.tokens) && q1 - x.q0 <= a.max_qo &&
-         x.kv0 >= max(uniform(a.kv_indptr[0]), 0) && k1 >= x.kv0 && k1 <= uniform(a.kv_indptr[a.batch]);
+  x.ok = q0 >= max(q_first, 0) && q1 >= q0 && q1 <= min(q_end, a.tokens) && q1 - q0 <= a.max_qo &&
+         kv0 >= max(kv_first, 0) && k1 >= kv0 && k1 <= kv_end;
   return x;
+}
+
+__device__ __forceinline__ Request request_of(const PrefixArgs& a, int r) {
+  return request_from(a, uniform(a.qo_indptr[r]), uniform(a.qo_indptr[r + 1]), uniform(a.kv_indptr[r]),
+                      uniform(a.kv_indptr[r + 1]), uniform(a.qo_indptr[0]), uniform(a.qo_indptr[a.batch]),
+                      uniform(a.kv_indptr[0]), uniform(a.kv_indptr[a.batch]));
 }
 
 __device__ __forceinline__ bf16x8_t as_bf16x8(const u32x4_t& v) {
@@ -570,6 +581,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(Prefix
   static_assert(sizeof(smem) >= kWaves * kWaveLds, "the waves' output rows take the tiles' place");
   const Split s = split_of(a);
   const int b = blockIdx.x;
+  if (b == a.blocks - 1 && threadIdx.x == 0)
+    *a.split = FoldSplit{s.first, s.rows, s.row_step, s.tiles, s.shares, static_cast<int>(s.run),
+                         static_cast<int>(s.W), 0};
   if (b < s.tile_blocks) {
     for (int v = b; v < s.per_head * a.hkv; v += s.tile_blocks) {
       const int j = v / a.hkv, h = v - j * a.hkv;
@@ -653,23 +667,41 @@ __device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request&
 template <int kSets>
 __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head_groups, int iters) {
   constexpr int kRows = 8 / kSets, kLoads = kSets == 1 ? 4 : 8;
-  __shared__ int before[4];
+  __shared__ int found[4][5];
   __shared__ float xch[kSets > 1 ? 6 : 1][8][32];
   const int t = uniform(blockIdx.x / static_cast<uint32_t>(head_groups));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // The token's request: those that end at or before it are counted.
-  int n = 0;
+  // The token's request, by one lane each; the first where offsets that decrease give
+  // it several.
+  int r = -1;
   for (int at = 64 * wave; at < a.batch; at += 256) {
-    const bool done = at + lane < a.batch && a.qo_indptr[at + lane + 1] <= t;
-    n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(done));
+    const int e = min(at + lane, a.batch - 1);
+    const int q0 = a.qo_indptr[e], q1 = a.qo_indptr[e + 1], k0 = a.kv_indptr[e], k1 = a.kv_indptr[e + 1];
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(at + lane < a.batch && q0 <= t && t < q1);
+    if (mask == 0) continue;
+    const int by = __builtin_ctzll(mask);
+    r = at + by;
+    if (lane == by) {
+      found[wave][1] = q0, found[wave][2] = q1;
+      found[wave][3] = k0, found[wave][4] = k1;
+    }
+    break;
   }
-  const Split sp = split_of(a);
-  if (lane == 0) before[wave] = n;
+  FoldSplit sp = *a.split;
+  const int q_first = a.qo_indptr[0], q_end = a.qo_indptr[a.batch];
+  const int kv_first = uniform(a.kv_indptr[0]), kv_end = a.kv_indptr[a.batch];
+  sp = FoldSplit{uniform(sp.first), uniform(sp.rows), uniform(sp.row_step), uniform(sp.tiles),
+                 uniform(sp.shares), uniform(sp.run), uniform(sp.W), 0};
+  if (lane == 0) found[wave][0] = r;
   __syncthreads();
-  const int r = uniform(before[0] + before[1] + before[2] + before[3]);
-  if (r >= a.batch || t < a.qo_indptr[0]) return;  // no request's row: left as it was
-  Request x = request_of(a, r);
-  x.ok = x.ok && t >= x.q0 && t - x.q0 < x.qo;  // not so where other requests' offsets decrease
+  int from = 3;
+#pragma unroll
+  for (int k = 2; k >= 0; --k) from = found[k][0] >= 0 ? k : from;
+  r = uniform(found[from][0]);
+  if (r < 0) return;  // no request's row: left as it was
+  const Request x = request_from(a, uniform(found[from][1]), uniform(found[from][2]), uniform(found[from][3]),
+                                 uniform(found[from][4]), uniform(q_first), uniform(q_end), kv_first,
+                                 uniform(kv_end));
   const int P = a.prefix, i = t - x.q0;
   const int64_t sees = static_cast<int64_t>(P) + x.kv - x.qo + i + 1;  // tokens this row sees, prefix first
   const bool folded = x.ok && sees >= P;
@@ -677,9 +709,10 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   int ns = 0;
   int64_t s1 = 0;
   if (x.kv > 0 && x.ok) {
-    const uint32_t own0 = (x.kv0 - max(uniform(a.kv_indptr[0]), 0)) + (r + 1) * kRequestTokens;
-    const uint32_t u0 = uniform(own0 / sp.W);
-    ns = uniform((own0 + x.kv - 1) / sp.W) - u0 + 1;
+    const uint32_t W = sp.W;
+    const uint32_t own0 = (x.kv0 - max(kv_first, 0)) + (r + 1) * kRequestTokens;
+    const uint32_t u0 = uniform(own0 / W);
+    ns = uniform((own0 + x.kv - 1) / W) - u0 + 1;
     s1 = (a.tokens + static_cast<int64_t>(u0) * a.max_qo + i) * a.hq;
   }
   const int64_t s0 = static_cast<int64_t>(t) * a.hq, s_step = static_cast<int64_t>(a.max_qo) * a.hq;
@@ -695,9 +728,9 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
       // Prefix pieces: np of them, p_step rows apart.
       const int prow = row_of_head + hh - h * a.group;
       int np = sp.shares;
-      if (sp.tile_blocks > 0 && np == 0) {
-        const uint32_t at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
-        np = static_cast<int>((at + sp.tiles - 1) / sp.run - at / sp.run) + 1;
+      if (np == 0 && sp.row_step > 0) {
+        const uint32_t run = sp.run, at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
+        np = static_cast<int>((at + sp.tiles - 1) / run - at / run) + 1;
       }
       const int64_t p_step = static_cast<int64_t>(a.hkv) * sp.rows, p0 = static_cast<int64_t>(h) * sp.rows + prow;
       for (int k0 = set; k0 < np + ns; k0 += kLoads * kSets) {
@@ -787,7 +820,7 @@ int heads_per_group(int hkv) {
 }
 
 struct Layout {
-  int64_t p_o, p_lse, s_o, s_lse, total;
+  int64_t p_o, p_lse, s_o, s_lse, split, total;
 };
 
 Layout workspace_layout(const sgl_prefix_plan_t& p) {
@@ -799,7 +832,8 @@ Layout workspace_layout(const sgl_prefix_plan_t& p) {
   l.p_lse = l.p_o + align(p.prefix_rows * kD * 4);
   l.s_o = l.p_lse + align(p.prefix_rows * 4);
   l.s_lse = l.s_o + align(own_rows * kD * 4);
-  l.total = l.s_lse + align(own_rows * 4);
+  l.split = l.s_lse + align(own_rows * 4);
+  l.total = l.split + align(sizeof(FoldSplit));
   return l;
 }
 
@@ -901,6 +935,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   a.o = static_cast<uint16_t*>(o), a.o_st = o_stride_token, a.o_sh = o_stride_head;
   a.p_o = reinterpret_cast<float*>(ws + l.p_o), a.p_lse = reinterpret_cast<float*>(ws + l.p_lse);
   a.s_o = reinterpret_cast<float*>(ws + l.s_o), a.s_lse = reinterpret_cast<float*>(ws + l.s_lse);
+  a.split = reinterpret_cast<FoldSplit*>(ws + l.split);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.max_qo_len * a.group <= 16) launch_attention<1>(a, s);
   else launch_attention<2>(a, s);
