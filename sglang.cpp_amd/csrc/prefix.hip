@@ -87,6 +87,7 @@ struct Split {
   uint32_t run;
   uint32_t all, W;
   int units;
+  int q_first, q_end, kv_first, kv_end;  // the batch's offsets
 };
 
 // What a tile takes on one workgroup, and a token of a kv head, ns. Half and twice of the
@@ -104,13 +105,28 @@ constexpr uint32_t kRequestTokens = 48;
 // keeps it in a vector one, as the kernel's stores might change the memory).
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-__device__ __forceinline__ Split split_of(const PrefixArgs& a) {
+// Offsets of 63 requests from request `base` on, lane i those of request base + i and the
+// end of the one before: in registers, so that neither finding a request nor the next one
+// of a walk waits for memory.
+struct Offsets {
+  int base, q, k;
+};
+
+constexpr int kWindow = kWave - 1;
+
+__device__ __forceinline__ Offsets offsets_from(const PrefixArgs& a, int base, int lane) {
+  const int e = min(base + lane, a.batch);
+  return Offsets{base, a.qo_indptr[e], a.kv_indptr[e]};
+}
+
+// `head`: the offsets from request 0 on.
+__device__ __forceinline__ Split split_of(const PrefixArgs& a, const Offsets& head) {
   Split s;
-  const int q_end = uniform(a.qo_indptr[a.batch]), kv_begin = uniform(a.kv_indptr[0]);
-  const int kv_end = uniform(a.kv_indptr[a.batch]);
-  s.first = max(uniform(a.qo_indptr[0]), 0);
-  s.rows = max(min(q_end, a.tokens) - s.first, 0) * a.group;
-  s.all = static_cast<uint32_t>(max(kv_end - max(kv_begin, 0), 0)) + a.batch * kRequestTokens;
+  s.q_end = uniform(a.qo_indptr[a.batch]), s.kv_end = uniform(a.kv_indptr[a.batch]);
+  s.q_first = uniform(head.q), s.kv_first = uniform(head.k);
+  s.first = max(s.q_first, 0);
+  s.rows = max(min(s.q_end, a.tokens) - s.first, 0) * a.group;
+  s.all = static_cast<uint32_t>(max(s.kv_end - max(s.kv_first, 0), 0)) + a.batch * kRequestTokens;
   s.tiles = (a.prefix + pf::kBN - 1) / pf::kBN;
   s.row_tiles = s.row_step = s.tile_blocks = s.per_head = s.shares = 0;
   s.run = 1;
@@ -166,12 +182,6 @@ __device__ __forceinline__ Request request_from(const PrefixArgs& a, int q0, int
   x.ok = q0 >= max(q_first, 0) && q1 >= q0 && q1 <= min(q_end, a.tokens) && q1 - q0 <= a.max_qo &&
          kv0 >= max(kv_first, 0) && k1 >= kv0 && k1 <= kv_end;
   return x;
-}
-
-__device__ __forceinline__ Request request_of(const PrefixArgs& a, int r) {
-  return request_from(a, uniform(a.qo_indptr[r]), uniform(a.qo_indptr[r + 1]), uniform(a.kv_indptr[r]),
-                      uniform(a.kv_indptr[r + 1]), uniform(a.qo_indptr[0]), uniform(a.qo_indptr[a.batch]),
-                      uniform(a.kv_indptr[0]), uniform(a.kv_indptr[a.batch]));
 }
 
 __device__ __forceinline__ bf16x8_t as_bf16x8(const u32x4_t& v) {
@@ -379,39 +389,40 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
   }
 }
 
-// Where request r begins among the requests in the stream.
-__device__ __forceinline__ int64_t place_of(const PrefixArgs& a, int r, int kv_first) {
-  return static_cast<int64_t>(a.kv_indptr[r]) - kv_first + static_cast<int64_t>(r) * kRequestTokens;
-}
-
 // Unit u's pieces of the stream for kv head h: places below 2^31 (the offsets are int32)
 // + 2^25 requests' kRequestTokens, 32 bits without a sign.
 template <int RB>
-__device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s, char* xch, uint32_t u, int h,
-                                            int lane) {
+__device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s, const Offsets& head, char* xch,
+                                            uint32_t u, int h, int lane) {
   if (static_cast<uint64_t>(u) * s.W >= s.all) return;
-  // The places [b0, b1), from request r on: those that end at or before b0 are passed
-  // over, 64 at a time.
+  // The places [b0, b1), from request r on: those that end at or before b0 are passed over.
   const uint32_t b0 = u * s.W, b1 = min(s.all, b0 + s.W);
-  const int kv_first = max(uniform(a.kv_indptr[0]), 0);
+  const int kv_first = max(s.kv_first, 0);
+  Offsets at = head;
   int r = 0;
-  for (int at = 0; at < a.batch; at += kWave) {
-    const int e = at + lane;
-    const bool before = e < a.batch && place_of(a, e + 1, kv_first) <= static_cast<int64_t>(b0);
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(before);
-    r += __builtin_popcountll(mask);
-    if (mask != ~0ull) break;
+  while (true) {
+    const int e = at.base + lane;  // this lane's offset is where request e - 1 ends
+    const int64_t end = static_cast<int64_t>(at.k) - kv_first + static_cast<int64_t>(e) * kRequestTokens;
+    const int passed = __builtin_popcountll(
+        __builtin_amdgcn_ballot_w64(lane > 0 && e <= a.batch && end <= static_cast<int64_t>(b0)));
+    r = at.base + passed;
+    if (passed < kWindow || r >= a.batch) break;
+    at = offsets_from(a, r, lane);
   }
   for (; r < a.batch; ++r) {
-    const Request x = request_of(a, r);
+    if (r - at.base >= kWindow) at = offsets_from(a, r, lane);
+    const int i = r - at.base;
+    const auto lane_of = [](int x, int i) { return __builtin_amdgcn_readlane(x, i); };
+    const Request x = request_from(a, lane_of(at.q, i), lane_of(at.q, i + 1), lane_of(at.k, i),
+                                   lane_of(at.k, i + 1), s.q_first, s.q_end, s.kv_first, s.kv_end);
     // Its kRequestTokens places, then its tokens'.
     const int64_t rb = static_cast<int64_t>(x.kv0) - kv_first + static_cast<int64_t>(r) * kRequestTokens;
     if (rb >= b1) return;
     if (!x.ok) continue;
-    const int64_t at = rb + kRequestTokens;
-    const int s0 = static_cast<int>(max(b0 - at, int64_t{0}));
+    const int64_t own = rb + kRequestTokens;
+    const int s0 = static_cast<int>(max(b0 - own, int64_t{0}));
     Piece w;
-    w.len = static_cast<int>(min(b1 - at, static_cast<int64_t>(x.kv))) - s0;
+    w.len = static_cast<int>(min(b1 - own, static_cast<int64_t>(x.kv))) - s0;
     if (w.len <= 0) continue;
     w.idx = a.indices + x.kv0 + s0;
     w.tok0 = x.q0;
@@ -579,7 +590,9 @@ template <int RB>
 __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(PrefixArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * pf::kTileBytes];
   static_assert(sizeof(smem) >= kWaves * kWaveLds, "the waves' output rows take the tiles' place");
-  const Split s = split_of(a);
+  const int lane = threadIdx.x & 63;
+  const Offsets head = offsets_from(a, 0, lane);
+  const Split s = split_of(a, head);
   const int b = blockIdx.x;
   if (b == a.blocks - 1 && threadIdx.x == 0)
     *a.split = FoldSplit{s.first, s.rows, s.row_step, s.tiles, s.shares, static_cast<int>(s.run),
@@ -612,14 +625,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(Prefix
     }
     return;
   }
-  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = wave / a.heads;
   if (g >= a.side) return;
   const int n = a.blocks - s.tile_blocks;
   for (int v = (b - s.tile_blocks) * a.side + g; v < s.units * a.rest; v += n * a.side) {
     const int u = v / a.rest;
-    unit_pieces<RB>(a, s, smem + wave * kWaveLds, u, (v - u * a.rest) * a.heads + wave - g * a.heads, lane);
+    unit_pieces<RB>(a, s, head, smem + wave * kWaveLds, u, (v - u * a.rest) * a.heads + wave - g * a.heads, lane);
   }
 }
 
