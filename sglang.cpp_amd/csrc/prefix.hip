@@ -33,7 +33,10 @@ constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
 constexpr int kMinUnit = 16;              // shortest unit
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
-constexpr int kFoldGroups = 1024;         // workgroups of the fold up to which a row has lanes of its own
+// Workgroups of the fold up to which a lane group has one row. 512 and 4,096: 256 tokens of
+// 32 heads 127 and 127 us in all (124 so), 384 of 32 44.6 and 41.4 (42.5), 32 of 32 23.8
+// and 22.6 (22.6).
+constexpr int kFoldGroups = 1024;
 constexpr int kWaves = 4;                 // waves of a workgroup, two workgroups per CU
 constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on their way to memory
 
@@ -584,8 +587,10 @@ __device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& s
 }
 
 // Two workgroups of four waves per CU: those that walk the prefix's tiles, bound by
-// the matrix cores, lie beside the others' units, bound by memory (a CU takes in about
-// 25 GB/s whatever it has in flight, so the units need every CU).
+// the matrix cores, lie beside the others' units, bound by memory. 256 requests of 528
+// own tokens behind 16,384, 32q/8kv: the prefix alone 102 us, the own tokens alone 90,
+// together 153 (fold included; 668 MB from memory, 92 us at a read's 7.2 TB/s, and 550
+// GFLOP, 60 us at a large product's 1.19 PFLOP/s).
 template <int RB>
 __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(PrefixArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * pf::kTileBytes];
@@ -949,22 +954,27 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   a.s_o = reinterpret_cast<float*>(ws + l.s_o), a.s_lse = reinterpret_cast<float*>(ws + l.s_lse);
   a.split = reinterpret_cast<FoldSplit*>(ws + l.split);
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  // Row blocks of a request's own tokens. One and two, 64 requests of 300 own tokens,
+  // 32q/8kv: 1 query token (4 rows) 21.0 and 21.5 us, 4 (16) 25.9 and 26.9, 5 38.6 and 29.6.
   if (p.max_qo_len * a.group <= 16) launch_attention<1>(a, s);
   else launch_attention<2>(a, s);
   st = launch_status();
   if (st != SGL_OK) return st;
-  // Many pieces a row: a workgroup for each. Few: 32 lanes a row, and of many rows
-  // several a lane group (2,048 workgroups of four heads each took 12.5 us for 256 tokens
-  // of 32 heads).
-  const int64_t pieces = a.prefix == 0 ? 2
-      : a.blocks / ((static_cast<int64_t>(max_tokens) * a.group + 127) / 128 * num_kv_heads) / 2 + 2;
-  const int rows_per = pieces > 16 ? 1 : 8;
+  // Lanes of a row. A row has about 32,768 / rows pieces of the prefix (two workgroups of
+  // tiles per 128 rows and CU), at most one a tile, and a group of 32 lanes takes 4 or 8 in
+  // turn. us with 1, 2 and 8 groups: 128 rows behind 4,096 tokens 19.1, 14.4 and 12.3,
+  // 1,024 behind 1,024 17.8, 13.9, 16.8, 2,048 behind 4,096 22.7, 21.1, 23.6, 4,096 behind
+  // 1,024 20.1, 24.5, 32.3.
+  const int64_t rows = static_cast<int64_t>(max_tokens) * num_qo_heads;
+  const int sets = p.prefix_len == 0 || rows > 2048 ? 1 : rows <= 256 && p.prefix_len > 16 * pf::kBN ? 8 : 2;
+  const int rows_per = 8 / sets;
   const int all_iters = (num_qo_heads + rows_per - 1) / rows_per;
   int iters = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(max_tokens) * all_iters + kFoldGroups - 1) / kFoldGroups, all_iters));
   iters = std::max(iters, 1);
   const int head_groups = (all_iters + iters - 1) / iters;
   const dim3 fold(static_cast<uint32_t>(max_tokens) * head_groups);
-  if (rows_per == 1) hipLaunchKernelGGL(prefix_fold_kernel<8>, fold, dim3(256), 0, s, a, head_groups, iters);
+  if (sets == 8) hipLaunchKernelGGL(prefix_fold_kernel<8>, fold, dim3(256), 0, s, a, head_groups, iters);
+  else if (sets == 2) hipLaunchKernelGGL(prefix_fold_kernel<2>, fold, dim3(256), 0, s, a, head_groups, iters);
   else hipLaunchKernelGGL(prefix_fold_kernel<1>, fold, dim3(256), 0, s, a, head_groups, iters);
   return launch_status();
 }
