@@ -18,8 +18,7 @@
 // sums and walks that slice alone. Bound by reading one target row and, where a
 // draft was rejected, one draft row per request: 48 requests of a vocabulary of 151,936
 // (38 slices) 13.7 us in all, 54 MB, 3.9 TB/s; one request 8.3 us, two launches and their
-// chains of dependent loads. One launch, whose last workgroup of a request draws, would
-// need counters that someone clears and its slices' sums made visible across the L2s.
+// chains of dependent loads.
 #include "common.h"
 
 namespace sgl {
@@ -58,7 +57,7 @@ struct Request {
 };
 
 // Accepted drafts of request r, the same in every thread of the calling wave.
-__device__ __forceinline__ Request judge(const VerifyArgs& v, int r, int lane) {
+__device__ __forceinline__ Request accepted_of(const VerifyArgs& v, int r, int lane) {
   Request q;
   const int64_t d0 = v.indptr[r], d1 = v.indptr[r + 1];
   q.d0 = d0;
@@ -165,13 +164,13 @@ __device__ __forceinline__ double lane_value(double x, int at) {
 }
 
 // kRun consecutive slices a workgroup, the next one's loads in flight while one is
-// summed: the dependent loads of judge() come before 16 KB or before 64.
+// summed: the dependent loads of accepted_of() come before 16 KB or before 64.
 template <int kRun>
 __global__ void __launch_bounds__(kThreads) verify_sums_kernel(VerifyArgs v) {
   __shared__ double part[kRun][2][kWaves];
   const int s0 = blockIdx.x * kRun, r = blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const Request q = judge(v, r, lane);
+  const Request q = accepted_of(v, r, lane);
   if (s0 == 0) {
     // The accepted drafts, and -1 behind the place of the drawn token.
     for (int i = t; i < q.n; i += kThreads) {

@@ -113,6 +113,16 @@ def test_many_requests(dev):
     check(x, run(x))
 
 
+@pytest.mark.parametrize("hq,hkv,qo", [(8, 8, 1), (24, 4, 4)])
+def test_many_requests_of_all_lengths(dev, hq, hkv, qo):
+    """Units that begin and end anywhere in a list of 200 requests, empty ones among them."""
+    rng = np.random.default_rng(qo)
+    kv = rng.integers(0, 300, 200) * (rng.random(200) > 0.3)
+    n = np.minimum(rng.integers(0, qo + 1, 200), kv)
+    x = make(dev, 130, kv, n, hq, hkv, 22)
+    check(x, run(x))
+
+
 def test_offsets_past_zero_and_rows_behind(dev):
     """A part of a larger batch: offsets that start past 0, rows before and behind that
     belong to no request stay as they were."""
@@ -245,8 +255,8 @@ def test_captured_steps_share_a_workspace(dev):
 
 
 @pytest.mark.parametrize("B,qo,hq,hkv,P,own", [
-    (9, 1, 32, 8, 65, 3),        # 36 rows: the smallest batch whose prefix has workgroups of its own
-    (33, 1, 32, 8, 640, 1),      # one row more than a row tile holds
+    (9, 1, 32, 8, 65, 3),        # 36 rows of a kv head: a wave's and four more
+    (33, 1, 32, 8, 640, 1),      # one token more than a row tile holds
     (65, 1, 32, 8, 63, 20),
     (257, 1, 16, 4, 1025, 2),
     (100, 8, 16, 2, 129, 9),     # 6,400 rows a kv head
