@@ -31,7 +31,6 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kStep = 16;                 // tokens a step
-constexpr int kMinUnit = 16;              // shortest unit
 constexpr float kRescaleSlack = 8.f;      // log2 units: p <= 256 between rescales
 // Workgroups of the fold up to which a lane group has one row. 512 and 4,096: 256 tokens of
 // 32 heads 127 and 127 us in all (124 so), 384 of 32 44.6 and 41.4 (42.5), 32 of 32 23.8
@@ -56,6 +55,7 @@ struct PrefixArgs {
   const int32_t* kv_indptr;
   const int32_t* qo_indptr;
   int batch, tokens, hq, hkv, group;
+  uint32_t inv_group;    // 2^16 / group, rounded up
   int prefix, max_qo;
   int blocks;            // workgroups of the launch
   int heads, side, rest; // kv heads of a unit, units side by side in a workgroup, head groups
@@ -74,7 +74,7 @@ struct PrefixArgs {
 };
 
 // How a launch is shared out, from the lengths as they are now (so a captured launch
-// follows them): every workgroup works it out alike, in whole numbers, and one leaves the
+// follows them): every workgroup works it out alike, by the same instructions, and one leaves the
 // fold what it needs of it.
 // Workgroups [0, tile_blocks) walk the prefix's 64-token tiles for one kv head and row
 // tile at a time, per_head of them for a head: with `shares` each row tile's tiles are
@@ -98,8 +98,8 @@ struct Split {
 // of 2,000 behind 1,024 183 and 177 (183), 32 of 300 behind 4,096 26.5 and 27.9 (26.2).
 constexpr uint32_t kTileNs = 1400;
 constexpr uint32_t kTokenNs = 16;
-// A request counts as this many tokens more in the units' stream: the loads that lead
-// to its first step, about 3.4 us. 0, 24, 48 and 96 measured: 64 requests of 5 own tokens
+// A request counts as this many tokens more in the units' stream: what begins and ends
+// its walk, about 3.4 us. 0, 24, 48 and 96 measured: 64 requests of 5 own tokens
 // 16.7, 11.2, 10.3, 11.2 us; 64 of 16 behind 1,024 tokens 25.2, 25.6, 22.7, 22.8; 256 of
 // 200 behind 16,384 121 to 125 with any.
 constexpr uint32_t kRequestTokens = 48;
@@ -107,6 +107,13 @@ constexpr uint32_t kRequestTokens = 48;
 // A loaded value that is the same in every lane, in a scalar register (the compiler
 // keeps it in a vector one, as the kernel's stores might change the memory).
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// x / d for x < 2^21, d > 0: the distance of (x + 1/2) / d from a whole number is at least
+// 1 / (2 d), the product with the reciprocal off by less than 2^-22 of itself. (The split
+// of a launch took 3,500 cycles with whole-number divisions, 1,800 so.)
+__device__ __forceinline__ int quotient(int x, int d) {
+  return static_cast<int>((static_cast<float>(x) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
+}
 
 // Offsets of 63 requests from request `base` on, lane i those of request base + i and the
 // end of the one before: in registers, so that neither finding a request nor the next one
@@ -134,38 +141,44 @@ __device__ __forceinline__ Split split_of(const PrefixArgs& a, const Offsets& he
   s.row_tiles = s.row_step = s.tile_blocks = s.per_head = s.shares = 0;
   s.run = 1;
   if (s.rows > 0 && s.tiles > 0) {
+    // 32 rows a wave, up to 4 waves a row tile, spread evenly.
     const int waves = (s.rows + 31) / 32;
     s.row_tiles = (waves + kWaves - 1) / kWaves;
-    const int each = (waves + s.row_tiles - 1) / s.row_tiles;
+    const int each = 1 + (waves > s.row_tiles) + (waves > 2 * s.row_tiles) + (waves > 3 * s.row_tiles);
     s.row_step = 32 * each;
-    s.row_tiles = (waves + each - 1) / each;
     const uint32_t list = static_cast<uint32_t>(s.row_tiles) * s.tiles;  // of a head
-    const uint64_t t = static_cast<uint64_t>(list) * a.hkv * kTileNs;
-    const uint64_t sum = t + static_cast<uint64_t>(s.all) * a.hkv * kTokenNs;
-    const int shift = max(0, 42 - __builtin_clzll(sum));  // to 22 bits
-    const uint32_t ts = static_cast<uint32_t>(t >> shift), ss = static_cast<uint32_t>(sum >> shift);
+    const float t = static_cast<float>(list) * kTileNs, own = static_cast<float>(s.all) * kTokenNs;
+    const int share = static_cast<int>(a.blocks * t * __builtin_amdgcn_rcpf(t + own) + 0.5f);
     // A second workgroup of tiles on a CU brings nothing (1.4 us a tile alone, 2.7 for
     // each of two).
-    s.tile_blocks = max(1, min(static_cast<int>((a.blocks * ts + ss / 2) / ss), a.blocks / 2));
-    s.per_head = max(1, s.tile_blocks / a.hkv);
+    s.tile_blocks = max(1, min(share, a.blocks / 2));
+    s.per_head = max(1, quotient(s.tile_blocks, a.hkv));
     if (s.per_head >= s.row_tiles) {
-      int n = (s.per_head + s.row_tiles / 2) / s.row_tiles;
+      int n = quotient(s.per_head + s.row_tiles / 2, s.row_tiles);
       if (n > 1 && n * s.row_tiles * a.hkv > a.blocks / 2) --n;
-      s.run = (s.tiles + n - 1) / n;
-      s.shares = static_cast<int>((s.tiles + s.run - 1) / s.run);
+      // At least tiles / n (up to 2^23 of them: off by less than two), and the runs that are.
+      int run = static_cast<int>(s.tiles * __builtin_amdgcn_rcpf(n));
+      run += run * n < s.tiles;
+      run += run * n < s.tiles;
+      s.shares = static_cast<int>(s.tiles * __builtin_amdgcn_rcpf(run));
+      s.shares += s.shares * run < s.tiles;
+      s.shares += s.shares * run < s.tiles;
+      s.shares -= (s.shares - 1) * run >= s.tiles;
+      s.run = run;
       s.per_head = s.shares * s.row_tiles;
     } else {
       s.run = (list + s.per_head - 1) / s.per_head;
     }
     s.tile_blocks = min(s.per_head * a.hkv, a.blocks - 1);
   }
-  s.units = max(1, (a.blocks - s.tile_blocks) * a.side / a.rest);
-  const uint32_t w = s.all / static_cast<uint32_t>(s.units) + 1;  // one more where it divides
-  s.W = max((w + kStep - 1) / kStep * kStep, static_cast<uint32_t>(kMinUnit));
+  s.units = max(1, quotient((a.blocks - s.tile_blocks) * a.side, a.rest));
+  // At least all / units: the product is off by less than 2^-20 of itself.
+  uint32_t w = static_cast<uint32_t>(s.all * __builtin_amdgcn_rcpf(s.units));
+  w += (w >> 20) + 1;
+  s.W = (w + kStep - 1) / kStep * kStep;
   // Quotients come from the vector unit.
-  s.row_tiles = uniform(s.row_tiles), s.row_step = uniform(s.row_step), s.tile_blocks = uniform(s.tile_blocks);
-  s.per_head = uniform(s.per_head), s.shares = uniform(s.shares), s.run = uniform(s.run);
-  s.W = uniform(s.W), s.units = uniform(s.units);
+  s.tile_blocks = uniform(s.tile_blocks), s.per_head = uniform(s.per_head), s.shares = uniform(s.shares);
+  s.run = uniform(s.run), s.W = uniform(s.W), s.units = uniform(s.units);
   return s;
 }
 
@@ -255,8 +268,8 @@ __device__ __forceinline__ void walk(const PrefixArgs& a, const Piece& w, char* 
   for (int i = 0; i < 2; ++i) slot[i] = w.idx[min((kDepth + i) * kStep + n, len - 1)];
   // Token and head of this lane's row of each block; rows past the last one read
   // its Q again and see nothing.
-  const int i0 = w.row0 / G, rem = w.row0 - i0 * G;
-  const uint32_t inv_g = (65536u + G - 1) / G;  // (rem + x) / G as a product, both below 128
+  const int i0 = uniform(quotient(w.row0, G)), rem = w.row0 - i0 * G;
+  const uint32_t inv_g = a.inv_group;  // (rem + x) / G as a product, both below 128
   int tok[RB], head[RB], sees[RB];
   u32x4_t q[RB][4];
 #pragma unroll
@@ -604,11 +617,11 @@ __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(Prefix
                          static_cast<int>(s.W), 0};
   if (b < s.tile_blocks) {
     for (int v = b; v < s.per_head * a.hkv; v += s.tile_blocks) {
-      const int j = v / a.hkv, h = v - j * a.hkv;
+      const int j = quotient(v, a.hkv), h = v - j * a.hkv;
       const int run = static_cast<int>(s.run);
       int rt, tb, left, piece;
       if (s.shares > 0) {
-        rt = j / s.shares;
+        rt = quotient(j, s.shares);
         piece = j - rt * s.shares;
         tb = piece * run;
         left = min(s.tiles - tb, run);
@@ -631,11 +644,11 @@ __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(Prefix
     return;
   }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = wave / a.heads;
+  const int g = uniform(quotient(wave, a.heads));
   if (g >= a.side) return;
   const int n = a.blocks - s.tile_blocks;
   for (int v = (b - s.tile_blocks) * a.side + g; v < s.units * a.rest; v += n * a.side) {
-    const int u = v / a.rest;
+    const int u = uniform(quotient(v, a.rest));
     unit_pieces<RB>(a, s, head, smem + wave * kWaveLds, u, (v - u * a.rest) * a.heads + wave - g * a.heads, lane);
   }
 }
@@ -946,6 +959,7 @@ extern "C" int sgl_prefix_attention(const sgl_prefix_plan_t* plan, const void* q
   a.pidx = prefix_indices, a.indices = indices, a.kv_indptr = kv_indptr, a.qo_indptr = qo_indptr;
   a.batch = batch_size, a.tokens = max_tokens;
   a.hq = num_qo_heads, a.hkv = num_kv_heads, a.group = num_qo_heads / num_kv_heads;
+  a.inv_group = (65536u + a.group - 1) / a.group;
   a.prefix = p.prefix_len, a.max_qo = p.max_qo_len, a.blocks = p.num_blocks;
   a.heads = heads_per_group(num_kv_heads), a.side = kWaves / a.heads, a.rest = num_kv_heads / a.heads;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
