@@ -559,8 +559,7 @@ int sgl_paged_mixed(const sgl_decode_plan_t* plan, const void* q,
  *     depend on the requests' own lengths, so it serves every step of a batch (graph
  *     capture and replay) behind a prefix of prefix_len. Up to 2^29 tokens of prefix,
  *     2^25 requests, 2^24 - 1 query tokens, 2^30 of them times the heads of a kv head, 2^31
- *     times num_qo_heads; and the 64-token tiles of the prefix times the 128-row tiles of
- *     the query tokens times num_kv_heads below 2^31.
+ *     times num_qo_heads.
  *   sgl_prefix_attention: q and o have max_tokens rows here (at most the plan's);
  *     rows outside [qo_indptr[0], qo_indptr[batch_size]) are left as they were. The
  *     offsets may start past 0 (a part of a larger batch); they must not decrease. A

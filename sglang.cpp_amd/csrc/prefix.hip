@@ -41,7 +41,7 @@ constexpr int kWaveLds = 8192;            // a wave's LDS for its output rows on
 
 // What the fold needs of a launch's Split.
 struct alignas(16) FoldSplit {
-  int first, rows, row_step, tiles, shares, run, W, pad;
+  int first, rows, shares, W;
 };
 
 struct PrefixArgs {
@@ -76,18 +76,16 @@ struct PrefixArgs {
 // How a launch is shared out, from the lengths as they are now (so a captured launch
 // follows them): every workgroup works it out alike, by the same instructions, and one leaves the
 // fold what it needs of it.
-// Workgroups [0, tile_blocks) walk the prefix's 64-token tiles for one kv head and row
-// tile at a time, per_head of them for a head: with `shares` each row tile's tiles are
-// cut into that many runs (all row tiles alike, so that the workgroups of a head, on the
-// same XCD where there are eight heads, read the same K/V at the same time), else the
-// list (row tile, tile) into per_head runs. The others' units walk the stream of `all`
-// tokens, W a unit.
+// Workgroups [0, tile_blocks) walk the prefix's 64-token tiles, `run` of them for one row
+// tile and kv head at a time: each row tile's tiles are cut into `shares` runs, all row
+// tiles alike and taken run by run, so that the `wide` workgroups of a head, on the same
+// XCD where there are eight heads, read the same K/V at about the same time. The others'
+// units walk the stream of `all` tokens, W a unit.
 struct Split {
   int first, rows;          // first query token, packed rows of a kv head
   int row_tiles, row_step;  // row tiles and their rows (32 a wave, spread evenly)
   int tiles;                // 64-token tiles of the prefix
-  int tile_blocks, per_head, shares;
-  uint32_t run;
+  int tile_blocks, wide, shares, run;
   uint32_t all, W;
   int units;
   int q_first, q_end, kv_first, kv_end;  // the batch's offsets
@@ -115,6 +113,20 @@ __device__ __forceinline__ int quotient(int x, int d) {
   return static_cast<int>((static_cast<float>(x) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
 }
 
+// Minimum over the wave: shifts by 1, 2, 4 and 8 in each row of 16, then the last lane of
+// a row to the next row, of the first half to the second, whose last lane has it.
+__device__ __forceinline__ float wave_min(float x) {
+  const auto with = [](float x, int y) { return fminf(x, __builtin_bit_cast(float, y)); };
+  const int inf = __builtin_bit_cast(int, INFINITY);
+  x = with(x, __builtin_amdgcn_update_dpp(inf, __builtin_bit_cast(int, x), 0x111, 0xF, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(inf, __builtin_bit_cast(int, x), 0x112, 0xF, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(inf, __builtin_bit_cast(int, x), 0x114, 0xF, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(inf, __builtin_bit_cast(int, x), 0x118, 0xF, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(inf, __builtin_bit_cast(int, x), 0x142, 0xA, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(inf, __builtin_bit_cast(int, x), 0x143, 0xC, 0xF, false));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
 // Offsets of 63 requests from request `base` on, lane i those of request base + i and the
 // end of the one before: in registers, so that neither finding a request nor the next one
 // of a walk waits for memory.
@@ -138,38 +150,51 @@ __device__ __forceinline__ Split split_of(const PrefixArgs& a, const Offsets& he
   s.rows = max(min(s.q_end, a.tokens) - s.first, 0) * a.group;
   s.all = static_cast<uint32_t>(max(s.kv_end - max(s.kv_first, 0), 0)) + a.batch * kRequestTokens;
   s.tiles = (a.prefix + pf::kBN - 1) / pf::kBN;
-  s.row_tiles = s.row_step = s.tile_blocks = s.per_head = s.shares = 0;
-  s.run = 1;
+  s.row_tiles = s.row_step = s.tile_blocks = s.wide = s.shares = s.run = 0;
   if (s.rows > 0 && s.tiles > 0) {
     // 32 rows a wave, up to 4 waves a row tile, spread evenly.
     const int waves = (s.rows + 31) / 32;
     s.row_tiles = (waves + kWaves - 1) / kWaves;
     const int each = 1 + (waves > s.row_tiles) + (waves > 2 * s.row_tiles) + (waves > 3 * s.row_tiles);
     s.row_step = 32 * each;
-    const uint32_t list = static_cast<uint32_t>(s.row_tiles) * s.tiles;  // of a head
-    const float t = static_cast<float>(list) * kTileNs, own = static_cast<float>(s.all) * kTokenNs;
+    const float t = static_cast<float>(s.row_tiles) * s.tiles * kTileNs, own = static_cast<float>(s.all) * kTokenNs;
     const int share = static_cast<int>(a.blocks * t * __builtin_amdgcn_rcpf(t + own) + 0.5f);
     // A second workgroup of tiles on a CU brings nothing (1.4 us a tile alone, 2.7 for
     // each of two).
     s.tile_blocks = max(1, min(share, a.blocks / 2));
-    s.per_head = max(1, quotient(s.tile_blocks, a.hkv));
-    if (s.per_head >= s.row_tiles) {
-      int n = quotient(s.per_head + s.row_tiles / 2, s.row_tiles);
-      if (n > 1 && n * s.row_tiles * a.hkv > a.blocks / 2) --n;
-      // At least tiles / n (up to 2^23 of them: off by less than two), and the runs that are.
-      int run = static_cast<int>(s.tiles * __builtin_amdgcn_rcpf(n));
-      run += run * n < s.tiles;
-      run += run * n < s.tiles;
-      s.shares = static_cast<int>(s.tiles * __builtin_amdgcn_rcpf(run));
-      s.shares += s.shares * run < s.tiles;
-      s.shares += s.shares * run < s.tiles;
-      s.shares -= (s.shares - 1) * run >= s.tiles;
-      s.run = run;
-      s.per_head = s.shares * s.row_tiles;
-    } else {
-      s.run = (list + s.per_head - 1) / s.per_head;
+    s.wide = max(1, quotient(s.tile_blocks, a.hkv));
+    s.wide = max(1, min(s.wide + s.wide / 8, quotient(a.blocks / 2, a.hkv)));
+    // The number of runs. Many workgroups a row tile: one each. Else candidates, one a lane:
+    // the tiles of the rounds that they take, what begins and ends a run (six tiles' time),
+    // and a 43rd of a tile for the partial rows of a run and row tile, written and folded.
+    // The workspace has room for two runs a row tile, or for as many as there are
+    // workgroups. 640 requests behind 16,384 tokens, 32q/8kv (20 row tiles for 32
+    // workgroups): one run each 295 us, three in two rounds 249.
+    int take = min(quotient(s.wide, s.row_tiles), s.tiles);
+    float k = 1.f;
+    if (s.wide < 8 * s.row_tiles) {
+      const int n = 1 + static_cast<int>(threadIdx.x & 63);
+      const float items = static_cast<float>(n) * s.row_tiles;
+      const float rounds = ceilf((items - 0.5f) * __builtin_amdgcn_rcpf(s.wide));
+      const float cost = rounds * (ceilf((s.tiles - 0.5f) * __builtin_amdgcn_rcpf(n)) + 6.f) + items * a.hkv * (1.f / 43.f);
+      const bool fits = n <= s.tiles && (n <= 2 || (items - 2.f * s.row_tiles) * a.hkv <= a.blocks);
+      const float best = wave_min(fits ? cost : INFINITY);
+      take = __builtin_ctzll(__builtin_amdgcn_ballot_w64(fits && cost == best));
+      k = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rounds), take));
+      ++take;
     }
-    s.tile_blocks = min(s.per_head * a.hkv, a.blocks - 1);
+    // At least tiles / take (up to 2^23 of them: off by less than two), and the runs that are.
+    int run = static_cast<int>(s.tiles * __builtin_amdgcn_rcpf(take));
+    run += run * take < s.tiles;
+    run += run * take < s.tiles;
+    int shares = static_cast<int>(s.tiles * __builtin_amdgcn_rcpf(run));
+    shares += shares * run < s.tiles;
+    shares += shares * run < s.tiles;
+    shares -= (shares - 1) * run >= s.tiles;
+    s.run = uniform(run), s.shares = uniform(shares);
+    const int all = s.shares * s.row_tiles;
+    s.wide = uniform(min(min(s.wide, all), static_cast<int>(all * __builtin_amdgcn_rcpf(k)) + 1));
+    s.tile_blocks = min(s.wide * a.hkv, a.blocks / 2);
   }
   s.units = max(1, quotient((a.blocks - s.tile_blocks) * a.side, a.rest));
   // At least all / units: the product is off by less than 2^-20 of itself.
@@ -177,8 +202,7 @@ __device__ __forceinline__ Split split_of(const PrefixArgs& a, const Offsets& he
   w += (w >> 20) + 1;
   s.W = (w + kStep - 1) / kStep * kStep;
   // Quotients come from the vector unit.
-  s.tile_blocks = uniform(s.tile_blocks), s.per_head = uniform(s.per_head), s.shares = uniform(s.shares);
-  s.run = uniform(s.run), s.W = uniform(s.W), s.units = uniform(s.units);
+  s.W = uniform(s.W), s.units = uniform(s.units);
   return s;
 }
 
@@ -613,32 +637,19 @@ __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(Prefix
   const Split s = split_of(a, head);
   const int b = blockIdx.x;
   if (b == a.blocks - 1 && threadIdx.x == 0)
-    *a.split = FoldSplit{s.first, s.rows, s.row_step, s.tiles, s.shares, static_cast<int>(s.run),
-                         static_cast<int>(s.W), 0};
+    *a.split = FoldSplit{s.first, s.rows, s.shares, static_cast<int>(s.W)};
   if (b < s.tile_blocks) {
-    for (int v = b; v < s.per_head * a.hkv; v += s.tile_blocks) {
-      const int j = quotient(v, a.hkv), h = v - j * a.hkv;
-      const int run = static_cast<int>(s.run);
-      int rt, tb, left, piece;
-      if (s.shares > 0) {
-        rt = quotient(j, s.shares);
-        piece = j - rt * s.shares;
-        tb = piece * run;
-        left = min(s.tiles - tb, run);
-      } else {
-        const uint32_t at = j * s.run, end = min(static_cast<uint32_t>(s.row_tiles) * s.tiles, at + s.run);
-        rt = static_cast<int>(at / static_cast<uint32_t>(s.tiles));
-        piece = j - static_cast<int>(rt * static_cast<uint32_t>(s.tiles) / s.run);
-        tb = static_cast<int>(at - rt * s.tiles);
-        left = end > at ? static_cast<int>(end - at) : 0;
-      }
-      while (left > 0) {
-        const int te = min(s.tiles, tb + left);
-        prefix_tiles(a, s, smem, uniform(rt), uniform(h), uniform(tb), uniform(te), uniform(piece));
-        left -= te - tb;
-        ++rt;  // its first run is number rt tiles / run
-        piece = j - static_cast<int>(rt * static_cast<uint32_t>(s.tiles) / s.run);
-        tb = 0;
+    // Workgroup b has head b % hkv and every wide-th item of it, or, with more heads than
+    // workgroups, every tile_blocks-th head and all of its items.
+    const bool few = s.wide * a.hkv > s.tile_blocks;
+    const int j0 = few ? 0 : uniform(quotient(b, a.hkv)), wide = few ? 1 : s.wide;
+    const int first_run = uniform(quotient(j0, s.row_tiles));
+    for (int h = b - j0 * a.hkv; h < a.hkv; h += few ? s.tile_blocks : a.hkv) {
+      int piece = first_run, rt = j0 - first_run * s.row_tiles;
+      while (piece < s.shares) {
+        const int tb = piece * s.run;
+        prefix_tiles(a, s, smem, rt, h, tb, min(s.tiles, tb + s.run), piece);
+        for (rt += wide; rt >= s.row_tiles; rt -= s.row_tiles) ++piece;
       }
     }
     return;
@@ -720,8 +731,7 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
   FoldSplit sp = *a.split;
   const int q_first = a.qo_indptr[0], q_end = a.qo_indptr[a.batch];
   const int kv_first = uniform(a.kv_indptr[0]), kv_end = a.kv_indptr[a.batch];
-  sp = FoldSplit{uniform(sp.first), uniform(sp.rows), uniform(sp.row_step), uniform(sp.tiles),
-                 uniform(sp.shares), uniform(sp.run), uniform(sp.W), 0};
+  sp = FoldSplit{uniform(sp.first), uniform(sp.rows), uniform(sp.shares), uniform(sp.W)};
   if (lane == 0) found[wave][0] = r;
   __syncthreads();
   int from = 3;
@@ -757,11 +767,7 @@ __global__ void __launch_bounds__(256) prefix_fold_kernel(PrefixArgs a, int head
     if (folded) {
       // Prefix pieces: np of them, p_step rows apart.
       const int prow = row_of_head + hh - h * a.group;
-      int np = sp.shares;
-      if (np == 0 && sp.row_step > 0) {
-        const uint32_t run = sp.run, at = static_cast<uint32_t>(prow / sp.row_step) * sp.tiles;
-        np = static_cast<int>((at + sp.tiles - 1) / run - at / run) + 1;
-      }
+      const int np = sp.shares;
       const int64_t p_step = static_cast<int64_t>(a.hkv) * sp.rows, p0 = static_cast<int64_t>(h) * sp.rows + prow;
       for (int k0 = set; k0 < np + ns; k0 += kLoads * kSets) {
         f32x4_t v[kLoads];
@@ -877,12 +883,11 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
   if (head_dim != kD || group > 64 || max_qo_len > SGL_PREFIX_MAX_QO ||
       num_kv_heads > 65535 || prefix_len > (1 << 29) || batch_size > (1 << 25))
     return SGL_ERR_UNSUPPORTED;
-  // Packed rows, and the list of tiles, are counted in 32 bits, and so are the threads of
-  // the fold's launch, a workgroup of 256 a token from kFoldGroups tokens on.
+  // Packed rows are counted in 32 bits, and so are the threads of the fold's launch, a
+  // workgroup of 256 a token from kFoldGroups tokens on.
   const int64_t rows = static_cast<int64_t>(max_tokens) * group;
-  const int64_t row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves), tiles = (prefix_len + pf::kBN - 1) / pf::kBN;
-  if (rows > (1 << 30) || max_tokens >= 1 << 24 || static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff ||
-      row_tiles * num_kv_heads > 0x7fffffff / (tiles > 0 ? tiles : 1))
+  const int64_t row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
+  if (rows > (1 << 30) || max_tokens >= 1 << 24 || static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff)
     return SGL_ERR_UNSUPPORTED;
   p = sgl_prefix_plan_t{};
   p.prefix_len = prefix_len, p.batch_size = batch_size, p.max_tokens = max_tokens, p.max_qo_len = max_qo_len;
@@ -891,8 +896,7 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
   const int heads = heads_per_group(num_kv_heads);
   const int64_t units = static_cast<int64_t>(blocks) * (kWaves / heads) / (num_kv_heads / heads);
   p.max_units = static_cast<int32_t>(units < 1 ? 1 : units);
-  // At most `blocks` shares of a row tile and head, or two runs that each of them lies in,
-  // of up to 128 rows.
+  // Two runs of a row tile and head, or as many as there are workgroups, of up to 128 rows.
   if (prefix_len > 0) p.prefix_rows = (blocks + 2 * row_tiles * num_kv_heads) * std::min<int64_t>(rows, 32 * kWaves);
   p.workspace_bytes = workspace_layout(p).total;
   return SGL_OK;
