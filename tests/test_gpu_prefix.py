@@ -140,6 +140,13 @@ def test_a_plan_for_more_and_the_backend(dev):
     assert torch.equal(o, run(x))
 
 
+@pytest.mark.parametrize("scale", [0.02, 0.15])
+def test_other_scales(dev, scale):
+    x = make(dev, 300, [20, 90, 1], [1, 2, 1], 16, 4, 24)
+    x["scale"] = scale
+    check(x, run(x))
+
+
 def test_equals_decode_and_prefill_of_the_joined_sequences(dev):
     """Within both sides' bounds: the paged decode kernel over prefix + own tokens."""
     x = make(dev, 400, [20, 90, 1, 300], [1, 1, 1, 1], 32, 8, 15)

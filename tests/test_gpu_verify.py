@@ -147,6 +147,16 @@ def test_views_streams_and_graphs(dev):
         check(batch([2, 2], 777, seed), dev)
 
 
+def test_rows_past_32_bits(dev):
+    """Rows 2^31 + 8 elements apart: the third one begins past 2^32."""
+    x = batch([2], 4099, 12)
+    wide = torch.empty((3, (1 << 31) + 8), device=dev)
+    target = wide[:, :4099]
+    target.copy_(torch.from_numpy(x["target"]))
+    for accept in (x["accept"], np.zeros(2, np.float32), np.full(2, 0.999, np.float32)):
+        check({**x, "accept": accept}, dev, target=target)
+
+
 def test_tokens_follow_the_target(dev):
     """20,000 requests with one draft each: the first emitted token has the target's
     distribution. Each count is binomial; 5 standard deviations (and a half) bound it."""
