@@ -19,9 +19,14 @@ namespace {
 
 constexpr int kMaxPairs = 256;
 
-// Quarter turns per position of each pair: f_i 2 / pi.
+constexpr int kFewPairs = 64;
+
+// Quarter turns per position of each pair: f_i 2 / pi. A launch copies its arguments, so
+// few pairs have a small one (4,096 positions of 32 pairs 6.8 us a call with room for 256
+// pairs, 6.4 with room for 64).
+template <int P>
 struct TurnArgs {
-  double turns[kMaxPairs];
+  double turns[P];
 };
 
 // cos and sin of x quarter turns, |x| < 2^31, x in 64 bits: the nearest whole
@@ -52,11 +57,11 @@ __device__ __forceinline__ void cos_sin_turns(double x, float& c, float& s) {
 // an entry costs one 64-bit product and the series. Bound by its stores: 131,072
 // positions of 64 pairs (67 MB) 12.2 us, 5.5 TB/s (a fill of 1 GiB 6.85); a few thousand
 // positions by the launch.
-template <int N>
+template <int N, int P>
 __global__ void __launch_bounds__(256) rope_table_kernel(float* __restrict__ cos_cache,
                                                          float* __restrict__ sin_cache,
                                                          int64_t max_pos, int half, float m,
-                                                         int rows, TurnArgs t) {
+                                                         int rows, TurnArgs<P> t) {
   const int cols = half / N;  // threads of a position
   const int r = threadIdx.x / cols;
   const int col = threadIdx.x - r * cols;
@@ -309,6 +314,21 @@ void launch_chunks(const AppendArgs& a, hipStream_t s) {
   }
 }
 
+template <int P>
+int launch_table(float* cos_cache, float* sin_cache, int64_t max_pos, int half, float m, const double* f, hipStream_t s) {
+  TurnArgs<P> t{};
+  for (int i = 0; i < half; ++i) t.turns[i] = f[i];
+  const bool wide = half % 4 == 0 && aligned16(cos_cache) && aligned16(sin_cache);
+  const int rows = 256 / (wide ? half / 4 : half);
+  const int64_t blocks = (max_pos + rows - 1) / rows;
+  const dim3 grid(static_cast<uint32_t>(blocks < 4096 ? blocks : 4096));
+  if (wide)
+    hipLaunchKernelGGL((rope_table_kernel<4, P>), grid, dim3(256), 0, s, cos_cache, sin_cache, max_pos, half, m, rows, t);
+  else
+    hipLaunchKernelGGL((rope_table_kernel<1, P>), grid, dim3(256), 0, s, cos_cache, sin_cache, max_pos, half, m, rows, t);
+  return launch_status();
+}
+
 template <int DT>
 void launch_chunks(const AppendArgs& a, bool interleaved, hipStream_t s) {
   const int64_t bytes = a.tokens * (static_cast<int64_t>(a.hq) + a.hk + a.hv) * a.d * 4;
@@ -397,25 +417,15 @@ extern "C" int sgl_rope_scaled_cache(float* cos_cache, float* sin_cache, int64_t
   if (st != SGL_OK) return st;
   if (max_pos == 0) return SGL_OK;
   if (!cos_cache || !sin_cache) return SGL_ERR_INVALID_ARG;
-  TurnArgs t;
   for (int i = 0; i < half; ++i) {
-    t.turns[i] = f[i] * 0.636619772367581343076;  // 2 / pi
+    f[i] *= 0.636619772367581343076;  // 2 / pi
     // The whole quarter turns of the last position are counted in 31 bits.
-    if (!(t.turns[i] * static_cast<double>(max_pos) < 2147483647.0)) return SGL_ERR_UNSUPPORTED;
+    if (!(f[i] * static_cast<double>(max_pos) < 2147483647.0)) return SGL_ERR_UNSUPPORTED;
   }
-  const bool wide = half % 4 == 0 && aligned16(cos_cache) && aligned16(sin_cache);
-  const int cols = wide ? half / 4 : half;
-  const int rows = 256 / cols;
-  const int64_t blocks = blocks_for(max_pos, rows);
-  const dim3 grid(static_cast<uint32_t>(blocks < 4096 ? blocks : 4096));
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (wide)
-    hipLaunchKernelGGL(rope_table_kernel<4>, grid, dim3(256), 0, s, cos_cache, sin_cache, max_pos,
-                       half, static_cast<float>(m), rows, t);
-  else
-    hipLaunchKernelGGL(rope_table_kernel<1>, grid, dim3(256), 0, s, cos_cache, sin_cache, max_pos,
-                       half, static_cast<float>(m), rows, t);
-  return launch_status();
+  if (half <= kFewPairs)
+    return launch_table<kFewPairs>(cos_cache, sin_cache, max_pos, half, static_cast<float>(m), f, s);
+  return launch_table<kMaxPairs>(cos_cache, sin_cache, max_pos, half, static_cast<float>(m), f, s);
 }
 
 extern "C" int sgl_rope_append(const sgl_rope_append_t* args, void* stream) {
