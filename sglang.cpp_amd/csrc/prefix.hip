@@ -674,6 +674,7 @@ __device__ __forceinline__ float half_sum(float x) {
 // The row again, token by token over those it sees, by 32 lanes (4 values each):
 // for rows that do not see the whole prefix, and for those whose products brought in
 // a V value that is not finite from a token they do not see (0 x inf).
+// Bound by its instructions: 12,288 rows of 6,000 tokens 4.9 ms (6.6 with one token's loads in flight).
 __device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request& x, int tok, int head,
                                              int64_t sees, int c) {
   const int h = head / a.group;
@@ -681,20 +682,34 @@ __device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request&
   const float q[4] = {bf16_lo(qw[0]), bf16_hi(qw[0]), bf16_lo(qw[1]), bf16_hi(qw[1])};
   float m = -INFINITY, l = 0.f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t t = 0; t < sees; ++t) {
-    const int64_t slot = static_cast<uint32_t>(t < a.prefix ? a.pidx[t] : a.indices[x.kv0 + (t - a.prefix)]);
-    const u32x2_t kw = *reinterpret_cast<const u32x2_t*>(a.kc + slot * a.kv_ss + h * a.kv_sh + 4 * c);
-    const u32x2_t vw = *reinterpret_cast<const u32x2_t*>(a.vc + slot * a.kv_ss + h * a.kv_sh + 4 * c);
-    float s = q[0] * bf16_lo(kw[0]) + q[1] * bf16_hi(kw[0]) + q[2] * bf16_lo(kw[1]) + q[3] * bf16_hi(kw[1]);
-    s = half_sum(s) * a.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float p = s == -INFINITY ? 0.f : exp2f(s - mn);  // NaN stays NaN
-    l = l * alpha + p;
-    const f32x4_t v = {bf16_lo(vw[0]), bf16_hi(vw[0]), bf16_lo(vw[1]), bf16_hi(vw[1])};
+  constexpr int kAhead = 8;  // tokens whose loads are in flight together
+  for (int64_t t0 = 0; t0 < sees; t0 += kAhead) {
+    u32x2_t kw[kAhead], vw[kAhead];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * alpha + p * v[i];
-    m = mn;
+    for (int e = 0; e < kAhead; ++e) {
+      const int64_t t = min(t0 + e, sees - 1);
+      const int64_t slot = static_cast<uint32_t>(t < a.prefix ? a.pidx[t] : a.indices[x.kv0 + (t - a.prefix)]);
+      kw[e] = *reinterpret_cast<const u32x2_t*>(a.kc + slot * a.kv_ss + h * a.kv_sh + 4 * c);
+      vw[e] = *reinterpret_cast<const u32x2_t*>(a.vc + slot * a.kv_ss + h * a.kv_sh + 4 * c);
+    }
+    float s[kAhead];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      s[e] = q[0] * bf16_lo(kw[e][0]) + q[1] * bf16_hi(kw[e][0]) + q[2] * bf16_lo(kw[e][1]) + q[3] * bf16_hi(kw[e][1]);
+      s[e] = half_sum(s[e]) * a.scale_log2;
+    }
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (t0 + e >= sees) break;
+      const float mn = fmaxf(m, s[e]);
+      const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
+      const float p = s[e] == -INFINITY ? 0.f : exp2f(s[e] - mn);  // NaN stays NaN
+      l = l * alpha + p;
+      const f32x4_t v = {bf16_lo(vw[e][0]), bf16_hi(vw[e][0]), bf16_lo(vw[e][1]), bf16_hi(vw[e][1])};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * alpha + p * v[i];
+      m = mn;
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   return acc * inv;
