@@ -552,7 +552,8 @@ int sgl_paged_mixed(const sgl_decode_plan_t* plan, const void* q,
  * i sees kv j with j <= i + kv_len - qo_len, kv_len = prefix_len + own length: the
  * result of sgl_paged_prefill over the joined sequences (of sgl_paged_decode for one
  * query token). A row that sees nothing is zero. K and V of tokens a row does not see
- * never reach it, whatever they hold. Rows that see less than the prefix (a request with
+ * never reach it, whatever they hold; a V value that it sees and that is not finite makes
+ * that element NaN or infinite. Rows that see less than the prefix (a request with
  * fewer own tokens than query tokens) are computed one by one: right, not fast.
  *   sgl_prefix_plan: host plan for up to batch_size requests with up to max_tokens query
  *     tokens together (max_qo_len of one request at most SGL_PREFIX_MAX_QO). It does not
