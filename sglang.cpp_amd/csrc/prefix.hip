@@ -888,11 +888,11 @@ Layout workspace_layout(const sgl_prefix_plan_t& p) {
   return l;
 }
 
-// The plan for workgroups `blocks`; everything else follows from the sizes.
-int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, int num_qo_heads,
-              int num_kv_heads, int head_dim, int blocks, sgl_prefix_plan_t& p) {
+// What a plan's sizes may be; the device is asked for its CUs only behind this.
+int check_sizes(int prefix_len, int batch_size, int max_tokens, int max_qo_len, int num_qo_heads,
+                int num_kv_heads, int head_dim) {
   if (prefix_len < 0 || batch_size < 0 || max_tokens < 0 || max_qo_len < 0 || num_qo_heads <= 0 ||
-      num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0 || blocks < 2 || blocks > 1022)
+      num_kv_heads <= 0 || num_qo_heads % num_kv_heads != 0)
     return SGL_ERR_INVALID_ARG;
   const int group = num_qo_heads / num_kv_heads;
   if (head_dim != kD || group > 64 || max_qo_len > SGL_PREFIX_MAX_QO ||
@@ -900,10 +900,20 @@ int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, in
     return SGL_ERR_UNSUPPORTED;
   // Packed rows are counted in 32 bits, and so are the threads of the fold's launch, a
   // workgroup of 256 a token from kFoldGroups tokens on.
-  const int64_t rows = static_cast<int64_t>(max_tokens) * group;
-  const int64_t row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
-  if (rows > (1 << 30) || max_tokens >= 1 << 24 || static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff)
+  if (static_cast<int64_t>(max_tokens) * group > (1 << 30) || max_tokens >= 1 << 24 ||
+      static_cast<int64_t>(max_tokens) * num_qo_heads > 0x7fffffff)
     return SGL_ERR_UNSUPPORTED;
+  return SGL_OK;
+}
+
+// The plan for workgroups `blocks`; everything else follows from the sizes.
+int make_plan(int prefix_len, int batch_size, int max_tokens, int max_qo_len, int num_qo_heads,
+              int num_kv_heads, int head_dim, int blocks, sgl_prefix_plan_t& p) {
+  const int st = check_sizes(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads, num_kv_heads, head_dim);
+  if (st != SGL_OK) return st;
+  if (blocks < 2 || blocks > 1022) return SGL_ERR_INVALID_ARG;
+  const int64_t rows = static_cast<int64_t>(max_tokens) * (num_qo_heads / num_kv_heads);
+  const int64_t row_tiles = (rows + 32 * kWaves - 1) / (32 * kWaves);
   p = sgl_prefix_plan_t{};
   p.prefix_len = prefix_len, p.batch_size = batch_size, p.max_tokens = max_tokens, p.max_qo_len = max_qo_len;
   p.num_qo_heads = num_qo_heads, p.num_kv_heads = num_kv_heads, p.head_dim = head_dim;
@@ -931,6 +941,8 @@ extern "C" int sgl_prefix_plan(int prefix_len, int batch_size, int max_tokens, i
                                int num_qo_heads, int num_kv_heads, int head_dim,
                                sgl_prefix_plan_t* plan) {
   if (!plan) return SGL_ERR_INVALID_ARG;
+  const int st = check_sizes(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads, num_kv_heads, head_dim);
+  if (st != SGL_OK) return st;
   return make_plan(prefix_len, batch_size, max_tokens, max_qo_len, num_qo_heads, num_kv_heads, head_dim,
                    std::min(2 * device_cus(), 1022), *plan);
 }

@@ -1,8 +1,13 @@
 """What the shared-prefix step's operators refuse, and their host logic, without a GPU:
-none of these calls reaches the HIP runtime. Status codes: -1 invalid argument, -2
+of these calls only a valid plan reaches the HIP runtime, for the device's CUs (256 where
+there is none). Status codes: -1 invalid argument, -2
 unsupported, -3 capacity, -4 alignment."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -155,3 +160,24 @@ def test_host_tensors_are_refused():
         be.verify_drafts(z(1, 4), None, z(0, dtype=torch.int32), z(2, dtype=torch.int32), z(0), z(1))
     with pytest.raises(RuntimeError):
         be.rope_scaled_cache(4, 7, 1e4)
+
+
+def test_refused_prefix_plans_do_not_ask_the_device():
+    """A refused plan is refused from its numbers alone: the runtime's own log of calls, in a
+    process of its own, holds none behind the mark (a valid plan asks for the device's CUs)."""
+    root = Path(__file__).resolve().parents[1]
+    code = """
+import ctypes, sys
+import __graft_entry__ as entry
+capi = entry.load_package().capi
+lib, p = capi.lib(), capi.PrefixPlan()
+print("mark", file=sys.stderr, flush=True)
+sizes = [(-1, 4, 8, 2, 8, 2, 128), (100, 4, 8, 2, 8, 3, 128), (100, 4, 8, 2, 8, 2, 64), (100, 4, 1 << 29, 2, 8, 2, 128)]
+print(*(lib.sgl_prefix_plan(*x, ctypes.byref(p)) for x in sizes), lib.sgl_prefix_plan(*sizes[0], None))
+print("mark", file=sys.stderr, flush=True)
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300,
+                          env={**os.environ, "AMD_LOG_LEVEL": "3"})
+    assert done.returncode == 0 and done.stdout.split() == ["-1", "-1", "-2", "-2", "-1"], done.stderr[-2000:]
+    between = done.stderr.split("mark\n")
+    assert len(between) == 3 and "hip" not in between[1], between[1]
