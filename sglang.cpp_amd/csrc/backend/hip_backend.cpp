@@ -1486,6 +1486,8 @@ AttentionLayer::AttentionLayer(int layer_id, int num_qo_heads, int num_kv_heads,
   TORCH_CHECK(backend_ && rotary_, "AttentionLayer needs a backend and a rotary embedding");
   TORCH_CHECK(static_cast<bool>(q_norm_) == static_cast<bool>(k_norm_),
               "the fused pass needs both q and k norms or neither");
+  TORCH_CHECK(rotary_->rotary_dim() <= head_dim_, "the rotary embedding turns ", rotary_->rotary_dim(),
+              " elements of a head of ", head_dim_);
 }
 
 torch::Tensor AttentionLayer::forward(const torch::Tensor& qkv, const torch::Tensor& positions,

@@ -224,3 +224,40 @@ def test_attention_layer_with_other_rotations(be, dev, decode, interleaved, rota
         outs.append((o, cache.buffer()))
     for a, c in zip(*outs):
         assert torch.equal(a.view(torch.int16), c.view(torch.int16))
+
+
+def layer_parts(be, dev, decode):
+    """A backend over a filled cache, one prepared batch and its qkv rows (32q/8kv)."""
+    hq, hkv, layers = 32, 8, 2
+    b = wl.make_paged_batch(np.random.default_rng(9), [49, 8] if decode else [0, 40],
+                            [50, 9] if decode else [33, 95], page_size=16, decode=decode)
+    g = torch.Generator(device=dev)
+    g.manual_seed(9)
+    cache = be.MHAKVCache(hkv, layers, D, b.num_pages + 1, 16, 0)
+    cache.buffer().copy_(torch.randn(cache.buffer().shape, generator=g, device=dev))
+    backend = be.HipAttnBackend(cache, hq, hkv, D)
+    backend.set_page_table(torch.from_numpy(b.page_table).to(dev))
+    reqs = [be.Req(int(b.table_idx[i]), int(b.cached_lens[i]), int(b.device_lens[i]))
+            for i in range(b.batch_size)]
+    batch = be.Batch(not decode, reqs, torch.from_numpy(b.positions).to(dev),
+                     torch.from_numpy(b.out_loc).to(dev))
+    backend.prepare_metadata(batch)
+    T = int(b.qo_indptr[-1])
+    qkv = torch.randn((T, (hq + 2 * hkv) * D), generator=g, device=dev).to(torch.bfloat16)
+    norms = be.RMSNorm(D, 1e-6, 0), be.RMSNorm(D, 1e-6, 0)
+    for n in norms:
+        n.weight = torch.randn(D, generator=g, device=dev).to(torch.bfloat16)
+    return cache, backend, batch, qkv, norms
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_attention_layer_refuses_a_rotation_wider_than_the_head(be, dev, interleaved):
+    """A rotary embedding of a larger head is refused when the layer is made; up to the
+    head's width it is taken."""
+    _, backend, _, _, norms = layer_parts(be, dev, True)
+    wide = be.RotaryEmbedding(2 * D, D + 2, 4096, 1e6, be.RopeScaling(), interleaved)
+    with pytest.raises(RuntimeError, match="rotary"):
+        be.AttentionLayer(1, 32, 8, D, backend, wide, *norms)
+    for rotary in (2, 64, D):
+        be.AttentionLayer(1, 32, 8, D, backend,
+                          be.RotaryEmbedding(2 * D, rotary, 4096, 1e6, be.RopeScaling(), interleaved), *norms)
