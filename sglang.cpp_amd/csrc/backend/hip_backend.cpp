@@ -1246,13 +1246,14 @@ std::pair<torch::Tensor, torch::Tensor> rope_scaled_cache(int64_t max_pos, int r
   return {cos, sin};
 }
 
-torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
-                          const torch::Tensor& k_cache, const torch::Tensor& v_cache,
-                          const torch::Tensor& cos, const torch::Tensor& sin,
-                          const torch::Tensor& positions, const torch::Tensor& out_loc,
-                          bool interleaved, const torch::Tensor& q_out) {
+namespace {
+// rope_append's arguments as the library takes them, checked; nothing is written.
+sgl_rope_append_t rope_append_args(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                   const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                                   const torch::Tensor& cos, const torch::Tensor& sin,
+                                   const torch::Tensor& positions, const torch::Tensor& out_loc,
+                                   bool interleaved, const torch::Tensor& out) {
   TORCH_CHECK(q.is_cuda(), "rope_append takes HIP device tensors");
-  const c10::DeviceGuard guard(q.device());
   sgl_rope_append_t a{};
   a.dtype = half_dtype(q, "q");
   check_heads(q, q, "q");
@@ -1283,9 +1284,8 @@ torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const 
     a.out_loc = out_loc.data_ptr();
     a.index_dtype = out_loc.scalar_type() == torch::kInt64 ? SGL_INDEX_I64 : SGL_INDEX_I32;
   }
-  if (q_out.defined()) check_heads(q_out, q, "q_out");
-  TORCH_CHECK(!q_out.defined() || q_out.sizes() == q.sizes(), "q_out must have q's shape");
-  auto out = q_out.defined() ? q_out : torch::empty({T, hq, d}, q.options());
+  check_heads(out, q, "q_out");
+  TORCH_CHECK(out.sizes() == q.sizes(), "q_out must have q's shape");
   a.q = q.data_ptr();
   a.q_out = out.data_ptr();
   a.k = k.data_ptr();
@@ -1313,6 +1313,20 @@ torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const 
   a.head_dim = narrow_dim(d, "head_dim");
   a.rotary_dim = narrow_dim(2 * cos.size(1), "rotary_dim");
   a.flags = interleaved ? SGL_ROPE_INTERLEAVED : 0;
+  return a;
+}
+}  // namespace
+
+torch::Tensor rope_append(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                          const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                          const torch::Tensor& cos, const torch::Tensor& sin,
+                          const torch::Tensor& positions, const torch::Tensor& out_loc,
+                          bool interleaved, const torch::Tensor& q_out) {
+  TORCH_CHECK(q.is_cuda(), "rope_append takes HIP device tensors");
+  const c10::DeviceGuard guard(q.device());
+  auto out = q_out.defined() ? q_out : torch::empty(q.sizes(), q.options());
+  const sgl_rope_append_t a = rope_append_args(q, k, v, k_cache, v_cache, cos, sin, positions, out_loc,
+                                               interleaved, out);
   check_sgl(sgl_rope_append(&a, current_stream(q.device())), "sgl_rope_append");
   return out;
 }
@@ -1507,18 +1521,22 @@ torch::Tensor AttentionLayer::forward(const torch::Tensor& qkv, const torch::Ten
   auto kc = backend_->kv_cache()->k_cache(layer_id_);
   auto vc = backend_->kv_cache()->v_cache(layer_id_);
   if (rotary_->interleaved() || rotary_->rotary_dim() != head_dim_) {
-    // Refused before the pool is written, as attend would behind it.
+    // Refused before anything is written, as rope_append and attend would behind the norm.
     TORCH_CHECK(num_qo_heads_ == backend_->num_qo_heads() && num_kv_heads_ == backend_->num_kv_heads() &&
                     head_dim_ == backend_->head_dim(),
                 "AttentionLayer: num_qo_heads, num_kv_heads and head_dim must be the backend's");
+    TORCH_CHECK(qkv.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+                "qkv rows must start on multiples of 16 bytes");
     auto heads = [&](int first, int count) {
       return qkv.narrow(1, first * head_dim_, count * head_dim_).view({-1, count, head_dim_});
     };
     auto q = heads(0, num_qo_heads_), k = heads(num_qo_heads_, num_kv_heads_);
+    const sgl_rope_append_t append = rope_append_args(
+        q, k, heads(num_qo_heads_ + num_kv_heads_, num_kv_heads_), kc, vc, rotary_->cos_cache(),
+        rotary_->sin_cache(), positions, batch.out_loc, rotary_->interleaved(), q);
+    const c10::DeviceGuard guard(qkv.device());
     if (q_norm_) fused_qk_rmsnorm_inplace_3d_strided(q, k, *q_norm_, *k_norm_);
-    rope_append(q, k, heads(num_qo_heads_ + num_kv_heads_, num_kv_heads_), kc, vc,
-                rotary_->cos_cache(), rotary_->sin_cache(), positions, batch.out_loc,
-                rotary_->interleaved(), q);
+    check_sgl(sgl_rope_append(&append, current_stream(qkv.device())), "sgl_rope_append");
     return backend_->attend(q, layer_id_, batch);
   }
   if (num_qo_heads_ == backend_->num_qo_heads() && num_kv_heads_ == backend_->num_kv_heads() &&

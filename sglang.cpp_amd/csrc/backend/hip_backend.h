@@ -366,7 +366,9 @@ std::pair<torch::Tensor, torch::Tensor> verify_drafts(
 
 // qkv [T, (Hq + 2 Hkv) D] -> o [T, Hq D]: qk-norm, RoPE and the KV store in
 // one fused pass, then paged attention (attention_layer.cc:17-51). A rotary embedding
-// of part of the head or of interleaved pairs takes the norm in place, then rope_append.
+// of part of the head or of interleaved pairs takes the norm in place, then rope_append;
+// rows, positions and slots that these or the attention refuse are refused before qkv or
+// the pool changes.
 class AttentionLayer {
  public:
   AttentionLayer(int layer_id, int num_qo_heads, int num_kv_heads, int head_dim,

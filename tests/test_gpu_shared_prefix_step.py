@@ -261,3 +261,44 @@ def test_attention_layer_refuses_a_rotation_wider_than_the_head(be, dev, interle
     for rotary in (2, 64, D):
         be.AttentionLayer(1, 32, 8, D, backend,
                           be.RotaryEmbedding(2 * D, rotary, 4096, 1e6, be.RopeScaling(), interleaved), *norms)
+
+
+def refused_calls(batch, qkv):
+    """(name, qkv, positions, out_loc) that the layer refuses."""
+    T, W = qkv.shape
+    pos, loc = batch.positions, batch.out_loc
+    wide = lambda first, more: torch.empty((T, W + more), device=qkv.device, dtype=qkv.dtype)[:, first:first + W].copy_(qkv)
+    apart = lambda x: torch.stack([x, x], 1)[:, 0]
+    yield "positions apart", qkv, apart(pos), loc
+    yield "positions on the host", qkv, pos.cpu(), loc
+    yield "positions of rank 2", qkv, pos[:, None], loc
+    yield "slots apart", qkv, pos, apart(loc)
+    yield "slots on the host", qkv, pos, loc.cpu()
+    yield "rows off the 16-byte grid", wide(1, 8), pos, loc
+    yield "rows a step off the grid", wide(0, 4), pos, loc
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("interleaved,rotary", [(True, D), (False, 32)])
+@pytest.mark.parametrize("norm", [True, False])
+def test_attention_layer_refuses_before_it_writes(be, dev, decode, interleaved, rotary, norm):
+    """A call that interleaved or partial rotations refuse leaves the caller's rows and the
+    pool as they were, so that it can be made again."""
+    cache, backend, batch, qkv, norms = layer_parts(be, dev, decode)
+    rot = be.RotaryEmbedding(D, rotary, 4096, 1e6, be.RopeScaling(), interleaved)
+    layer = be.AttentionLayer(1, 32, 8, D, backend, rot, *(norms if norm else (None, None)))
+    pool, pos, loc = cache.buffer().clone(), batch.positions, batch.out_loc
+    bits = lambda x: x.view(torch.int16)
+    touched = []
+    for name, rows, p, slots in refused_calls(batch, qkv):
+        before = rows.clone()
+        batch.out_loc = slots
+        with pytest.raises(RuntimeError):
+            layer.forward(rows, p, batch)
+        batch.out_loc = loc
+        if not torch.equal(bits(rows.contiguous()), bits(before.contiguous())) or \
+                not torch.equal(bits(cache.buffer()), bits(pool)):
+            touched.append(name)
+        cache.buffer().copy_(pool)
+    assert not touched
+    layer.forward(qkv, pos, batch)  # the same objects take the call that holds
