@@ -1,5 +1,7 @@
 """GPU tests (marked gpu) of the verification of drafted tokens against its 64-bit
 form: whole numbers, so equal."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -171,3 +173,38 @@ def test_tokens_follow_the_target(dev):
     tokens, _ = run(x, dev)
     first = np.bincount(np.array(tokens)[::2], minlength=V)
     assert (np.abs(first - N * p) <= 5 * np.sqrt(N * p * (1 - p)) + 0.5).all()
+
+
+@pytest.mark.parametrize("with_probs", [True, False])
+@pytest.mark.parametrize("bad", [[0, 2, 1, 6], [0, 2, 7, 6], [-1, 2, 4, 6], [0, 2, 2 ** 31 - 1, -5], [3, 1, 4, 6]])
+def test_invalid_requests_write_nothing_but_their_mark(dev, bad, with_probs):
+    """Outputs full of a sentinel: a request whose offsets do not hold gets accepted = -1 and
+    no token is written for it; the others, whose places do not meet, have their 64-bit
+    results."""
+    V, N, B, mark = 4099, 6, 3, -77
+    x = batch([2, 2, 2], V, 13, with_probs=with_probs)
+    t = {k: None if v is None else torch.from_numpy(v).to(dev) for k, v in x.items()}
+    indptr = torch.tensor(bad, dtype=torch.int32, device=dev)
+    tokens = torch.full((N + B,), mark, dtype=torch.int32, device=dev)
+    accepted = torch.full((B,), mark, dtype=torch.int32, device=dev)
+    size = capi.lib().sgl_verify_workspace_bytes(B, V)
+    ws = torch.full((size,), 0x7F, dtype=torch.uint8, device=dev)
+    args = capi.VerifyArgs(t["target"].data_ptr(), t["draft"].data_ptr() if with_probs else 0,
+                           t["tokens"].data_ptr(), indptr.data_ptr(), t["accept"].data_ptr(),
+                           t["sample"].data_ptr(), tokens.data_ptr(), accepted.data_ptr(), V, V, N, B, V)
+    assert capi.lib().sgl_verify_drafts(ctypes.byref(args), ws.data_ptr(), size,
+                                        torch.cuda.current_stream().cuda_stream) == 0
+    want, counts = [mark] * (N + B), []
+    for r in range(B):
+        a, b = bad[r], bad[r + 1]
+        if not 0 <= a <= b <= N:
+            counts.append(-1)
+            continue
+        # The request alone: its own rows, drafts and random numbers.
+        one, n = refs.verify(x["target"][a + r:b + r + 1], x["draft"][a:b] if with_probs else None,
+                             x["tokens"][a:b], [0, b - a], x["accept"][a:b], x["sample"][r:r + 1])
+        assert want[a + r:b + r + 1] == [mark] * (b - a + 1)
+        want[a + r:b + r + 1] = one
+        counts.append(n[0])
+    assert accepted.cpu().tolist() == counts
+    assert tokens.cpu().tolist() == want
