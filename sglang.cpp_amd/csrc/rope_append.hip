@@ -447,8 +447,8 @@ extern "C" int sgl_rope_append(const sgl_rope_append_t* args, void* stream) {
       !x.sin || !x.positions)
     return SGL_ERR_INVALID_ARG;
   // In place means the same rows at the same places.
-  if (x.q == x.q_out && (x.q_stride_token != x.q_out_stride_token ||
-                         x.q_stride_head != x.q_out_stride_head))
+  if (x.num_qo_heads && x.q == x.q_out && (x.q_stride_token != x.q_out_stride_token ||
+                                           x.q_stride_head != x.q_out_stride_head))
     return SGL_ERR_INVALID_ARG;
   AppendArgs a{};
   a.q = static_cast<const uint16_t*>(x.q), a.q_st = x.q_stride_token, a.q_sh = x.q_stride_head;

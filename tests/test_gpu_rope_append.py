@@ -7,6 +7,8 @@ the factor m once: below 6 x 2^-24 of m. The 64-bit angle is off by less than
 2^-33. Rotation: two products and a sum in fp32 (at most 2 x 2^-24 of the absolute
 products), then one rounding to the type: half a step, 2^-8 (bf16) or 2^-11 (fp16)
 of the value, and for fp16 half its smallest step, 2^-25."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -240,3 +242,22 @@ def test_append_many_tokens(dev, interleaved):
                                 x["pos"][a:b], x["loc"][a:b], interleaved)
         assert torch.equal(part, q[a:b])
     assert torch.equal(kc, x["kc"]) and torch.equal(vc, x["vc"])
+
+
+def test_append_without_q_takes_any_q_strides(dev):
+    """num_qo_heads 0: no q, whatever its pointers and strides say; k and v as with it."""
+    x = make(dev, 9, 4, 2, 128, 64, "bf16", 12)
+    kc, vc = x["kc"].clone(), x["vc"].clone()
+    capi.rope_append(x["q"], x["k"], x["v"], x["kc"], x["vc"], x["cos"], x["sin"], x["pos"], x["loc"])
+    for st in (0, 512):
+        k2, v2 = kc.clone(), vc.clone()
+        args = capi.RopeAppendArgs(
+            k=x["k"].data_ptr(), v=x["v"].data_ptr(), k_cache=k2.data_ptr(), v_cache=v2.data_ptr(),
+            cos=x["cos"].data_ptr(), sin=x["sin"].data_ptr(), positions=x["pos"].data_ptr(),
+            out_loc=x["loc"].data_ptr(), tokens=9, num_slots=k2.shape[0], max_pos=x["cos"].shape[0],
+            q_stride_token=st, q_stride_head=128, k_stride_token=256, k_stride_head=128,
+            v_stride_token=256, v_stride_head=128, kv_stride_slot=256, kv_stride_head=128,
+            num_qo_heads=0, num_kv_heads=2, head_dim=128, rotary_dim=64)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert capi.lib().sgl_rope_append(ctypes.byref(args), stream) == 0
+        assert torch.equal(k2, x["kc"]) and torch.equal(v2, x["vc"])
