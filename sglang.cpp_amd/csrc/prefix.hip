@@ -162,14 +162,21 @@ __device__ __forceinline__ Split split_of(const PrefixArgs& a, const Offsets& he
     // A second workgroup of tiles on a CU brings nothing (1.4 us a tile alone, 2.7 for
     // each of two).
     s.tile_blocks = max(1, min(share, a.blocks / 2));
+    // An eighth more than its share: within 1% of none in most batches. us with none, an
+    // eighth and a quarter: 160 requests of 20 own tokens behind 16,384 64.5, 63.6, 65.2; 64 of
+    // 16 behind 1,024 14.4, 14.4, 16.5; 32 of 300 behind 4,096 22.2, 23.0, 23.1.
     s.wide = max(1, quotient(s.tile_blocks, a.hkv));
     s.wide = max(1, min(s.wide + s.wide / 8, quotient(a.blocks / 2, a.hkv)));
     // The number of runs. Many workgroups a row tile: one each. Else candidates, one a lane:
     // the tiles of the rounds that they take, what begins and ends a run (six tiles' time),
     // and a 43rd of a tile for the partial rows of a run and row tile, written and folded.
     // The workspace has room for two runs a row tile, or for as many as there are
-    // workgroups. 640 requests behind 16,384 tokens, 32q/8kv (20 row tiles for 32
-    // workgroups): one run each 295 us, three in two rounds 249.
+    // workgroups. 640 requests of 20 own tokens behind 16,384, 32q/8kv (20 row tiles for 32
+    // workgroups): one run each 319 us, three in two rounds 235. The constants hardly matter.
+    // us with 3, 6 and 12 tiles: 160 of 20 behind 16,384 64.2, 63.6, 63.4; 96 of 100 behind
+    // 4,096, 32q/4kv, 25.2, 25.4, 25.9. With a 21st, 43rd and 86th: 640 of 20 behind 2,048
+    // 53.9, 53.7, 56.4. With candidates below 4, 8, 16 and 64 workgroups a row tile: 96 of 100
+    // 25.5, 25.4, 24.3, 24.2; 4 requests of 40 behind 1,500, 16q/8kv, 11.2, 11.1, 11.2, 11.9.
     int take = min(quotient(s.wide, s.row_tiles), s.tiles);
     float k = 1.f;
     if (s.wide < 8 * s.row_tiles) {
@@ -479,9 +486,10 @@ __device__ __forceinline__ void unit_pieces(const PrefixArgs& a, const Split& s,
 // The prefix: W waves with 32 packed rows each share the 64-token K/V
 // tiles that they gather into LDS (two buffers, K one tile ahead of V), and tile t + 1's
 // scores are on the matrix cores while tile t's become weights; the prefill kernel's
-// tile steps without a causal bound. 1.4 us a tile of 128 rows, 0.77 PFLOP/s on all CUs. Tiles [tb, te) of the prefix for row tile rt of kv
-// head h, the item's piece number `piece`. Bound by the matrix cores: 4 x 64 x 128 flops
-// a row and tile.
+// tile steps without a causal bound, P in bf16 for the product with V as there and in the
+// units. Tiles [tb, te) of the prefix for row tile rt of kv head h, the item's piece number
+// `piece`. 4 x 64 x 128 flops a row and tile: 1.4 us a tile of 128 rows, 0.77 PFLOP/s on all
+// CUs, the matrix cores busy in 41% of the cycles (the prefill's 256 rows a tile: 1.0).
 __device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& sp, char* lds_raw, int rt,
                                              int h, int tb, int te, int piece) {
   using namespace pf;
@@ -624,9 +632,9 @@ __device__ __forceinline__ void prefix_tiles(const PrefixArgs& a, const Split& s
 }
 
 // Two workgroups of four waves per CU: those that walk the prefix's tiles, bound by
-// the matrix cores, lie beside the others' units, bound by memory. 256 requests of 528
-// own tokens behind 16,384, 32q/8kv: the prefix alone 102 us, the own tokens alone 90,
-// together 153 (fold included; 621 MB of K/V, 87 us at a read's 7.1 TB/s, and 71 GFLOP,
+// their products, lie beside the others' units, bound by memory. 256 requests of 528
+// own tokens each behind 16,384, 32q/8kv: the prefix alone 103 us, the own tokens alone 89,
+// together 152 (fold included; 621 MB of K/V, 87 us at a read's 7.1 TB/s, and 71 GFLOP,
 // 60 us at a large product's 1.19 PFLOP/s).
 template <int RB>
 __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attention_kernel(PrefixArgs a) {
@@ -674,7 +682,8 @@ __device__ __forceinline__ float half_sum(float x) {
 // The row again, token by token over those it sees, by 32 lanes (4 values each):
 // for rows that do not see the whole prefix, and for those whose products brought in
 // a V value that is not finite from a token they do not see (0 x inf).
-// Bound by its instructions: 12,288 rows of 6,000 tokens 4.9 ms (6.6 with one token's loads in flight).
+// No reuse between rows and no matrix cores: 12,288 rows of 6,000 tokens 4.9 ms (6.6 with
+// one token's loads in flight), 4 requests of 8 query and 2 own tokens behind 16,384 6.4 ms.
 __device__ __forceinline__ f32x4_t plain_row(const PrefixArgs& a, const Request& x, int tok, int head,
                                              int64_t sees, int c) {
   const int h = head / a.group;

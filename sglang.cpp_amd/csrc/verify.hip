@@ -17,8 +17,9 @@
 // workgroup per request picks the slice the draw falls into from the slices'
 // sums and walks that slice alone. Bound by reading one target row and, where a
 // draft was rejected, one draft row per request: 48 requests of a vocabulary of 151,936
-// (38 slices) 13.7 us in all, 54 MB, 3.9 TB/s; one request 8.3 us, two launches and their
-// chains of dependent loads.
+// (38 slices), some 23 of them with a rejected draft, 13.7 us in all, 43 MB, 3.1 TB/s (the
+// first launch 10.5 us, 4.1 TB/s); one request 8.7 us, two launches and their chains of
+// dependent loads.
 #include "common.h"
 
 namespace sgl {
