@@ -40,7 +40,7 @@ const char* sgl_status_string(int status);
 
 /* Library version, to check that the loaded .so matches this header. */
 int sgl_abi_version(void);
-#define SGL_ABI_VERSION 17
+#define SGL_ABI_VERSION 18
 
 /* ------------------------------------------------------------------ */
 /* KV-cache store                                                      */
@@ -649,6 +649,95 @@ int sgl_silu_and_mul(void* out, const void* input, int64_t tokens, int64_t d,
 int sgl_gelu_and_mul(void* out, const void* input, int64_t tokens, int64_t d,
                      int64_t in_stride_row, int64_t out_stride_row, int dtype,
                      void* stream);
+
+/* ------------------------------------------------------------------ */
+/* Projections and experts                                             */
+/* ------------------------------------------------------------------ */
+
+/*
+ * A projection and what follows it:
+ *   out[t, j] = T(act(sum_i x[t, i] weight[j, i] + bias[j]) + residual[t, j]),
+ * t < tokens, j < n, i < k, and for the *_AND_MUL activations, whose weight and bias have
+ * 2 n rows (gate, then up),
+ *   out[t, j] = T(act(g_j) u_j + residual[t, j]), g and u the biased sums of rows j, n + j.
+ * fp32 sums and arithmetic, one rounding. x, weight, bias and residual are bf16 or fp16
+ * (dtype), out that type or fp32 (out_dtype SGL_DTYPE_F32: logits). bias and residual may
+ * be NULL; out may be residual (same type and strides), other overlaps are the caller's
+ * error. Any sizes up to 2^31 - 256, strides and alignment; fastest where k is a multiple of 64
+ * and rows start on 16 bytes. workspace: sgl_linear_workspace_bytes (0 for most sizes),
+ * 16-byte aligned, written before it is read; calls that share one must be
+ * stream-ordered. With NULL the launch has fewer workgroups, and sums another order.
+ * Replaces: Linear::forward and what the model runs on its output
+ *           (src/layers/linear.cc:9-78; activation.cu:15-77).
+ */
+#define SGL_ACT_NONE 0
+#define SGL_ACT_SILU 1
+#define SGL_ACT_GELU 2 /* tanh, as sgl_gelu_and_mul */
+#define SGL_ACT_SILU_AND_MUL 3
+#define SGL_ACT_GELU_AND_MUL 4
+typedef struct {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* residual;
+  void* out;
+  int64_t tokens, n, k;
+  int64_t x_stride_row, weight_stride_row, residual_stride_row, out_stride_row;
+  int32_t dtype;
+  int32_t out_dtype;
+  int32_t activation;
+  int32_t reserved; /* 0 */
+} sgl_linear_t;
+int64_t sgl_linear_workspace_bytes(int64_t tokens, int64_t n, int64_t k, int activation);
+int sgl_linear(const sgl_linear_t* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The experts of each token from the router's logits (bf16, fp16 or fp32 [tokens,
+ * num_experts], rows logits_stride_row elements apart): experts[t, j], j < top_k, are the
+ * experts of the top_k largest logits, largest first, equal ones by their number;
+ * weights[t, j] their probabilities in the softmax over all experts, with renormalize
+ * divided by their sum. int32 and fp32 [tokens, top_k], contiguous. NaN is ranked below
+ * -inf; a row with a NaN, an infinite or no finite logit above -inf has NaN weights. Up
+ * to 512 experts and top_k 32.
+ * Replaces: the softmax, top-k and renormalisation of the router (src/moe/moe.cc:47-60).
+ */
+int sgl_moe_route(const void* logits, int64_t logits_stride_row, int logits_dtype, int64_t tokens,
+                  int num_experts, int top_k, int renormalize, float* weights, int32_t* experts,
+                  void* stream);
+
+/*
+ * The experts of a mixture-of-experts layer:
+ *   out[t] = T(sum_j weights[t, j] down[e] h + residual[t]), e = experts[t, j],
+ *   h = T(act(gate_up[e][:I] x[t]) * (gate_up[e][I:] x[t])), I = intermediate,
+ * with x, out and residual [tokens, hidden], gate_up [num_experts, 2 I, hidden] and down
+ * [num_experts, hidden, I] bf16 or fp16, weights fp32 and experts int32 [tokens, top_k]
+ * contiguous. Sums in fp32, over j in its order; h is rounded to the type, as the
+ * matrix instructions take it. A slot whose expert is outside [0, num_experts) adds
+ * nothing (padding, experts of another device). An expert may be chosen more than once.
+ * activation: SGL_ACT_SILU_AND_MUL or SGL_ACT_GELU_AND_MUL. residual may be NULL, out may
+ * be residual (same strides). workspace: sgl_moe_workspace_bytes, 16-byte aligned,
+ * written before it is read; calls that share one must be stream-ordered. hidden and
+ * intermediate up to 2^20, 65,536 experts.
+ * Replaces: the loop over the experts (src/moe/moe.cc:62-98).
+ */
+typedef struct {
+  const void* x;
+  const void* gate_up;
+  const void* down;
+  const float* weights;
+  const int32_t* experts;
+  const void* residual;
+  void* out;
+  int64_t tokens;
+  int64_t x_stride_row, residual_stride_row, out_stride_row;
+  int64_t gate_up_stride_expert, gate_up_stride_row, down_stride_expert, down_stride_row;
+  int32_t top_k, num_experts, hidden, intermediate;
+  int32_t dtype;
+  int32_t activation;
+} sgl_moe_t;
+int64_t sgl_moe_workspace_bytes(int64_t tokens, int top_k, int num_experts, int hidden,
+                                int intermediate);
+int sgl_moe_experts(const sgl_moe_t* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Probabilities from logits, then sampling from probabilities         */

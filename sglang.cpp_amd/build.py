@@ -37,7 +37,8 @@ HIP_FLAGS = [
 ]
 
 SOURCES = ["kv_store.hip", "metadata.hip", "rope_norm.hip", "decode.hip", "prefill.hip", "residual.hip",
-           "sampling.hip", "softmax.hip", "rope_append.hip", "verify.hip", "prefix.hip"]
+           "sampling.hip", "softmax.hip", "rope_append.hip", "verify.hip", "prefix.hip",
+           "linear.hip", "moe.hip"]
 
 
 def _compile(src: Path, obj: Path) -> None:

@@ -27,7 +27,7 @@ SGL_INDEX_I64 = 1
 SGL_DTYPE_BF16 = 0
 SGL_DTYPE_F16 = 1
 SGL_DTYPE_F32 = 2
-ABI_VERSION = 17
+ABI_VERSION = 18
 FUSED_NO_K_WRITEBACK = 1  # SGL_FUSED_NO_K_WRITEBACK
 
 
@@ -142,6 +142,31 @@ class VerifyArgs(ctypes.Structure):
                 ("batch_size", ctypes.c_int32), ("vocab", ctypes.c_int32)]
 
 
+class LinearArgs(ctypes.Structure):
+    """sgl_linear_t."""
+    _fields_ = [*[(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "residual", "out")],
+                *[(n, ctypes.c_int64) for n in ("tokens", "n", "k", "x_stride_row",
+                                                "weight_stride_row", "residual_stride_row",
+                                                "out_stride_row")],
+                *[(n, ctypes.c_int32) for n in ("dtype", "out_dtype", "activation", "reserved")]]
+
+
+# SGL_ACT_*
+ACTIVATION = {"none": 0, "silu": 1, "gelu": 2, "silu_and_mul": 3, "gelu_and_mul": 4}
+
+
+class MoeArgs(ctypes.Structure):
+    """sgl_moe_t."""
+    _fields_ = [*[(n, ctypes.c_void_p) for n in ("x", "gate_up", "down", "weights", "experts",
+                                                 "residual", "out")],
+                *[(n, ctypes.c_int64) for n in ("tokens", "x_stride_row", "residual_stride_row",
+                                                "out_stride_row", "gate_up_stride_expert",
+                                                "gate_up_stride_row", "down_stride_expert",
+                                                "down_stride_row")],
+                *[(n, ctypes.c_int32) for n in ("top_k", "num_experts", "hidden", "intermediate",
+                                                "dtype", "activation")]]
+
+
 class I32Copy(ctypes.Structure):
     """sgl_i32_copy_t."""
     _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("count", ctypes.c_int64)]
@@ -218,6 +243,11 @@ _SIGNATURES = {
                               _i64, _vp, _i64, _vp], _i32),
     "sgl_verify_workspace_bytes": ([_i32, _i32], _i64),
     "sgl_verify_drafts": ([ctypes.POINTER(VerifyArgs), _vp, _i64, _vp], _i32),
+    "sgl_linear_workspace_bytes": ([_i64, _i64, _i64, _i32], _i64),
+    "sgl_linear": ([ctypes.POINTER(LinearArgs), _vp, _i64, _vp], _i32),
+    "sgl_moe_route": ([_vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _vp], _i32),
+    "sgl_moe_workspace_bytes": ([_i64, _i32, _i32, _i32, _i32], _i64),
+    "sgl_moe_experts": ([ctypes.POINTER(MoeArgs), _vp, _i64, _vp], _i32),
     "sgl_mixed_decode_cus": ([_i64, _i32, _i32, ctypes.c_double], _i32),
     "sgl_decode_plan_cus": ([_vp, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(DecodePlan)], _i32),
     "sgl_paged_mixed": ([ctypes.POINTER(DecodePlan), _vp, _i64, _i64, _vp, _vp, _i64, _i64,
@@ -1120,3 +1150,116 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
                                        workspace.numel() * workspace.element_size(), _stream(dev)),
                "sgl_verify_drafts")
     return tokens, accepted
+
+
+# ---------------------------------------------------------------- projections and experts
+
+_HALF = {torch.bfloat16: SGL_DTYPE_BF16, torch.float16: SGL_DTYPE_F16}
+
+
+def _rows(t: torch.Tensor, shape, dtype, what: str) -> int:
+    """Row stride of a [rows, columns] tensor with contiguous rows."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or (t.numel() > 0 and shape[1] > 1
+                                                              and t.stride(1) != 1):
+        raise ValueError(f"{what} must be {dtype} {list(shape)} with contiguous rows")
+    return max(t.stride(0), shape[1]) if shape[0] <= 1 else t.stride(0)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           activation: str = "none", residual: Optional[torch.Tensor] = None,
+           out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual (sgl_linear): x [T, k], weight [n, k], or [2 n, k]
+    for "silu_and_mul" and "gelu_and_mul". Returns [T, n] of out_dtype (x's, or float32)."""
+    dev = _need_gpu(x, weight, bias, residual, out, workspace)
+    if activation not in ACTIVATION:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATION)}")
+    if x.dtype not in _HALF or x.dim() != 2 or weight.dim() != 2:
+        raise ValueError("x and weight must be bf16 or fp16 matrices")
+    T, k = x.shape
+    gated = activation.endswith("_and_mul")
+    if gated and weight.shape[0] % 2:
+        raise ValueError("a gated projection needs as many gate rows as up rows")
+    n = weight.shape[0] // 2 if gated else weight.shape[0]
+    out_dtype = out_dtype or (x.dtype if out is None else out.dtype)
+    if out_dtype not in (x.dtype, torch.float32):
+        raise ValueError("out must have x's type or float32")
+    if out is None:
+        out = torch.empty((T, n), dtype=out_dtype, device=dev)
+    if bias is not None and (bias.dtype != x.dtype or bias.shape != (weight.shape[0],)
+                             or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous vector of weight's rows, of x's type")
+    args = LinearArgs(
+        x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if residual is None else residual.data_ptr(), out.data_ptr(), T, n, k,
+        _rows(x, (T, k), x.dtype, "x"), _rows(weight, weight.shape[:1] + (k,), x.dtype, "weight"),
+        0 if residual is None else _rows(residual, (T, n), x.dtype, "residual"),
+        _rows(out, (T, n), out_dtype, "out"), _HALF[x.dtype],
+        _HALF.get(out_dtype, SGL_DTYPE_F32), ACTIVATION[activation], 0)
+    need = lib().sgl_linear_workspace_bytes(T, n, k, ACTIVATION[activation])
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib().sgl_linear(ctypes.byref(args), _p(workspace),
+                                0 if workspace is None else workspace.numel()
+                                * workspace.element_size(), _stream(dev)), "sgl_linear")
+    return out
+
+
+def moe_route(logits: torch.Tensor, top_k: int,
+              renormalize: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """(weights float32, experts int32), both [T, top_k], of sgl_moe_route: logits
+    [T, num_experts] bf16, fp16 or float32 with contiguous rows."""
+    dev = _need_gpu(logits)
+    kinds = {**_HALF, torch.float32: SGL_DTYPE_F32}
+    if logits.dim() != 2 or logits.dtype not in kinds:
+        raise ValueError("logits must be a bf16, fp16 or float32 matrix")
+    T, E = logits.shape
+    weights = torch.empty((T, max(top_k, 0)), dtype=torch.float32, device=dev)
+    experts = torch.empty((T, max(top_k, 0)), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib().sgl_moe_route(_p(logits), _rows(logits, (T, E), logits.dtype, "logits"),
+                                   kinds[logits.dtype], T, E, top_k, int(renormalize), _p(weights),
+                                   _p(experts), _stream(dev)), "sgl_moe_route")
+    return weights, experts
+
+
+def moe_experts(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weights: torch.Tensor,
+                experts: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                activation: str = "silu_and_mul", out: Optional[torch.Tensor] = None,
+                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The experts' weighted outputs (+ residual) of sgl_moe_experts: x [T, H], gate_up
+    [E, 2 I, H], down [E, H, I] (contiguous rows), weights float32 and experts int32 [T, top_k]."""
+    dev = _need_gpu(x, gate_up, down, weights, experts, residual, out, workspace)
+    if x.dim() != 2 or x.dtype not in _HALF or gate_up.dim() != 3 or down.dim() != 3:
+        raise ValueError("x must be [T, H] bf16 or fp16, gate_up [E, 2 I, H], down [E, H, I]")
+    T, H = x.shape
+    E, I = gate_up.shape[0], down.shape[2]
+    for t, shape, what in ((gate_up, (E, 2 * I, H), "gate_up"), (down, (E, H, I), "down")):
+        if tuple(t.shape) != shape or t.dtype != x.dtype or (shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{what} must be {x.dtype} {list(shape)} with contiguous rows")
+    if weights.dim() != 2 or any(
+            t.shape != weights.shape or t.dtype != d or not t.is_contiguous()
+            for t, d in ((weights, torch.float32), (experts, torch.int32))) or weights.shape[0] != T:
+        raise ValueError("weights float32 and experts int32 must be contiguous [T, top_k]")
+    if activation not in ("silu_and_mul", "gelu_and_mul"):
+        raise ValueError("activation must be silu_and_mul or gelu_and_mul")
+    if out is None:
+        out = torch.empty((T, H), dtype=x.dtype, device=dev)
+    K = weights.shape[1]
+    row = lambda t: max(t.stride(1), t.shape[2]) if t.shape[1] <= 1 else t.stride(1)
+    args = MoeArgs(
+        x.data_ptr(), gate_up.data_ptr(), down.data_ptr(), weights.data_ptr(), experts.data_ptr(),
+        0 if residual is None else residual.data_ptr(), out.data_ptr(), T,
+        _rows(x, (T, H), x.dtype, "x"),
+        0 if residual is None else _rows(residual, (T, H), x.dtype, "residual"),
+        _rows(out, (T, H), x.dtype, "out"), gate_up.stride(0), row(gate_up), down.stride(0),
+        row(down), K, E, H, I, _HALF[x.dtype], ACTIVATION[activation])
+    if workspace is None:
+        workspace = torch.empty(lib().sgl_moe_workspace_bytes(T, K, E, H, I), dtype=torch.uint8,
+                                device=dev)
+    with torch.cuda.device(dev):
+        _check(lib().sgl_moe_experts(ctypes.byref(args), _p(workspace),
+                                     workspace.numel() * workspace.element_size(), _stream(dev)),
+               "sgl_moe_experts")
+    return out

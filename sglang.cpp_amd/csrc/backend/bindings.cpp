@@ -189,6 +189,62 @@ PYBIND11_MODULE(sgl_backend, m) {
   m.def("silu_and_mul", [](torch::Tensor out, torch::Tensor input) { silu_and_mul(out, input); });
   m.def("gelu_and_mul", [](torch::Tensor out, torch::Tensor input) { gelu_and_mul(out, input); });
 
+  m.def("linear",
+        [](const torch::Tensor& x, const torch::Tensor& w, c10::optional<torch::Tensor> bias,
+           const std::string& activation, c10::optional<torch::Tensor> residual,
+           c10::optional<torch::Tensor> out, c10::optional<torch::Dtype> out_dtype) {
+          return linear(x, w, bias.value_or(torch::Tensor()), activation,
+                        residual.value_or(torch::Tensor()), out.value_or(torch::Tensor()), out_dtype);
+        },
+        py::arg("x"), py::arg("weight"), py::arg("bias") = py::none(),
+        py::arg("activation") = "none", py::arg("residual") = py::none(),
+        py::arg("out") = py::none(), py::arg("out_dtype") = py::none());
+  m.def("moe_route", &moe_route, py::arg("logits"), py::arg("top_k"), py::arg("renormalize") = true);
+  m.def("moe_experts",
+        [](const torch::Tensor& x, const torch::Tensor& gate_up, const torch::Tensor& down,
+           const torch::Tensor& weights, const torch::Tensor& experts,
+           c10::optional<torch::Tensor> residual, const std::string& activation,
+           c10::optional<torch::Tensor> out) {
+          return moe_experts(x, gate_up, down, weights, experts, residual.value_or(torch::Tensor()),
+                             activation, out.value_or(torch::Tensor()));
+        },
+        py::arg("x"), py::arg("gate_up"), py::arg("down"), py::arg("weights"), py::arg("experts"),
+        py::arg("residual") = py::none(), py::arg("activation") = "silu_and_mul",
+        py::arg("out") = py::none());
+  auto forward = [](const auto& mlp, const torch::Tensor& x, c10::optional<torch::Tensor> residual) {
+    return mlp.forward(x, residual.value_or(torch::Tensor()));
+  };
+  py::class_<GatedMLP, std::shared_ptr<GatedMLP>>(m, "GatedMLP")
+      .def(py::init([](int hidden, int inter, const std::string& activation, int device) {
+             return std::make_shared<GatedMLP>(hidden, inter, activation, cuda(device));
+           }),
+           py::arg("hidden_size"), py::arg("intermediate_size"),
+           py::arg("activation") = "silu_and_mul", py::arg("device") = 0)
+      .def_readwrite("gate_up", &GatedMLP::gate_up)
+      .def_readwrite("down", &GatedMLP::down)
+      .def("forward",
+           [forward](const GatedMLP& m, const torch::Tensor& x, c10::optional<torch::Tensor> r) {
+             return forward(m, x, r);
+           },
+           py::arg("x"), py::arg("residual") = py::none());
+  py::class_<MoEMLP, std::shared_ptr<MoEMLP>>(m, "MoEMLP")
+      .def(py::init([](int hidden, int inter, int experts, int top_k, bool renormalize,
+                       const std::string& activation, int device) {
+             return std::make_shared<MoEMLP>(hidden, inter, experts, top_k, renormalize, activation,
+                                             cuda(device));
+           }),
+           py::arg("hidden_size"), py::arg("intermediate_size"), py::arg("num_experts"),
+           py::arg("top_k"), py::arg("renormalize") = true,
+           py::arg("activation") = "silu_and_mul", py::arg("device") = 0)
+      .def_readwrite("router", &MoEMLP::router)
+      .def_readwrite("gate_up", &MoEMLP::gate_up)
+      .def_readwrite("down", &MoEMLP::down)
+      .def("forward",
+           [forward](const MoEMLP& m, const torch::Tensor& x, c10::optional<torch::Tensor> r) {
+             return forward(m, x, r);
+           },
+           py::arg("x"), py::arg("residual") = py::none());
+
   m.def("fused_qk_rmsnorm_inplace_3d_strided",
         [](torch::Tensor q, torch::Tensor k, const RMSNorm& qn, const RMSNorm& kn) {
           fused_qk_rmsnorm_inplace_3d_strided(q, k, qn, kn);

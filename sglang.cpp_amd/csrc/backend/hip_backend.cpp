@@ -895,6 +895,11 @@ namespace {
 // SGL_DTYPE_* of a 16-bit floating tensor; the reference's kernels take
 // fp16 and bf16 (normalization.cu:253-268,346-372, activation.cu:25-44,
 // rotary_embedding.cu:124-168).
+int32_t narrow_dim(int64_t v, const char* what) {
+  TORCH_CHECK(v >= 0 && v <= 0x7fffffff, what, " out of range");
+  return static_cast<int32_t>(v);
+}
+
 int half_dtype(const torch::Tensor& t, const char* what) {
   if (t.scalar_type() == torch::kBFloat16) return SGL_DTYPE_BF16;
   TORCH_CHECK(t.scalar_type() == torch::kFloat16, what, " must be bf16 or fp16");
@@ -999,6 +1004,177 @@ static void act_and_mul(bool gelu, torch::Tensor& out, const torch::Tensor& inpu
 void silu_and_mul(torch::Tensor& out, const torch::Tensor& input) { act_and_mul(false, out, input); }
 void gelu_and_mul(torch::Tensor& out, const torch::Tensor& input) { act_and_mul(true, out, input); }
 
+// ---------------------------------------------------------------- projections and experts
+
+namespace {
+int activation_of(const std::string& name) {
+  static const char* const names[] = {"none", "silu", "gelu", "silu_and_mul", "gelu_and_mul"};
+  for (int i = 0; i < 5; ++i)
+    if (name == names[i]) return i;  // SGL_ACT_NONE .. SGL_ACT_GELU_AND_MUL
+  TORCH_CHECK(false, "activation must be none, silu, gelu, silu_and_mul or gelu_and_mul, got ", name);
+}
+
+// Row stride of a [rows, columns] tensor with contiguous rows.
+int64_t row_stride(const torch::Tensor& t, int64_t rows, int64_t cols, const torch::Tensor& like,
+                   torch::Dtype type, const char* what) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == type && t.dim() == 2 &&
+                  t.size(0) == rows && t.size(1) == cols &&
+                  (rows == 0 || cols <= 1 || t.stride(1) == 1),
+              what, " must be ", type, " [", rows, ", ", cols, "] on x's device, with contiguous rows");
+  return rows <= 1 ? std::max<int64_t>(t.stride(0), cols) : t.stride(0);
+}
+
+void check_experts(const torch::Tensor& t, const torch::Tensor& like, int64_t experts, int64_t rows,
+                   int64_t cols, const char* what) {
+  TORCH_CHECK(t.defined() && t.device() == like.device() && t.scalar_type() == like.scalar_type() &&
+                  t.dim() == 3 && t.size(0) == experts && t.size(1) == rows && t.size(2) == cols &&
+                  (cols <= 1 || t.stride(2) == 1),
+              what, " must be [", experts, ", ", rows, ", ", cols,
+              "] of x's type and device, with contiguous rows");
+}
+}  // namespace
+
+torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& bias,
+                     const std::string& activation, const torch::Tensor& residual,
+                     const torch::Tensor& out, c10::optional<torch::Dtype> out_dtype) {
+  sgl_linear_t a{};
+  a.activation = activation_of(activation);
+  TORCH_CHECK(x.defined() && x.is_cuda() && x.dim() == 2, "x must be a [T, k] device tensor");
+  TORCH_CHECK(weight.defined() && weight.dim() == 2, "weight must be a matrix");
+  const c10::DeviceGuard guard(x.device());
+  a.dtype = half_dtype(x, "x");
+  const bool gated = a.activation >= SGL_ACT_SILU_AND_MUL;
+  TORCH_CHECK(!gated || weight.size(0) % 2 == 0,
+              "a gated projection needs as many gate rows as up rows");
+  const auto type = x.scalar_type();
+  const auto to = out_dtype.value_or(out.defined() ? out.scalar_type() : type);
+  TORCH_CHECK(to == type || to == torch::kFloat32, "out must have x's type or float32");
+  a.tokens = x.size(0), a.k = x.size(1);
+  a.n = gated ? weight.size(0) / 2 : weight.size(0);
+  a.x_stride_row = row_stride(x, a.tokens, a.k, x, type, "x");
+  a.weight_stride_row = row_stride(weight, weight.size(0), a.k, x, type, "weight");
+  if (bias.defined()) {
+    TORCH_CHECK(bias.device() == x.device() && bias.scalar_type() == type && bias.dim() == 1 &&
+                    bias.size(0) == weight.size(0) && bias.is_contiguous(),
+                "bias must be a contiguous vector of weight's rows, of x's type and device");
+    a.bias = bias.data_ptr();
+  }
+  if (residual.defined()) {
+    a.residual_stride_row = row_stride(residual, a.tokens, a.n, x, type, "residual");
+    a.residual = residual.data_ptr();
+  }
+  auto o = out.defined() ? out : torch::empty({a.tokens, a.n}, x.options().dtype(to));
+  a.out_stride_row = row_stride(o, a.tokens, a.n, x, to, "out");
+  a.out_dtype = to == type ? a.dtype : SGL_DTYPE_F32;
+  a.x = x.data_ptr(), a.weight = weight.data_ptr(), a.out = o.data_ptr();
+  const int64_t bytes = sgl_linear_workspace_bytes(a.tokens, a.n, a.k, a.activation);
+  torch::Tensor ws;
+  if (bytes > 0) ws = torch::empty({bytes}, x.options().dtype(torch::kUInt8));
+  check_sgl(sgl_linear(&a, bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream(x.device())),
+            "sgl_linear");
+  return o;
+}
+
+std::pair<torch::Tensor, torch::Tensor> moe_route(const torch::Tensor& logits, int64_t top_k,
+                                                  bool renormalize) {
+  TORCH_CHECK(logits.defined() && logits.is_cuda() && logits.dim() == 2,
+              "logits must be a [T, experts] device tensor");
+  const c10::DeviceGuard guard(logits.device());
+  const int dt = logits.scalar_type() == torch::kFloat32 ? SGL_DTYPE_F32 : half_dtype(logits, "logits");
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  const int64_t stride = row_stride(logits, tokens, experts, logits, logits.scalar_type(), "logits");
+  TORCH_CHECK(top_k > 0 && top_k <= experts, "top_k must be in [1, experts]");
+  auto weights = torch::empty({tokens, top_k}, logits.options().dtype(torch::kFloat32));
+  auto ids = torch::empty({tokens, top_k}, logits.options().dtype(torch::kInt32));
+  check_sgl(sgl_moe_route(logits.data_ptr(), stride, dt, tokens, narrow_dim(experts, "experts"),
+                          static_cast<int>(top_k), renormalize, weights.data_ptr<float>(),
+                          ids.data_ptr<int32_t>(), current_stream(logits.device())),
+            "sgl_moe_route");
+  return {weights, ids};
+}
+
+torch::Tensor moe_experts(const torch::Tensor& x, const torch::Tensor& gate_up,
+                          const torch::Tensor& down, const torch::Tensor& weights,
+                          const torch::Tensor& experts, const torch::Tensor& residual,
+                          const std::string& activation, const torch::Tensor& out) {
+  sgl_moe_t a{};
+  a.activation = activation_of(activation);
+  TORCH_CHECK(a.activation >= SGL_ACT_SILU_AND_MUL, "activation must be silu_and_mul or gelu_and_mul");
+  TORCH_CHECK(x.defined() && x.is_cuda() && x.dim() == 2, "x must be a [T, H] device tensor");
+  TORCH_CHECK(gate_up.defined() && gate_up.dim() == 3 && down.defined() && down.dim() == 3,
+              "gate_up must be [E, 2 I, H] and down [E, H, I]");
+  const c10::DeviceGuard guard(x.device());
+  a.dtype = half_dtype(x, "x");
+  const int64_t hidden = x.size(1), inter = down.size(2), num = gate_up.size(0);
+  a.tokens = x.size(0);
+  check_experts(gate_up, x, num, 2 * inter, hidden, "gate_up");
+  check_experts(down, x, num, hidden, inter, "down");
+  for (const auto& t : {weights, experts})
+    TORCH_CHECK(t.defined() && t.device() == x.device() && t.dim() == 2 && t.size(0) == a.tokens &&
+                    t.size(1) == weights.size(1) && t.is_contiguous(),
+                "weights and experts must be contiguous [T, top_k] on x's device");
+  TORCH_CHECK(weights.scalar_type() == torch::kFloat32 && experts.scalar_type() == torch::kInt32,
+              "weights must be float32 and experts int32");
+  a.num_experts = narrow_dim(num, "experts"), a.top_k = narrow_dim(weights.size(1), "top_k");
+  a.hidden = narrow_dim(hidden, "hidden"), a.intermediate = narrow_dim(inter, "intermediate");
+  a.x_stride_row = row_stride(x, a.tokens, hidden, x, x.scalar_type(), "x");
+  auto o = out.defined() ? out : torch::empty({a.tokens, hidden}, x.options());
+  a.out_stride_row = row_stride(o, a.tokens, hidden, x, x.scalar_type(), "out");
+  if (residual.defined()) {
+    a.residual_stride_row = row_stride(residual, a.tokens, hidden, x, x.scalar_type(), "residual");
+    a.residual = residual.data_ptr();
+  }
+  auto rows = [](const torch::Tensor& t) {
+    return t.size(1) <= 1 ? std::max<int64_t>(t.stride(1), t.size(2)) : t.stride(1);
+  };
+  a.gate_up_stride_expert = gate_up.stride(0), a.gate_up_stride_row = rows(gate_up);
+  a.down_stride_expert = down.stride(0), a.down_stride_row = rows(down);
+  a.x = x.data_ptr(), a.gate_up = gate_up.data_ptr(), a.down = down.data_ptr(), a.out = o.data_ptr();
+  a.weights = weights.data_ptr<float>(), a.experts = experts.data_ptr<int32_t>();
+  const int64_t bytes =
+      sgl_moe_workspace_bytes(a.tokens, a.top_k, a.num_experts, a.hidden, a.intermediate);
+  auto ws = torch::empty({bytes}, x.options().dtype(torch::kUInt8));
+  check_sgl(sgl_moe_experts(&a, ws.data_ptr(), bytes, current_stream(x.device())), "sgl_moe_experts");
+  return o;
+}
+
+GatedMLP::GatedMLP(int hidden, int intermediate, const std::string& activation, torch::Device device)
+    : activation_(activation) {
+  TORCH_CHECK(activation_of(activation) >= SGL_ACT_SILU_AND_MUL,
+              "GatedMLP: activation must be silu_and_mul or gelu_and_mul");
+  TORCH_CHECK(hidden > 0 && intermediate > 0, "GatedMLP: sizes must be positive");
+  const auto opts = torch::TensorOptions().dtype(torch::kBFloat16).device(device);
+  gate_up = torch::zeros({2 * static_cast<int64_t>(intermediate), hidden}, opts);
+  down = torch::zeros({hidden, intermediate}, opts);
+}
+
+torch::Tensor GatedMLP::forward(const torch::Tensor& x, const torch::Tensor& residual) const {
+  const auto h = linear(x, gate_up, torch::Tensor(), activation_, torch::Tensor(), torch::Tensor(), {});
+  return linear(h, down, torch::Tensor(), "none", residual, torch::Tensor(), {});
+}
+
+MoEMLP::MoEMLP(int hidden, int intermediate, int num_experts, int top_k, bool renormalize,
+               const std::string& activation, torch::Device device)
+    : top_k_(top_k), renormalize_(renormalize), activation_(activation) {
+  TORCH_CHECK(activation_of(activation) >= SGL_ACT_SILU_AND_MUL,
+              "MoEMLP: activation must be silu_and_mul or gelu_and_mul");
+  TORCH_CHECK(hidden > 0 && intermediate > 0 && num_experts > 0 && top_k > 0 && top_k <= num_experts,
+              "MoEMLP: sizes must be positive and top_k at most the experts");
+  const auto opts = torch::TensorOptions().dtype(torch::kBFloat16).device(device);
+  router = torch::zeros({num_experts, hidden}, opts);
+  gate_up = torch::zeros({num_experts, 2 * static_cast<int64_t>(intermediate), hidden}, opts);
+  down = torch::zeros({num_experts, hidden, intermediate}, opts);
+}
+
+torch::Tensor MoEMLP::forward(const torch::Tensor& x, const torch::Tensor& residual) const {
+  // The logits in fp32: rounded to 16 bits, near ones would tie and the lower expert win.
+  const auto logits =
+      linear(x, router, torch::Tensor(), "none", torch::Tensor(), torch::Tensor(), torch::kFloat32);
+  const auto chosen = moe_route(logits, top_k_, renormalize_);
+  return moe_experts(x, gate_up, down, chosen.first, chosen.second, residual, activation_,
+                     torch::Tensor());
+}
+
 // ---------------------------------------------------------------- sampling
 
 namespace {
@@ -1031,11 +1207,6 @@ FlashInferSamplingResult sampling_outputs(const torch::Tensor& probs) {
   auto opts = probs.options();
   return {torch::empty({probs.size(0)}, opts.dtype(torch::kInt32)),
           torch::empty({probs.size(0)}, opts.dtype(torch::kBool))};
-}
-
-int32_t narrow_dim(int64_t v, const char* what) {
-  TORCH_CHECK(v >= 0 && v <= 0x7fffffff, what, " out of range");
-  return static_cast<int32_t>(v);
 }
 
 // One draw over the rows, with the workspace a small batch is split over.

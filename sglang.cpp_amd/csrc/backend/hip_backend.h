@@ -247,6 +247,52 @@ void fused_qk_rmsnorm_inplace_3d_strided(torch::Tensor& q, torch::Tensor& k, con
 void silu_and_mul(torch::Tensor& out, const torch::Tensor& input);
 void gelu_and_mul(torch::Tensor& out, const torch::Tensor& input);
 
+// act(x weight^T + bias) + residual (sgl_linear; src/layers/linear.cc:9-78): x [T, k],
+// weight [n, k], or [2 n, k] (gate rows, then up rows) with "silu_and_mul" and
+// "gelu_and_mul"; activation "none", "silu" or "gelu" otherwise. bf16 or fp16; undefined
+// bias, residual and out: none, none, a new tensor of out_dtype (x's type, or fp32).
+torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& bias,
+                     const std::string& activation, const torch::Tensor& residual,
+                     const torch::Tensor& out, c10::optional<torch::Dtype> out_dtype);
+
+// (weights fp32, experts int32), [T, top_k], from the router's logits [T, experts]
+// (sgl_moe_route; src/moe/moe.cc:47-60).
+std::pair<torch::Tensor, torch::Tensor> moe_route(const torch::Tensor& logits, int64_t top_k,
+                                                  bool renormalize);
+
+// The chosen experts' weighted outputs + residual (sgl_moe_experts; src/moe/moe.cc:62-98):
+// x [T, H], gate_up [E, 2 I, H], down [E, H, I], weights and experts [T, top_k].
+torch::Tensor moe_experts(const torch::Tensor& x, const torch::Tensor& gate_up,
+                          const torch::Tensor& down, const torch::Tensor& weights,
+                          const torch::Tensor& experts, const torch::Tensor& residual,
+                          const std::string& activation, const torch::Tensor& out);
+
+// The dense MLP of a decoder layer (GatedMLP, src/models/utils.cc): down(act(gate) * up),
+// + residual where it is defined. Weights bf16 until they are set; fp16 ones serve fp16.
+class GatedMLP {
+ public:
+  GatedMLP(int hidden, int intermediate, const std::string& activation, torch::Device device);
+  torch::Tensor forward(const torch::Tensor& x, const torch::Tensor& residual) const;
+  torch::Tensor gate_up, down;  // [2 I, H], [H, I]
+
+ private:
+  std::string activation_;
+};
+
+// The mixture-of-experts MLP (MoEMLP, src/moe/moe.cc:36-98): router, choice, experts.
+class MoEMLP {
+ public:
+  MoEMLP(int hidden, int intermediate, int num_experts, int top_k, bool renormalize,
+         const std::string& activation, torch::Device device);
+  torch::Tensor forward(const torch::Tensor& x, const torch::Tensor& residual) const;
+  torch::Tensor router, gate_up, down;  // [E, H], [E, 2 I, H], [E, H, I]
+
+ private:
+  int top_k_;
+  bool renormalize_;
+  std::string activation_;
+};
+
 // Sampling from probabilities, the reference's Sampler kernels
 // (include/sglang/engine/sampling.h:7-36, src/engine/sampling.cu:65-194):
 // same names, arguments and checks; the HIP kernels replace FlashInfer's.

@@ -1,0 +1,268 @@
+// Device code shared by the projections (linear.hip) and the experts (moe.hip):
+// y[t, n] = sum_k x[t, k] w[n, k] and what follows it.
+//
+// The matrix instruction's rows are weight rows and its columns tokens, so a lane
+// ends with four consecutive outputs of one token (one 8-byte store). Products of
+// 16-bit values, sums, bias, activation, weighting and residual are fp32; the result
+// is rounded once. Gate and up projections (GATED) are one matrix of 2 n rows: a tile
+// alternates blocks of 16 gate rows with the 16 up rows of the same outputs, which so
+// meet in one lane.
+#pragma once
+
+#include "common.h"
+
+namespace sgl {
+namespace gemm {
+
+enum Mode : int {
+  kLinear = 0,  // rows of x are the tokens
+  kGateUp = 1,  // experts: sorted places read their token's row of x, written in order
+  kDown = 2,    // experts: sorted places read in order, weighted, written to their slot
+};
+
+struct Args {
+  const uint16_t* x;
+  const uint16_t* w;
+  const uint16_t* bias;  // kLinear
+  const uint16_t* res;   // kLinear
+  void* out;
+  int64_t x_st, w_st, w_se, r_st, o_st;  // strides of a row (w_se: of an expert)
+  int32_t tokens, n, k;
+  int32_t act;      // SGL_ACT_*
+  int32_t out_f32;  // out is fp32
+  int32_t wide;     // outputs, bias and residual of four columns can go in one access
+  int32_t tiles_n;  // tiles over the outputs
+  int32_t top_k;
+  const int4* tiles;     // experts: {expert, first place, places, 0} of a tile of places
+  const int32_t* order;  // experts: slot (token top_k + j) of each place
+  const float* scale;    // kDown: weight of each slot
+};
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// D += A B with 16 x 32 and 32 x 16 operands: lane l holds elements 8 (l / 16) .. + 7 of
+// A's row l % 16 and of B's column l % 16, and rows 4 (l / 16) .. + 3 of D's column l % 16.
+template <int DT>
+__device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
+  if constexpr (DT == SGL_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// x sigmoid(z), z = x (SiLU) or 2 * 0.7978845608 (x + 0.044715 x^3) (tanh GELU, since
+// (1 + tanh(u)) / 2 = sigmoid(2 u)), on the hardware exp2 and reciprocal: an fp32 ulp or
+// two, where the output is rounded to 16 bits.
+__device__ __forceinline__ float activate(int act, float x) {
+  if (act == SGL_ACT_NONE) return x;
+  float z = x;
+  if (act == SGL_ACT_GELU || act == SGL_ACT_GELU_AND_MUL)
+    z = 2.0f * 0.7978845608f * (x + 0.044715f * x * x * x);
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-z * 1.4426950408889634f));
+}
+
+// Eight elements of a row from element e on, zero from element k on. VEC: rows start on
+// 16 bytes and k is a multiple of 8.
+template <bool VEC>
+__device__ __forceinline__ u32x4_t load8(const uint16_t* row, int e, int k) {
+  u32x4_t v = {0, 0, 0, 0};
+  if constexpr (VEC) {
+    if (e < k) v = ldg128(row + e);
+  } else if (e + 8 <= k) {
+    __builtin_memcpy(&v, row + e, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e + i < k) v[i / 2] |= static_cast<uint32_t>(row[e + i]) << (16 * (i & 1));
+  }
+  return v;
+}
+
+// Outputs n0 .. n0 + 3 of one row: g (and, gated, u) from the accumulators.
+template <int DT, int MODE, bool GATED>
+__device__ __forceinline__ void finish4(const Args& a, int n0, int64_t row, float scale, f32x4_t g,
+                                        f32x4_t u) {
+  if (n0 >= a.n) return;
+  if (a.wide && n0 + 4 <= a.n) {
+    if constexpr (MODE == kLinear) {
+      if (a.bias) {
+        const u32x2_t b = *reinterpret_cast<const u32x2_t*>(a.bias + n0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] += to_f32<DT>((b[i / 2] >> (16 * (i & 1))) & 0xffffu);
+        if constexpr (GATED) {
+          const u32x2_t c = *reinterpret_cast<const u32x2_t*>(a.bias + a.n + n0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[i] += to_f32<DT>((c[i / 2] >> (16 * (i & 1))) & 0xffffu);
+        }
+      }
+    }
+    if constexpr (MODE != kDown) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = activate(a.act, g[i]);
+    }
+    if constexpr (GATED) g *= u;
+    if constexpr (MODE == kDown) g *= scale;
+    if constexpr (MODE == kLinear) {
+      if (a.res) {
+        const u32x2_t r = *reinterpret_cast<const u32x2_t*>(a.res + row * a.r_st + n0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] += to_f32<DT>((r[i / 2] >> (16 * (i & 1))) & 0xffffu);
+      }
+    }
+    if (a.out_f32) {
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + row * a.o_st + n0) = g;
+    } else {
+      const u32x2_t v = {pack2_t<DT>(g[0], g[1]), pack2_t<DT>(g[2], g[3])};
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + row * a.o_st + n0) = v;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = n0 + i;
+    if (n >= a.n) break;
+    float y = g[i];
+    if constexpr (MODE == kLinear) {
+      if (a.bias) y += to_f32<DT>(a.bias[n]);
+    }
+    if constexpr (MODE != kDown) y = activate(a.act, y);
+    if constexpr (GATED) {
+      float z = u[i];
+      if constexpr (MODE == kLinear) {
+        if (a.bias) z += to_f32<DT>(a.bias[a.n + n]);
+      }
+      y *= z;
+    }
+    if constexpr (MODE == kDown) y *= scale;
+    if constexpr (MODE == kLinear) {
+      if (a.res) y += to_f32<DT>(a.res[row * a.r_st + n]);
+    }
+    if (a.out_f32) static_cast<float*>(a.out)[row * a.o_st + n] = y;
+    else static_cast<uint16_t*>(a.out)[row * a.o_st + n] = static_cast<uint16_t>(from_f32<DT>(y));
+  }
+}
+
+// The part of a launch that a workgroup has: rows [first, first + rows) of the tokens, or
+// of an expert's places.
+struct Part {
+  int expert, first, rows;
+};
+
+template <int MODE>
+__device__ __forceinline__ Part part_of(const Args& a, int tile, int tile_rows) {
+  if constexpr (MODE == kLinear) {
+    const int first = tile * tile_rows;
+    return {0, first, min(tile_rows, a.tokens - first)};
+  } else {
+    const int4 t = a.tiles[tile];
+    return {t.x, t.y, t.z};
+  }
+}
+
+// Row of x, row of the output and weight of place or token i.
+template <int MODE>
+__device__ __forceinline__ int64_t source_row(const Args& a, int i) {
+  return MODE == kGateUp ? a.order[i] / a.top_k : i;
+}
+template <int MODE>
+__device__ __forceinline__ int64_t target_row(const Args& a, int i, float& scale) {
+  scale = 1.f;
+  if constexpr (MODE == kDown) {
+    const int slot = a.order[i];
+    scale = a.scale[slot];
+    return slot;
+  }
+  return i;
+}
+
+// Weight row of row r of a tile whose first output is n0, -1 past the last output.
+template <bool GATED>
+__device__ __forceinline__ int64_t weight_row(const Args& a, int n0, int r) {
+  const int n = GATED ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
+  if (n >= a.n) return -1;
+  return GATED && (r & 16) ? static_cast<int64_t>(a.n) + n : n;
+}
+
+// Any sizes, strides and alignment: tiles of 64 weight rows x 64 tokens, staged through
+// registers and LDS, four waves of 32 x 32 outputs.
+constexpr int kAnyTile = 64;
+constexpr int kAnyPitch = 40;  // 32 elements and 16 bytes: rows start on different banks
+
+template <int DT, int MODE, bool GATED, bool VEC>
+__global__ __launch_bounds__(256) void any_kernel(const Args a) {
+  __shared__ uint16_t sw[kAnyTile * kAnyPitch], sx[kAnyTile * kAnyPitch];
+  const int tn = blockIdx.x % a.tiles_n, tt = blockIdx.x / a.tiles_n;
+  const Part p = part_of<MODE>(a, tt, kAnyTile);
+  if (p.rows <= 0) return;
+  const int n0 = tn * (GATED ? kAnyTile / 2 : kAnyTile);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r = tid >> 2, c = (tid & 3) * 8;
+  const int64_t wr = weight_row<GATED>(a, n0, r);
+  const uint16_t* wp = a.w + p.expert * a.w_se + (wr < 0 ? 0 : wr) * a.w_st;
+  const bool has_x = r < p.rows;
+  const uint16_t* xp = a.x + (has_x ? source_row<MODE>(a, p.first + r) : 0) * a.x_st;
+  const u32x4_t zero = {0, 0, 0, 0};
+  f32x4_t acc[2][2] = {};
+  const int aw = (wave & 1) * 32 + (lane & 15), ax = (wave >> 1) * 32 + (lane & 15);
+  const int ac = (lane >> 4) * 8;
+  u32x4_t vw = wr < 0 ? zero : load8<VEC>(wp, c, a.k);
+  u32x4_t vx = has_x ? load8<VEC>(xp, c, a.k) : zero;
+  for (int k0 = 0; k0 < a.k; k0 += 32) {
+    stg128(&sw[r * kAnyPitch + c], vw);
+    stg128(&sx[r * kAnyPitch + c], vx);
+    __syncthreads();
+    if (k0 + 32 < a.k) {
+      vw = wr < 0 ? zero : load8<VEC>(wp, k0 + 32 + c, a.k);
+      vx = has_x ? load8<VEC>(xp, k0 + 32 + c, a.k) : zero;
+    }
+    u32x4_t fw[2], fx[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      fw[i] = ldg128(&sw[(aw + 16 * i) * kAnyPitch + ac]);
+      fx[i] = ldg128(&sx[(ax + 16 * i) * kAnyPitch + ac]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<DT>(fw[i], fx[j], acc[i][j]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int t = ax + 16 * j;
+    if (t >= p.rows) continue;
+    float scale;
+    const int64_t row = target_row<MODE>(a, p.first + t, scale);
+    const int q = 4 * (lane >> 4);
+    if constexpr (GATED) {
+      finish4<DT, MODE, true>(a, n0 + (wave & 1) * 16 + q, row, scale, acc[0][j], acc[1][j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        finish4<DT, MODE, false>(a, n0 + (wave & 1) * 32 + 16 * i + q, row, scale, acc[i][j],
+                                 acc[i][j]);
+    }
+  }
+}
+
+// Workgroups of a launch, or -1 where it has more than a grid.
+inline int64_t grid_of(int64_t tiles_n, int64_t tiles_t) {
+  return tiles_t > 0 && tiles_n > 0x7fffffff / tiles_t ? -1 : tiles_n * tiles_t;
+}
+
+template <int DT, int MODE, bool GATED>
+int launch_any(Args a, bool vec, int64_t tiles_t, hipStream_t s) {
+  const int out = GATED ? kAnyTile / 2 : kAnyTile;
+  a.tiles_n = static_cast<int32_t>((static_cast<int64_t>(a.n) + out - 1) / out);
+  const int64_t grid = grid_of(a.tiles_n, tiles_t);
+  if (grid < 0) return SGL_ERR_UNSUPPORTED;
+  const dim3 g(static_cast<uint32_t>(grid)), b(256);
+  if (vec) hipLaunchKernelGGL((any_kernel<DT, MODE, GATED, true>), g, b, 0, s, a);
+  else hipLaunchKernelGGL((any_kernel<DT, MODE, GATED, false>), g, b, 0, s, a);
+  return launch_status();
+}
+
+}  // namespace gemm
+}  // namespace sgl

@@ -1,0 +1,325 @@
+// Mixture of experts: sgl_moe_route (the experts of each token from the router's logits)
+// and sgl_moe_experts (their gate, up and down projections and the weighted sum).
+#include "gemm.h"
+
+namespace sgl {
+namespace {
+
+// ------------------------------------------------------------------ route
+
+constexpr int kMostExperts = 512;
+constexpr int kMostChosen = 32;
+
+struct RouteArgs {
+  const void* logits;
+  int64_t stride;
+  float* weights;
+  int32_t* experts;
+  int64_t tokens;
+  int32_t num_experts, top_k, renormalize;
+};
+
+template <int DT>
+__device__ __forceinline__ float load_logit(const void* p, int64_t i) {
+  if constexpr (DT == SGL_DTYPE_F32) return static_cast<const float*>(p)[i];
+  else return to_f32<DT>(static_cast<const uint16_t*>(p)[i]);
+}
+
+// Order of a logit as a whole number: larger logits are larger, NaN is below -inf, and
+// -0 is 0. Never 0, which marks an expert already taken.
+__device__ __forceinline__ uint32_t rank_of(float x) {
+  if (x != x) return 1;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// One wave a token: expert lane + 64 i in register i. Each round takes the largest
+// (rank, lowest expert) of the wave.
+template <int DT, int V>
+__global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (t >= a.tokens) return;
+  const int64_t row = t * a.stride;
+  float x[V];
+  uint32_t key[V];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 64 * i;
+    x[i] = e < a.num_experts ? load_logit<DT>(a.logits, row + e) : -INFINITY;
+    key[i] = e < a.num_experts ? rank_of(x[i]) : 0;
+    top = fmaxf(top, x[i]);
+  }
+  top = group_max<64>(top);
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) total += lane + 64 * i < a.num_experts ? expf(x[i] - top) : 0.f;
+  total = group_sum<64>(total);
+  float mine = 0.f, sum = 0.f;
+  int32_t my_expert = 0;
+  for (int j = 0; j < a.top_k; ++j) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint64_t c = (static_cast<uint64_t>(key[i]) << 32) | ~static_cast<uint32_t>(lane + 64 * i);
+      if (key[i] && c > best) best = c;
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+      const uint64_t other = __shfl_xor(best, off, kWave);
+      best = other > best ? other : best;
+    }
+    const int e = static_cast<int>(~static_cast<uint32_t>(best));
+    float value = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane + 64 * i == e) {
+        value = expf(x[i] - top);
+        key[i] = 0;
+      }
+    value = __shfl(value, e & 63, kWave);
+    sum += value;
+    if (lane == j) mine = value, my_expert = e;
+  }
+  // A row with a NaN, or no finite logit, has a NaN total and NaN weights.
+  if (lane < a.top_k) {
+    a.weights[t * a.top_k + lane] = mine / (a.renormalize ? sum + (total - total) : total);
+    a.experts[t * a.top_k + lane] = my_expert;
+  }
+}
+
+template <int DT>
+void launch_route(const RouteArgs& a, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>((a.tokens + 3) / 4)), block(256);
+  if (a.num_experts <= 64) hipLaunchKernelGGL((route_kernel<DT, 1>), grid, block, 0, s, a);
+  else if (a.num_experts <= 128) hipLaunchKernelGGL((route_kernel<DT, 2>), grid, block, 0, s, a);
+  else if (a.num_experts <= 256) hipLaunchKernelGGL((route_kernel<DT, 4>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((route_kernel<DT, 8>), grid, block, 0, s, a);
+}
+
+// ------------------------------------------------------------------ experts
+
+struct SortArgs {
+  const int32_t* experts;  // [slots]
+  int32_t* order;          // slots by expert, those of one expert in their own order
+  int4* tiles;
+  int32_t slots, num_experts, tile_rows, num_tiles;
+};
+
+constexpr int kSortThreads = 256;
+
+// One workgroup an expert counts the slots of lower experts (its first place) and writes
+// its own slots and tiles. Expert e's tiles start at entry first / tile_rows + e: a later
+// expert's cannot start inside them, so no expert needs another's tiles.
+__global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
+  __shared__ int32_t lower_of[kSortThreads / kWave], own_of[kSortThreads / kWave];
+  const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int kWaves = kSortThreads / kWave;
+  // Wave w has the slots [w per, (w + 1) per).
+  const int per = (a.slots + kSortThreads - 1) / kSortThreads * kWave;
+  const int begin = min(a.slots, wave * per), end = min(a.slots, begin + per);
+  int lower = 0, own = 0;
+  for (int i = begin; i < end; i += kWave) {
+    const int x = i + lane < end ? a.experts[i + lane] : -1;
+    lower += __popcll(__ballot(x >= 0 && x < e));
+    own += __popcll(__ballot(x == e));
+  }
+  if (lane == 0) lower_of[wave] = lower, own_of[wave] = own;
+  __syncthreads();
+  int first = 0, at = 0, count = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    first += lower_of[w];
+    at += w < wave ? own_of[w] : 0;
+    count += own_of[w];
+  }
+  at += first;
+  for (int i = begin; i < end; i += kWave) {
+    const bool hit = i + lane < end && a.experts[i + lane] == e;
+    const uint64_t hits = __ballot(hit);
+    if (hit) a.order[at + __popcll(hits & ((1ull << lane) - 1))] = i + lane;
+    at += __popcll(hits);
+  }
+  const int t0 = first / a.tile_rows + e;
+  const int t1 = e + 1 == a.num_experts ? a.num_tiles : (first + count) / a.tile_rows + e + 1;
+  for (int t = t0 + tid; t < t1; t += kSortThreads) {
+    const int done = (t - t0) * a.tile_rows;
+    a.tiles[t] = int4{e, first + done, min(a.tile_rows, count - done), 0};
+  }
+}
+
+struct CombineArgs {
+  const float* y;  // [slots, stride] weighted outputs of the slots
+  const int32_t* experts;
+  const uint16_t* res;
+  uint16_t* out;
+  int64_t y_st, r_st, o_st;
+  int32_t hidden, top_k, num_experts, wide;
+};
+
+// out[t] = the sum of its slots in their order (+ residual); slots of no expert are skipped.
+template <int DT>
+__global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
+  const int64_t t = blockIdx.x;
+  const int32_t* ids = a.experts + t * a.top_k;
+  for (int h = 4 * threadIdx.x; h < a.hidden; h += 4 * 256) {
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < a.top_k; ++j)
+      if (ids[j] >= 0 && ids[j] < a.num_experts)
+        sum += *reinterpret_cast<const f32x4_t*>(a.y + (t * a.top_k + j) * a.y_st + h);
+    uint16_t* o = a.out + t * a.o_st + h;
+    const uint16_t* r = a.res ? a.res + t * a.r_st + h : nullptr;
+    if (a.wide && h + 4 <= a.hidden) {
+      if (r) {
+        const u32x2_t v = *reinterpret_cast<const u32x2_t*>(r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += to_f32<DT>((v[i / 2] >> (16 * (i & 1))) & 0xffffu);
+      }
+      *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack2_t<DT>(sum[0], sum[1]), pack2_t<DT>(sum[2], sum[3])};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (h + i < a.hidden)
+          o[i] = static_cast<uint16_t>(from_f32<DT>(sum[i] + (r ? to_f32<DT>(r[i]) : 0.f)));
+    }
+  }
+}
+
+bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0);
+}
+
+constexpr int64_t kMost = 0x7fffff00;
+constexpr int kTileRows = gemm::kAnyTile;
+
+// The workspace: slots in order, tiles, the rows between the projections and the
+// weighted outputs. Rows are padded to whole 16 bytes.
+struct Layout {
+  int64_t num_tiles, h_st, y_st, order, tiles, h, y, bytes;
+};
+
+Layout layout_of(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) {
+  const auto up = [](int64_t x, int64_t to) { return (x + to - 1) / to * to; };
+  Layout l;
+  l.num_tiles = slots / kTileRows + experts;
+  l.h_st = up(inter, 8);
+  l.y_st = up(hidden, 4);
+  l.order = 0;
+  l.tiles = up(slots * 4, 256);
+  l.h = l.tiles + up(l.num_tiles * 16, 256);
+  l.y = l.h + up(slots * l.h_st * 2, 256);
+  l.bytes = l.y + up(slots * l.y_st * 4, 256);
+  return l;
+}
+
+bool sizes_ok(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden, int64_t inter) {
+  return tokens >= 0 && top_k > 0 && experts > 0 && hidden > 0 && inter > 0;
+}
+bool sizes_built(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden, int64_t inter) {
+  return top_k <= kMost && tokens <= kMost / top_k && experts <= 65536 && hidden <= 1 << 20 &&
+         inter <= 1 << 20;
+}
+
+template <int DT>
+int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
+  const int slots = static_cast<int>(x.tokens * x.top_k);
+  int32_t* order = reinterpret_cast<int32_t*>(ws + l.order);
+  int4* tiles = reinterpret_cast<int4*>(ws + l.tiles);
+  uint16_t* h = reinterpret_cast<uint16_t*>(ws + l.h);
+  float* y = reinterpret_cast<float*>(ws + l.y);
+  const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, kTileRows,
+                      static_cast<int32_t>(l.num_tiles)};
+  hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
+  int st = launch_status();
+  if (st != SGL_OK) return st;
+
+  gemm::Args a{};
+  a.tiles = tiles, a.order = order, a.top_k = x.top_k, a.scale = x.weights;
+  a.x = static_cast<const uint16_t*>(x.x), a.x_st = x.x_stride_row;
+  a.w = static_cast<const uint16_t*>(x.gate_up);
+  a.w_st = x.gate_up_stride_row, a.w_se = x.gate_up_stride_expert;
+  a.out = h, a.o_st = l.h_st, a.wide = 1;
+  a.tokens = slots, a.n = x.intermediate, a.k = x.hidden, a.act = x.activation;
+  bool vec = x.hidden % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
+             aligned(x.gate_up, x.gate_up_stride_row, 16, 2) && x.gate_up_stride_expert % 8 == 0;
+  st = gemm::launch_any<DT, gemm::kGateUp, true>(a, vec, l.num_tiles, s);
+  if (st != SGL_OK) return st;
+
+  a.x = h, a.x_st = l.h_st;
+  a.w = static_cast<const uint16_t*>(x.down);
+  a.w_st = x.down_stride_row, a.w_se = x.down_stride_expert;
+  a.out = y, a.o_st = l.y_st, a.out_f32 = 1;
+  a.n = x.hidden, a.k = x.intermediate;
+  vec = x.intermediate % 8 == 0 && aligned(x.down, x.down_stride_row, 16, 2) &&
+        x.down_stride_expert % 8 == 0;
+  st = gemm::launch_any<DT, gemm::kDown, false>(a, vec, l.num_tiles, s);
+  if (st != SGL_OK) return st;
+
+  CombineArgs c{};
+  c.y = y, c.y_st = l.y_st, c.experts = x.experts;
+  c.res = static_cast<const uint16_t*>(x.residual), c.r_st = x.residual_stride_row;
+  c.out = static_cast<uint16_t*>(x.out), c.o_st = x.out_stride_row;
+  c.hidden = x.hidden, c.top_k = x.top_k, c.num_experts = x.num_experts;
+  c.wide = aligned(x.out, x.out_stride_row, 8, 2) && aligned(x.residual, x.residual_stride_row, 8, 2);
+  hipLaunchKernelGGL((combine_kernel<DT>), dim3(static_cast<uint32_t>(x.tokens)), dim3(256), 0, s, c);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace sgl
+
+using namespace sgl;
+
+extern "C" int sgl_moe_route(const void* logits, int64_t logits_stride_row, int logits_dtype,
+                             int64_t tokens, int num_experts, int top_k, int renormalize,
+                             float* weights, int32_t* experts, void* stream) {
+  if (tokens < 0 || num_experts <= 0 || top_k <= 0 || top_k > num_experts) return SGL_ERR_INVALID_ARG;
+  if (num_experts > kMostExperts || top_k > kMostChosen || tokens > kMost) return SGL_ERR_UNSUPPORTED;
+  if (logits_dtype < SGL_DTYPE_BF16 || logits_dtype > SGL_DTYPE_F32) return SGL_ERR_UNSUPPORTED;
+  if (tokens == 0) return SGL_OK;
+  if (!logits || !weights || !experts || logits_stride_row < num_experts) return SGL_ERR_INVALID_ARG;
+  const RouteArgs a{logits, logits_stride_row, weights, experts, tokens, num_experts, top_k,
+                    renormalize != 0};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (logits_dtype == SGL_DTYPE_F32) launch_route<SGL_DTYPE_F32>(a, s);
+  else if (logits_dtype == SGL_DTYPE_BF16) launch_route<SGL_DTYPE_BF16>(a, s);
+  else launch_route<SGL_DTYPE_F16>(a, s);
+  return launch_status();
+}
+
+extern "C" int64_t sgl_moe_workspace_bytes(int64_t tokens, int top_k, int num_experts, int hidden,
+                                           int intermediate) {
+  if (!sizes_ok(tokens, top_k, num_experts, hidden, intermediate) ||
+      !sizes_built(tokens, top_k, num_experts, hidden, intermediate))
+    return 0;
+  return layout_of(tokens * top_k, num_experts, hidden, intermediate).bytes;
+}
+
+extern "C" int sgl_moe_experts(const sgl_moe_t* args, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+  if (!args) return SGL_ERR_INVALID_ARG;
+  const sgl_moe_t& x = *args;
+  if (!sizes_ok(x.tokens, x.top_k, x.num_experts, x.hidden, x.intermediate)) return SGL_ERR_INVALID_ARG;
+  if (x.dtype != SGL_DTYPE_BF16 && x.dtype != SGL_DTYPE_F16) return SGL_ERR_UNSUPPORTED;
+  if (x.activation != SGL_ACT_SILU_AND_MUL && x.activation != SGL_ACT_GELU_AND_MUL)
+    return SGL_ERR_UNSUPPORTED;
+  if (!sizes_built(x.tokens, x.top_k, x.num_experts, x.hidden, x.intermediate))
+    return SGL_ERR_UNSUPPORTED;
+  if (x.tokens == 0) return SGL_OK;
+  if (!x.x || !x.gate_up || !x.down || !x.weights || !x.experts || !x.out) return SGL_ERR_INVALID_ARG;
+  if (x.x_stride_row < x.hidden || x.out_stride_row < x.hidden ||
+      x.gate_up_stride_row < x.hidden || x.down_stride_row < x.intermediate ||
+      (x.residual && x.residual_stride_row < x.hidden) ||
+      (x.num_experts > 1 &&
+       (x.gate_up_stride_expert < x.gate_up_stride_row * 2 * x.intermediate ||
+        x.down_stride_expert < x.down_stride_row * x.hidden)))
+    return SGL_ERR_INVALID_ARG;
+  if (x.out == x.x || (x.residual == x.out && x.residual_stride_row != x.out_stride_row))
+    return SGL_ERR_INVALID_ARG;
+  const Layout l = layout_of(x.tokens * x.top_k, x.num_experts, x.hidden, x.intermediate);
+  if (!workspace || workspace_bytes < l.bytes) return SGL_ERR_CAPACITY;
+  if (!aligned16(workspace)) return SGL_ERR_ALIGNMENT;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  return x.dtype == SGL_DTYPE_BF16 ? run<SGL_DTYPE_BF16>(x, l, ws, s) : run<SGL_DTYPE_F16>(x, l, ws, s);
+}
