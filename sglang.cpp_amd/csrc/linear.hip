@@ -1,13 +1,21 @@
 // sgl_linear: a projection with its epilogue.
-#include "gemm.h"
+#include "stream.h"
 
 namespace sgl {
 namespace {
 
 bool gated(int act) { return act == SGL_ACT_SILU_AND_MUL || act == SGL_ACT_GELU_AND_MUL; }
 
+constexpr int kStreamTokens = 64;
+
 template <int DT>
 int run(const gemm::Args& a, bool vec, hipStream_t s) {
+  if (vec && a.tokens <= kStreamTokens) {
+    gemm::StreamArgs st{};
+    st.g = a;
+    return gated(a.act) ? gemm::launch_stream<DT, gemm::kLinear, true>(st, a.tokens, 1, s)
+                        : gemm::launch_stream<DT, gemm::kLinear, false>(st, a.tokens, 1, s);
+  }
   const int64_t tiles_t = (static_cast<int64_t>(a.tokens) + gemm::kAnyTile - 1) / gemm::kAnyTile;
   return gated(a.act) ? gemm::launch_any<DT, gemm::kLinear, true>(a, vec, tiles_t, s)
                       : gemm::launch_any<DT, gemm::kLinear, false>(a, vec, tiles_t, s);

@@ -1,6 +1,8 @@
 // Mixture of experts: sgl_moe_route (the experts of each token from the router's logits)
 // and sgl_moe_experts (their gate, up and down projections and the weighted sum).
-#include "gemm.h"
+#include "stream.h"
+
+#include <algorithm>
 
 namespace sgl {
 namespace {
@@ -191,6 +193,7 @@ bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) {
 
 constexpr int64_t kMost = 0x7fffff00;
 constexpr int kTileRows = gemm::kAnyTile;
+constexpr int64_t kFewRows = 64;  // tokens of the kernels that stream the weights at most
 
 // The workspace: slots in order, tiles, the rows between the projections and the
 // weighted outputs. Rows are padded to whole 16 bytes.
@@ -221,40 +224,7 @@ bool sizes_built(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
 }
 
 template <int DT>
-int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
-  const int slots = static_cast<int>(x.tokens * x.top_k);
-  int32_t* order = reinterpret_cast<int32_t*>(ws + l.order);
-  int4* tiles = reinterpret_cast<int4*>(ws + l.tiles);
-  uint16_t* h = reinterpret_cast<uint16_t*>(ws + l.h);
-  float* y = reinterpret_cast<float*>(ws + l.y);
-  const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, kTileRows,
-                      static_cast<int32_t>(l.num_tiles)};
-  hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
-  int st = launch_status();
-  if (st != SGL_OK) return st;
-
-  gemm::Args a{};
-  a.tiles = tiles, a.order = order, a.top_k = x.top_k, a.scale = x.weights;
-  a.x = static_cast<const uint16_t*>(x.x), a.x_st = x.x_stride_row;
-  a.w = static_cast<const uint16_t*>(x.gate_up);
-  a.w_st = x.gate_up_stride_row, a.w_se = x.gate_up_stride_expert;
-  a.out = h, a.o_st = l.h_st, a.wide = 1;
-  a.tokens = slots, a.n = x.intermediate, a.k = x.hidden, a.act = x.activation;
-  bool vec = x.hidden % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
-             aligned(x.gate_up, x.gate_up_stride_row, 16, 2) && x.gate_up_stride_expert % 8 == 0;
-  st = gemm::launch_any<DT, gemm::kGateUp, true>(a, vec, l.num_tiles, s);
-  if (st != SGL_OK) return st;
-
-  a.x = h, a.x_st = l.h_st;
-  a.w = static_cast<const uint16_t*>(x.down);
-  a.w_st = x.down_stride_row, a.w_se = x.down_stride_expert;
-  a.out = y, a.o_st = l.y_st, a.out_f32 = 1;
-  a.n = x.hidden, a.k = x.intermediate;
-  vec = x.intermediate % 8 == 0 && aligned(x.down, x.down_stride_row, 16, 2) &&
-        x.down_stride_expert % 8 == 0;
-  st = gemm::launch_any<DT, gemm::kDown, false>(a, vec, l.num_tiles, s);
-  if (st != SGL_OK) return st;
-
+int combine(const sgl_moe_t& x, const Layout& l, const float* y, hipStream_t s) {
   CombineArgs c{};
   c.y = y, c.y_st = l.y_st, c.experts = x.experts;
   c.res = static_cast<const uint16_t*>(x.residual), c.r_st = x.residual_stride_row;
@@ -263,6 +233,75 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   c.wide = aligned(x.out, x.out_stride_row, 8, 2) && aligned(x.residual, x.residual_stride_row, 8, 2);
   hipLaunchKernelGGL((combine_kernel<DT>), dim3(static_cast<uint32_t>(x.tokens)), dim3(256), 0, s, c);
   return launch_status();
+}
+
+// Few slots: the workgroups find their expert's slots themselves, rows of h and y are slots.
+template <int DT>
+int run_few(const sgl_moe_t& x, const Layout& l, gemm::Args up, gemm::Args down, hipStream_t s) {
+  const int slots = static_cast<int>(x.tokens * x.top_k), tokens = static_cast<int>(x.tokens);
+  gemm::StreamArgs st{};
+  st.experts = x.experts, st.slots = slots, st.num_experts = x.num_experts;
+  st.by_slot = slots < x.num_experts;
+  const int rows = st.by_slot ? slots : x.num_experts;
+  // Columns an expert is expected to need: three times its share of the slots; more take
+  // another pass over its weights.
+  const int share = 3 * slots / x.num_experts;
+  const int columns = std::min(tokens, std::max(share, 16));
+  st.g = up;
+  int status = gemm::launch_stream<DT, gemm::kGateUp, true>(st, columns, rows, s);
+  if (status != SGL_OK) return status;
+  st.g = down;
+  if (tokens <= gemm::kFewTokens && slots <= gemm::kFewSlots) {
+    st.g.out = x.out, st.g.o_st = x.out_stride_row, st.g.out_f32 = 0;
+    st.g.tokens = tokens;
+    st.g.wide = aligned(x.out, x.out_stride_row, 8, 2) && aligned(x.residual, x.residual_stride_row, 8, 2);
+    constexpr int kTiles = 2, kOut = 4 * kTiles;
+    hipLaunchKernelGGL((gemm::down_few_kernel<DT, kTiles, 8>), dim3((x.hidden + kOut - 1) / kOut), dim3(512),
+                       0, s, st, static_cast<const uint16_t*>(x.residual), x.residual_stride_row);
+    return launch_status();
+  }
+  status = gemm::launch_stream<DT, gemm::kDown, false>(st, columns, rows, s);
+  if (status != SGL_OK) return status;
+  return combine<DT>(x, l, static_cast<const float*>(down.out), s);
+}
+
+template <int DT>
+int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
+  const int slots = static_cast<int>(x.tokens * x.top_k);
+  int32_t* order = reinterpret_cast<int32_t*>(ws + l.order);
+  int4* tiles = reinterpret_cast<int4*>(ws + l.tiles);
+  uint16_t* h = reinterpret_cast<uint16_t*>(ws + l.h);
+  float* y = reinterpret_cast<float*>(ws + l.y);
+  gemm::Args up{};
+  up.tiles = tiles, up.order = order, up.top_k = x.top_k, up.scale = x.weights;
+  gemm::Args down = up;
+  up.x = static_cast<const uint16_t*>(x.x), up.x_st = x.x_stride_row;
+  up.w = static_cast<const uint16_t*>(x.gate_up);
+  up.w_st = x.gate_up_stride_row, up.w_se = x.gate_up_stride_expert;
+  up.out = h, up.o_st = l.h_st, up.wide = 1;
+  up.tokens = slots, up.n = x.intermediate, up.k = x.hidden, up.act = x.activation;
+  const bool up_vec = x.hidden % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
+                      aligned(x.gate_up, x.gate_up_stride_row, 16, 2) && x.gate_up_stride_expert % 8 == 0;
+  down.x = h, down.x_st = l.h_st;
+  down.w = static_cast<const uint16_t*>(x.down);
+  down.w_st = x.down_stride_row, down.w_se = x.down_stride_expert;
+  down.out = y, down.o_st = l.y_st, down.out_f32 = 1, down.wide = 1;
+  down.tokens = slots, down.n = x.hidden, down.k = x.intermediate;
+  const bool down_vec = x.intermediate % 8 == 0 && aligned(x.down, x.down_stride_row, 16, 2) &&
+                        x.down_stride_expert % 8 == 0;
+  if (up_vec && down_vec && slots <= gemm::kMostSlots && x.tokens <= kFewRows)
+    return run_few<DT>(x, l, up, down, s);
+
+  const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, kTileRows,
+                      static_cast<int32_t>(l.num_tiles)};
+  hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
+  int st = launch_status();
+  if (st != SGL_OK) return st;
+  st = gemm::launch_any<DT, gemm::kGateUp, true>(up, up_vec, l.num_tiles, s);
+  if (st != SGL_OK) return st;
+  st = gemm::launch_any<DT, gemm::kDown, false>(down, down_vec, l.num_tiles, s);
+  if (st != SGL_OK) return st;
+  return combine<DT>(x, l, y, s);
 }
 
 }  // namespace
