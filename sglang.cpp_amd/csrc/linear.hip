@@ -10,7 +10,7 @@ constexpr int kStreamTokens = 64;
 
 template <int DT>
 int run(const gemm::Args& a, bool vec, hipStream_t s) {
-  if (vec && a.tokens <= kStreamTokens) {
+  if (vec && a.tokens <= kStreamTokens && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride) {
     gemm::StreamArgs st{};
     st.g = a;
     return gated(a.act) ? gemm::launch_stream<DT, gemm::kLinear, true>(st, a.tokens, 1, s)

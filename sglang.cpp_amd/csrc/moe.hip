@@ -289,7 +289,8 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   down.tokens = slots, down.n = x.hidden, down.k = x.intermediate;
   const bool down_vec = x.intermediate % 8 == 0 && aligned(x.down, x.down_stride_row, 16, 2) &&
                         x.down_stride_expert % 8 == 0;
-  if (up_vec && down_vec && slots <= gemm::kMostSlots && x.tokens <= kFewRows)
+  if (up_vec && down_vec && slots <= gemm::kMostSlots && x.tokens <= kFewRows &&
+      std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride)
     return run_few<DT>(x, l, up, down, s);
 
   const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, kTileRows,
