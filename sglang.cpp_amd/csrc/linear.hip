@@ -6,11 +6,9 @@ namespace {
 
 bool gated(int act) { return act == SGL_ACT_SILU_AND_MUL || act == SGL_ACT_GELU_AND_MUL; }
 
-constexpr int kStreamTokens = 64;
-
 template <int DT>
 int run(const gemm::Args& a, bool vec, hipStream_t s) {
-  if (vec && a.tokens <= kStreamTokens && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride) {
+  if (vec && a.tokens <= (gated(a.act) ? gemm::stream_tokens<true>() : gemm::stream_tokens<false>()) && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride) {
     gemm::StreamArgs st{};
     st.g = a;
     return gated(a.act) ? gemm::launch_stream<DT, gemm::kLinear, true>(st, a.tokens, 1, s)

@@ -1,14 +1,20 @@
 // Few tokens: every weight is read once, straight into the registers of the matrix
 // instruction that takes it, and everything else is kept out of its way.
 //
-// A workgroup has MT tiles of weight rows, its waves share out the inputs (k) in steps and
-// fold their sums through LDS at the end. One instruction multiplies 16 rows by 16
-// columns over 32 inputs. Where there are at most 16 / P tokens (P = 2, 4), rows and
-// columns stand for 16 / P rows and tokens times P parts of 32 P inputs instead: row and
-// column blocks of the same part meet on the diagonal, whose P blocks are summed, and
-// what is off it is dropped. A load then covers 64 P contiguous bytes of a row instead of
-// 64 and a tile fewer rows, so that short launches spread over more workgroups; the
-// wasted products cost nothing where the weights' bytes are what bounds the kernel.
+// A workgroup has MT tiles of weight rows, its waves share out the inputs (k) in units of
+// 128 or 256 bytes of a row and fold their sums through LDS at the end. One instruction
+// multiplies 16 rows by 16 columns over 32 inputs.
+//
+// Up to 4 or 8 tokens (P = 4, 2): rows and columns stand for 16 / P rows and tokens times P
+// parts of the inputs; row and column blocks of the same part meet on the diagonal, whose P
+// blocks are summed, and what is off it is dropped. Neighbouring lanes then hold
+// neighbouring inputs of a row, so operands are loaded straight into registers, and a tile
+// has fewer rows, so that short launches spread over more workgroups. The wasted products
+// cost nothing where the weights' bytes are what bounds the kernel.
+//
+// More tokens (P = 1): neighbouring lanes hold different rows, which makes every lane's 16
+// bytes an access of its own; each wave brings whole 128-byte pieces of rows into a ring of
+// its own in LDS (no registers, no barriers) and reads the operands from there.
 #pragma once
 
 #include "gemm.h"
@@ -91,15 +97,39 @@ __device__ __forceinline__ Rows weight_rows(const Args& a, int expert, int n0, i
                  static_cast<uint32_t>(min(r, a.n - 1 - n)) * static_cast<uint32_t>(a.w_st) + koff);
 }
 
-// acc[i][j] += the products of the units first, first + stride ..: a unit is 32 P inputs, but
-// 64 at least (128 bytes of a row, a whole cache line). Loads go round a ring of kRing
-// instructions' operands, so that what is in flight never runs dry between batches.
+// First input of a lane's 16 bytes in a unit of 32 P.
+template <int P>
+__device__ __forceinline__ int lane_input(int lane) {
+  return ((lane >> 4) * P + (lane & 15) % P) * 8;
+}
+
+// The inputs from `at` on, fewer than a unit; what is behind the last one is zero.
+template <int DT, int P, int MT, int NT>
+__device__ __forceinline__ void stream_tail(const Rows (&w)[MT], const Rows (&x)[NT], int k, int at,
+                                            f32x4_t (&acc)[MT][NT]) {
+  for (; at < k; at += 32 * P) {
+    const bool in = at + lane_input<P>(threadIdx.x & 63) < k;
+    u32x4_t fw[MT], fx[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) fw[i] = stream_load<true>(w[i], at, in);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) fx[j] = stream_load<false>(x[j], at, in);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<DT>(fw[i], fx[j], acc[i][j]);
+  }
+}
+
+// acc[i][j] += the products of the units first, first + stride .. of 32 P inputs. Loads go
+// round a ring of kRing instructions' operands, so that what is in flight never runs dry
+// between batches. turn: the first unit of a workgroup.
 template <int DT, int P, int MT, int NT>
 __device__ __forceinline__ void stream_units(const Rows (&w)[MT], const Rows (&x)[NT], int k,
                                              int first, int stride, int turn,
                                              f32x4_t (&acc)[MT][NT]) {
-  constexpr int kStep = 32 * P, kSub = P == 1 ? 2 : 1, kUnit = kStep * kSub;
-  constexpr int kRing = (20 / (MT + NT)) / kSub < 1 ? kSub : (20 / (MT + NT)) / kSub * kSub;
+  constexpr int kUnit = 32 * P;
+  constexpr int kRing = 20 / (MT + NT);
   const int whole = k / kUnit;  // units without a tail
   u32x4_t fw[kRing][MT], fx[kRing][NT];
   auto load = [&](int d, int at) {
@@ -115,11 +145,10 @@ __device__ __forceinline__ void stream_units(const Rows (&w)[MT], const Rows (&x
       for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<DT>(fw[d][i], fx[d][j], acc[i][j]);
   };
   turn = whole > 0 ? turn % whole : 0;
-  const int n = first < whole ? ((whole - first - 1) / stride + 1) * kSub : 0;  // its steps
+  const int n = first < whole ? (whole - first - 1) / stride + 1 : 0;  // its units
   auto place = [&](int q) {
-    int u = first + q / kSub * stride + turn;
-    u = u < whole ? u : u - whole;
-    return u * kUnit + (q % kSub) * kStep;
+    const int u = first + q * stride + turn;
+    return (u < whole ? u : u - whole) * kUnit;
   };
 #pragma unroll
   for (int d = 0; d < kRing; ++d)
@@ -142,42 +171,133 @@ __device__ __forceinline__ void stream_units(const Rows (&w)[MT], const Rows (&x
       if (q + d + kRing < n) load(d, place(q + kRing + d));
     }
   }
-  if (whole * kUnit < k && whole % stride == first) {  // the last unit is a part of one
-    const int m = threadIdx.x & 15, koff = ((m / (16 / P)) * 4 + ((threadIdx.x & 63) >> 4)) * 8;
+  if (whole * kUnit < k && whole % stride == first)  // the last unit is a part of one
+    stream_tail<DT, P, MT, NT>(w, x, k, whole * kUnit, acc);
+}
+
+// P = 1: tiles of 16 rows x 64 inputs in LDS, row r's 16-byte piece c at place c ^ ((r >> 1) &
+// 7) of its 128 bytes, so that the 16 rows' reads of one piece are spread over all banks.
+constexpr int kPiece = 64;           // inputs of a unit
+constexpr int kTileBytes = 2048;     // 16 rows of one
+
+// Lane offsets of a tile's two loads of 8 rows: lane i has row 8 h + i / 8 and the piece that
+// belongs at place i % 8.
+struct Staged {
+  __amdgpu_buffer_rsrc_t base;
+  uint32_t lane[2];
+};
+__device__ __forceinline__ int staged_input(int lane, int h) {
+  return ((lane & 7) ^ ((4 * h + (lane >> 4)) & 7)) * 8;
+}
+
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "i"(N) : "memory");
+}
+
+template <int OFF>
+__device__ __forceinline__ u32x4_t lds_read(uint32_t addr) {
+  u32x4_t v;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFF));
+  return v;
+}
+
+// The operands have arrived (the reads are in order: the first wait is the only one).
+__device__ __forceinline__ void lds_wait(u32x4_t& a, u32x4_t& b) {
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a), "+v"(b) : : "memory");
+}
+
+// Waits until at most `left` units of kEach loads are in flight, left < kMost.
+template <int kMost, int kEach>
+__device__ __forceinline__ void units_wait(int left) {
+  static_for<0, kMost>([&](auto i) {
+    if (left == i.value) vm_wait<i.value * kEach>();
+  });
+}
+
+template <int DT, int MT, int NT, int D>
+__device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* ring, int k, int first,
+                                             int stride, int turn, f32x4_t (&acc)[MT][NT]) {
+  constexpr int kTiles = MT + NT, kSlot = kTiles * kTileBytes;
+  const int whole = k / kPiece;
+  turn = whole > 0 ? turn % whole : 0;
+  const int n = first < whole ? (whole - first - 1) / stride + 1 : 0;
+  const int lane = threadIdx.x & 63;
+  auto fetch = [&](int q, int slot) {
+    const int u = first + q * stride + turn;
+    const int at = (u < whole ? u : u - whole) * kPiece * 2;
+    static_for<0, kTiles>([&](auto i) {
 #pragma unroll
-    for (int d = 0; d < kSub; ++d) {
-      const int at = whole * kUnit + d * kStep;
-      if (at >= k) break;
-      const bool in = at + koff < k;
+      for (int h = 0; h < 2; ++h)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            t[i.value].base,
+            (__attribute__((address_space(3))) void*)(ring + slot * kSlot + i.value * kTileBytes + h * 1024),
+            16, t[i.value].lane[h], at, 0, i.value < MT ? 2 : 0);
+    });
+  };
+  // Place of this lane's operand: row l % 16, piece l / 16 (and 4 further for the second half).
+  const int r = lane & 15;
+  const uint32_t at0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+                           (__attribute__((address_space(3))) char*)ring)) +
+                       r * 128 + (((lane >> 4) ^ (r >> 1)) & 7) * 16;
+  for (int d = 0; d < D; ++d)
+    if (d < n) fetch(d, d);
+  int slot = 0;
+  for (int q = 0; q < n; ++q) {
+    units_wait<D, 2 * kTiles>(min(n - 1 - q, D - 1));
+    u32x4_t f[2][kTiles];
+    const uint32_t at = at0 + slot * kSlot, at1 = at ^ 64;
+    static_for<0, kTiles>([&](auto i) {
+      f[0][i.value] = lds_read<i.value * kTileBytes>(at);
+      f[1][i.value] = lds_read<i.value * kTileBytes>(at1);
+    });
+    static_for<0, kTiles>([&](auto i) { lds_wait(f[0][i.value], f[1][i.value]); });
+    if (q + D < n) fetch(q + D, slot);
+    slot = slot + 1 == D ? 0 : slot + 1;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) fw[0][i] = stream_load<true>(w[i], at, in);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fx[0][j] = stream_load<false>(x[j], at, in);
-      multiply(0);
-    }
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<DT>(f[h][i], f[h][MT + j], acc[i][j]);
   }
 }
 
-// The waves' sums, each wave's own in LDS: the sum of unit (tile i, column tile j, quad q
-// of rows, column c) over waves and parts.
+// Units of a ring: 16 to 20 KB a wave, 8 waves a CU.
+constexpr int stream_depth(int mt, int nt) { return mt + nt <= 2 ? 4 : mt + nt <= 3 ? 3 : 2; }
+
+// The waves' sums, each wave's own in LDS: outputs 4 q .. + 3 of (tile i, column tile j),
+// column c, over waves and parts. Row r and column c of part p are the instruction's row
+// r P + p and column c P + p.
 template <int P, int MT, int NT, int NW>
 __device__ __forceinline__ f32x4_t folded(const f32x4_t* red, int i, int j, int q, int c) {
-  constexpr int R = 16 / P;
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int w = 0; w < NW; ++w)
+  for (int w = 0; w < NW; ++w) {
+    const f32x4_t* of = red + ((w * MT + i) * NT + j) * 64;
+    if constexpr (P == 1) {
+      sum += of[q * 16 + c];
+    } else {
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-      sum += red[((w * MT + i) * NT + j) * 64 + (p * (R / 4) + q) * 16 + p * R + c];
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const int row = (4 * q + r) * P + p;
+          sum[r] += reinterpret_cast<const float*>(&of[row / 4 * 16 + c * P + p])[row % 4];
+        }
+    }
+  }
   return sum;
 }
 
 template <int DT, int MODE, bool GATED, int P, int MT, int NT, int NW>
-__global__ __launch_bounds__(64 * NW, 4) void stream_kernel(const StreamArgs s) {
+__global__ __launch_bounds__(64 * NW, P == 1 ? 2 : 4) void stream_kernel(const StreamArgs s) {
   static_assert((P == 1 || NT == 1) && (!GATED || MT % 2 == 0), "tiles");
+  constexpr int kDepth = stream_depth(MT, NT);
   constexpr int R = 16 / P;                        // rows of a tile, columns of a column tile
   constexpr int kOut = (GATED ? MT / 2 : MT) * R;  // outputs of a workgroup
-  __shared__ f32x4_t red[NW * MT * NT * 64];
+  // The rings of P = 1 and, behind the last unit, the waves' sums.
+  __shared__ f32x4_t red[NW * (P == 1 ? kDepth * (MT + NT) * kTileBytes / 16 : MT * NT * 64)];
   __shared__ int32_t list[MODE == kLinear ? 1 : kMostSlots];
   const Args& a = s.g;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -188,24 +308,49 @@ __global__ __launch_bounds__(64 * NW, 4) void stream_kernel(const StreamArgs s) 
     count = find_slots(s, list, expert);
     if (count == 0) return;
   }
-  const int m = lane & 15, koff = ((m / R) * 4 + (lane >> 4)) * 8;
+  // Row of x of column c; columns past the last are computed from it and dropped.
+  auto source = [&](int c) -> uint32_t {
+    c = min(c, count - 1);
+    return MODE == kGateUp ? list[c] / a.top_k : MODE == kDown ? list[c] : c;
+  };
+  const uint32_t x_st = static_cast<uint32_t>(a.x_st);
+  const int turn = 5 * blockIdx.x + 11 * expert;
+  const int m = lane & 15, in = lane_input<P>(lane);
   Rows w[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) w[i] = weight_rows<GATED, R>(a, expert, n0, i, m % R, koff);
+  for (int i = 0; i < MT; ++i) w[i] = weight_rows<GATED, R>(a, expert, n0, i, m / P, in);
   for (int first = 0; first < count; first += R * NT) {
     Rows x[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      // Columns past the last are computed from it and dropped.
-      const int c = min(first + j * 16 + m % R, count - 1);
-      uint32_t row = c;
-      if constexpr (MODE == kGateUp) row = list[c] / a.top_k;
-      if constexpr (MODE == kDown) row = list[c];
-      x[j] = rows_at(a.x, row * static_cast<uint32_t>(a.x_st) + koff);
-    }
+    for (int j = 0; j < NT; ++j) x[j] = rows_at(a.x, source(first + j * 16 + m / P) * x_st + in);
     f32x4_t acc[MT][NT] = {};
-    stream_units<DT, P, MT, NT>(w, x, a.k, wave, NW, 5 * blockIdx.x + 11 * expert, acc);
-    if (MODE != kLinear && first > 0) __syncthreads();
+    if constexpr (P == 1) {
+      Staged t[MT + NT];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 8 * h + (lane >> 3), at = staged_input(lane, h);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const Rows row = weight_rows<GATED, R>(a, expert, n0, i, r, at);
+          t[i].base = row.base, t[i].lane[h] = row.lane;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          t[MT + j].base = x[j].base;
+          t[MT + j].lane[h] = 2u * (source(first + j * 16 + r) * x_st + at);
+        }
+      }
+      if (MODE != kLinear && first > 0) __syncthreads();  // the sums in the rings were read
+      char* ring = reinterpret_cast<char*>(red) + wave * (kDepth * (MT + NT) * kTileBytes);
+      staged_units<DT, MT, NT, kDepth>(t, ring, a.k, wave, NW, turn, acc);
+      const int whole = a.k / kPiece;
+      if (whole * kPiece < a.k && whole % NW == wave)
+        stream_tail<DT, P, MT, NT>(w, x, a.k, whole * kPiece, acc);
+      __syncthreads();  // every wave is done with its ring
+    } else {
+      stream_units<DT, P, MT, NT>(w, x, a.k, wave, NW, turn, acc);
+      if (MODE != kLinear && first > 0) __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -272,7 +417,7 @@ __global__ __launch_bounds__(64 * NW) void down_few_kernel(const StreamArgs s, c
   }
   __syncthreads();
   const int experts = num;
-  const int m = lane & 15, c = m % R, koff = ((m / R) * 4 + (lane >> 4)) * 8;
+  const int c = (lane & 15) / P, in = lane_input<P>(lane);
   // Fewer experts than waves: each is shared by as many waves as there are for it.
   const int parts = experts > 0 ? max(1, NW / experts) : 1;
   f32x4_t total[MT] = {};
@@ -285,7 +430,7 @@ __global__ __launch_bounds__(64 * NW) void down_few_kernel(const StreamArgs s, c
     float weight = 0.f;
     Rows w[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) w[i] = weight_rows<false, R>(a, e, n0, i, c, koff);
+    for (int i = 0; i < MT; ++i) w[i] = weight_rows<false, R>(a, e, n0, i, c, in);
     if (c < s.g.tokens)
       for (int j = 0; j < a.top_k; ++j)
         if (chosen[c * a.top_k + j] == e) {
@@ -294,7 +439,7 @@ __global__ __launch_bounds__(64 * NW) void down_few_kernel(const StreamArgs s, c
           mine = true;
           weight += weight_of[c * a.top_k + j];
         }
-    const Rows x[1] = {rows_at(a.x, static_cast<uint32_t>(slot) * static_cast<uint32_t>(a.x_st) + koff)};
+    const Rows x[1] = {rows_at(a.x, static_cast<uint32_t>(slot) * static_cast<uint32_t>(a.x_st) + in)};
     f32x4_t acc[MT][1] = {};
     stream_units<DT, P, MT, NT>(w, x, a.k, unit % parts, parts, 5 * blockIdx.x + 11 * e, acc);
     // A token that did not choose e has another token's products: dropped, not weighted.
@@ -323,29 +468,36 @@ void launch_stream_as(const StreamArgs& s, int rows, hipStream_t st) {
   hipLaunchKernelGGL((stream_kernel<DT, MODE, GATED, P, MT, NT, NW>), grid, dim3(64 * NW), 0, st, s);
 }
 
-// MT tiles a workgroup where that leaves a workgroup for every CU, a half otherwise; as many
-// waves as fill the CUs with 16 each.
+// Half of the tiles a workgroup where MT would leave CUs without one; as many waves as fill
+// the CUs.
 template <int DT, int MODE, bool GATED, int P, int MT, int NT>
 void launch_stream_at(const StreamArgs& s, int rows, hipStream_t st) {
   constexpr int kOut = (GATED ? MT / 2 : MT) * 16 / P;
-  constexpr int kLess = GATED && MT == 2 ? 2 : MT > 1 ? MT / 2 : 1;
+  constexpr int kLess = (GATED ? MT > 2 : MT > 1) ? MT / 2 : MT;
   const int64_t groups = static_cast<int64_t>((s.g.n + kOut - 1) / kOut) * rows;
-  if (groups >= 1024) launch_stream_as<DT, MODE, GATED, P, MT, NT, 4>(s, rows, st);
+  if (groups >= (P == 1 ? 512 : 1024)) launch_stream_as<DT, MODE, GATED, P, MT, NT, 4>(s, rows, st);
   else if (groups >= 256) launch_stream_as<DT, MODE, GATED, P, MT, NT, 8>(s, rows, st);
   else launch_stream_as<DT, MODE, GATED, P, kLess, NT, 8>(s, rows, st);
 }
+
+// Tokens of a call that these kernels take at most: the rings of a workgroup's waves fill
+// the LDS.
+template <bool GATED>
+constexpr int stream_tokens() { return GATED ? 48 : 64; }
 
 // columns: tokens of the call, or the most places an expert is expected to have. rows:
 // the grid's second extent.
 template <int DT, int MODE, bool GATED>
 int launch_stream(const StreamArgs& s, int columns, int rows, hipStream_t st) {
-  constexpr int kWide = GATED ? 2 : 1;
   if (columns <= 4) launch_stream_at<DT, MODE, GATED, 4, 4, 1>(s, rows, st);
   else if (columns <= 8) launch_stream_at<DT, MODE, GATED, 2, 4, 1>(s, rows, st);
-  else if (columns <= 16) launch_stream_at<DT, MODE, GATED, 1, 4, 1>(s, rows, st);
-  else if (columns <= 32) launch_stream_at<DT, MODE, GATED, 1, 2, 2>(s, rows, st);
-  else if (columns <= 48) launch_stream_at<DT, MODE, GATED, 1, 2, 3>(s, rows, st);
-  else launch_stream_at<DT, MODE, GATED, 1, 2, 4>(s, rows, st);
+  else if (columns <= 16) launch_stream_at<DT, MODE, GATED, 1, 2, 1>(s, rows, st);
+  else if (columns <= 32 || MODE != kLinear) launch_stream_at<DT, MODE, GATED, 1, 2, 2>(s, rows, st);
+  else if constexpr (MODE == kLinear) {
+    constexpr int kTiles = GATED ? 2 : 1;
+    if (columns <= 48) launch_stream_as<DT, MODE, GATED, 1, kTiles, 3, 8>(s, rows, st);
+    else if constexpr (!GATED) launch_stream_as<DT, MODE, GATED, 1, 1, 4, 8>(s, rows, st);
+  }
   return launch_status();
 }
 
