@@ -1,10 +1,19 @@
 // sgl_linear: a projection with its epilogue.
-#include "stream.h"
+#include "tile.h"
 
 namespace sgl {
 namespace {
 
 bool gated(int act) { return act == SGL_ACT_SILU_AND_MUL || act == SGL_ACT_GELU_AND_MUL; }
+
+// Tiles of 256 x 256 where they fill the CUs, of 128 x 128 otherwise.
+template <int DT, bool GATED>
+int run_tiles(const gemm::Args& a, hipStream_t s) {
+  const int64_t t = a.tokens, rows = static_cast<int64_t>(a.n) * (GATED ? 2 : 1);
+  if ((t + 255) / 256 * ((rows + 255) / 256) >= 256)
+    return gemm::launch_tile<DT, gemm::kLinear, GATED, 2, 4, 4, 2>(a, (t + 255) / 256, s);
+  return gemm::launch_tile<DT, gemm::kLinear, GATED, 2, 2, 2, 2>(a, (t + 127) / 128, s);
+}
 
 template <int DT>
 int run(const gemm::Args& a, bool vec, hipStream_t s) {
@@ -14,6 +23,8 @@ int run(const gemm::Args& a, bool vec, hipStream_t s) {
     return gated(a.act) ? gemm::launch_stream<DT, gemm::kLinear, true>(st, a.tokens, 1, s)
                         : gemm::launch_stream<DT, gemm::kLinear, false>(st, a.tokens, 1, s);
   }
+  if (vec && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride)
+    return gated(a.act) ? run_tiles<DT, true>(a, s) : run_tiles<DT, false>(a, s);
   const int64_t tiles_t = (static_cast<int64_t>(a.tokens) + gemm::kAnyTile - 1) / gemm::kAnyTile;
   return gated(a.act) ? gemm::launch_any<DT, gemm::kLinear, true>(a, vec, tiles_t, s)
                       : gemm::launch_any<DT, gemm::kLinear, false>(a, vec, tiles_t, s);

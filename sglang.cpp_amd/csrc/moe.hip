@@ -1,6 +1,6 @@
 // Mixture of experts: sgl_moe_route (the experts of each token from the router's logits)
 // and sgl_moe_experts (their gate, up and down projections and the weighted sum).
-#include "stream.h"
+#include "tile.h"
 
 #include <algorithm>
 
@@ -293,14 +293,19 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
       std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride)
     return run_few<DT>(x, l, up, down, s);
 
-  const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, kTileRows,
-                      static_cast<int32_t>(l.num_tiles)};
+  const bool fast = up_vec && down_vec && x.tokens * up.x_st < (1ll << 30) &&
+                    std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride;
+  const int rows = fast ? 128 : gemm::kAnyTile;
+  const int num_tiles = slots / rows + x.num_experts;
+  const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, rows, num_tiles};
   hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
   int st = launch_status();
   if (st != SGL_OK) return st;
-  st = gemm::launch_any<DT, gemm::kGateUp, true>(up, up_vec, l.num_tiles, s);
+  st = fast ? gemm::launch_tile<DT, gemm::kGateUp, true, 2, 2, 2, 2>(up, num_tiles, s)
+            : gemm::launch_any<DT, gemm::kGateUp, true>(up, up_vec, num_tiles, s);
   if (st != SGL_OK) return st;
-  st = gemm::launch_any<DT, gemm::kDown, false>(down, down_vec, l.num_tiles, s);
+  st = fast ? gemm::launch_tile<DT, gemm::kDown, false, 2, 2, 2, 2>(down, num_tiles, s)
+            : gemm::launch_any<DT, gemm::kDown, false>(down, down_vec, num_tiles, s);
   if (st != SGL_OK) return st;
   return combine<DT>(x, l, y, s);
 }

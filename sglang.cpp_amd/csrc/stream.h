@@ -190,6 +190,17 @@ __device__ __forceinline__ int staged_input(int lane, int h) {
   return ((lane & 7) ^ ((4 * h + (lane >> 4)) & 7)) * 8;
 }
 
+// 16 bytes a lane into LDS, lane i's at `place` + 16 i; NT: read once. (Only the device pass
+// knows loads of 16 bytes.)
+template <bool NT>
+__device__ __forceinline__ void stage16(const __amdgpu_buffer_rsrc_t& base, char* place, uint32_t lane,
+                                        int at) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (__attribute__((address_space(3))) void*)place, 16, lane,
+                                           at, 0, NT ? 2 : 0);
+#endif
+}
+
 template <int N>
 __device__ __forceinline__ void vm_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "i"(N) : "memory");
@@ -229,10 +240,8 @@ __device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* r
     static_for<0, kTiles>([&](auto i) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            t[i.value].base,
-            (__attribute__((address_space(3))) void*)(ring + slot * kSlot + i.value * kTileBytes + h * 1024),
-            16, t[i.value].lane[h], at, 0, i.value < MT ? 2 : 0);
+        stage16<(i.value < MT)>(t[i.value].base, ring + slot * kSlot + i.value * kTileBytes + h * 1024,
+                                t[i.value].lane[h], at);
     });
   };
   // Place of this lane's operand: row l % 16, piece l / 16 (and 4 further for the second half).
