@@ -35,68 +35,95 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// One wave a token: expert lane + 64 i in register i. Each round takes the largest
-// (rank, lowest expert) of the wave.
+// The logit of a rank.
+__device__ __forceinline__ float logit_of(uint32_t rank) {
+  if (rank == 1) return __builtin_nanf("");
+  return __uint_as_float(rank & 0x80000000u ? rank & 0x7fffffffu : ~rank);
+}
+
+// Largest and smallest of a row of 16 lanes, in all of them.
+__device__ __forceinline__ uint32_t max16(uint32_t x) {
+  x = max(x, dpp_u32<0xB1>(x));
+  x = max(x, dpp_u32<0x4E>(x));
+  x = max(x, dpp_u32<0x141>(x));
+  return max(x, dpp_u32<0x140>(x));
+}
+__device__ __forceinline__ uint32_t min16(uint32_t x) {
+  x = min(x, dpp_u32<0xB1>(x));
+  x = min(x, dpp_u32<0x4E>(x));
+  x = min(x, dpp_u32<0x141>(x));
+  return min(x, dpp_u32<0x140>(x));
+}
+
+// 16 lanes a token (lane exchanges inside 16 lanes are register moves): expert l + 16 i in
+// register i. Each round takes the largest rank and of its experts the lowest; lane j % 16
+// keeps the j-th choice.
 template <int DT, int V>
 __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (t >= a.tokens) return;
-  const int64_t row = t * a.stride;
+  const int l = threadIdx.x & 15;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const bool real = t < a.tokens;
+  const int64_t row = (real ? t : a.tokens - 1) * a.stride;
   float x[V];
-  uint32_t key[V];
-  float top = -INFINITY;
+  uint32_t rank[V];
+  uint32_t top_rank = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int e = lane + 64 * i;
-    x[i] = e < a.num_experts ? load_logit<DT>(a.logits, row + e) : -INFINITY;
-    key[i] = e < a.num_experts ? rank_of(x[i]) : 0;
-    top = fmaxf(top, x[i]);
+    const int e = l + 16 * i;
+    x[i] = e < a.num_experts ? load_logit<DT>(a.logits, row + e) : 0.f;
   }
-  top = group_max<64>(top);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    rank[i] = l + 16 * i < a.num_experts ? rank_of(x[i]) : 0;
+    top_rank = max(top_rank, rank[i]);
+  }
+  const float top = logit_of(max16(top_rank));
   float total = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) total += lane + 64 * i < a.num_experts ? expf(x[i] - top) : 0.f;
-  total = group_sum<64>(total);
-  float mine = 0.f, sum = 0.f;
-  int32_t my_expert = 0;
-  for (int j = 0; j < a.top_k; ++j) {
-    uint64_t best = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const uint64_t c = (static_cast<uint64_t>(key[i]) << 32) | ~static_cast<uint32_t>(lane + 64 * i);
-      if (key[i] && c > best) best = c;
-    }
-    for (int off = 32; off > 0; off >>= 1) {
-      const uint64_t other = __shfl_xor(best, off, kWave);
-      best = other > best ? other : best;
-    }
-    const int e = static_cast<int>(~static_cast<uint32_t>(best));
-    float value = 0.f;
+  for (int i = 0; i < V; ++i) total += l + 16 * i < a.num_experts ? expf(x[i] - top) : 0.f;
+  total = group_sum<16>(total);
+  uint32_t kept[kMostChosen / 16] = {};
+  int32_t expert[kMostChosen / 16] = {};
+  auto round = [&](int j, uint32_t& kept_rank, int32_t& kept_expert) {
+    uint32_t best = 0, at = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (lane + 64 * i == e) {
-        value = expf(x[i] - top);
-        key[i] = 0;
-      }
-    value = __shfl(value, e & 63, kWave);
-    sum += value;
-    if (lane == j) mine = value, my_expert = e;
+      if (rank[i] > best) best = rank[i], at = i;  // of equal ones the first
+    const uint32_t most = max16(best);
+    const uint32_t e = min16(best == most ? l + 16 * at : 0xffffffffu);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (e == static_cast<uint32_t>(l + 16 * i)) rank[i] = 0;
+    if (l == (j & 15)) kept_rank = most, kept_expert = static_cast<int32_t>(e);
+  };
+  for (int j = 0; j < min(a.top_k, 16); ++j) round(j, kept[0], expert[0]);
+  for (int j = 16; j < a.top_k; ++j) round(j, kept[1], expert[1]);
+  float w[kMostChosen / 16], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMostChosen / 16; ++i) {
+    w[i] = l + 16 * i < a.top_k ? expf(logit_of(kept[i]) - top) : 0.f;
+    sum += w[i];
   }
+  sum = group_sum<16>(sum);
   // A row with a NaN, or no finite logit, has a NaN total and NaN weights.
-  if (lane < a.top_k) {
-    a.weights[t * a.top_k + lane] = mine / (a.renormalize ? sum + (total - total) : total);
-    a.experts[t * a.top_k + lane] = my_expert;
+  const float under = a.renormalize ? sum + (total - total) : total;
+#pragma unroll
+  for (int i = 0; i < kMostChosen / 16; ++i) {
+    const int j = l + 16 * i;
+    if (real && j < a.top_k) {
+      a.weights[t * a.top_k + j] = w[i] / under;
+      a.experts[t * a.top_k + j] = expert[i];
+    }
   }
 }
 
 template <int DT>
 void launch_route(const RouteArgs& a, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>((a.tokens + 3) / 4)), block(256);
-  if (a.num_experts <= 64) hipLaunchKernelGGL((route_kernel<DT, 1>), grid, block, 0, s, a);
-  else if (a.num_experts <= 128) hipLaunchKernelGGL((route_kernel<DT, 2>), grid, block, 0, s, a);
-  else if (a.num_experts <= 256) hipLaunchKernelGGL((route_kernel<DT, 4>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((route_kernel<DT, 8>), grid, block, 0, s, a);
+  const dim3 grid(static_cast<uint32_t>((a.tokens + 15) / 16)), block(256);
+  if (a.num_experts <= 64) hipLaunchKernelGGL((route_kernel<DT, 4>), grid, block, 0, s, a);
+  else if (a.num_experts <= 128) hipLaunchKernelGGL((route_kernel<DT, 8>), grid, block, 0, s, a);
+  else if (a.num_experts <= 256) hipLaunchKernelGGL((route_kernel<DT, 16>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((route_kernel<DT, 32>), grid, block, 0, s, a);
 }
 
 // ------------------------------------------------------------------ experts
@@ -108,7 +135,8 @@ struct SortArgs {
   int32_t slots, num_experts, tile_rows, num_tiles;
 };
 
-constexpr int kSortThreads = 256;
+constexpr int kSortThreads = 1024;
+constexpr int kSortAhead = 8;  // choices a lane has in flight
 
 // One workgroup an expert counts the slots of lower experts (its first place) and writes
 // its own slots and tiles. Expert e's tiles start at entry first / tile_rows + e: a later
@@ -118,13 +146,25 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
   const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int kWaves = kSortThreads / kWave;
   // Wave w has the slots [w per, (w + 1) per).
-  const int per = (a.slots + kSortThreads - 1) / kSortThreads * kWave;
+  constexpr int kStep = kWave * kSortAhead;
+  const int per = (a.slots / kSortThreads + 1) * kWave;
   const int begin = min(a.slots, wave * per), end = min(a.slots, begin + per);
+  int32_t x[kSortAhead];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int at = i + kWave * u + lane;
+      x[u] = at < end ? a.experts[at] : -1;
+    }
+  };
   int lower = 0, own = 0;
-  for (int i = begin; i < end; i += kWave) {
-    const int x = i + lane < end ? a.experts[i + lane] : -1;
-    lower += __popcll(__ballot(x >= 0 && x < e));
-    own += __popcll(__ballot(x == e));
+  for (int i = begin; i < end; i += kStep) {
+    load(i);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      lower += __popcll(__ballot(x[u] >= 0 && x[u] < e));
+      own += __popcll(__ballot(x[u] == e));
+    }
   }
   if (lane == 0) lower_of[wave] = lower, own_of[wave] = own;
   __syncthreads();
@@ -136,11 +176,14 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
     count += own_of[w];
   }
   at += first;
-  for (int i = begin; i < end; i += kWave) {
-    const bool hit = i + lane < end && a.experts[i + lane] == e;
-    const uint64_t hits = __ballot(hit);
-    if (hit) a.order[at + __popcll(hits & ((1ull << lane) - 1))] = i + lane;
-    at += __popcll(hits);
+  for (int i = begin; i < end && own > 0; i += kStep) {
+    if (begin + kStep < end) load(i);  // else they are still there
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const uint64_t hits = __ballot(x[u] == e);
+      if (x[u] == e) a.order[at + __popcll(hits & ((1ull << lane) - 1))] = i + kWave * u + lane;
+      at += __popcll(hits);
+    }
   }
   const int t0 = first / a.tile_rows + e;
   const int t1 = e + 1 == a.num_experts ? a.num_tiles : (first + count) / a.tile_rows + e + 1;
@@ -151,7 +194,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
 }
 
 struct CombineArgs {
-  const float* y;  // [slots, stride] weighted outputs of the slots
+  const void* y;  // [slots, stride] weighted outputs of the slots
   const int32_t* experts;
   const uint16_t* res;
   uint16_t* out;
@@ -160,30 +203,58 @@ struct CombineArgs {
 };
 
 // out[t] = the sum of its slots in their order (+ residual); slots of no expert are skipped.
-template <int DT>
+// Eight outputs a thread, eight slots' loads in flight. YT: type of y (16 bits or fp32).
+template <int DT, int YT>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
+  constexpr int kAhead = 8;
   const int64_t t = blockIdx.x;
+  const int h = 8 * (blockIdx.y * 256 + threadIdx.x);
+  if (h >= a.hidden) return;
   const int32_t* ids = a.experts + t * a.top_k;
-  for (int h = 4 * threadIdx.x; h < a.hidden; h += 4 * 256) {
-    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < a.top_k; ++j)
-      if (ids[j] >= 0 && ids[j] < a.num_experts)
-        sum += *reinterpret_cast<const f32x4_t*>(a.y + (t * a.top_k + j) * a.y_st + h);
-    uint16_t* o = a.out + t * a.o_st + h;
-    const uint16_t* r = a.res ? a.res + t * a.r_st + h : nullptr;
-    if (a.wide && h + 4 <= a.hidden) {
-      if (r) {
-        const u32x2_t v = *reinterpret_cast<const u32x2_t*>(r);
+  float sum[8] = {};
+  for (int j0 = 0; j0 < a.top_k; j0 += kAhead) {
+    u32x4_t v[kAhead][YT == SGL_DTYPE_F32 ? 2 : 1];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] += to_f32<DT>((v[i / 2] >> (16 * (i & 1))) & 0xffffu);
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = j0 + u;
+      const u32x4_t zero = {0, 0, 0, 0};
+      const bool in = j < a.top_k && ids[j] >= 0 && ids[j] < a.num_experts;
+      const int64_t at = (t * a.top_k + j) * a.y_st + h;
+      if constexpr (YT == SGL_DTYPE_F32) {
+        v[u][0] = in ? ldg128_nt<true>(static_cast<const float*>(a.y) + at) : zero;
+        v[u][1] = in ? ldg128_nt<true>(static_cast<const float*>(a.y) + at + 4) : zero;
+      } else {
+        v[u][0] = in ? ldg128_nt<true>(static_cast<const uint16_t*>(a.y) + at) : zero;
       }
-      *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack2_t<DT>(sum[0], sum[1]), pack2_t<DT>(sum[2], sum[3])};
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (h + i < a.hidden)
-          o[i] = static_cast<uint16_t>(from_f32<DT>(sum[i] + (r ? to_f32<DT>(r[i]) : 0.f)));
     }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      float f[8];
+      if constexpr (YT == SGL_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[u][i / 4][i % 4]);
+      } else {
+        unpack8_t<YT>(v[u][0], f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += f[i];
+    }
+  }
+  uint16_t* o = a.out + t * a.o_st + h;
+  const uint16_t* r = a.res ? a.res + t * a.r_st + h : nullptr;
+  if (a.wide && h + 8 <= a.hidden) {
+    if (r) {
+      float f[8];
+      unpack8_t<DT>(ldg128(r), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += f[i];
+    }
+    stg128(o, pack8_t<DT>(sum));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (h + i < a.hidden)
+        o[i] = static_cast<uint16_t>(from_f32<DT>(sum[i] + (r ? to_f32<DT>(r[i]) : 0.f)));
   }
 }
 
@@ -206,7 +277,7 @@ Layout layout_of(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) 
   Layout l;
   l.num_tiles = slots / kTileRows + experts;
   l.h_st = up(inter, 8);
-  l.y_st = up(hidden, 4);
+  l.y_st = up(hidden, 8);
   l.order = 0;
   l.tiles = up(slots * 4, 256);
   l.h = l.tiles + up(l.num_tiles * 16, 256);
@@ -223,15 +294,16 @@ bool sizes_built(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
          inter <= 1 << 20;
 }
 
-template <int DT>
-int combine(const sgl_moe_t& x, const Layout& l, const float* y, hipStream_t s) {
+template <int DT, int YT>
+int combine(const sgl_moe_t& x, const Layout& l, const void* y, hipStream_t s) {
   CombineArgs c{};
   c.y = y, c.y_st = l.y_st, c.experts = x.experts;
   c.res = static_cast<const uint16_t*>(x.residual), c.r_st = x.residual_stride_row;
   c.out = static_cast<uint16_t*>(x.out), c.o_st = x.out_stride_row;
   c.hidden = x.hidden, c.top_k = x.top_k, c.num_experts = x.num_experts;
-  c.wide = aligned(x.out, x.out_stride_row, 8, 2) && aligned(x.residual, x.residual_stride_row, 8, 2);
-  hipLaunchKernelGGL((combine_kernel<DT>), dim3(static_cast<uint32_t>(x.tokens)), dim3(256), 0, s, c);
+  c.wide = aligned(x.out, x.out_stride_row, 16, 2) && aligned(x.residual, x.residual_stride_row, 16, 2);
+  const dim3 grid(static_cast<uint32_t>(x.tokens), (x.hidden + 2047) / 2048);
+  hipLaunchKernelGGL((combine_kernel<DT, YT>), grid, dim3(256), 0, s, c);
   return launch_status();
 }
 
@@ -262,7 +334,7 @@ int run_few(const sgl_moe_t& x, const Layout& l, gemm::Args up, gemm::Args down,
   }
   status = gemm::launch_stream<DT, gemm::kDown, false>(st, columns, rows, s);
   if (status != SGL_OK) return status;
-  return combine<DT>(x, l, static_cast<const float*>(down.out), s);
+  return combine<DT, SGL_DTYPE_F32>(x, l, down.out, s);
 }
 
 template <int DT>
@@ -293,6 +365,13 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
       std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride)
     return run_few<DT>(x, l, up, down, s);
 
+  // Many tokens: the slots' weighted outputs are rounded to bf16 before their sum. That is
+  // half of what the sum reads (8,192 tokens x 8 slots x 2,048: 268 MB instead of 537) for
+  // errors of at most half a step of each term, as the rounding of h and of the result. In
+  // fp16 a term could pass 65,504 where the sum does not, so they stay fp32.
+  constexpr bool kRounded = DT == SGL_DTYPE_BF16;
+  if (kRounded) down.out_f32 = 0;
+
   const bool fast = up_vec && down_vec && x.tokens * up.x_st < (1ll << 30) &&
                     std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride;
   const int rows = fast ? 128 : gemm::kAnyTile;
@@ -307,7 +386,7 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   st = fast ? gemm::launch_tile<DT, gemm::kDown, false, 2, 2, 2, 2>(down, num_tiles, s)
             : gemm::launch_any<DT, gemm::kDown, false>(down, down_vec, num_tiles, s);
   if (st != SGL_OK) return st;
-  return combine<DT>(x, l, y, s);
+  return kRounded ? combine<DT, DT>(x, l, y, s) : combine<DT, SGL_DTYPE_F32>(x, l, y, s);
 }
 
 }  // namespace
