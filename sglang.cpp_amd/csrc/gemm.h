@@ -36,6 +36,8 @@ struct Args {
   const int4* tiles;     // experts: {expert, first place, places, 0} of a tile of places
   const int32_t* order;  // experts: slot (token top_k + j) of each place
   const float* scale;    // kDown: weight of each slot
+  float* part;           // sums of the parts of k, where a tile's is split
+  int32_t splits;        // parts
 };
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));

@@ -6,25 +6,71 @@ namespace {
 
 bool gated(int act) { return act == SGL_ACT_SILU_AND_MUL || act == SGL_ACT_GELU_AND_MUL; }
 
-// Tiles of 256 x 256 where they fill the CUs, of 128 x 128 otherwise.
-template <int DT, bool GATED>
-int run_tiles(const gemm::Args& a, hipStream_t s) {
-  const int64_t t = a.tokens, rows = static_cast<int64_t>(a.n) * (GATED ? 2 : 1);
-  if ((t + 255) / 256 * ((rows + 255) / 256) >= 256)
-    return gemm::launch_tile<DT, gemm::kLinear, GATED, 2, 4, 4, 2>(a, (t + 255) / 256, s);
-  return gemm::launch_tile<DT, gemm::kLinear, GATED, 2, 2, 2, 2>(a, (t + 127) / 128, s);
+// The tile kernels' shapes and what a stage of 64 inputs takes them (us, measured): with a
+// workgroup for each CU at most, and with all a CU holds.
+struct Shape {
+  int rows, tokens, per_cu;
+  double alone, full;
+};
+constexpr Shape kShapes[] = {
+    {256, 256, 1, 1.55, 1.55},  // 1,384 TFLOP/s where they fill the CUs (8,192 x 24,576 x 4,096)
+    {128, 128, 2, 0.70, 1.05},  // 1,090 there; 2,048 x 4,096 x 4,096 takes 72 us, the larger ones 100
+    {64, 128, 2, 0.40, 0.55},   // 512 x 4,096 x 4,096: 28 us, the others 48 and 92
+};
+constexpr int kCus = 256;
+constexpr int kMostSplits = 8;
+
+struct Plan {
+  int shape, splits;
+  int64_t bytes;  // of the parts' sums
+};
+
+// The shape and the number of parts of k with the least estimated time: rounds of
+// workgroups x stages, and for parts their sums written and read at 5 TB/s and another
+// launch (333 x 4,096 x 12,288: 128 x 128 tiles in five parts 59 us, in one 163; 100 x 4,096
+// x 4,096: 64 x 128 in four 15.6, in one 26).
+Plan plan_of(int64_t tokens, int64_t n, int64_t k, int act, bool may_split) {
+  const int64_t rows = n * (gated(act) ? 2 : 1), stages = (k + 63) / 64;
+  Plan best{0, 1, 0};
+  double least = 1e300;
+  for (int i = 0; i < 3; ++i) {
+    const Shape& x = kShapes[i];
+    const int64_t tiles = ((rows + x.rows - 1) / x.rows) * ((tokens + x.tokens - 1) / x.tokens);
+    for (int s = 1; s <= kMostSplits && (s == 1 || (may_split && tiles <= 2 * kCus && stages >= 4 * s)); ++s) {
+      const int64_t groups = tiles * s, each = (stages + s - 1) / s;
+      const int64_t bytes = s > 1 ? groups * x.rows * x.tokens * 4 : 0;
+      const int64_t rounds = (groups + kCus * x.per_cu - 1) / (kCus * x.per_cu);
+      const double us = (groups <= kCus ? x.alone : x.full) * static_cast<double>(rounds * each) +
+                        (s > 1 ? 2.5 + 2.0 * static_cast<double>(bytes) / 5e6 : 0.0);
+      if (us < least) least = us, best = Plan{i, s, bytes};
+    }
+  }
+  return best;
 }
 
+template <int DT, bool GATED>
+int run_tiles(gemm::Args a, void* workspace, hipStream_t s) {
+  const Plan p = plan_of(a.tokens, a.n, a.k, a.act, workspace != nullptr);
+  a.splits = p.splits, a.part = static_cast<float*>(workspace);
+  const int64_t tiles_t = (static_cast<int64_t>(a.tokens) + kShapes[p.shape].tokens - 1) / kShapes[p.shape].tokens;
+  if (p.shape == 0) return gemm::launch_tile<DT, gemm::kLinear, GATED, 2, 4, 4, 2, 2>(a, tiles_t, s);
+  if (p.shape == 1) return gemm::launch_tile<DT, gemm::kLinear, GATED, 2, 2, 2, 2, 2>(a, tiles_t, s);
+  return gemm::launch_tile<DT, gemm::kLinear, GATED, 1, 4, 2, 1, 3>(a, tiles_t, s);
+}
+
+// Tokens that the stream kernels take.
+int stream_tokens(int act) { return gated(act) ? gemm::stream_tokens<true>() : gemm::stream_tokens<false>(); }
+
 template <int DT>
-int run(const gemm::Args& a, bool vec, hipStream_t s) {
-  if (vec && a.tokens <= (gated(a.act) ? gemm::stream_tokens<true>() : gemm::stream_tokens<false>()) && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride) {
+int run(const gemm::Args& a, bool vec, void* workspace, hipStream_t s) {
+  const bool fast = vec && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride;
+  if (fast && a.tokens <= stream_tokens(a.act)) {
     gemm::StreamArgs st{};
     st.g = a;
     return gated(a.act) ? gemm::launch_stream<DT, gemm::kLinear, true>(st, a.tokens, 1, s)
                         : gemm::launch_stream<DT, gemm::kLinear, false>(st, a.tokens, 1, s);
   }
-  if (vec && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride)
-    return gated(a.act) ? run_tiles<DT, true>(a, s) : run_tiles<DT, false>(a, s);
+  if (fast) return gated(a.act) ? run_tiles<DT, true>(a, workspace, s) : run_tiles<DT, false>(a, workspace, s);
   const int64_t tiles_t = (static_cast<int64_t>(a.tokens) + gemm::kAnyTile - 1) / gemm::kAnyTile;
   return gated(a.act) ? gemm::launch_any<DT, gemm::kLinear, true>(a, vec, tiles_t, s)
                       : gemm::launch_any<DT, gemm::kLinear, false>(a, vec, tiles_t, s);
@@ -42,8 +88,10 @@ constexpr int64_t kMost = 0x7fffff00;  // tokens, outputs and inputs: room for a
 using namespace sgl;
 
 extern "C" int64_t sgl_linear_workspace_bytes(int64_t tokens, int64_t n, int64_t k, int activation) {
-  (void)tokens, (void)n, (void)k, (void)activation;
-  return 0;
+  if (tokens <= 0 || n <= 0 || k <= 0 || tokens > kMost || n > kMost || k > kMost ||
+      activation < SGL_ACT_NONE || activation > SGL_ACT_GELU_AND_MUL || tokens <= stream_tokens(activation))
+    return 0;
+  return plan_of(tokens, n, k, activation, true).bytes;
 }
 
 extern "C" int sgl_linear(const sgl_linear_t* args, void* workspace, int64_t workspace_bytes,
@@ -82,5 +130,6 @@ extern "C" int sgl_linear(const sgl_linear_t* args, void* workspace, int64_t wor
   const bool vec = x.k % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
                    aligned(x.weight, x.weight_stride_row, 16, 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return x.dtype == SGL_DTYPE_BF16 ? run<SGL_DTYPE_BF16>(a, vec, s) : run<SGL_DTYPE_F16>(a, vec, s);
+  return x.dtype == SGL_DTYPE_BF16 ? run<SGL_DTYPE_BF16>(a, vec, workspace, s)
+                                   : run<SGL_DTYPE_F16>(a, vec, workspace, s);
 }

@@ -374,17 +374,24 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
 
   const bool fast = up_vec && down_vec && x.tokens * up.x_st < (1ll << 30) &&
                     std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride;
-  const int rows = fast ? 128 : gemm::kAnyTile;
+  const int share = slots / x.num_experts;  // places of an expert, on average
+  const int rows = !fast ? gemm::kAnyTile : share <= 64 ? 64 : share < 256 ? 128 : 256;
   const int num_tiles = slots / rows + x.num_experts;
   const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, rows, num_tiles};
   hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
   int st = launch_status();
   if (st != SGL_OK) return st;
-  st = fast ? gemm::launch_tile<DT, gemm::kGateUp, true, 2, 2, 2, 2>(up, num_tiles, s)
-            : gemm::launch_any<DT, gemm::kGateUp, true>(up, up_vec, num_tiles, s);
+  const auto product = [&](auto mode, auto gate, const gemm::Args& a, bool vec) {
+    constexpr int kMode = decltype(mode)::value;
+    constexpr bool kGated = decltype(gate)::value;
+    if (!fast) return gemm::launch_any<DT, kMode, kGated>(a, vec, num_tiles, s);
+    if (rows == 64) return gemm::launch_tile<DT, kMode, kGated, 2, 2, 2, 1, 3>(a, num_tiles, s);
+    if (rows == 128) return gemm::launch_tile<DT, kMode, kGated, 2, 2, 2, 2, 2>(a, num_tiles, s);
+    return gemm::launch_tile<DT, kMode, kGated, 2, 4, 4, 2, 2>(a, num_tiles, s);
+  };
+  st = product(std::integral_constant<int, gemm::kGateUp>{}, std::true_type{}, up, up_vec);
   if (st != SGL_OK) return st;
-  st = fast ? gemm::launch_tile<DT, gemm::kDown, false, 2, 2, 2, 2>(down, num_tiles, s)
-            : gemm::launch_any<DT, gemm::kDown, false>(down, down_vec, num_tiles, s);
+  st = product(std::integral_constant<int, gemm::kDown>{}, std::false_type{}, down, down_vec);
   if (st != SGL_OK) return st;
   return kRounded ? combine<DT, DT>(x, l, y, s) : combine<DT, SGL_DTYPE_F32>(x, l, y, s);
 }

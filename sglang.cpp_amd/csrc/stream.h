@@ -218,6 +218,10 @@ __device__ __forceinline__ void lds_wait(u32x4_t& a, u32x4_t& b) {
   asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a), "+v"(b) : : "memory");
 }
 
+__device__ __forceinline__ void lds_wait(u32x4_t& a) {
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a) : : "memory");
+}
+
 // Waits until at most `left` units of kEach loads are in flight, left < kMost.
 template <int kMost, int kEach>
 __device__ __forceinline__ void units_wait(int left) {

@@ -1,11 +1,11 @@
 // Many tokens: tiles of weight rows x tokens whose operands go through LDS.
 //
 // WR x WC waves of 32 AT weight rows x 32 BT tokens each. 64 inputs of the tile's rows are a
-// stage; two stages are in LDS. A stage is loaded as four pieces, in the order they are
+// stage; D stages are in LDS. A stage is loaded as four pieces, in the order they are
 // needed: the first halves of every wave's weight rows and of its tokens, the second half
 // of the tokens, the second half of the rows. A piece's place is free as soon as its
-// operands are in registers, a phase later the piece two stages ahead is on its way into
-// it: loads have between one and two stages' products to arrive and no register holds them.
+// operands are in registers, a phase later the piece D stages ahead is on its way into
+// it: loads have between D - 1 and D stages' products to arrive and no register holds them.
 //
 // A stage is four phases of AT BT 2 matrix instructions: rows 0 x tokens 0, rows 0 x tokens
 // 1, rows 1 x tokens 1, rows 1 x tokens 0, each behind the reads of what it needs anew.
@@ -20,7 +20,7 @@ namespace gemm {
 
 constexpr int kXcds = 8;  // chiplets, each with an L2 of its own, take workgroups in turn
 
-template <int WR, int WC, int AT, int BT>
+template <int WR, int WC, int AT, int BT, int D>
 struct TileShape {
   static constexpr int kWaves = WR * WC;
   static constexpr int kM = WR * AT * 32, kN = WC * BT * 32;        // weight rows, tokens
@@ -28,7 +28,7 @@ struct TileShape {
   static constexpr int kLoadA = kPieceA / 8 / kWaves, kLoadB = kPieceB / 8 / kWaves;
   static constexpr int kOffA0 = 0, kOffB0 = kPieceA * 128, kOffB1 = kOffB0 + kPieceB * 128,
                        kOffA1 = kOffB1 + kPieceB * 128, kStage = kOffA1 + kPieceA * 128;
-  static constexpr int kBytes = 2 * kStage;
+  static constexpr int kBytes = D * kStage, kLoads = 2 * kLoadA + 2 * kLoadB;
 };
 
 template <int OFF, int N>
@@ -56,6 +56,61 @@ __device__ __forceinline__ void multiply(const u32x4_t (&a)[2][AT], const u32x4_
   __builtin_amdgcn_s_setprio(0);
 }
 
+// The operands of a whole stage and their products, for waves that have their SIMD's matrix
+// unit to themselves: [half of 64 inputs][half of the rows or tokens][tile].
+template <int AT, int BT>
+struct Operands {
+  u32x4_t a[2][2][AT], b[2][2][BT];
+
+  // Reads the stage in `slot`; between the reads, part(i) for i = 0 .. 4 (AT + BT) - 1.
+  template <typename S, int D, typename F>
+  __device__ __forceinline__ void read(uint32_t base_a, uint32_t base_b, int slot, F&& part) {
+    const uint32_t at_a[2] = {base_a + slot * S::kStage, (base_a + slot * S::kStage) ^ 64};
+    const uint32_t at_b[2] = {base_b + slot * S::kStage, (base_b + slot * S::kStage) ^ 64};
+    static_for<0, 4 * (AT + BT)>([&](auto i) {
+      constexpr int k = i.value / (2 * (AT + BT)), r = i.value % (2 * (AT + BT));
+      if constexpr (r < 2 * AT)
+        a[k][r / AT][r % AT] = lds_read<(r / AT ? S::kOffA1 : S::kOffA0) + r % AT * 2048>(at_a[k]);
+      else
+        b[k][(r - 2 * AT) / BT][(r - 2 * AT) % BT] =
+            lds_read<((r - 2 * AT) / BT ? S::kOffB1 : S::kOffB0) + (r - 2 * AT) % BT * 2048>(at_b[k]);
+      part(i);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+
+  __device__ __forceinline__ void wait() {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < AT; ++i) lds_wait(a[k][h][i]);
+#pragma unroll
+        for (int j = 0; j < BT; ++j) lds_wait(b[k][h][j]);
+      }
+  }
+
+  // The I-th of 4 (AT + BT) shares of the products.
+  template <int DT, typename I>
+  __device__ __forceinline__ void multiply(I, f32x4_t (&acc)[2][2][AT][BT]) const {
+    constexpr int kAll = 8 * AT * BT, kParts = 4 * (AT + BT);
+    static_for<I::value * kAll / kParts, (I::value + 1) * kAll / kParts>([&](auto n) {
+      constexpr int k = n.value / (4 * AT * BT), m = n.value % (4 * AT * BT);
+      constexpr int ha = m / (2 * AT * BT), i = m / (2 * BT) % AT, hb = m / BT % 2, j = m % BT;
+      acc[ha][hb][i][j] = mfma16<DT>(a[k][ha][i], b[k][hb][j], acc[ha][hb][i][j]);
+    });
+  }
+};
+
+// Waits until at most `left` whole stages and kMore loads are in flight, left < D.
+template <int D, int kLoads, int kMore>
+__device__ __forceinline__ void stages_wait(int left) {
+  static_for<0, D>([&](auto i) {
+    if (left == i.value) vm_wait<i.value * kLoads + kMore>();
+  });
+}
+
 // A barrier that no memory operation and no matrix instruction moves across; the waits in
 // front of it are explicit.
 __device__ __forceinline__ void phase_barrier() {
@@ -64,21 +119,65 @@ __device__ __forceinline__ void phase_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT>
+// The tile of a workgroup. Consecutive workgroups go to the chiplets in turn: each chiplet
+// has a run of tiles, eight tiles of weights by all tiles of tokens after another, so that
+// those it works on at a time share rows of both.
+struct Tile {
+  int n, t;
+};
+__device__ __forceinline__ Tile tile_of(int block, int total, int tiles_n) {
+  const int xcd = block % kXcds;
+  const int at = xcd * (total / kXcds) + min(xcd, total % kXcds) + block / kXcds;
+  const int tiles_t = total / tiles_n, band = at / (8 * tiles_t), in_band = at - band * 8 * tiles_t;
+  const int wide = min(8, tiles_n - 8 * band);
+  return {8 * band + in_band % wide, in_band / wide};
+}
+
+// What follows a quarter (second or first half of a wave's weight rows and of its tokens)
+// of a wave's sums.
+template <int DT, int MODE, bool GATED, int AT, int BT>
+__device__ __forceinline__ void finish_quarter(const Args& a, const Part& p, int n0, int wr, int wc, int ha,
+                                               int hb, const f32x4_t (&acc)[AT][BT]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < BT; ++j) {
+    const int t = wc * BT * 32 + hb * BT * 16 + j * 16 + (lane & 15);
+    if (t >= p.rows) continue;
+    float scale;
+    const int64_t row = target_row<MODE>(a, p.first + t, scale);
+    const int n = n0 + (wr * AT * 32 + ha * AT * 16) / (GATED ? 2 : 1) + 4 * (lane >> 4);
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < AT; i += 2)
+        finish4<DT, MODE, true>(a, n + i * 8, row, scale, acc[i][j], acc[i + 1][j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < AT; ++i)
+        finish4<DT, MODE, false>(a, n + i * 16, row, scale, acc[i][j], acc[i][j]);
+    }
+  }
+}
+
+// Place of a lane's four sums: part, tile, quarter, piece of it; whole waves store whole lines.
+template <int WR, int WC, int AT, int BT>
+__device__ __forceinline__ f32x4_t* part_at(const Args& a, int tiles, int split, int tile, int quarter) {
+  constexpr int kThreads = 64 * WR * WC;
+  return reinterpret_cast<f32x4_t*>(a.part) +
+         ((static_cast<int64_t>(split) * tiles + tile) * 4 + quarter) * (AT * BT * kThreads) + threadIdx.x;
+}
+
+template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT, int D>
 __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
-  using S = TileShape<WR, WC, AT, BT>;
+  using S = TileShape<WR, WC, AT, BT, D>;
   constexpr int LA = S::kLoadA, LB = S::kLoadB;
   constexpr bool kPhased = S::kWaves == 8;
-  static_assert(LA == 2 && LB == 2, "a wave's loads of gate or up rows");
+  static_assert(LA <= 4 && LB <= 4, "a wave's loads of gate or up rows");
   __shared__ __attribute__((aligned(1024))) char lds[S::kBytes];
-  // Consecutive workgroups go to the chiplets in turn: each chiplet has a run of tiles,
-  // eight tiles of weights by all tiles of tokens after another, so that those it works on
-  // at a time share rows of both.
-  const int total = gridDim.x, xcd = blockIdx.x % kXcds;
-  const int at = xcd * (total / kXcds) + min(xcd, total % kXcds) + static_cast<int>(blockIdx.x) / kXcds;
-  const int tiles_t = total / a.tiles_n, band = at / (8 * tiles_t), in_band = at - band * 8 * tiles_t;
-  const int wide = min(8, a.tiles_n - 8 * band);
-  const int tn = 8 * band + in_band % wide, tt = in_band / wide;
+  // Parts of k: all tiles of the first one, then of the next.
+  const int total = static_cast<int>(gridDim.x) / a.splits;
+  const int split = static_cast<int>(blockIdx.x) / total, block = blockIdx.x - split * total;
+  const Tile tile = tile_of(block, total, a.tiles_n);
+  const int tn = tile.n, tt = tile.t;
   const Part p = part_of<MODE>(a, tt, S::kN);
   if (p.rows <= 0) return;
   const int n0 = tn * (GATED ? S::kM / 2 : S::kM);
@@ -115,9 +214,12 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
   const auto xr_src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(xbase), 0, kNowhere, 0x00027000);
   // Stage s is inputs 64 s .. + 63; where k is not a whole number of stages, the part of one
   // comes first (the order of the sum is free) and the others follow from input 0 on.
-  const int tail = a.k % 64, stages = a.k / 64 + (tail ? 1 : 0);
+  const int k_tail = a.k % 64, all = a.k / 64 + (k_tail ? 1 : 0);
+  const int begin = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
+  const int stages = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - begin;
+  const int tail = begin == 0 ? k_tail : 0, shift = begin - (k_tail ? 1 : 0);
   auto fetch_a = [&](int s, auto h, int slot) {
-    const int k_at = __builtin_amdgcn_readfirstlane((s - (tail ? 1 : 0)) * 128);
+    const int k_at = __builtin_amdgcn_readfirstlane((s + shift) * 128);
 #pragma unroll
     for (int u = 0; u < LA; ++u)
       stage16<false>(wr_src,
@@ -125,7 +227,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
                      wo[h.value][u], k_at);
   };
   auto fetch_b = [&](int s, auto h, int slot) {
-    const int k_at = __builtin_amdgcn_readfirstlane((s - (tail ? 1 : 0)) * 128);
+    const int k_at = __builtin_amdgcn_readfirstlane((s + shift) * 128);
 #pragma unroll
     for (int u = 0; u < LB; ++u)
       stage16<false>(xr_src,
@@ -152,12 +254,10 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
   } else {
     fetch_a(0, i0, 0), fetch_b(0, i0, 0), fetch_b(0, i1, 0), fetch_a(0, i1, 0);
   }
-  if (stages > 1) {
-    fetch_a(1, i0, 1), fetch_b(1, i0, 1), fetch_b(1, i1, 1), fetch_a(1, i1, 1);
-    vm_wait<3 * LA + 3 * LB>();
-  } else {
-    vm_wait<0>();
-  }
+  for (int d = 1; d < D; ++d)
+    if (d < stages) fetch_a(d, i0, d), fetch_b(d, i0, d), fetch_b(d, i1, d), fetch_a(d, i1, d);
+  if (kPhased) stages_wait<D, S::kLoads, LA + LB>(min(stages, D) - 1);
+  else stages_wait<D, S::kLoads, 0>(min(stages, D) - 1);
   phase_barrier();
   if (kPhased && wave >= 4) phase_barrier();
 
@@ -167,81 +267,139 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
                         r * 128 + (((lane >> 4) ^ (r >> 1)) & 7) * 16;
   const uint32_t base_a = base + wr * AT * 2048, base_b = base + wc * BT * 2048;
   f32x4_t acc[2][2][AT][BT] = {};
-  u32x4_t fa[2][AT], fb0[2][BT], fb1[2][BT];
-  for (int s = 0; s < stages; ++s) {
-    const int slot = s & 1;
-    const uint32_t at_a = base_a + slot * S::kStage, at_b = base_b + slot * S::kStage;
-    const bool more = s + 2 < stages;
-    // Rows 0 x tokens 0.
-    read_tiles<S::kOffB0>(at_b, fb0);
-    read_tiles<S::kOffA0>(at_a, fa);
-    if (more) vm_wait<3 * LA + 2 * LB>();  // tokens 1 of this stage
-    else vm_wait<0>();
-    wait_tiles(fb0), wait_tiles(fa);
-    phase_barrier();
-    multiply<DT>(fa, fb0, acc[0][0]);
-    if constexpr (kPhased) phase_barrier();
-    // Rows 0 x tokens 1.
-    read_tiles<S::kOffB1>(at_b, fb1);
-    if (more) {
-      fetch_a(s + 2, i0, slot), fetch_b(s + 2, i0, slot);
-      vm_wait<3 * LA + 3 * LB>();  // rows 1 of this stage
-    }
-    wait_tiles(fb1);
-    phase_barrier();
-    multiply<DT>(fa, fb1, acc[0][1]);
-    if constexpr (kPhased) phase_barrier();
-    // Rows 1 x tokens 1.
-    read_tiles<S::kOffA1>(at_a, fa);
-    if (more) fetch_b(s + 2, i1, slot);
-    wait_tiles(fa);
-    phase_barrier();
-    multiply<DT>(fa, fb1, acc[1][1]);
-    if constexpr (kPhased) phase_barrier();
-    // Rows 1 x tokens 0.
-    if (more) {
-      fetch_a(s + 2, i1, slot);
-      vm_wait<3 * LA + 3 * LB>();  // rows 0 and tokens 0 of the next stage
-    }
-    phase_barrier();
-    multiply<DT>(fa, fb0, acc[1][0]);
-    if constexpr (kPhased) phase_barrier();
-  }
-  if (kPhased && wave < 4) phase_barrier();
-
-#pragma unroll
-  for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-    for (int j = 0; j < BT; ++j) {
-      const int t = wc * BT * 32 + hb * BT * 16 + j * 16 + (lane & 15);
-      if (t >= p.rows) continue;
-      float scale;
-      const int64_t row = target_row<MODE>(a, p.first + t, scale);
-#pragma unroll
-      for (int ha = 0; ha < 2; ++ha) {
-        const int n = n0 + (wr * AT * 32 + ha * AT * 16) / (GATED ? 2 : 1) + 4 * (lane >> 4);
-        if constexpr (GATED) {
-#pragma unroll
-          for (int i = 0; i < AT; i += 2)
-            finish4<DT, MODE, true>(a, n + i * 8, row, scale, acc[ha][hb][i][j], acc[ha][hb][i + 1][j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < AT; ++i)
-            finish4<DT, MODE, false>(a, n + i * 16, row, scale, acc[ha][hb][i][j], acc[ha][hb][i][j]);
-        }
+  const std::true_type steady;
+  const std::false_type ending;
+  int slot = 0, s = 0;
+  if constexpr (kPhased) {
+    u32x4_t fa[2][AT], fb0[2][BT], fb1[2][BT];
+    // steady: stage s + D exists, so that what is in flight is known.
+    auto stage = [&](auto more) {
+      const uint32_t at_a = base_a + slot * S::kStage, at_b = base_b + slot * S::kStage;
+      const int left = min(stages - 1 - s, D - 1);  // stages on their way behind this one
+      // Rows 0 x tokens 0.
+      read_tiles<S::kOffB0>(at_b, fb0);
+      read_tiles<S::kOffA0>(at_a, fa);
+      if constexpr (more.value) vm_wait<(D - 1) * S::kLoads + LA>();  // tokens 1 of this stage
+      else stages_wait<D, S::kLoads, LA>(left);
+      wait_tiles(fb0), wait_tiles(fa);
+      phase_barrier();
+      multiply<DT>(fa, fb0, acc[0][0]);
+      phase_barrier();
+      // Rows 0 x tokens 1.
+      read_tiles<S::kOffB1>(at_b, fb1);
+      if constexpr (more.value) {
+        fetch_a(s + D, i0, slot), fetch_b(s + D, i0, slot);
+        vm_wait<(D - 1) * S::kLoads + LA + LB>();  // rows 1 of this stage
+      } else {
+        stages_wait<D, S::kLoads, 0>(left);
       }
+      wait_tiles(fb1);
+      phase_barrier();
+      multiply<DT>(fa, fb1, acc[0][1]);
+      phase_barrier();
+      // Rows 1 x tokens 1.
+      read_tiles<S::kOffA1>(at_a, fa);
+      if constexpr (more.value) fetch_b(s + D, i1, slot);
+      wait_tiles(fa);
+      phase_barrier();
+      multiply<DT>(fa, fb1, acc[1][1]);
+      phase_barrier();
+      // Rows 1 x tokens 0.
+      if constexpr (more.value) {
+        fetch_a(s + D, i1, slot);
+        vm_wait<(D - 1) * S::kLoads + LA + LB>();  // rows 0 and tokens 0 of the next stage
+      } else if (left > 0) {
+        stages_wait<D, S::kLoads, LA + LB>(left - 1);
+      }
+      phase_barrier();
+      multiply<DT>(fa, fb0, acc[1][0]);
+      phase_barrier();
+      slot = slot + 1 == D ? 0 : slot + 1;
+      ++s;
+    };
+    while (s + D < stages) stage(steady);
+    while (s < stages) stage(ending);
+    if (wave < 4) phase_barrier();
+  } else {
+    Operands<AT, BT> f[2];
+    f[0].template read<S, D>(base_a, base_b, 0, [](auto) {});
+    f[0].wait();
+    // One stage: the operands of the next one are read between its products.
+    auto stage = [&](auto more, Operands<AT, BT>& now, Operands<AT, BT>& next) {
+      if constexpr (more.value) vm_wait<(D - 2) * S::kLoads>();
+      else if (s + 1 < stages) stages_wait<D - 1, S::kLoads, 0>(min(stages - 2 - s, D - 2));
+      phase_barrier();  // the next stage is there, and every wave has this one in registers
+      if (more.value || s + D < stages)
+        fetch_a(s + D, i0, slot), fetch_b(s + D, i0, slot), fetch_b(s + D, i1, slot), fetch_a(s + D, i1, slot);
+      slot = slot + 1 == D ? 0 : slot + 1;
+      // Behind the last stage the reads find what was there and nobody takes it.
+      next.template read<S, D>(base_a, base_b, slot, [&](auto i) { now.template multiply<DT>(i, acc); });
+      next.wait();
+      ++s;
+    };
+    while (s + D + 1 < stages) stage(steady, f[0], f[1]), stage(steady, f[1], f[0]);
+    for (;;) {
+      stage(ending, f[0], f[1]);
+      if (s == stages) break;
+      stage(ending, f[1], f[0]);
+      if (s == stages) break;
     }
+  }
+
+  static_for<0, 4>([&](auto q) {
+    constexpr int ha = q.value / 2, hb = q.value % 2;
+    if (MODE == kLinear && a.splits > 1) {
+      f32x4_t* out = part_at<WR, WC, AT, BT>(a, total, split, block, q.value);
+#pragma unroll
+      for (int i = 0; i < AT; ++i)
+#pragma unroll
+        for (int j = 0; j < BT; ++j) out[(i * BT + j) * 64 * S::kWaves] = acc[ha][hb][i][j];
+    } else {
+      finish_quarter<DT, MODE, GATED, AT, BT>(a, p, n0, wr, wc, ha, hb, acc[ha][hb]);
+    }
+  });
 }
 
-template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT>
+// The sum of a tile's parts, in their order, and what follows it: a workgroup for each
+// quarter of the waves' sums.
+template <int DT, bool GATED, int WR, int WC, int AT, int BT>
+__global__ __launch_bounds__(64 * WR * WC) void fold_kernel(const Args a) {
+  using S = TileShape<WR, WC, AT, BT, 2>;
+  const int total = gridDim.x, block = blockIdx.x, quarter = blockIdx.y;
+  const Tile tile = tile_of(block, total, a.tiles_n);
+  const Part p = part_of<kLinear>(a, tile.t, S::kN);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  f32x4_t acc[AT][BT] = {};
+  for (int split = 0; split < a.splits; ++split) {
+    const f32x4_t* in = part_at<WR, WC, AT, BT>(a, total, split, block, quarter);
+#pragma unroll
+    for (int i = 0; i < AT; ++i)
+#pragma unroll
+      for (int j = 0; j < BT; ++j)
+        acc[i][j] += __builtin_nontemporal_load(&in[(i * BT + j) * 64 * S::kWaves]);
+  }
+  finish_quarter<DT, kLinear, GATED, AT, BT>(a, p, tile.n * (GATED ? S::kM / 2 : S::kM), wave % WR, wave / WR,
+                                             quarter / 2, quarter % 2, acc);
+}
+
+template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT, int D>
 int launch_tile(Args a, int64_t tiles_t, hipStream_t s) {
-  using S = TileShape<WR, WC, AT, BT>;
+  using S = TileShape<WR, WC, AT, BT, D>;
   constexpr int out = GATED ? S::kM / 2 : S::kM;
   a.tiles_n = static_cast<int32_t>((static_cast<int64_t>(a.n) + out - 1) / out);
   const int64_t grid = grid_of(a.tiles_n, tiles_t);
   if (grid < 0) return SGL_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((tile_kernel<DT, MODE, GATED, WR, WC, AT, BT>), dim3(static_cast<uint32_t>(grid)),
-                     dim3(64 * S::kWaves), 0, s, a);
+  if (a.splits < 1) a.splits = 1;
+  hipLaunchKernelGGL((tile_kernel<DT, MODE, GATED, WR, WC, AT, BT, D>),
+                     dim3(static_cast<uint32_t>(grid * a.splits)), dim3(64 * S::kWaves), 0, s, a);
+  if constexpr (MODE == kLinear) {
+    if (a.splits > 1) {
+      const int st = launch_status();
+      if (st != SGL_OK) return st;
+      hipLaunchKernelGGL((fold_kernel<DT, GATED, WR, WC, AT, BT>), dim3(static_cast<uint32_t>(grid), 4),
+                         dim3(64 * S::kWaves), 0, s, a);
+    }
+  }
   return launch_status();
 }
 
