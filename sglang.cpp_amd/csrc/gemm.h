@@ -30,7 +30,7 @@ struct Args {
   int32_t tokens, n, k;
   int32_t act;      // SGL_ACT_*
   int32_t out_f32;  // out is fp32
-  int32_t wide;     // outputs, bias and residual of four columns can go in one access
+  int32_t wide;     // outputs, bias and residual: 1 of four columns, 2 of eight in whole accesses
   int32_t tiles_n;  // tiles over the outputs
   int32_t top_k;
   const int4* tiles;     // experts: {expert, first place, places, 0} of a tile of places
@@ -80,6 +80,61 @@ __device__ __forceinline__ u32x4_t load8(const uint16_t* row, int e, int k) {
       if (e + i < k) v[i / 2] |= static_cast<uint32_t>(row[e + i]) << (16 * (i & 1));
   }
   return v;
+}
+
+// Bias and activation of outputs n0 .. n0 + 3 (columns past the last are dropped later).
+template <int DT, int MODE, bool GATED>
+__device__ __forceinline__ f32x4_t activated4(const Args& a, int n0, f32x4_t g, f32x4_t u) {
+  if constexpr (MODE == kLinear) {
+    if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = min(n0 + i, a.n - 1);
+        g[i] += to_f32<DT>(a.bias[n]);
+        if constexpr (GATED) u[i] += to_f32<DT>(a.bias[a.n + n]);
+      }
+    }
+  }
+  if constexpr (MODE != kDown) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = activate(a.act, g[i]);
+  }
+  if constexpr (GATED) g *= u;
+  return g;
+}
+
+// Weight, residual and rounding of the activated outputs n0 .. n0 + 7 of one row.
+template <int DT, int MODE>
+__device__ __forceinline__ void store8(const Args& a, int n0, int64_t row, float scale, float (&y)[8]) {
+  if (n0 >= a.n) return;
+  if constexpr (MODE == kDown) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= scale;
+  }
+  const uint16_t* r = MODE == kLinear && a.res ? a.res + row * a.r_st + n0 : nullptr;
+  if (a.wide == 2 && n0 + 8 <= a.n) {
+    if (r) {
+      float f[8];
+      unpack8_t<DT>(ldg128(r), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += f[i];
+    }
+    if (a.out_f32) {
+      float* o = static_cast<float*>(a.out) + row * a.o_st + n0;
+      *reinterpret_cast<f32x4_t*>(o) = f32x4_t{y[0], y[1], y[2], y[3]};
+      *reinterpret_cast<f32x4_t*>(o + 4) = f32x4_t{y[4], y[5], y[6], y[7]};
+    } else {
+      stg128(static_cast<uint16_t*>(a.out) + row * a.o_st + n0, pack8_t<DT>(y));
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (n0 + i >= a.n) break;
+    const float v = r ? y[i] + to_f32<DT>(r[i]) : y[i];
+    if (a.out_f32) static_cast<float*>(a.out)[row * a.o_st + n0 + i] = v;
+    else static_cast<uint16_t*>(a.out)[row * a.o_st + n0 + i] = static_cast<uint16_t>(from_f32<DT>(v));
+  }
 }
 
 // Outputs n0 .. n0 + 3 of one row: g (and, gated, u) from the accumulators.

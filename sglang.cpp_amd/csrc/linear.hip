@@ -1,6 +1,8 @@
 // sgl_linear: a projection with its epilogue.
 #include "tile.h"
 
+#include <algorithm>
+
 namespace sgl {
 namespace {
 
@@ -124,9 +126,12 @@ extern "C" int sgl_linear(const sgl_linear_t* args, void* workspace, int64_t wor
   a.k = static_cast<int32_t>(x.k), a.act = x.activation;
   a.out_f32 = x.out_dtype == SGL_DTYPE_F32;
   const int64_t size = a.out_f32 ? 4 : 2;
-  a.wide = aligned(x.out, x.out_stride_row, 4 * size, size) &&
-           aligned(x.residual, x.residual_stride_row, 8, 2) &&
-           aligned(x.bias, gated(x.activation) ? x.n : 0, 8, 2);
+  const int64_t rows = gated(x.activation) ? x.n : 0;
+  const auto wide = [&](int64_t columns) {
+    return aligned(x.out, x.out_stride_row, std::min<int64_t>(16, columns * size), size) &&
+           aligned(x.residual, x.residual_stride_row, 2 * columns, 2) && aligned(x.bias, rows, 8, 2);
+  };
+  a.wide = wide(8) ? 2 : wide(4) ? 1 : 0;
   const bool vec = x.k % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
                    aligned(x.weight, x.weight_stride_row, 16, 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);

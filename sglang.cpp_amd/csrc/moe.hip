@@ -350,14 +350,14 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   up.x = static_cast<const uint16_t*>(x.x), up.x_st = x.x_stride_row;
   up.w = static_cast<const uint16_t*>(x.gate_up);
   up.w_st = x.gate_up_stride_row, up.w_se = x.gate_up_stride_expert;
-  up.out = h, up.o_st = l.h_st, up.wide = 1;
+  up.out = h, up.o_st = l.h_st, up.wide = 2;
   up.tokens = slots, up.n = x.intermediate, up.k = x.hidden, up.act = x.activation;
   const bool up_vec = x.hidden % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
                       aligned(x.gate_up, x.gate_up_stride_row, 16, 2) && x.gate_up_stride_expert % 8 == 0;
   down.x = h, down.x_st = l.h_st;
   down.w = static_cast<const uint16_t*>(x.down);
   down.w_st = x.down_stride_row, down.w_se = x.down_stride_expert;
-  down.out = y, down.o_st = l.y_st, down.out_f32 = 1, down.wide = 1;
+  down.out = y, down.o_st = l.y_st, down.out_f32 = 1, down.wide = 2;
   down.tokens = slots, down.n = x.hidden, down.k = x.intermediate;
   const bool down_vec = x.intermediate % 8 == 0 && aligned(x.down, x.down_stride_row, 16, 2) &&
                         x.down_stride_expert % 8 == 0;

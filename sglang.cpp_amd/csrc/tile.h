@@ -31,6 +31,13 @@ struct TileShape {
   static constexpr int kBytes = D * kStage, kLoads = 2 * kLoadA + 2 * kLoadB;
 };
 
+// LDS operations of a wave are in order; this keeps the compiler from changing it.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int OFF, int N>
 __device__ __forceinline__ void read_tiles(uint32_t at, u32x4_t (&f)[2][N]) {
   static_for<0, N>([&](auto i) {
@@ -158,6 +165,55 @@ __device__ __forceinline__ void finish_quarter(const Args& a, const Part& p, int
   }
 }
 
+// What follows a wave's sums, by way of its own part of LDS, half of its tokens at a time:
+// the matrix instruction leaves four outputs of a token to a lane, stores of which would
+// touch 32 bytes of each of 16 rows (8 slots of 8,192 tokens x 2,048 outputs: half of the
+// kernel's time); from LDS every 16 lanes (8, 4) store a token's whole run of outputs.
+// Rows of outputs are in pieces of four, piece c of token t at place c ^ t (mod 16) or c ^
+// (t / 2) (mod 8), so that 16 tokens' pieces are spread over all banks.
+template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT>
+__device__ __forceinline__ void finish_wave(const Args& a, const Part& p, int n0, int wr, int wc, char* lds,
+                                            const f32x4_t (&acc)[2][2][AT][BT]) {
+  constexpr int kOut = GATED ? AT * 16 : AT * 32, kPieces = kOut / 4;  // of a wave
+  constexpr int kTokens = BT * 16, kLanes = kOut / 8, kRows = 64 / kLanes;
+  constexpr int kSteps = kTokens / kRows;
+  const int lane = threadIdx.x & 63;
+  f32x4_t* stage = reinterpret_cast<f32x4_t*>(lds) + (wc * WR + wr) * (kTokens * kPieces);
+  const auto place = [&](int t, int c) {
+    return t * kPieces + (kPieces >= 16 ? c ^ (t & 15) : c ^ ((t >> 1) & 7));
+  };
+  const int first_n = n0 + wr * kOut;
+  static_for<0, 2>([&](auto hb) {
+    const int t0 = (wc * 2 + hb.value) * kTokens, mine = lane / kLanes;
+    int64_t row[kSteps];
+    float scale[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      row[s] = target_row<MODE>(a, p.first + min(t0 + s * kRows + mine, p.rows - 1), scale[s]);
+#pragma unroll
+    for (int j = 0; j < BT; ++j)
+#pragma unroll
+      for (int ha = 0; ha < 2; ++ha)
+#pragma unroll
+        for (int i = 0; i < AT; i += GATED ? 2 : 1) {
+          const int n = (ha * AT + i) * (GATED ? 8 : 16) + 4 * (lane >> 4);  // of the wave's
+          const f32x4_t& u = acc[ha][hb.value][GATED ? i + 1 : i][j];
+          stage[place(j * 16 + (lane & 15), n / 4)] =
+              activated4<DT, MODE, GATED>(a, first_n + n, acc[ha][hb.value][i][j], u);
+        }
+    wave_sync();
+    const int c = 2 * (lane % kLanes);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int t = s * kRows + mine;
+      const f32x4_t lo = stage[place(t, c)], hi = stage[place(t, c + 1)];
+      float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if (t0 + t < p.rows) store8<DT, MODE>(a, first_n + 4 * c, row[s], scale[s], y);
+    }
+    wave_sync();
+  });
+}
+
 // Place of a lane's four sums: part, tile, quarter, piece of it; whole waves store whole lines.
 template <int WR, int WC, int AT, int BT>
 __device__ __forceinline__ f32x4_t* part_at(const Args& a, int tiles, int split, int tile, int quarter) {
@@ -167,7 +223,7 @@ __device__ __forceinline__ f32x4_t* part_at(const Args& a, int tiles, int split,
 }
 
 template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT, int D>
-__global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
+__global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2) void tile_kernel(const Args a) {
   using S = TileShape<WR, WC, AT, BT, D>;
   constexpr int LA = S::kLoadA, LB = S::kLoadB;
   constexpr bool kPhased = S::kWaves == 8;
@@ -267,6 +323,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
                         r * 128 + (((lane >> 4) ^ (r >> 1)) & 7) * 16;
   const uint32_t base_a = base + wr * AT * 2048, base_b = base + wc * BT * 2048;
   f32x4_t acc[2][2][AT][BT] = {};
+  const bool idle = wc * BT * 32 >= p.rows;  // no token of this wave's: it only loads and waits
   const std::true_type steady;
   const std::false_type ending;
   int slot = 0, s = 0;
@@ -283,7 +340,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
       else stages_wait<D, S::kLoads, LA>(left);
       wait_tiles(fb0), wait_tiles(fa);
       phase_barrier();
-      multiply<DT>(fa, fb0, acc[0][0]);
+      if (!idle) multiply<DT>(fa, fb0, acc[0][0]);
       phase_barrier();
       // Rows 0 x tokens 1.
       read_tiles<S::kOffB1>(at_b, fb1);
@@ -295,14 +352,14 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
       }
       wait_tiles(fb1);
       phase_barrier();
-      multiply<DT>(fa, fb1, acc[0][1]);
+      if (!idle) multiply<DT>(fa, fb1, acc[0][1]);
       phase_barrier();
       // Rows 1 x tokens 1.
       read_tiles<S::kOffA1>(at_a, fa);
       if constexpr (more.value) fetch_b(s + D, i1, slot);
       wait_tiles(fa);
       phase_barrier();
-      multiply<DT>(fa, fb1, acc[1][1]);
+      if (!idle) multiply<DT>(fa, fb1, acc[1][1]);
       phase_barrier();
       // Rows 1 x tokens 0.
       if constexpr (more.value) {
@@ -312,7 +369,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
         stages_wait<D, S::kLoads, LA + LB>(left - 1);
       }
       phase_barrier();
-      multiply<DT>(fa, fb0, acc[1][0]);
+      if (!idle) multiply<DT>(fa, fb0, acc[1][0]);
       phase_barrier();
       slot = slot + 1 == D ? 0 : slot + 1;
       ++s;
@@ -346,18 +403,19 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
     }
   }
 
-  static_for<0, 4>([&](auto q) {
-    constexpr int ha = q.value / 2, hb = q.value % 2;
-    if (MODE == kLinear && a.splits > 1) {
+  if (MODE == kLinear && a.splits > 1) {
+    static_for<0, 4>([&](auto q) {
+      constexpr int ha = q.value / 2, hb = q.value % 2;
       f32x4_t* out = part_at<WR, WC, AT, BT>(a, total, split, block, q.value);
 #pragma unroll
       for (int i = 0; i < AT; ++i)
 #pragma unroll
         for (int j = 0; j < BT; ++j) out[(i * BT + j) * 64 * S::kWaves] = acc[ha][hb][i][j];
-    } else {
-      finish_quarter<DT, MODE, GATED, AT, BT>(a, p, n0, wr, wc, ha, hb, acc[ha][hb]);
-    }
-  });
+    });
+    return;
+  }
+  phase_barrier();  // every wave is done with the operands
+  finish_wave<DT, MODE, GATED, WR, WC, AT, BT>(a, p, n0, wr, wc, lds, acc);
 }
 
 // The sum of a tile's parts, in their order, and what follows it: a workgroup for each
