@@ -19,12 +19,13 @@ constexpr Shape kShapes[] = {
     {128, 128, 2, 0.70, 1.05},  // 1,090 there; 2,048 x 4,096 x 4,096 takes 72 us, the larger ones 100
     {64, 128, 2, 0.40, 0.55},   // 512 x 4,096 x 4,096: 28 us, the others 48 and 92
 };
-constexpr int kCus = 256;
+using gemm::kCus;
 constexpr int kMostSplits = 8;
 
 struct Plan {
   int shape, splits;
   int64_t bytes;  // of the parts' sums
+  double us;
 };
 
 // The shape and the number of parts of k with the least estimated time: rounds of
@@ -33,8 +34,7 @@ struct Plan {
 // x 4,096: 64 x 128 in four 15.6, in one 26).
 Plan plan_of(int64_t tokens, int64_t n, int64_t k, int act, bool may_split) {
   const int64_t rows = n * (gated(act) ? 2 : 1), stages = (k + 63) / 64;
-  Plan best{0, 1, 0};
-  double least = 1e300;
+  Plan best{0, 1, 0, 1e300};
   for (int i = 0; i < 3; ++i) {
     const Shape& x = kShapes[i];
     const int64_t tiles = ((rows + x.rows - 1) / x.rows) * ((tokens + x.tokens - 1) / x.tokens);
@@ -42,12 +42,27 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t k, int act, bool may_split) {
       const int64_t groups = tiles * s, each = (stages + s - 1) / s;
       const int64_t bytes = s > 1 ? groups * x.rows * x.tokens * 4 : 0;
       const int64_t rounds = (groups + kCus * x.per_cu - 1) / (kCus * x.per_cu);
-      const double us = (groups <= kCus ? x.alone : x.full) * static_cast<double>(rounds * each) +
+      const double us = 4.0 + (groups <= kCus ? x.alone : x.full) * static_cast<double>(rounds * each) +
                         (s > 1 ? 2.5 + 2.0 * static_cast<double>(bytes) / 5e6 : 0.0);
-      if (us < least) least = us, best = Plan{i, s, bytes};
+      if (us < best.us) best = Plan{i, s, bytes, us};
     }
   }
   return best;
+}
+
+// Whether the stream kernels take a call: always up to 16 tokens (their rows of x cost what
+// the weights' do), above where their estimate, the weights at 5.8 TB/s or what a CU
+// stages at 50 GB/s, is the lower one (48 tokens x 4,096 x 4,096: 13 us, tiles 16; 60 x
+// 4,096 x 12,288: 37, tiles 29).
+bool streams(int64_t tokens, int64_t n, int64_t k, int act, bool may_split) {
+  if (tokens > gemm::stream_tokens(gated(act), n)) return false;
+  if (tokens <= 16) return true;
+  const int tiles = gemm::stream_tiles(gated(act), n, 1);
+  const int64_t rows = n * (gated(act) ? 2 : 1), groups = (rows + 16 * tiles - 1) / (16 * tiles);
+  const double staged = static_cast<double>((groups + kCus - 1) / kCus * (tiles + (tokens + 15) / 16)) * 32.0 *
+                        static_cast<double>(k);
+  const double read = 2.0 * static_cast<double>(rows) * static_cast<double>(k);
+  return 2.5 + std::max(staged / 5e4, read / 5.8e6) <= plan_of(tokens, n, k, act, may_split).us;
 }
 
 template <int DT, bool GATED>
@@ -60,13 +75,10 @@ int run_tiles(gemm::Args a, void* workspace, hipStream_t s) {
   return gemm::launch_tile<DT, gemm::kLinear, GATED, 1, 4, 2, 1, 3>(a, tiles_t, s);
 }
 
-// Tokens that the stream kernels take.
-int stream_tokens(int act) { return gated(act) ? gemm::stream_tokens<true>() : gemm::stream_tokens<false>(); }
-
 template <int DT>
 int run(const gemm::Args& a, bool vec, void* workspace, hipStream_t s) {
   const bool fast = vec && a.x_st <= gemm::kMostStride && a.w_st <= gemm::kMostStride;
-  if (fast && a.tokens <= stream_tokens(a.act)) {
+  if (fast && streams(a.tokens, a.n, a.k, a.act, workspace != nullptr)) {
     gemm::StreamArgs st{};
     st.g = a;
     return gated(a.act) ? gemm::launch_stream<DT, gemm::kLinear, true>(st, a.tokens, 1, s)
@@ -91,7 +103,7 @@ using namespace sgl;
 
 extern "C" int64_t sgl_linear_workspace_bytes(int64_t tokens, int64_t n, int64_t k, int activation) {
   if (tokens <= 0 || n <= 0 || k <= 0 || tokens > kMost || n > kMost || k > kMost ||
-      activation < SGL_ACT_NONE || activation > SGL_ACT_GELU_AND_MUL || tokens <= stream_tokens(activation))
+      activation < SGL_ACT_NONE || activation > SGL_ACT_GELU_AND_MUL || streams(tokens, n, k, activation, true))
     return 0;
   return plan_of(tokens, n, k, activation, true).bytes;
 }

@@ -1,20 +1,12 @@
-// Few tokens: every weight is read once, straight into the registers of the matrix
-// instruction that takes it, and everything else is kept out of its way.
+// Few tokens: every weight is read once and everything else is kept out of its way.
 //
-// A workgroup has MT tiles of weight rows, its waves share out the inputs (k) in units of
-// 128 or 256 bytes of a row and fold their sums through LDS at the end. One instruction
-// multiplies 16 rows by 16 columns over 32 inputs.
-//
-// Up to 4 or 8 tokens (P = 4, 2): rows and columns stand for 16 / P rows and tokens times P
-// parts of the inputs; row and column blocks of the same part meet on the diagonal, whose P
-// blocks are summed, and what is off it is dropped. Neighbouring lanes then hold
-// neighbouring inputs of a row, so operands are loaded straight into registers, and a tile
-// has fewer rows, so that short launches spread over more workgroups. The wasted products
-// cost nothing where the weights' bytes are what bounds the kernel.
-//
-// More tokens (P = 1): neighbouring lanes hold different rows, which makes every lane's 16
-// bytes an access of its own; each wave brings whole 128-byte pieces of rows into a ring of
-// its own in LDS (no registers, no barriers) and reads the operands from there.
+// A workgroup has MT tiles of 16 weight rows, its waves share out the inputs (k) in units of
+// 64 (128 bytes of a row, a cache line) and fold their sums through LDS at the end. One
+// instruction multiplies 16 rows by 16 columns (tokens) over 32 inputs. Its operands have
+// neighbouring lanes in different rows: loaded straight into registers, every lane's 16
+// bytes are an access of their own (24 tokens through 84 experts of 2 x 768 x 2,048: 129 us
+// where this takes 85). So each wave brings whole pieces of rows into a ring of its own in
+// LDS, which holds no registers and needs no barrier, and reads the operands from there.
 #pragma once
 
 #include "gemm.h"
@@ -25,6 +17,7 @@ namespace gemm {
 // Slots of one expert, found by every workgroup of a launch for itself: a few hundred
 // choices are read faster than another launch would sort them.
 constexpr int kMostSlots = 1024;
+constexpr int kCus = 256;
 // Strides whose 16 weight rows, 64 rows of x or 1,024 rows of h stay below 2^31 bytes.
 constexpr int64_t kMostStride = 1 << 20;
 
@@ -230,10 +223,11 @@ __device__ __forceinline__ void units_wait(int left) {
   });
 }
 
-template <int DT, int MT, int NT, int D>
+// EIGHT: at most eight tokens, whose rows alone are loaded; the other columns are dropped.
+template <int DT, int MT, int NT, int D, bool EIGHT>
 __device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* ring, int k, int first,
                                              int stride, int turn, f32x4_t (&acc)[MT][NT]) {
-  constexpr int kTiles = MT + NT, kSlot = kTiles * kTileBytes;
+  constexpr int kTiles = MT + NT, kSlot = kTiles * kTileBytes, kLoads = 2 * kTiles - (EIGHT ? 1 : 0);
   const int whole = k / kPiece;
   turn = whole > 0 ? turn % whole : 0;
   const int n = first < whole ? (whole - first - 1) / stride + 1 : 0;
@@ -243,7 +237,7 @@ __device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* r
     const int at = (u < whole ? u : u - whole) * kPiece * 2;
     static_for<0, kTiles>([&](auto i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < (EIGHT && i.value == MT ? 1 : 2); ++h)
         stage16<(i.value < MT)>(t[i.value].base, ring + slot * kSlot + i.value * kTileBytes + h * 1024,
                                 t[i.value].lane[h], at);
     });
@@ -257,7 +251,7 @@ __device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* r
     if (d < n) fetch(d, d);
   int slot = 0;
   for (int q = 0; q < n; ++q) {
-    units_wait<D, 2 * kTiles>(min(n - 1 - q, D - 1));
+    units_wait<D, kLoads>(min(n - 1 - q, D - 1));
     u32x4_t f[2][kTiles];
     const uint32_t at = at0 + slot * kSlot, at1 = at ^ 64;
     static_for<0, kTiles>([&](auto i) {
@@ -280,37 +274,22 @@ __device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* r
 constexpr int stream_depth(int mt, int nt) { return mt + nt <= 2 ? 4 : mt + nt <= 3 ? 3 : 2; }
 
 // The waves' sums, each wave's own in LDS: outputs 4 q .. + 3 of (tile i, column tile j),
-// column c, over waves and parts. Row r and column c of part p are the instruction's row
-// r P + p and column c P + p.
-template <int P, int MT, int NT, int NW>
+// column c.
+template <int MT, int NT, int NW>
 __device__ __forceinline__ f32x4_t folded(const f32x4_t* red, int i, int j, int q, int c) {
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int w = 0; w < NW; ++w) {
-    const f32x4_t* of = red + ((w * MT + i) * NT + j) * 64;
-    if constexpr (P == 1) {
-      sum += of[q * 16 + c];
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const int row = (4 * q + r) * P + p;
-          sum[r] += reinterpret_cast<const float*>(&of[row / 4 * 16 + c * P + p])[row % 4];
-        }
-    }
-  }
+  for (int w = 0; w < NW; ++w) sum += red[((w * MT + i) * NT + j) * 64 + q * 16 + c];
   return sum;
 }
 
-template <int DT, int MODE, bool GATED, int P, int MT, int NT, int NW>
-__global__ __launch_bounds__(64 * NW, P == 1 ? 2 : 4) void stream_kernel(const StreamArgs s) {
-  static_assert((P == 1 || NT == 1) && (!GATED || MT % 2 == 0), "tiles");
+template <int DT, int MODE, bool GATED, int MT, int NT, int NW, bool EIGHT>
+__global__ __launch_bounds__(64 * NW, 2) void stream_kernel(const StreamArgs s) {
+  static_assert((!EIGHT || NT == 1) && (!GATED || MT % 2 == 0), "tiles");
   constexpr int kDepth = stream_depth(MT, NT);
-  constexpr int R = 16 / P;                        // rows of a tile, columns of a column tile
-  constexpr int kOut = (GATED ? MT / 2 : MT) * R;  // outputs of a workgroup
-  // The rings of P = 1 and, behind the last unit, the waves' sums.
-  __shared__ f32x4_t red[NW * (P == 1 ? kDepth * (MT + NT) * kTileBytes / 16 : MT * NT * 64)];
+  constexpr int kOut = (GATED ? MT / 2 : MT) * 16;  // outputs of a workgroup
+  // The rings and, behind the last unit, the waves' sums.
+  __shared__ f32x4_t red[NW * kDepth * (MT + NT) * kTileBytes / 16];
   __shared__ int32_t list[MODE == kLinear ? 1 : kMostSlots];
   const Args& a = s.g;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -327,64 +306,58 @@ __global__ __launch_bounds__(64 * NW, P == 1 ? 2 : 4) void stream_kernel(const S
     return MODE == kGateUp ? list[c] / a.top_k : MODE == kDown ? list[c] : c;
   };
   const uint32_t x_st = static_cast<uint32_t>(a.x_st);
-  const int turn = 5 * blockIdx.x + 11 * expert;
-  const int m = lane & 15, in = lane_input<P>(lane);
-  Rows w[MT];
+  const int whole = a.k / kPiece;
+  constexpr int kStep = EIGHT ? 8 : 16 * NT;
+  for (int first = 0; first < count; first += kStep) {
+    Staged t[MT + NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) w[i] = weight_rows<GATED, R>(a, expert, n0, i, m / P, in);
-  for (int first = 0; first < count; first += R * NT) {
-    Rows x[NT];
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * h + (lane >> 3), at = staged_input(lane, h);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = rows_at(a.x, source(first + j * 16 + m / P) * x_st + in);
-    f32x4_t acc[MT][NT] = {};
-    if constexpr (P == 1) {
-      Staged t[MT + NT];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 8 * h + (lane >> 3), at = staged_input(lane, h);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const Rows row = weight_rows<GATED, R>(a, expert, n0, i, r, at);
-          t[i].base = row.base, t[i].lane[h] = row.lane;
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          t[MT + j].base = x[j].base;
-          t[MT + j].lane[h] = 2u * (source(first + j * 16 + r) * x_st + at);
-        }
+      for (int i = 0; i < MT; ++i) {
+        const Rows row = weight_rows<GATED, 16>(a, expert, n0, i, r, at);
+        t[i].base = row.base, t[i].lane[h] = row.lane;
       }
-      if (MODE != kLinear && first > 0) __syncthreads();  // the sums in the rings were read
-      char* ring = reinterpret_cast<char*>(red) + wave * (kDepth * (MT + NT) * kTileBytes);
-      staged_units<DT, MT, NT, kDepth>(t, ring, a.k, wave, NW, turn, acc);
-      const int whole = a.k / kPiece;
-      if (whole * kPiece < a.k && whole % NW == wave)
-        stream_tail<DT, P, MT, NT>(w, x, a.k, whole * kPiece, acc);
-      __syncthreads();  // every wave is done with its ring
-    } else {
-      stream_units<DT, P, MT, NT>(w, x, a.k, wave, NW, turn, acc);
-      if (MODE != kLinear && first > 0) __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const Rows row = rows_at(a.x, source(first + j * 16 + r) * x_st + at);
+        t[MT + j].base = row.base, t[MT + j].lane[h] = row.lane;
+      }
     }
+    if (MODE != kLinear && first > 0) __syncthreads();  // the sums in the rings were read
+    char* ring = reinterpret_cast<char*>(red) + wave * (kDepth * (MT + NT) * kTileBytes);
+    f32x4_t acc[MT][NT] = {};
+    staged_units<DT, MT, NT, kDepth, EIGHT>(t, ring, a.k, wave, NW, 5 * blockIdx.x + 11 * expert, acc);
+    if (whole * kPiece < a.k && whole % NW == wave) {  // the last unit is a part of one
+      const int r = lane & 15, in = lane_input<1>(lane);
+      Rows w[MT], x[NT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) w[i] = weight_rows<GATED, 16>(a, expert, n0, i, r, in);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) x[j] = rows_at(a.x, source(first + j * 16 + r) * x_st + in);
+      stream_tail<DT, 1, MT, NT>(w, x, a.k, whole * kPiece, acc);
+    }
+    __syncthreads();  // every wave is done with its ring
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) red[((wave * MT + i) * NT + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    constexpr int kUnits = kOut / 4 * R * NT;
+    constexpr int kUnits = kOut * 4 * NT;
     for (int unit = tid; unit < kUnits; unit += 64 * NW) {
-      const int c = unit % R, q = unit / R % (R / 4), rest = unit / R / (R / 4);
-      const int j = rest % NT, i = rest / NT;
+      const int c = unit % 16, q = unit / 16 % 4, j = unit / 64 % NT, i = unit / 64 / NT;
       const int col = first + j * 16 + c;
-      if (col >= count) continue;
-      const int n = n0 + i * R + 4 * q;
+      if (col >= count || c >= kStep) continue;
+      const int n = n0 + i * 16 + 4 * q;
       float scale = 1.f;
       int64_t row = col;
       if constexpr (MODE != kLinear) row = list[col];
       if constexpr (MODE == kDown) scale = a.scale[row];
-      if constexpr (GATED)
-        finish4<DT, MODE, true>(a, n, row, scale, folded<P, MT, NT, NW>(red, 2 * i, j, q, c),
-                                folded<P, MT, NT, NW>(red, 2 * i + 1, j, q, c));
-      else {
-        const f32x4_t y = folded<P, MT, NT, NW>(red, i, j, q, c);
+      if constexpr (GATED) {
+        finish4<DT, MODE, true>(a, n, row, scale, folded<MT, NT, NW>(red, 2 * i, j, q, c),
+                                folded<MT, NT, NW>(red, 2 * i + 1, j, q, c));
+      } else {
+        const f32x4_t y = folded<MT, NT, NW>(red, i, j, q, c);
         finish4<DT, MODE, false>(a, n, row, scale, y, y);
       }
     }
@@ -393,7 +366,13 @@ __global__ __launch_bounds__(64 * NW, P == 1 ? 2 : 4) void stream_kernel(const S
 
 // The down projections of at most four tokens with their weighted sum: the waves share out
 // (expert, part of its inputs), each adds its weighted sums, and the fold is the token's
-// output. kOut = 4 MT outputs a workgroup.
+// output, 4 MT of them a workgroup.
+//
+// The instruction's rows and columns stand for 4 rows and tokens times 4 parts of 128 inputs:
+// row and column blocks of the same part meet on the diagonal, whose blocks are summed, and
+// what is off it is dropped. Neighbouring lanes then hold neighbouring inputs of a row, so
+// operands come straight into registers, and a workgroup has few outputs, so that all CUs
+// have one (hidden 2,048: 256 workgroups of 8).
 constexpr int kFewTokens = 4;
 constexpr int kFewSlots = 128;
 
@@ -468,48 +447,62 @@ __global__ __launch_bounds__(64 * NW) void down_few_kernel(const StreamArgs s, c
     if (col < s.g.tokens) {
       Args o = a;
       o.res = res, o.r_st = r_st, o.act = SGL_ACT_NONE;
-      const f32x4_t y = folded<P, MT, 1, NW>(red, i, 0, 0, col);
+      // Row r and column c of part p are the instruction's row 4 r + p and column 4 c + p.
+      f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+      for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+            y[r] += reinterpret_cast<const float*>(&red[(w * MT + i) * 64 + r * 16 + col * P + p])[p];
       finish4<DT, kLinear, false>(o, n0 + i * R, col, 1.f, y, y);
     }
   }
 }
 
-template <int DT, int MODE, bool GATED, int P, int MT, int NT, int NW>
+template <int DT, int MODE, bool GATED, int MT, int NT, int NW, bool EIGHT>
 void launch_stream_as(const StreamArgs& s, int rows, hipStream_t st) {
-  constexpr int kOut = (GATED ? MT / 2 : MT) * 16 / P;
+  constexpr int kOut = (GATED ? MT / 2 : MT) * 16;
   const dim3 grid((s.g.n + kOut - 1) / kOut, rows);
-  hipLaunchKernelGGL((stream_kernel<DT, MODE, GATED, P, MT, NT, NW>), grid, dim3(64 * NW), 0, st, s);
+  hipLaunchKernelGGL((stream_kernel<DT, MODE, GATED, MT, NT, NW, EIGHT>), grid, dim3(64 * NW), 0, st, s);
 }
 
-// Half of the tiles a workgroup where MT would leave CUs without one; as many waves as fill
-// the CUs.
-template <int DT, int MODE, bool GATED, int P, int MT, int NT>
+// Weight tiles of a workgroup: one where that leaves every CU at most one workgroup (4,096
+// outputs of one token 7.6 us, with two tiles 8.9; 6,144: 12.2 and 10.2), two otherwise.
+inline int stream_tiles(bool gated, int64_t n, int rows) {
+  return gated || (n + 15) / 16 * rows > kCus ? 2 : 1;
+}
+
+// Eight waves a workgroup, four where CUs have two workgroups (24,576 rows: 33.5 us, 36.1 with
+// eight).
+template <int DT, int MODE, bool GATED, int NT, bool EIGHT>
 void launch_stream_at(const StreamArgs& s, int rows, hipStream_t st) {
-  constexpr int kOut = (GATED ? MT / 2 : MT) * 16 / P;
-  constexpr int kLess = (GATED ? MT > 2 : MT > 1) ? MT / 2 : MT;
-  const int64_t groups = static_cast<int64_t>((s.g.n + kOut - 1) / kOut) * rows;
-  if (groups >= (P == 1 ? 512 : 1024)) launch_stream_as<DT, MODE, GATED, P, MT, NT, 4>(s, rows, st);
-  else if (groups >= 256) launch_stream_as<DT, MODE, GATED, P, MT, NT, 8>(s, rows, st);
-  else launch_stream_as<DT, MODE, GATED, P, kLess, NT, 8>(s, rows, st);
+  constexpr int kTwo = GATED ? 16 : 32;
+  const int64_t groups = static_cast<int64_t>((s.g.n + kTwo - 1) / kTwo) * rows;
+  if constexpr (!GATED) {
+    if (stream_tiles(false, s.g.n, rows) == 1) return launch_stream_as<DT, MODE, GATED, 1, NT, 8, EIGHT>(s, rows, st);
+  }
+  if constexpr (NT <= 2) {
+    if (groups <= kCus) return launch_stream_as<DT, MODE, GATED, 2, NT, 8, EIGHT>(s, rows, st);
+  }
+  if constexpr (NT <= 3) launch_stream_as<DT, MODE, GATED, 2, NT, 4, EIGHT>(s, rows, st);
 }
 
 // Tokens of a call that these kernels take at most: the rings of a workgroup's waves fill
 // the LDS.
-template <bool GATED>
-constexpr int stream_tokens() { return GATED ? 48 : 64; }
+inline int stream_tokens(bool gated, int64_t n) { return stream_tiles(gated, n, 1) == 2 ? 48 : 64; }
 
 // columns: tokens of the call, or the most places an expert is expected to have. rows:
 // the grid's second extent.
 template <int DT, int MODE, bool GATED>
 int launch_stream(const StreamArgs& s, int columns, int rows, hipStream_t st) {
-  if (columns <= 4) launch_stream_at<DT, MODE, GATED, 4, 4, 1>(s, rows, st);
-  else if (columns <= 8) launch_stream_at<DT, MODE, GATED, 2, 4, 1>(s, rows, st);
-  else if (columns <= 16) launch_stream_at<DT, MODE, GATED, 1, 2, 1>(s, rows, st);
-  else if (columns <= 32 || MODE != kLinear) launch_stream_at<DT, MODE, GATED, 1, 2, 2>(s, rows, st);
+  if (columns <= 8) launch_stream_at<DT, MODE, GATED, 1, true>(s, rows, st);
+  else if (columns <= 16) launch_stream_at<DT, MODE, GATED, 1, false>(s, rows, st);
+  else if (columns <= 32 || MODE != kLinear) launch_stream_at<DT, MODE, GATED, 2, false>(s, rows, st);
   else if constexpr (MODE == kLinear) {
-    constexpr int kTiles = GATED ? 2 : 1;
-    if (columns <= 48) launch_stream_as<DT, MODE, GATED, 1, kTiles, 3, 8>(s, rows, st);
-    else if constexpr (!GATED) launch_stream_as<DT, MODE, GATED, 1, 1, 4, 8>(s, rows, st);
+    if (columns <= 48) launch_stream_at<DT, MODE, GATED, 3, false>(s, rows, st);
+    else if constexpr (!GATED) launch_stream_at<DT, MODE, GATED, 4, false>(s, rows, st);
   }
   return launch_status();
 }
