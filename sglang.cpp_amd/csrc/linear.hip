@@ -81,8 +81,8 @@ int run(const gemm::Args& a, bool vec, void* workspace, hipStream_t s) {
   if (fast && streams(a.tokens, a.n, a.k, a.act, workspace != nullptr)) {
     gemm::StreamArgs st{};
     st.g = a;
-    return gated(a.act) ? gemm::launch_stream<DT, gemm::kLinear, true>(st, a.tokens, 1, s)
-                        : gemm::launch_stream<DT, gemm::kLinear, false>(st, a.tokens, 1, s);
+    return gated(a.act) ? gemm::launch_stream<DT, true>(st, s)
+                        : gemm::launch_stream<DT, false>(st, s);
   }
   if (fast) return gated(a.act) ? run_tiles<DT, true>(a, workspace, s) : run_tiles<DT, false>(a, workspace, s);
   const int64_t tiles_t = (static_cast<int64_t>(a.tokens) + gemm::kAnyTile - 1) / gemm::kAnyTile;

@@ -264,7 +264,10 @@ bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) {
 
 constexpr int64_t kMost = 0x7fffff00;
 constexpr int kTileRows = gemm::kAnyTile;
-constexpr int64_t kFewRows = 64;  // tokens of the kernels that stream the weights at most
+// Slots an expert has on average at most where the weights are streamed: 16 at a time, more
+// take another pass (128 experts of 2,048 x 768, 8 a token: 96 tokens 215 us, tiles 234; 128
+// tokens 229 and 229).
+constexpr int64_t kFewPlaces = 7;
 
 // The workspace: slots in order, tiles, the rows between the projections and the
 // weighted outputs. Rows are padded to whole 16 bytes.
@@ -315,12 +318,8 @@ int run_few(const sgl_moe_t& x, const Layout& l, gemm::Args up, gemm::Args down,
   st.experts = x.experts, st.slots = slots, st.num_experts = x.num_experts;
   st.by_slot = slots < x.num_experts;
   const int rows = st.by_slot ? slots : x.num_experts;
-  // Columns an expert is expected to need: three times its share of the slots; more take
-  // another pass over its weights.
-  const int share = 3 * slots / x.num_experts;
-  const int columns = std::min(tokens, std::max(share, 16));
   st.g = up;
-  int status = gemm::launch_stream<DT, gemm::kGateUp, true>(st, columns, rows, s);
+  int status = gemm::launch_experts<DT, gemm::kGateUp, true>(st, rows, s);
   if (status != SGL_OK) return status;
   st.g = down;
   if (tokens <= gemm::kFewTokens && slots <= gemm::kFewSlots) {
@@ -332,7 +331,7 @@ int run_few(const sgl_moe_t& x, const Layout& l, gemm::Args up, gemm::Args down,
                        0, s, st, static_cast<const uint16_t*>(x.residual), x.residual_stride_row);
     return launch_status();
   }
-  status = gemm::launch_stream<DT, gemm::kDown, false>(st, columns, rows, s);
+  status = gemm::launch_experts<DT, gemm::kDown, false>(st, rows, s);
   if (status != SGL_OK) return status;
   return combine<DT, SGL_DTYPE_F32>(x, l, down.out, s);
 }
@@ -361,7 +360,7 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   down.tokens = slots, down.n = x.hidden, down.k = x.intermediate;
   const bool down_vec = x.intermediate % 8 == 0 && aligned(x.down, x.down_stride_row, 16, 2) &&
                         x.down_stride_expert % 8 == 0;
-  if (up_vec && down_vec && slots <= gemm::kMostSlots && x.tokens <= kFewRows &&
+  if (up_vec && down_vec && slots <= gemm::kMostSlots && slots <= kFewPlaces * x.num_experts &&
       std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride)
     return run_few<DT>(x, l, up, down, s);
 

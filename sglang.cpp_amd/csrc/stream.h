@@ -223,11 +223,10 @@ __device__ __forceinline__ void units_wait(int left) {
   });
 }
 
-// EIGHT: at most eight tokens, whose rows alone are loaded; the other columns are dropped.
-template <int DT, int MT, int NT, int D, bool EIGHT>
+template <int DT, int MT, int NT, int D>
 __device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* ring, int k, int first,
                                              int stride, int turn, f32x4_t (&acc)[MT][NT]) {
-  constexpr int kTiles = MT + NT, kSlot = kTiles * kTileBytes, kLoads = 2 * kTiles - (EIGHT ? 1 : 0);
+  constexpr int kTiles = MT + NT, kSlot = kTiles * kTileBytes, kLoads = 2 * kTiles;
   const int whole = k / kPiece;
   turn = whole > 0 ? turn % whole : 0;
   const int n = first < whole ? (whole - first - 1) / stride + 1 : 0;
@@ -237,7 +236,7 @@ __device__ __forceinline__ void staged_units(const Staged (&t)[MT + NT], char* r
     const int at = (u < whole ? u : u - whole) * kPiece * 2;
     static_for<0, kTiles>([&](auto i) {
 #pragma unroll
-      for (int h = 0; h < (EIGHT && i.value == MT ? 1 : 2); ++h)
+      for (int h = 0; h < 2; ++h)
         stage16<(i.value < MT)>(t[i.value].base, ring + slot * kSlot + i.value * kTileBytes + h * 1024,
                                 t[i.value].lane[h], at);
     });
@@ -283,9 +282,9 @@ __device__ __forceinline__ f32x4_t folded(const f32x4_t* red, int i, int j, int 
   return sum;
 }
 
-template <int DT, int MODE, bool GATED, int MT, int NT, int NW, bool EIGHT>
+template <int DT, int MODE, bool GATED, int MT, int NT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void stream_kernel(const StreamArgs s) {
-  static_assert((!EIGHT || NT == 1) && (!GATED || MT % 2 == 0), "tiles");
+  static_assert(!GATED || MT % 2 == 0, "gate and up rows");
   constexpr int kDepth = stream_depth(MT, NT);
   constexpr int kOut = (GATED ? MT / 2 : MT) * 16;  // outputs of a workgroup
   // The rings and, behind the last unit, the waves' sums.
@@ -307,8 +306,7 @@ __global__ __launch_bounds__(64 * NW, 2) void stream_kernel(const StreamArgs s) 
   };
   const uint32_t x_st = static_cast<uint32_t>(a.x_st);
   const int whole = a.k / kPiece;
-  constexpr int kStep = EIGHT ? 8 : 16 * NT;
-  for (int first = 0; first < count; first += kStep) {
+  for (int first = 0; first < count; first += 16 * NT) {
     Staged t[MT + NT];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -327,7 +325,7 @@ __global__ __launch_bounds__(64 * NW, 2) void stream_kernel(const StreamArgs s) 
     if (MODE != kLinear && first > 0) __syncthreads();  // the sums in the rings were read
     char* ring = reinterpret_cast<char*>(red) + wave * (kDepth * (MT + NT) * kTileBytes);
     f32x4_t acc[MT][NT] = {};
-    staged_units<DT, MT, NT, kDepth, EIGHT>(t, ring, a.k, wave, NW, 5 * blockIdx.x + 11 * expert, acc);
+    staged_units<DT, MT, NT, kDepth>(t, ring, a.k, wave, NW, 5 * blockIdx.x + 11 * expert, acc);
     if (whole * kPiece < a.k && whole % NW == wave) {  // the last unit is a part of one
       const int r = lane & 15, in = lane_input<1>(lane);
       Rows w[MT], x[NT];
@@ -347,7 +345,7 @@ __global__ __launch_bounds__(64 * NW, 2) void stream_kernel(const StreamArgs s) 
     for (int unit = tid; unit < kUnits; unit += 64 * NW) {
       const int c = unit % 16, q = unit / 16 % 4, j = unit / 64 % NT, i = unit / 64 / NT;
       const int col = first + j * 16 + c;
-      if (col >= count || c >= kStep) continue;
+      if (col >= count) continue;
       const int n = n0 + i * 16 + 4 * q;
       float scale = 1.f;
       int64_t row = col;
@@ -461,49 +459,51 @@ __global__ __launch_bounds__(64 * NW) void down_few_kernel(const StreamArgs s, c
   }
 }
 
-template <int DT, int MODE, bool GATED, int MT, int NT, int NW, bool EIGHT>
+template <int DT, int MODE, bool GATED, int MT, int NT, int NW>
 void launch_stream_as(const StreamArgs& s, int rows, hipStream_t st) {
   constexpr int kOut = (GATED ? MT / 2 : MT) * 16;
   const dim3 grid((s.g.n + kOut - 1) / kOut, rows);
-  hipLaunchKernelGGL((stream_kernel<DT, MODE, GATED, MT, NT, NW, EIGHT>), grid, dim3(64 * NW), 0, st, s);
+  hipLaunchKernelGGL((stream_kernel<DT, MODE, GATED, MT, NT, NW>), grid, dim3(64 * NW), 0, st, s);
 }
 
 // Weight tiles of a workgroup: one where that leaves every CU at most one workgroup (4,096
-// outputs of one token 7.6 us, with two tiles 8.9; 6,144: 12.2 and 10.2), two otherwise.
+// outputs of one token 7.6 us, with two tiles 8.9; 6,144: 12.3 and 10.3), two otherwise.
 inline int stream_tiles(bool gated, int64_t n, int rows) {
   return gated || (n + 15) / 16 * rows > kCus ? 2 : 1;
-}
-
-// Eight waves a workgroup, four where CUs have two workgroups (24,576 rows: 33.5 us, 36.1 with
-// eight).
-template <int DT, int MODE, bool GATED, int NT, bool EIGHT>
-void launch_stream_at(const StreamArgs& s, int rows, hipStream_t st) {
-  constexpr int kTwo = GATED ? 16 : 32;
-  const int64_t groups = static_cast<int64_t>((s.g.n + kTwo - 1) / kTwo) * rows;
-  if constexpr (!GATED) {
-    if (stream_tiles(false, s.g.n, rows) == 1) return launch_stream_as<DT, MODE, GATED, 1, NT, 8, EIGHT>(s, rows, st);
-  }
-  if constexpr (NT <= 2) {
-    if (groups <= kCus) return launch_stream_as<DT, MODE, GATED, 2, NT, 8, EIGHT>(s, rows, st);
-  }
-  if constexpr (NT <= 3) launch_stream_as<DT, MODE, GATED, 2, NT, 4, EIGHT>(s, rows, st);
 }
 
 // Tokens of a call that these kernels take at most: the rings of a workgroup's waves fill
 // the LDS.
 inline int stream_tokens(bool gated, int64_t n) { return stream_tiles(gated, n, 1) == 2 ? 48 : 64; }
 
-// columns: tokens of the call, or the most places an expert is expected to have. rows:
-// the grid's second extent.
-template <int DT, int MODE, bool GATED>
-int launch_stream(const StreamArgs& s, int columns, int rows, hipStream_t st) {
-  if (columns <= 8) launch_stream_at<DT, MODE, GATED, 1, true>(s, rows, st);
-  else if (columns <= 16) launch_stream_at<DT, MODE, GATED, 1, false>(s, rows, st);
-  else if (columns <= 32 || MODE != kLinear) launch_stream_at<DT, MODE, GATED, 2, false>(s, rows, st);
-  else if constexpr (MODE == kLinear) {
-    if (columns <= 48) launch_stream_at<DT, MODE, GATED, 3, false>(s, rows, st);
-    else if constexpr (!GATED) launch_stream_at<DT, MODE, GATED, 4, false>(s, rows, st);
+// A projection of up to stream_tokens: eight waves a workgroup, four where CUs have two
+// workgroups (24,576 rows: 33.5 us, 36.1 with eight).
+template <int DT, bool GATED, int NT>
+void launch_stream_at(const StreamArgs& s, hipStream_t st) {
+  constexpr int kTwo = GATED ? 16 : 32;
+  if constexpr (!GATED) {
+    if (stream_tiles(false, s.g.n, 1) == 1) return launch_stream_as<DT, kLinear, GATED, 1, NT, 8>(s, 1, st);
   }
+  if constexpr (NT <= 2) {
+    if ((s.g.n + kTwo - 1) / kTwo <= kCus) return launch_stream_as<DT, kLinear, GATED, 2, NT, 8>(s, 1, st);
+  }
+  if constexpr (NT <= 3) launch_stream_as<DT, kLinear, GATED, 2, NT, 4>(s, 1, st);
+}
+template <int DT, bool GATED>
+int launch_stream(const StreamArgs& s, hipStream_t st) {
+  if (s.g.tokens <= 16) launch_stream_at<DT, GATED, 1>(s, st);
+  else if (s.g.tokens <= 32) launch_stream_at<DT, GATED, 2>(s, st);
+  else if (s.g.tokens <= 48) launch_stream_at<DT, GATED, 3>(s, st);
+  else if constexpr (!GATED) launch_stream_at<DT, GATED, 4>(s, st);
+  return launch_status();
+}
+
+// A projection of the experts, `rows` of them or slots: workgroups of two waves, several of
+// which a CU holds while others look for their slots (64 tokens x 8 of 128 experts of 2,048 x
+// 768: 68 us, 82 with four waves).
+template <int DT, int MODE, bool GATED>
+int launch_experts(const StreamArgs& s, int rows, hipStream_t st) {
+  launch_stream_as<DT, MODE, GATED, 2, 1, 2>(s, rows, st);
   return launch_status();
 }
 
