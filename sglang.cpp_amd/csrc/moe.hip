@@ -194,7 +194,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
 }
 
 struct CombineArgs {
-  const void* y;  // [slots, stride] weighted outputs of the slots
+  const void* y;      // [slots, stride] weighted outputs of the slots
+  const float* unit;  // of each 64 of them where they are fp16, [slots, units]
+  int32_t units;
   const int32_t* experts;
   const uint16_t* res;
   uint16_t* out;
@@ -203,8 +205,8 @@ struct CombineArgs {
 };
 
 // out[t] = the sum of its slots in their order (+ residual); slots of no expert are skipped.
-// Eight outputs a thread, eight slots' loads in flight. YT: type of y (16 bits or fp32).
-template <int DT, int YT>
+// Eight outputs a thread, eight slots' loads in flight. SCALED: y is fp16 in units, else fp32.
+template <int DT, bool SCALED>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   constexpr int kAhead = 8;
   const int64_t t = blockIdx.x;
@@ -213,28 +215,33 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   const int32_t* ids = a.experts + t * a.top_k;
   float sum[8] = {};
   for (int j0 = 0; j0 < a.top_k; j0 += kAhead) {
-    u32x4_t v[kAhead][YT == SGL_DTYPE_F32 ? 2 : 1];
+    u32x4_t v[kAhead][SCALED ? 1 : 2];
+    float unit[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int j = j0 + u;
       const u32x4_t zero = {0, 0, 0, 0};
       const bool in = j < a.top_k && ids[j] >= 0 && ids[j] < a.num_experts;
       const int64_t at = (t * a.top_k + j) * a.y_st + h;
-      if constexpr (YT == SGL_DTYPE_F32) {
+      unit[u] = 1.f;
+      if constexpr (SCALED) {
+        v[u][0] = in ? ldg128_nt<true>(static_cast<const uint16_t*>(a.y) + at) : zero;
+        if (in) unit[u] = a.unit[(t * a.top_k + j) * a.units + h / 64];
+      } else {
         v[u][0] = in ? ldg128_nt<true>(static_cast<const float*>(a.y) + at) : zero;
         v[u][1] = in ? ldg128_nt<true>(static_cast<const float*>(a.y) + at + 4) : zero;
-      } else {
-        v[u][0] = in ? ldg128_nt<true>(static_cast<const uint16_t*>(a.y) + at) : zero;
       }
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       float f[8];
-      if constexpr (YT == SGL_DTYPE_F32) {
+      if constexpr (SCALED) {
+        unpack8_t<SGL_DTYPE_F16>(v[u][0], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= unit[u];
+      } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[u][i / 4][i % 4]);
-      } else {
-        unpack8_t<YT>(v[u][0], f);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += f[i];
@@ -272,7 +279,7 @@ constexpr int64_t kFewPlaces = 7;
 // The workspace: slots in order, tiles, the rows between the projections and the
 // weighted outputs. Rows are padded to whole 16 bytes.
 struct Layout {
-  int64_t num_tiles, h_st, y_st, order, tiles, h, y, bytes;
+  int64_t num_tiles, h_st, y_st, units, order, tiles, h, y, unit, bytes;
 };
 
 Layout layout_of(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) {
@@ -285,7 +292,9 @@ Layout layout_of(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) 
   l.tiles = up(slots * 4, 256);
   l.h = l.tiles + up(l.num_tiles * 16, 256);
   l.y = l.h + up(slots * l.h_st * 2, 256);
-  l.bytes = l.y + up(slots * l.y_st * 4, 256);
+  l.units = up(hidden, 64) / 64;
+  l.unit = l.y + up(slots * std::max(l.y_st * 4, l.units * 128), 256);
+  l.bytes = l.unit + up(slots * l.units * 4, 256);
   return l;
 }
 
@@ -297,22 +306,22 @@ bool sizes_built(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
          inter <= 1 << 20;
 }
 
-template <int DT, int YT>
-int combine(const sgl_moe_t& x, const Layout& l, const void* y, hipStream_t s) {
+template <int DT, bool SCALED>
+int combine(const sgl_moe_t& x, const gemm::Args& down, hipStream_t s) {
   CombineArgs c{};
-  c.y = y, c.y_st = l.y_st, c.experts = x.experts;
+  c.y = down.out, c.y_st = down.o_st, c.unit = down.unit, c.units = down.units, c.experts = x.experts;
   c.res = static_cast<const uint16_t*>(x.residual), c.r_st = x.residual_stride_row;
   c.out = static_cast<uint16_t*>(x.out), c.o_st = x.out_stride_row;
   c.hidden = x.hidden, c.top_k = x.top_k, c.num_experts = x.num_experts;
   c.wide = aligned(x.out, x.out_stride_row, 16, 2) && aligned(x.residual, x.residual_stride_row, 16, 2);
   const dim3 grid(static_cast<uint32_t>(x.tokens), (x.hidden + 2047) / 2048);
-  hipLaunchKernelGGL((combine_kernel<DT, YT>), grid, dim3(256), 0, s, c);
+  hipLaunchKernelGGL((combine_kernel<DT, SCALED>), grid, dim3(256), 0, s, c);
   return launch_status();
 }
 
 // Few slots: the workgroups find their expert's slots themselves, rows of h and y are slots.
 template <int DT>
-int run_few(const sgl_moe_t& x, const Layout& l, gemm::Args up, gemm::Args down, hipStream_t s) {
+int run_few(const sgl_moe_t& x, gemm::Args up, gemm::Args down, hipStream_t s) {
   const int slots = static_cast<int>(x.tokens * x.top_k), tokens = static_cast<int>(x.tokens);
   gemm::StreamArgs st{};
   st.experts = x.experts, st.slots = slots, st.num_experts = x.num_experts;
@@ -333,7 +342,7 @@ int run_few(const sgl_moe_t& x, const Layout& l, gemm::Args up, gemm::Args down,
   }
   status = gemm::launch_experts<DT, gemm::kDown, false>(st, rows, s);
   if (status != SGL_OK) return status;
-  return combine<DT, SGL_DTYPE_F32>(x, l, down.out, s);
+  return combine<DT, false>(x, down, s);
 }
 
 template <int DT>
@@ -362,20 +371,17 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
                         x.down_stride_expert % 8 == 0;
   if (up_vec && down_vec && slots <= gemm::kMostSlots && slots <= kFewPlaces * x.num_experts &&
       std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride)
-    return run_few<DT>(x, l, up, down, s);
-
-  // Many tokens: the slots' weighted outputs are rounded to bf16 before their sum. That is
-  // half of what the sum reads (8,192 tokens x 8 slots x 2,048: 268 MB instead of 537) for
-  // errors of at most half a step of each term, as the rounding of h and of the result. In
-  // fp16 a term could pass 65,504 where the sum does not, so they stay fp32.
-  constexpr bool kRounded = DT == SGL_DTYPE_BF16;
-  if (kRounded) down.out_f32 = 0;
+    return run_few<DT>(x, up, down, s);
 
   const bool fast = up_vec && down_vec && x.tokens * up.x_st < (1ll << 30) &&
                     std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride;
   const int share = slots / x.num_experts;  // places of an expert, on average
   const int rows = !fast ? gemm::kAnyTile : share <= 64 ? 64 : share < 256 ? 128 : 256;
   const int num_tiles = slots / rows + x.num_experts;
+  if (fast) {
+    down.out_f32 = 0, down.o_st = l.units * 64;
+    down.unit = reinterpret_cast<float*>(ws + l.unit), down.units = static_cast<int32_t>(l.units);
+  }
   const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, rows, num_tiles};
   hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
   int st = launch_status();
@@ -392,7 +398,7 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   if (st != SGL_OK) return st;
   st = product(std::integral_constant<int, gemm::kDown>{}, std::false_type{}, down, down_vec);
   if (st != SGL_OK) return st;
-  return kRounded ? combine<DT, DT>(x, l, y, s) : combine<DT, SGL_DTYPE_F32>(x, l, y, s);
+  return fast ? combine<DT, true>(x, down, s) : combine<DT, false>(x, down, s);
 }
 
 }  // namespace

@@ -189,6 +189,29 @@ def test_experts_of_strided_tensors(dev, off, pad):
         assert (flat == 7.0).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_terms_of_any_size(dev, dtype):
+    """Weights and rows far apart in size: a slot's outputs, large or tiny, reach the sum with
+    their own precision, and one that is infinite leaves its neighbours what they are."""
+    for T in (3, 60, 400):
+        x, gu, d, w, ids = make(dev, T, 8, 2, 128, 64, dtype)
+        far = torch.tensor([1e-3, 1.0, 1e3] if dtype == "fp16" else [1e-20, 1.0, 1e20], device=dev)
+        w = (w * far[torch.arange(T, device=dev) % 3][:, None]).contiguous()
+        rows = torch.ones(128, device=dev)
+        rows[::5], rows[1::7] = 2.0 ** -10, 2.0 ** 4
+        d = (d.float() * rows[None, :, None]).to(d.dtype)
+        if dtype == "fp16":
+            w = w.clamp(max=100.0)
+        check_experts((x, gu, d, w, ids))
+        want, bound = ref.experts(x, gu, d, w, ids)
+        d[3, 17] = math.inf
+        got = capi.moe_experts(x, gu, d, w, ids).cpu()
+        ok = torch.ones(T, 128, dtype=torch.bool)
+        ok[(ids == 3).any(1).cpu(), 17] = False
+        assert not torch.isfinite(got[~ok]).any()
+        ref.check(got[ok], want[ok], bound[ok])
+
+
 def test_experts_of_no_tokens(dev):
     a = make(dev, 0, 4, 2, 64, 32)
     assert capi.moe_experts(*a).shape == (0, 64)
