@@ -170,10 +170,11 @@ __device__ __forceinline__ void finish_quarter(const Args& a, const Part& p, int
 // touch 32 bytes of each of 16 rows (8 slots of 8,192 tokens x 2,048 outputs: half of the
 // kernel's time); from LDS every 16 lanes (8, 4) store a token's whole run of outputs.
 // Rows of outputs are in pieces of four, piece c of token t at place c ^ t (mod 16) or c ^
-// (t / 2) (mod 8), so that 16 tokens' pieces are spread over all banks.
+// (t / 2) (mod 8), so that 16 tokens' pieces are spread over all banks. kDown: lane l has the
+// slot and weight of the wave's token l.
 template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT>
 __device__ __forceinline__ void finish_wave(const Args& a, const Part& p, int n0, int wr, int wc, char* lds,
-                                            const f32x4_t (&acc)[2][2][AT][BT]) {
+                                            int32_t slot, float weight, const f32x4_t (&acc)[2][2][AT][BT]) {
   constexpr int kOut = GATED ? AT * 16 : AT * 32, kPieces = kOut / 4;  // of a wave
   constexpr int kTokens = BT * 16, kLanes = kOut / 8, kRows = 64 / kLanes;
   constexpr int kSteps = kTokens / kRows;
@@ -188,8 +189,13 @@ __device__ __forceinline__ void finish_wave(const Args& a, const Part& p, int n0
     int64_t row[kSteps];
     float scale[kSteps];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      row[s] = target_row<MODE>(a, p.first + min(t0 + s * kRows + mine, p.rows - 1), scale[s]);
+    for (int s = 0; s < kSteps; ++s) {
+      row[s] = p.first + t0 + s * kRows + mine, scale[s] = 1.f;
+      if constexpr (MODE == kDown) {
+        const int from = hb.value * kTokens + s * kRows + mine;
+        row[s] = __shfl(slot, from, kWave), scale[s] = __shfl(weight, from, kWave);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < BT; ++j)
 #pragma unroll
@@ -292,6 +298,8 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2)
   };
   const std::integral_constant<int, 0> i0;
   const std::integral_constant<int, 1> i1;
+  int32_t slot_of = 0;
+  if constexpr (MODE == kDown) slot_of = a.order[p.first + min(wc * BT * 32 + lane % (BT * 32), p.rows - 1)];
   if (tail) {
     const int k_at = a.k - tail;
     auto part = [&](const __amdgpu_buffer_rsrc_t& src, uint32_t off, int q, int place) {
@@ -317,6 +325,8 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2)
   phase_barrier();
   if (kPhased && wave >= 4) phase_barrier();
 
+  float weight_of = 0.f;  // on its way while the products are summed
+  if constexpr (MODE == kDown) weight_of = a.scale[slot_of];
   const int r = lane & 15;
   const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
                             (__attribute__((address_space(3))) char*)lds)) +
@@ -415,7 +425,7 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2)
     return;
   }
   phase_barrier();  // every wave is done with the operands
-  finish_wave<DT, MODE, GATED, WR, WC, AT, BT>(a, p, n0, wr, wc, lds, acc);
+  finish_wave<DT, MODE, GATED, WR, WC, AT, BT>(a, p, n0, wr, wc, lds, slot_of, weight_of, acc);
 }
 
 // The sum of a tile's parts, in their order, and what follows it: a workgroup for each
