@@ -49,6 +49,46 @@ def test_sizes_of_many_tokens(dev, T, n, k, dtype):
     run(dev, T, n, k, dtype, "silu_and_mul", bias=True, residual=True)
 
 
+# Sizes that take each tile shape with the inputs whole and in parts, a part of a stage among them.
+@pytest.mark.parametrize("T,n,k,gated", [
+    (4100, 1000, 72, True), (4100, 500, 4104, True), (4100, 500, 9000, False),
+    (4100, 500, 72, True), (400, 2500, 6000, True), (257, 2000, 9000, True),
+    (257, 1000, 2056, True), (130, 500, 1032, True), (70, 64, 1000, False),
+    (130, 500, 2056, True), (130, 500, 4104, True), (70, 64, 2056, False), (70, 64, 4104, False)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_tiles_and_parts(dev, T, n, k, gated, dtype):
+    run(dev, T, n, k, dtype, "gelu_and_mul" if gated else "none", bias=True, residual=True)
+    run(dev, T, n, k, dtype, "silu_and_mul" if gated else "silu", fp32=True)
+
+
+@pytest.mark.parametrize("T", [80, 300, 1100])
+def test_a_call_without_a_workspace(dev, T):
+    """The C entry with no workspace: the inputs in one part, the same sums to rounding."""
+    n, k = 512, 4096
+    x, w, b, r = make(dev, T, n, k)
+    out = torch.empty(T, n, dtype=x.dtype, device=dev)
+    a = capi.LinearArgs(x.data_ptr(), w.data_ptr(), b.data_ptr(), r.data_ptr(), out.data_ptr(), T, n, k,
+                        k, k, n, n, 0, 0, 1, 0)
+    import ctypes
+    assert capi.lib().sgl_linear_workspace_bytes(T, n, k, 1) > 0
+    assert capi.lib().sgl_linear(ctypes.byref(a), None, 0,
+                                 ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    ref.check(out, *ref.linear(x, w, b, "silu", r))
+
+
+@pytest.mark.parametrize("T", [1, 20, 90])
+def test_subnormal_values(dev, T):
+    """fp16 values below its smallest normal one count with their own precision."""
+    x, w, _, _ = make(dev, T, 64, 128, "fp16")
+    x = (x.float() * 2.0 ** -20).half()
+    want, bound = ref.linear(x, w, out_dtype=torch.float32)
+    ref.check(capi.linear(x, w, out_dtype=torch.float32), want, bound)
+    w = (w.float() * 2.0 ** -16).half()
+    x = x.float().mul(2.0 ** 20).half()
+    want, bound = ref.linear(x, w)
+    ref.check(capi.linear(x, w), want, bound)
+
+
 EPILOGUES = list(itertools.product(["none", "silu", "gelu", "silu_and_mul", "gelu_and_mul"],
                                    [False, True], [False, True], [False, True]))
 

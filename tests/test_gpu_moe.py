@@ -156,6 +156,15 @@ def test_all_tokens_at_one_expert(dev, T):
     check_experts((x, gu, d, w, ids))
 
 
+@pytest.mark.parametrize("T", [17, 40, 100])
+def test_one_expert_of_many_for_all_tokens(dev, T):
+    x, gu, d, w, ids = make(dev, T, 64, 2, 136, 64)
+    ids[:, 0], ids[:, 1] = 63, torch.arange(T, device=dev) % 63
+    check_experts((x, gu, d, w, ids))
+    ids[:, 1] = 63
+    check_experts((x, gu, d, w, ids))
+
+
 def test_values_that_are_not_finite_stay_with_their_token(dev):
     for T in (3, 40, 300):
         x, gu, d, w, ids = make(dev, T, 8, 2, 128, 64)
