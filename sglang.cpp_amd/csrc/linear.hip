@@ -20,7 +20,7 @@ constexpr Shape kShapes[] = {
     {64, 128, 2, 0.40, 0.55},   // 512 x 4,096 x 4,096: 28 us, the others 48 and 92
 };
 using gemm::kCus;
-constexpr int kMostSplits = 8;
+using gemm::kMostSplits;
 
 struct Plan {
   int shape, splits;

@@ -140,31 +140,6 @@ __device__ __forceinline__ Tile tile_of(int block, int total, int tiles_n) {
   return {8 * band + in_band % wide, in_band / wide};
 }
 
-// What follows a quarter (second or first half of a wave's weight rows and of its tokens)
-// of a wave's sums.
-template <int DT, int MODE, bool GATED, int AT, int BT>
-__device__ __forceinline__ void finish_quarter(const Args& a, const Part& p, int n0, int wr, int wc, int ha,
-                                               int hb, const f32x4_t (&acc)[AT][BT]) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int j = 0; j < BT; ++j) {
-    const int t = wc * BT * 32 + hb * BT * 16 + j * 16 + (lane & 15);
-    if (t >= p.rows) continue;
-    float scale;
-    const int64_t row = target_row<MODE>(a, p.first + t, scale);
-    const int n = n0 + (wr * AT * 32 + ha * AT * 16) / (GATED ? 2 : 1) + 4 * (lane >> 4);
-    if constexpr (GATED) {
-#pragma unroll
-      for (int i = 0; i < AT; i += 2)
-        finish4<DT, MODE, true>(a, n + i * 8, row, scale, acc[i][j], acc[i + 1][j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < AT; ++i)
-        finish4<DT, MODE, false>(a, n + i * 16, row, scale, acc[i][j], acc[i][j]);
-    }
-  }
-}
-
 // What follows a wave's sums, by way of its own part of LDS, half of its tokens at a time:
 // the matrix instruction leaves four outputs of a token to a lane, stores of which would
 // touch 32 bytes of each of 16 rows (8 slots of 8,192 tokens x 2,048 outputs: half of the
@@ -428,26 +403,40 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2)
   finish_wave<DT, MODE, GATED, WR, WC, AT, BT>(a, p, n0, wr, wc, lds, slot_of, weight_of, acc);
 }
 
-// The sum of a tile's parts, in their order, and what follows it: a workgroup for each
-// quarter of the waves' sums.
+// The sum of a tile's parts, in their order, and what follows it: a workgroup for each piece
+// of a quarter of the waves' sums, so that every part's loads are in flight at once.
+constexpr int kMostSplits = 8;
+
 template <int DT, bool GATED, int WR, int WC, int AT, int BT>
 __global__ __launch_bounds__(64 * WR * WC) void fold_kernel(const Args a) {
   using S = TileShape<WR, WC, AT, BT, 2>;
-  const int total = gridDim.x, block = blockIdx.x, quarter = blockIdx.y;
+  constexpr int kPair = GATED ? 2 : 1, kPieces = AT / kPair * BT;
+  const int total = gridDim.x, block = blockIdx.x, quarter = blockIdx.y / kPieces, piece = blockIdx.y % kPieces;
+  const int i = piece / BT * kPair, j = piece % BT;
   const Tile tile = tile_of(block, total, a.tiles_n);
   const Part p = part_of<kLinear>(a, tile.t, S::kN);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  f32x4_t acc[AT][BT] = {};
-  for (int split = 0; split < a.splits; ++split) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  f32x4_t v[kMostSplits][kPair];
+#pragma unroll
+  for (int split = 0; split < kMostSplits; ++split) {
+    if (split >= a.splits) break;
     const f32x4_t* in = part_at<WR, WC, AT, BT>(a, total, split, block, quarter);
 #pragma unroll
-    for (int i = 0; i < AT; ++i)
-#pragma unroll
-      for (int j = 0; j < BT; ++j)
-        acc[i][j] += __builtin_nontemporal_load(&in[(i * BT + j) * 64 * S::kWaves]);
+    for (int e = 0; e < kPair; ++e)
+      v[split][e] = __builtin_nontemporal_load(&in[((i + e) * BT + j) * 64 * S::kWaves]);
   }
-  finish_quarter<DT, kLinear, GATED, AT, BT>(a, p, tile.n * (GATED ? S::kM / 2 : S::kM), wave % WR, wave / WR,
-                                             quarter / 2, quarter % 2, acc);
+  f32x4_t g = {0.f, 0.f, 0.f, 0.f}, u = g;
+#pragma unroll
+  for (int split = 0; split < kMostSplits; ++split) {
+    if (split >= a.splits) break;
+    g += v[split][0];
+    if constexpr (GATED) u += v[split][1];
+  }
+  const int wr = wave % WR, wc = wave / WR, ha = quarter / 2, hb = quarter % 2;
+  const int t = ((wc * 2 + hb) * BT + j) * 16 + (lane & 15);
+  if (t >= p.rows) return;
+  const int n0 = tile.n * (S::kM / kPair) + ((wr * 2 + ha) * AT + i) * 16 / kPair + 4 * (lane >> 4);
+  finish4<DT, kLinear, GATED>(a, n0, p.first + t, 1.f, g, u);
 }
 
 template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT, int D>
@@ -464,8 +453,8 @@ int launch_tile(Args a, int64_t tiles_t, hipStream_t s) {
     if (a.splits > 1) {
       const int st = launch_status();
       if (st != SGL_OK) return st;
-      hipLaunchKernelGGL((fold_kernel<DT, GATED, WR, WC, AT, BT>), dim3(static_cast<uint32_t>(grid), 4),
-                         dim3(64 * S::kWaves), 0, s, a);
+      hipLaunchKernelGGL((fold_kernel<DT, GATED, WR, WC, AT, BT>), dim3(static_cast<uint32_t>(grid), 4 * BT * (GATED ? AT / 2 : AT)), dim3(64 * S::kWaves), 0,
+                         s, a);
     }
   }
   return launch_status();
