@@ -663,10 +663,11 @@ int sgl_gelu_and_mul(void* out, const void* input, int64_t tokens, int64_t d,
  * fp32 sums and arithmetic, one rounding. x, weight, bias and residual are bf16 or fp16
  * (dtype), out that type or fp32 (out_dtype SGL_DTYPE_F32: logits). bias and residual may
  * be NULL; out may be residual (same type and strides), other overlaps are the caller's
- * error. Any sizes up to 2^31 - 256, strides and alignment; fastest where k is a multiple of 64
- * and rows start on 16 bytes. workspace: sgl_linear_workspace_bytes (0 for most sizes),
- * 16-byte aligned, written before it is read; calls that share one must be
- * stream-ordered. With NULL the launch has fewer workgroups, and sums another order.
+ * error. Any sizes up to 2^31 - 256, strides and alignment; fast where k is a multiple of 8 (best
+ * of 64) and rows start on 16 bytes. workspace: sgl_linear_workspace_bytes (0 where the
+ * inputs are summed in one part; up to 134 MB), 16-byte aligned, written before it is
+ * read; calls that share one must be stream-ordered. With NULL they are summed in one part:
+ * slower, another order of the sum.
  * Replaces: Linear::forward and what the model runs on its output
  *           (src/layers/linear.cc:9-78; activation.cu:15-77).
  */
@@ -697,8 +698,8 @@ int sgl_linear(const sgl_linear_t* args, void* workspace, int64_t workspace_byte
  * experts of the top_k largest logits, largest first, equal ones by their number;
  * weights[t, j] their probabilities in the softmax over all experts, with renormalize
  * divided by their sum. int32 and fp32 [tokens, top_k], contiguous. NaN is ranked below
- * -inf; a row with a NaN, an infinite or no finite logit above -inf has NaN weights. Up
- * to 512 experts and top_k 32.
+ * -inf; a row with a NaN, with +inf or with nothing above -inf has NaN weights. Up to 512
+ * experts, top_k 32, 2^30 tokens.
  * Replaces: the softmax, top-k and renormalisation of the router (src/moe/moe.cc:47-60).
  */
 int sgl_moe_route(const void* logits, int64_t logits_stride_row, int logits_dtype, int64_t tokens,
@@ -711,13 +712,15 @@ int sgl_moe_route(const void* logits, int64_t logits_stride_row, int logits_dtyp
  *   h = T(act(gate_up[e][:I] x[t]) * (gate_up[e][I:] x[t])), I = intermediate,
  * with x, out and residual [tokens, hidden], gate_up [num_experts, 2 I, hidden] and down
  * [num_experts, hidden, I] bf16 or fp16, weights fp32 and experts int32 [tokens, top_k]
- * contiguous. Sums in fp32, over j in its order; h is rounded to the type, as the
- * matrix instructions take it. A slot whose expert is outside [0, num_experts) adds
+ * contiguous. Sums in fp32; h is rounded to the type, as the matrix instructions take it,
+ * and with many tokens the weighted terms are rounded once, to below 2^-11 of the largest
+ * of 64 outputs. A slot whose expert is outside [0, num_experts) adds
  * nothing (padding, experts of another device). An expert may be chosen more than once.
  * activation: SGL_ACT_SILU_AND_MUL or SGL_ACT_GELU_AND_MUL. residual may be NULL, out may
  * be residual (same strides). workspace: sgl_moe_workspace_bytes, 16-byte aligned,
  * written before it is read; calls that share one must be stream-ordered. hidden and
- * intermediate up to 2^20, 65,536 experts.
+ * intermediate up to 2^20, 65,536 experts, 2^30 choices (tokens x top_k). Fast where hidden
+ * and intermediate are multiples of 8 and rows start on 16 bytes.
  * Replaces: the loop over the experts (src/moe/moe.cc:62-98).
  */
 typedef struct {

@@ -67,14 +67,10 @@ __device__ __forceinline__ float activate(int act, float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-z * 1.4426950408889634f));
 }
 
-// Eight elements of a row from element e on, zero from element k on. VEC: rows start on
-// 16 bytes and k is a multiple of 8.
-template <bool VEC>
+// Eight elements of a row from element e on, zero from element k on; a row starts anywhere.
 __device__ __forceinline__ u32x4_t load8(const uint16_t* row, int e, int k) {
   u32x4_t v = {0, 0, 0, 0};
-  if constexpr (VEC) {
-    if (e < k) v = ldg128(row + e);
-  } else if (e + 8 <= k) {
+  if (e + 8 <= k) {
     __builtin_memcpy(&v, row + e, 16);
   } else {
 #pragma unroll
@@ -93,7 +89,7 @@ __device__ __forceinline__ f32x4_t activated4(const Args& a, int n0, f32x4_t g, 
       for (int i = 0; i < 4; ++i) {
         const int n = min(n0 + i, a.n - 1);
         g[i] += to_f32<DT>(a.bias[n]);
-        if constexpr (GATED) u[i] += to_f32<DT>(a.bias[a.n + n]);
+        if constexpr (GATED) u[i] += to_f32<DT>(a.bias[static_cast<int64_t>(a.n) + n]);
       }
     }
   }
@@ -213,7 +209,7 @@ __device__ __forceinline__ void finish4(const Args& a, int n0, int64_t row, floa
     if constexpr (GATED) {
       float z = u[i];
       if constexpr (MODE == kLinear) {
-        if (a.bias) z += to_f32<DT>(a.bias[a.n + n]);
+        if (a.bias) z += to_f32<DT>(a.bias[static_cast<int64_t>(a.n) + n]);
       }
       y *= z;
     }
@@ -268,11 +264,13 @@ __device__ __forceinline__ int64_t weight_row(const Args& a, int n0, int r) {
 }
 
 // Any sizes, strides and alignment: tiles of 64 weight rows x 64 tokens, staged through
-// registers and LDS, four waves of 32 x 32 outputs.
+// registers and LDS, four waves of 32 x 32 outputs. Taken where rows are not whole 16 bytes
+// or strides pass what the other kernels' 32-bit offsets reach (7 x 128 x 2,048: 21 us, the
+// stream kernel 4; 8,192 x 24,576 x 4,096: 4.3 ms, tiles 1.2).
 constexpr int kAnyTile = 64;
 constexpr int kAnyPitch = 40;  // 32 elements and 16 bytes: rows start on different banks
 
-template <int DT, int MODE, bool GATED, bool VEC>
+template <int DT, int MODE, bool GATED>
 __global__ __launch_bounds__(256) void any_kernel(const Args a) {
   __shared__ uint16_t sw[kAnyTile * kAnyPitch], sx[kAnyTile * kAnyPitch];
   const int tn = blockIdx.x % a.tiles_n, tt = blockIdx.x / a.tiles_n;
@@ -289,15 +287,15 @@ __global__ __launch_bounds__(256) void any_kernel(const Args a) {
   f32x4_t acc[2][2] = {};
   const int aw = (wave & 1) * 32 + (lane & 15), ax = (wave >> 1) * 32 + (lane & 15);
   const int ac = (lane >> 4) * 8;
-  u32x4_t vw = wr < 0 ? zero : load8<VEC>(wp, c, a.k);
-  u32x4_t vx = has_x ? load8<VEC>(xp, c, a.k) : zero;
+  u32x4_t vw = wr < 0 ? zero : load8(wp, c, a.k);
+  u32x4_t vx = has_x ? load8(xp, c, a.k) : zero;
   for (int k0 = 0; k0 < a.k; k0 += 32) {
     stg128(&sw[r * kAnyPitch + c], vw);
     stg128(&sx[r * kAnyPitch + c], vx);
     __syncthreads();
     if (k0 + 32 < a.k) {
-      vw = wr < 0 ? zero : load8<VEC>(wp, k0 + 32 + c, a.k);
-      vx = has_x ? load8<VEC>(xp, k0 + 32 + c, a.k) : zero;
+      vw = wr < 0 ? zero : load8(wp, k0 + 32 + c, a.k);
+      vx = has_x ? load8(xp, k0 + 32 + c, a.k) : zero;
     }
     u32x4_t fw[2], fx[2];
 #pragma unroll
@@ -329,20 +327,22 @@ __global__ __launch_bounds__(256) void any_kernel(const Args a) {
   }
 }
 
+inline bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0);
+}
+
 // Workgroups of a launch, or -1 where it has more than a grid.
 inline int64_t grid_of(int64_t tiles_n, int64_t tiles_t) {
   return tiles_t > 0 && tiles_n > 0x7fffffff / tiles_t ? -1 : tiles_n * tiles_t;
 }
 
 template <int DT, int MODE, bool GATED>
-int launch_any(Args a, bool vec, int64_t tiles_t, hipStream_t s) {
+int launch_any(Args a, int64_t tiles_t, hipStream_t s) {
   const int out = GATED ? kAnyTile / 2 : kAnyTile;
   a.tiles_n = static_cast<int32_t>((static_cast<int64_t>(a.n) + out - 1) / out);
   const int64_t grid = grid_of(a.tiles_n, tiles_t);
   if (grid < 0) return SGL_ERR_UNSUPPORTED;
-  const dim3 g(static_cast<uint32_t>(grid)), b(256);
-  if (vec) hipLaunchKernelGGL((any_kernel<DT, MODE, GATED, true>), g, b, 0, s, a);
-  else hipLaunchKernelGGL((any_kernel<DT, MODE, GATED, false>), g, b, 0, s, a);
+  hipLaunchKernelGGL((any_kernel<DT, MODE, GATED>), dim3(static_cast<uint32_t>(grid)), dim3(256), 0, s, a);
   return launch_status();
 }
 

@@ -38,7 +38,7 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t k, int act, bool may_split) {
   for (int i = 0; i < 3; ++i) {
     const Shape& x = kShapes[i];
     const int64_t tiles = ((rows + x.rows - 1) / x.rows) * ((tokens + x.tokens - 1) / x.tokens);
-    for (int s = 1; s <= kMostSplits && (s == 1 || (may_split && tiles <= 2 * kCus && stages >= 4 * s)); ++s) {
+    for (int s = 1; s <= kMostSplits && (s == 1 || (may_split && tiles * s <= 2 * kCus && stages >= 4 * s)); ++s) {
       const int64_t groups = tiles * s, each = (stages + s - 1) / s;
       const int64_t bytes = s > 1 ? groups * x.rows * x.tokens * 4 : 0;
       const int64_t rounds = (groups + kCus * x.per_cu - 1) / (kCus * x.per_cu);
@@ -86,14 +86,11 @@ int run(const gemm::Args& a, bool vec, void* workspace, hipStream_t s) {
   }
   if (fast) return gated(a.act) ? run_tiles<DT, true>(a, workspace, s) : run_tiles<DT, false>(a, workspace, s);
   const int64_t tiles_t = (static_cast<int64_t>(a.tokens) + gemm::kAnyTile - 1) / gemm::kAnyTile;
-  return gated(a.act) ? gemm::launch_any<DT, gemm::kLinear, true>(a, vec, tiles_t, s)
-                      : gemm::launch_any<DT, gemm::kLinear, false>(a, vec, tiles_t, s);
+  return gated(a.act) ? gemm::launch_any<DT, gemm::kLinear, true>(a, tiles_t, s)
+                      : gemm::launch_any<DT, gemm::kLinear, false>(a, tiles_t, s);
 }
 
-bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) {
-  return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0);
-}
-
+using gemm::aligned;
 constexpr int64_t kMost = 0x7fffff00;  // tokens, outputs and inputs: room for a tile below 2^31
 
 }  // namespace
@@ -129,22 +126,24 @@ extern "C" int sgl_linear(const sgl_linear_t* args, void* workspace, int64_t wor
   if (workspace && workspace_bytes < need) return SGL_ERR_CAPACITY;
   if (workspace && !aligned16(workspace)) return SGL_ERR_ALIGNMENT;
   gemm::Args a{};
-  a.x = static_cast<const uint16_t*>(x.x), a.x_st = x.x_stride_row;
+  // A single row's stride is nothing that alignment depends on.
+  const bool one = x.tokens == 1;
+  a.x = static_cast<const uint16_t*>(x.x), a.x_st = one ? 0 : x.x_stride_row;
   a.w = static_cast<const uint16_t*>(x.weight), a.w_st = x.weight_stride_row;
   a.bias = static_cast<const uint16_t*>(x.bias);
-  a.res = static_cast<const uint16_t*>(x.residual), a.r_st = x.residual_stride_row;
-  a.out = x.out, a.o_st = x.out_stride_row;
+  a.res = static_cast<const uint16_t*>(x.residual), a.r_st = one ? 0 : x.residual_stride_row;
+  a.out = x.out, a.o_st = one ? 0 : x.out_stride_row;
   a.tokens = static_cast<int32_t>(x.tokens), a.n = static_cast<int32_t>(x.n);
   a.k = static_cast<int32_t>(x.k), a.act = x.activation;
   a.out_f32 = x.out_dtype == SGL_DTYPE_F32;
   const int64_t size = a.out_f32 ? 4 : 2;
   const int64_t rows = gated(x.activation) ? x.n : 0;
   const auto wide = [&](int64_t columns) {
-    return aligned(x.out, x.out_stride_row, std::min<int64_t>(16, columns * size), size) &&
-           aligned(x.residual, x.residual_stride_row, 2 * columns, 2) && aligned(x.bias, rows, 8, 2);
+    return aligned(x.out, a.o_st, std::min<int64_t>(16, columns * size), size) &&
+           aligned(x.residual, a.r_st, 2 * columns, 2) && aligned(x.bias, rows, 8, 2);
   };
   a.wide = wide(8) ? 2 : wide(4) ? 1 : 0;
-  const bool vec = x.k % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
+  const bool vec = x.k % 8 == 0 && aligned(x.x, a.x_st, 16, 2) &&
                    aligned(x.weight, x.weight_stride_row, 16, 2);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return x.dtype == SGL_DTYPE_BF16 ? run<SGL_DTYPE_BF16>(a, vec, workspace, s)

@@ -265,11 +265,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   }
 }
 
-bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) {
-  return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0);
-}
+using gemm::aligned;
 
-constexpr int64_t kMost = 0x7fffff00;
+constexpr int64_t kMost = 1 << 30;  // choices: a workgroup's share of them stays an int
 constexpr int kTileRows = gemm::kAnyTile;
 // Slots an expert has on average at most where the weights are streamed: 16 at a time, more
 // take another pass (128 experts of 2,048 x 768, 8 a token: 96 tokens 215 us, tiles 234; 128
@@ -355,20 +353,21 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   gemm::Args up{};
   up.tiles = tiles, up.order = order, up.top_k = x.top_k, up.scale = x.weights;
   gemm::Args down = up;
-  up.x = static_cast<const uint16_t*>(x.x), up.x_st = x.x_stride_row;
+  up.x = static_cast<const uint16_t*>(x.x), up.x_st = x.tokens == 1 ? 0 : x.x_stride_row;
   up.w = static_cast<const uint16_t*>(x.gate_up);
   up.w_st = x.gate_up_stride_row, up.w_se = x.gate_up_stride_expert;
   up.out = h, up.o_st = l.h_st, up.wide = 2;
   up.tokens = slots, up.n = x.intermediate, up.k = x.hidden, up.act = x.activation;
-  const bool up_vec = x.hidden % 8 == 0 && aligned(x.x, x.x_stride_row, 16, 2) &&
-                      aligned(x.gate_up, x.gate_up_stride_row, 16, 2) && x.gate_up_stride_expert % 8 == 0;
+  const bool up_vec = x.hidden % 8 == 0 && aligned(x.x, up.x_st, 16, 2) &&
+                      aligned(x.gate_up, x.gate_up_stride_row, 16, 2) &&
+                      (x.num_experts == 1 || x.gate_up_stride_expert % 8 == 0);
   down.x = h, down.x_st = l.h_st;
   down.w = static_cast<const uint16_t*>(x.down);
   down.w_st = x.down_stride_row, down.w_se = x.down_stride_expert;
   down.out = y, down.o_st = l.y_st, down.out_f32 = 1, down.wide = 2;
   down.tokens = slots, down.n = x.hidden, down.k = x.intermediate;
   const bool down_vec = x.intermediate % 8 == 0 && aligned(x.down, x.down_stride_row, 16, 2) &&
-                        x.down_stride_expert % 8 == 0;
+                        (x.num_experts == 1 || x.down_stride_expert % 8 == 0);
   if (up_vec && down_vec && slots <= gemm::kMostSlots && slots <= kFewPlaces * x.num_experts &&
       std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride)
     return run_few<DT>(x, up, down, s);
@@ -386,17 +385,17 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
   int st = launch_status();
   if (st != SGL_OK) return st;
-  const auto product = [&](auto mode, auto gate, const gemm::Args& a, bool vec) {
+  const auto product = [&](auto mode, auto gate, const gemm::Args& a) {
     constexpr int kMode = decltype(mode)::value;
     constexpr bool kGated = decltype(gate)::value;
-    if (!fast) return gemm::launch_any<DT, kMode, kGated>(a, vec, num_tiles, s);
+    if (!fast) return gemm::launch_any<DT, kMode, kGated>(a, num_tiles, s);
     if (rows == 64) return gemm::launch_tile<DT, kMode, kGated, 2, 2, 2, 1, 3>(a, num_tiles, s);
     if (rows == 128) return gemm::launch_tile<DT, kMode, kGated, 2, 2, 2, 2, 2>(a, num_tiles, s);
     return gemm::launch_tile<DT, kMode, kGated, 2, 4, 4, 2, 2>(a, num_tiles, s);
   };
-  st = product(std::integral_constant<int, gemm::kGateUp>{}, std::true_type{}, up, up_vec);
+  st = product(std::integral_constant<int, gemm::kGateUp>{}, std::true_type{}, up);
   if (st != SGL_OK) return st;
-  st = product(std::integral_constant<int, gemm::kDown>{}, std::false_type{}, down, down_vec);
+  st = product(std::integral_constant<int, gemm::kDown>{}, std::false_type{}, down);
   if (st != SGL_OK) return st;
   return fast ? combine<DT, true>(x, down, s) : combine<DT, false>(x, down, s);
 }

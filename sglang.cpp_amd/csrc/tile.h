@@ -204,11 +204,11 @@ __device__ __forceinline__ f32x4_t* part_at(const Args& a, int tiles, int split,
 }
 
 template <int DT, int MODE, bool GATED, int WR, int WC, int AT, int BT, int D>
-__global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2) void tile_kernel(const Args a) {
+__global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
   using S = TileShape<WR, WC, AT, BT, D>;
   constexpr int LA = S::kLoadA, LB = S::kLoadB;
   constexpr bool kPhased = S::kWaves == 8;
-  static_assert(LA <= 4 && LB <= 4, "a wave's loads of gate or up rows");
+  static_assert(LA <= 2, "a wave's loads are of gate rows or of up rows");
   __shared__ __attribute__((aligned(1024))) char lds[S::kBytes];
   // Parts of k: all tiles of the first one, then of the next.
   const int total = static_cast<int>(gridDim.x) / a.splits;
@@ -235,14 +235,14 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2)
       const int q = wave * LA + u, r = 8 * q + (lane >> 3);
       const int row = r / (AT * 16) * (AT * 32) + h * (AT * 16) + r % (AT * 16);  // of the tile
       const int n = GATED ? (row >> 5) * 16 + (row & 15) : row;
-      const int c = ((lane & 7) ^ ((4 * q + (lane >> 4)) & 7)) * 8;
+      const int c = staged_input(lane, q);
       wo[h][u] = 2u * (static_cast<uint32_t>(min(n, a.n - 1 - first_n)) * static_cast<uint32_t>(a.w_st) + c);
     }
 #pragma unroll
     for (int u = 0; u < LB; ++u) {
       const int q = wave * LB + u, r = 8 * q + (lane >> 3);
       const int row = min(r / (BT * 16) * (BT * 32) + h * (BT * 16) + r % (BT * 16), p.rows - 1);
-      const int c = ((lane & 7) ^ ((4 * q + (lane >> 4)) & 7)) * 8;
+      const int c = staged_input(lane, q);
       const uint32_t src = MODE == kGateUp ? a.order[p.first + row] / a.top_k : row;
       xo[h][u] = 2u * (src * static_cast<uint32_t>(a.x_st) + c);
     }
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && AT * BT >= 8 ? 1 : 2)
   if (tail) {
     const int k_at = a.k - tail;
     auto part = [&](const __amdgpu_buffer_rsrc_t& src, uint32_t off, int q, int place) {
-      const int c = ((lane & 7) ^ ((4 * q + (lane >> 4)) & 7)) * 8;
+      const int c = staged_input(lane, q);
       const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(src, c < tail ? off : kNowhere, 2 * k_at, 0);
       stg128(lds + place + q * 1024 + lane * 16, v);
     };
