@@ -130,13 +130,13 @@ void launch_route(const RouteArgs& a, hipStream_t s) {
 
 struct SortArgs {
   const int32_t* experts;  // [slots]
-  int32_t* order;          // slots by expert, those of one expert in their own order
+  int32_t* order;          // slots by expert
   int4* tiles;
   int32_t slots, num_experts, tile_rows, num_tiles;
 };
 
 constexpr int kSortThreads = 1024;
-constexpr int kSortAhead = 8;  // choices a lane has in flight
+constexpr int kSortAhead = 16;  // loads of four choices a lane has in flight
 
 // One workgroup an expert counts the slots of lower experts (its first place) and writes
 // its own slots and tiles. Expert e's tiles start at entry first / tile_rows + e: a later
@@ -146,27 +146,44 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
   const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int kWaves = kSortThreads / kWave;
   // Wave w has the slots [w per, (w + 1) per).
-  constexpr int kStep = kWave * kSortAhead;
-  const int per = (a.slots / kSortThreads + 1) * kWave;
+  constexpr int kRun = 4 * kWave, kStep = kRun * kSortAhead;
+  const int per = (a.slots + kSortThreads - 1) / kSortThreads * kWave;
   const int begin = min(a.slots, wave * per), end = min(a.slots, begin + per);
-  int32_t x[kSortAhead];
+  int32_t x[kSortAhead][4];
   auto load = [&](int i) {
 #pragma unroll
     for (int u = 0; u < kSortAhead; ++u) {
-      const int at = i + kWave * u + lane;
-      x[u] = at < end ? a.experts[at] : -1;
+      const int at = i + kRun * u + 4 * lane;
+      if (i + kRun * u >= end) break;
+      if (i + kRun * (u + 1) <= end) {
+        __builtin_memcpy(x[u], a.experts + at, 16);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[u][c] = at + c < end ? a.experts[at + c] : -1;
+      }
     }
   };
-  int lower = 0, own = 0;
+  int lower = 0, own = 0;  // of this lane's choices; no expert's number is below none
   for (int i = begin; i < end; i += kStep) {
     load(i);
 #pragma unroll
     for (int u = 0; u < kSortAhead; ++u) {
-      lower += __popcll(__ballot(x[u] >= 0 && x[u] < e));
-      own += __popcll(__ballot(x[u] == e));
+      if (i + kRun * u >= end) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        lower += static_cast<uint32_t>(x[u][c]) < static_cast<uint32_t>(e);
+        own += x[u][c] == e;
+      }
     }
   }
-  if (lane == 0) lower_of[wave] = lower, own_of[wave] = own;
+  int before = own;  // in this lane and those below
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int low = __shfl_up(before, d, kWave);
+    if (lane >= d) before += low;
+    lower += __shfl_xor(lower, d, kWave);
+  }
+  if (lane == kWave - 1) lower_of[wave] = lower, own_of[wave] = before;
   __syncthreads();
   int first = 0, at = 0, count = 0;
 #pragma unroll
@@ -175,14 +192,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
     at += w < wave ? own_of[w] : 0;
     count += own_of[w];
   }
-  at += first;
-  for (int i = begin; i < end && own > 0; i += kStep) {
+  at += first + before - own;
+  for (int i = begin; i < end; i += kStep) {
     if (begin + kStep < end) load(i);  // else they are still there
 #pragma unroll
     for (int u = 0; u < kSortAhead; ++u) {
-      const uint64_t hits = __ballot(x[u] == e);
-      if (x[u] == e) a.order[at + __popcll(hits & ((1ull << lane) - 1))] = i + kWave * u + lane;
-      at += __popcll(hits);
+      if (i + kRun * u >= end) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (x[u][c] == e) a.order[at++] = i + kRun * u + 4 * lane + c;
     }
   }
   const int t0 = first / a.tile_rows + e;
