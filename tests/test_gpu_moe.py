@@ -221,6 +221,47 @@ def test_terms_of_any_size(dev, dtype):
         ref.check(got[ok], want[ok], bound[ok])
 
 
+@pytest.mark.parametrize("T,K", [(8192, 8), (9001, 8), (30001, 3), (140000, 1)])
+def test_many_choices(dev, T, K):
+    check_experts(make(dev, T, 40, K, 16, 8))
+
+
+@pytest.mark.parametrize("T", [3, 130, 1501])
+def test_choices_at_any_place(dev, T):
+    x, gu, d, w, ids = make(dev, T, 12, 3, 64, 32)
+    for off in (1, 2, 3):
+        at = torch.full((off + 3 * T,), 5, dtype=torch.int32, device=dev)
+        weights = torch.zeros(off + 3 * T, device=dev)
+        at[off:], weights[off:] = ids.view(-1), w.view(-1)
+        check_experts((x, gu, d, weights[off:].view(T, 3), at[off:].view(T, 3)))
+
+
+@pytest.mark.parametrize("T", [3, 20, 500])
+def test_experts_past_32_bits(dev, T):
+    """Weights whose elements, and rows of x whose bytes, pass 2^31."""
+    x, gu, d, w, ids = make(dev, T, 4, 2, 64, 32)
+    apart = 2 ** 30 + 8
+    big = torch.empty(3 * apart + 64 * 64, dtype=x.dtype, device=dev)
+    gate_up = big.as_strided((4, 64, 64), (apart, 64, 1))
+    gate_up.copy_(gu)
+    want = check_experts((x, gate_up, d, w, ids))
+    down = big.as_strided((4, 64, 32), (apart, 32, 1))
+    down.copy_(d)
+    assert torch.equal(capi.moe_experts(x, gu, down, w, ids), want)
+
+
+@pytest.mark.parametrize("T", [500, 1000, 1100])
+def test_rows_of_experts_past_32_bits(dev, T):
+    x, gu, d, w, ids = make(dev, T, 4, 2, 64, 32)
+    far = torch.empty(T * 2 ** 20, dtype=x.dtype, device=dev).as_strided((T, 64), (2 ** 20, 1))
+    far.copy_(x)
+    check_experts((far, gu, d, w, ids))
+    out = far[:, 16:]
+    a = make(dev, T, 4, 2, 48, 32)
+    want = capi.moe_experts(*a)
+    assert torch.equal(capi.moe_experts(*a, out=out), want)
+
+
 def test_experts_of_no_tokens(dev):
     a = make(dev, 0, 4, 2, 64, 32)
     assert capi.moe_experts(*a).shape == (0, 64)
