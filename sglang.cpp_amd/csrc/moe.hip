@@ -395,7 +395,8 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   const int share = slots / x.num_experts;  // places of an expert, on average
   const int rows = !fast ? gemm::kAnyTile : share <= 64 ? 64 : share < 256 ? 128 : 256;
   const int num_tiles = slots / rows + x.num_experts;
-  if (fast) {
+  const bool scaled = fast && gemm::kScaledTerms<DT>;
+  if (scaled) {
     down.out_f32 = 0, down.o_st = l.units * 64;
     down.unit = reinterpret_cast<float*>(ws + l.unit), down.units = static_cast<int32_t>(l.units);
   }
@@ -415,7 +416,10 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   if (st != SGL_OK) return st;
   st = product(std::integral_constant<int, gemm::kDown>{}, std::false_type{}, down);
   if (st != SGL_OK) return st;
-  return fast ? combine<DT, true>(x, down, s) : combine<DT, false>(x, down, s);
+  if constexpr (gemm::kScaledTerms<DT>) {
+    if (scaled) return combine<DT, true>(x, down, s);
+  }
+  return combine<DT, false>(x, down, s);
 }
 
 }  // namespace

@@ -221,6 +221,17 @@ def test_terms_of_any_size(dev, dtype):
         ref.check(got[ok], want[ok], bound[ok])
 
 
+@pytest.mark.parametrize("T", [3, 60, 130, 400])
+def test_terms_of_fp16_are_not_rounded(dev, T):
+    """2,049 - 2,048, of which fp16 has the first only as 2,048 or 2,050."""
+    x, gu, d, w, ids = make(dev, T, 2, 2, 128, 64, "fp16")
+    x.zero_(), gu.zero_(), d.zero_()
+    x[:, 5], gu[:, :64, 5], gu[:, 64:, 5] = 1, 32, 1   # silu(32) is 32 to 2^-40
+    d[:, :, 3], d[0, :, 40] = 64, 2.0 ** -5
+    w.copy_(torch.where(ids == 0, 1.0, -1.0))
+    assert (capi.moe_experts(x, gu, d, w, ids) == 1).all()
+
+
 @pytest.mark.parametrize("T,K", [(8192, 8), (9001, 8), (30001, 3), (140000, 1)])
 def test_many_choices(dev, T, K):
     check_experts(make(dev, T, 40, K, 16, 8))
