@@ -3,7 +3,8 @@
 The extension holds HipAttnBackend, MHAKVCache, RMSNorm, RotaryEmbedding and
 AttentionLayer — the reference's BaseAttnBackend contract and the layer
 around it (include/sglang/attention/backend.h:16-41,
-src/layers/attention_layer.cc:17-51) — over libsgl_attn.so. It is built
+src/layers/attention_layer.cc:17-51) — and the layer's products, linear, GatedMLP
+and MoEMLP (src/layers/linear.cc:9-78, src/moe/moe.cc:36-98), over libsgl_attn.so. It is built
 in-tree by build.py; loading fails loudly when it is missing.
 """
 from __future__ import annotations

@@ -168,7 +168,7 @@ __device__ __forceinline__ void stream_units(const Rows (&w)[MT], const Rows (&x
     stream_tail<DT, P, MT, NT>(w, x, k, whole * kUnit, acc);
 }
 
-// P = 1: tiles of 16 rows x 64 inputs in LDS, row r's 16-byte piece c at place c ^ ((r >> 1) &
+// The ring's tiles: 16 rows x 64 inputs, row r's 16-byte piece c at place c ^ ((r >> 1) &
 // 7) of its 128 bytes, so that the 16 rows' reads of one piece are spread over all banks.
 constexpr int kPiece = 64;           // inputs of a unit
 constexpr int kTileBytes = 2048;     // 16 rows of one
