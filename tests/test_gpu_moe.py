@@ -237,6 +237,12 @@ def test_many_choices(dev, T, K):
     check_experts(make(dev, T, 40, K, 16, 8))
 
 
+@pytest.mark.parametrize("T,E,K", [(1, 700, 6), (300, 700, 4), (1500, 1025, 2), (1, 64, 40), (3, 64, 40),
+                                   (4, 64, 32), (4, 64, 33), (30, 200, 33), (100, 64, 40)])
+def test_many_experts_and_many_of_a_token(dev, T, E, K):
+    check_experts(make(dev, T, E, K, 72, 40))
+
+
 @pytest.mark.parametrize("T", [3, 130, 1501])
 def test_choices_at_any_place(dev, T):
     x, gu, d, w, ids = make(dev, T, 12, 3, 64, 32)
@@ -348,6 +354,34 @@ def test_mlp_layers(dev, T):
     weights, ids = ref.route(logits, 4, True)
     want, bound = ref.experts(x, moe.gate_up, moe.down, weights.float(), ids, res)
     ref.check(moe.forward(x, res), want, bound)
+
+
+def test_mlp_layers_in_fp16_and_captured(dev):
+    be = pkg.backend.load()
+    g = torch.Generator().manual_seed(12)
+    r = lambda *s: torch.randn(s, generator=g).to(torch.float16).to(dev)
+    mlp, moe = be.GatedMLP(128, 192, "silu_and_mul"), be.MoEMLP(128, 64, 8, 2)
+    mlp.gate_up, mlp.down = r(384, 128) / 12, r(128, 192) / 14
+    moe.router, moe.gate_up, moe.down = r(8, 128) / 4, r(8, 128, 128) / 12, r(8, 128, 64) / 8
+    for T in (1, 40, 300):
+        x, out = r(T, 128), torch.empty(T, 128, dtype=torch.float16, device=dev)
+        step = lambda: out.copy_(moe.forward(mlp.forward(x, x), x))
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for _ in range(3):
+            x.copy_(r(T, 128))
+            h = mlp.forward(x, x)
+            want, bound = ref.linear(be.linear(x, mlp.gate_up, activation="silu_and_mul"), mlp.down,
+                                     residual=x)
+            ref.check(h, want, bound)
+            want = moe.forward(h, x)
+            out.fill_(9.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
 
 
 @pytest.mark.parametrize("decode", [True, False])
