@@ -274,8 +274,8 @@ __device__ __forceinline__ int64_t weight_row(const Args& a, int n0, int r) {
 
 // Any sizes, strides and alignment: tiles of 64 weight rows x 64 tokens, staged through
 // registers and LDS, four waves of 32 x 32 outputs. Taken where rows are not whole 16 bytes
-// or strides pass what the other kernels' 32-bit offsets reach (7 x 128 x 2,048: 21 us, the
-// stream kernel 4; 8,192 x 24,576 x 4,096: 4.3 ms, tiles 1.2).
+// or strides pass what the other kernels' 32-bit offsets reach (8,192 x 24,576 x 4,096: 4.3 ms,
+// the other tiles 1.2).
 constexpr int kAnyTile = 64;
 constexpr int kAnyPitch = 40;  // 32 elements and 16 bytes: rows start on different banks
 
@@ -336,6 +336,63 @@ __global__ __launch_bounds__(256) void any_kernel(const Args a) {
   }
 }
 
+// Few tokens of any layout: 16 outputs (GATED: and their 16 up rows) and 16 tokens a workgroup,
+// whose waves share out units of 32 inputs and fold their sums. Operands come straight into
+// registers, 64 bytes of a row by four lanes, kAhead units in flight a wave. Taken up to 16
+// tokens, and above while there are at most three workgroups a CU, since each 16 tokens read
+// the weights again (1 x 6,144 x 4,097: 30 us, tiles 90; 48 x 4,096 x 12,287, 768 workgroups:
+// 224 and 284; 64 tokens: 298 and 290).
+template <int DT, bool GATED, int NW>
+__global__ __launch_bounds__(64 * NW) void any_few_kernel(const Args a) {
+  constexpr int MT = GATED ? 2 : 1, kAhead = 4;
+  __shared__ f32x4_t red[NW * MT * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = 16 * static_cast<int>(blockIdx.x), t0 = 16 * static_cast<int>(blockIdx.y);
+  const int r = lane & 15, c = 8 * (lane >> 4);
+  // Rows past the last output or token are computed from it and dropped.
+  const int64_t n = min(n0 + r, a.n - 1);
+  const uint16_t* w[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) w[i] = a.w + (i * static_cast<int64_t>(a.n) + n) * a.w_st;
+  const uint16_t* x = a.x + min(t0 + r, a.tokens - 1) * a.x_st;
+  const int whole = a.k / 32;
+  const int units = wave < whole ? (whole - wave - 1) / NW + 1 : 0;
+  f32x4_t acc[MT] = {};
+  u32x4_t fw[kAhead][MT], fx[kAhead];
+  auto load = [&](int d, int q) {
+    const int at = (wave + q * NW) * 32 + c;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) __builtin_memcpy(&fw[d][i], w[i] + at, 16);
+    __builtin_memcpy(&fx[d], x + at, 16);
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d)
+    if (d < units) load(d, d);
+  for (int q = 0; q < units; q += kAhead) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      if (q + d >= units) break;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = mfma16<DT>(fw[d][i], fx[d], acc[i]);
+      if (q + d + kAhead < units) load(d, q + d + kAhead);
+    }
+  }
+  if (whole * 32 < a.k && whole % NW == wave) {  // the last unit is a part of one
+    const u32x4_t v = load8(x, whole * 32 + c, a.k);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = mfma16<DT>(load8(w[i], whole * 32 + c, a.k), v, acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) red[(wave * MT + i) * 64 + lane] = acc[i];
+  __syncthreads();
+  if (wave > 0 || t0 + r >= a.tokens) return;
+  f32x4_t sum[MT] = {};
+  for (int v = 0; v < NW; ++v)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sum[i] += red[(v * MT + i) * 64 + lane];
+  finish4<DT, kLinear, GATED>(a, n0 + 4 * (lane >> 4), t0 + r, 1.f, sum[0], sum[MT - 1]);
+}
+
 inline bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) {
   return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0);
 }
@@ -343,6 +400,23 @@ inline bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) 
 // Workgroups of a launch, or -1 where it has more than a grid.
 inline int64_t grid_of(int64_t tiles_n, int64_t tiles_t) {
   return tiles_t > 0 && tiles_n > 0x7fffffff / tiles_t ? -1 : tiles_n * tiles_t;
+}
+
+constexpr int kCus = 256;
+constexpr int kFewWaves = 8;
+
+inline bool takes_any_few(const Args& a) {
+  const int64_t x = (static_cast<int64_t>(a.n) + 15) / 16, y = (static_cast<int64_t>(a.tokens) + 15) / 16;
+  if (x > 0xffffffffll / (64 * kFewWaves)) return false;  // a grid has fewer than 2^32 threads
+  return y == 1 || x * y <= 3 * kCus;
+}
+
+template <int DT, bool GATED>
+int launch_any_few(const Args& a, hipStream_t s) {
+  constexpr int kWaves = kFewWaves;
+  const dim3 grid(static_cast<uint32_t>((static_cast<int64_t>(a.n) + 15) / 16), (a.tokens + 15) / 16);
+  hipLaunchKernelGGL((any_few_kernel<DT, GATED, kWaves>), grid, dim3(64 * kWaves), 0, s, a);
+  return launch_status();
 }
 
 template <int DT, int MODE, bool GATED>

@@ -85,6 +85,8 @@ int run(const gemm::Args& a, bool vec, void* workspace, hipStream_t s) {
                         : gemm::launch_stream<DT, false>(st, s);
   }
   if (fast) return gated(a.act) ? run_tiles<DT, true>(a, workspace, s) : run_tiles<DT, false>(a, workspace, s);
+  if (gemm::takes_any_few(a))
+    return gated(a.act) ? gemm::launch_any_few<DT, true>(a, s) : gemm::launch_any_few<DT, false>(a, s);
   const int64_t tiles_t = (static_cast<int64_t>(a.tokens) + gemm::kAnyTile - 1) / gemm::kAnyTile;
   return gated(a.act) ? gemm::launch_any<DT, gemm::kLinear, true>(a, tiles_t, s)
                       : gemm::launch_any<DT, gemm::kLinear, false>(a, tiles_t, s);

@@ -17,7 +17,6 @@ namespace gemm {
 // Slots of one expert, found by every workgroup of a launch for itself: a few hundred
 // choices are read faster than another launch would sort them.
 constexpr int kMostSlots = 1024;
-constexpr int kCus = 256;
 // Strides whose 16 weight rows, 64 rows of x or 1,024 rows of h stay below 2^31 bytes.
 constexpr int64_t kMostStride = 1 << 20;
 

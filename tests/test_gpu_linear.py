@@ -161,6 +161,21 @@ def test_nothing_to_do(dev):
     assert pkg.backend.load().linear(x[:0], w).shape == (0, 16)
 
 
+@pytest.mark.parametrize("T,n", [(1, 700), (16, 13_000), (17, 40), (17, 13_000), (100, 40), (800, 40),
+                                 (800, 700), (12_300, 5)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_inputs_of_odd_length(dev, T, n, dtype):
+    for k in (31, 33, 333, 1025):
+        run(dev, T, n, k, dtype, "silu_and_mul" if k == 333 else "gelu", k != 31, k != 33, k == 1025)
+
+
+@pytest.mark.parametrize("n", [2 ** 27 - 16, 2 ** 27, 2 ** 27 + 5])
+def test_more_outputs_than_a_grid_of_few_tokens(dev, n):
+    x = torch.full((1, 1), 3.0, dtype=torch.bfloat16, device=dev)
+    w = (torch.arange(n, device=dev) % 251 - 125).to(torch.bfloat16).view(n, 1)
+    assert torch.equal(capi.linear(x, w).view(-1), (w * 3.0).view(-1))  # one rounding on both sides
+
+
 @pytest.mark.parametrize("T", [1, 7, 20, 60, 300])
 def test_logits_of_a_vocabulary(dev, T):
     x, w, _, _ = make(dev, T, 151_936, 128)
