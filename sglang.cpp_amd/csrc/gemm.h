@@ -32,8 +32,9 @@ struct Args {
   int32_t out_f32;  // out is fp32
   int32_t wide;     // outputs, bias and residual: 1 of four columns, 2 of eight in whole accesses
   int32_t tiles_n;  // tiles over the outputs
+  int32_t tiles;    // tiles in all
   int32_t top_k;
-  const int4* tiles;     // experts: {expert, first place, places, 0} of a tile of places
+  const int4* places;    // experts: {expert, first place, places, 0} of a tile of places
   const int32_t* order;  // experts: slot (token top_k + j) of each place
   const float* scale;    // kDown: weight of each slot
   float* unit;           // kDown in 16 bits: unit of each 64 outputs of a slot, [slots, units]
@@ -41,6 +42,18 @@ struct Args {
   float* part;           // sums of the parts of k, where a tile's is split
   int32_t splits;        // parts
 };
+
+// A dimension of a grid has fewer than 2^32 threads, and a launch with more is cut short without
+// an error. Workgroups past a row of kRow are the next row's; the last row may reach past the
+// last of them. Up to 2^31 of them, of up to 512 threads.
+constexpr int kRowShift = 22;
+constexpr int64_t kRow = 1 << kRowShift;
+
+inline dim3 rows_of(int64_t groups) {
+  return dim3(static_cast<uint32_t>(groups < kRow ? groups : kRow),
+              static_cast<uint32_t>((groups + kRow - 1) / kRow));
+}
+__device__ __forceinline__ uint32_t group_index() { return blockIdx.y << kRowShift | blockIdx.x; }
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
@@ -243,7 +256,7 @@ __device__ __forceinline__ Part part_of(const Args& a, int tile, int tile_rows) 
     const int first = tile * tile_rows;
     return {0, first, min(tile_rows, a.tokens - first)};
   } else {
-    const int4 t = a.tiles[tile];
+    const int4 t = a.places[tile];
     return {t.x, t.y, t.z};
   }
 }
@@ -282,7 +295,8 @@ constexpr int kAnyPitch = 40;  // 32 elements and 16 bytes: rows start on differ
 template <int DT, int MODE, bool GATED>
 __global__ __launch_bounds__(256) void any_kernel(const Args a) {
   __shared__ uint16_t sw[kAnyTile * kAnyPitch], sx[kAnyTile * kAnyPitch];
-  const int tn = blockIdx.x % a.tiles_n, tt = blockIdx.x / a.tiles_n;
+  if (group_index() >= static_cast<uint32_t>(a.tiles)) return;
+  const int tn = group_index() % a.tiles_n, tt = group_index() / a.tiles_n;
   const Part p = part_of<MODE>(a, tt, kAnyTile);
   if (p.rows <= 0) return;
   const int n0 = tn * (GATED ? kAnyTile / 2 : kAnyTile);
@@ -397,8 +411,8 @@ inline bool aligned(const void* p, int64_t stride, int64_t bytes, int64_t size) 
   return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0);
 }
 
-// Workgroups of a launch, or -1 where it has more than a grid.
-inline int64_t grid_of(int64_t tiles_n, int64_t tiles_t) {
+// Tiles of a product, or -1 where a launch has no numbers for them.
+inline int64_t all_tiles(int64_t tiles_n, int64_t tiles_t) {
   return tiles_t > 0 && tiles_n > 0x7fffffff / tiles_t ? -1 : tiles_n * tiles_t;
 }
 
@@ -423,9 +437,10 @@ template <int DT, int MODE, bool GATED>
 int launch_any(Args a, int64_t tiles_t, hipStream_t s) {
   const int out = GATED ? kAnyTile / 2 : kAnyTile;
   a.tiles_n = static_cast<int32_t>((static_cast<int64_t>(a.n) + out - 1) / out);
-  const int64_t grid = grid_of(a.tiles_n, tiles_t);
-  if (grid < 0) return SGL_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((any_kernel<DT, MODE, GATED>), dim3(static_cast<uint32_t>(grid)), dim3(256), 0, s, a);
+  const int64_t tiles = all_tiles(a.tiles_n, tiles_t);
+  if (tiles < 0) return SGL_ERR_UNSUPPORTED;
+  a.tiles = static_cast<int32_t>(tiles);
+  hipLaunchKernelGGL((any_kernel<DT, MODE, GATED>), rows_of(tiles), dim3(256), 0, s, a);
   return launch_status();
 }
 

@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t min16(uint32_t x) {
 template <int DT, int V>
 __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   const int l = threadIdx.x & 15;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const int64_t t = static_cast<int64_t>(gemm::group_index()) * 16 + (threadIdx.x >> 4);
   const bool real = t < a.tokens;
   const int64_t row = (real ? t : a.tokens - 1) * a.stride;
   float x[V];
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
 
 template <int DT>
 void launch_route(const RouteArgs& a, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>((a.tokens + 15) / 16)), block(256);
+  const dim3 grid = gemm::rows_of((a.tokens + 15) / 16), block(256);
   if (a.num_experts <= 64) hipLaunchKernelGGL((route_kernel<DT, 4>), grid, block, 0, s, a);
   else if (a.num_experts <= 128) hipLaunchKernelGGL((route_kernel<DT, 8>), grid, block, 0, s, a);
   else if (a.num_experts <= 256) hipLaunchKernelGGL((route_kernel<DT, 16>), grid, block, 0, s, a);
@@ -222,7 +222,7 @@ struct CombineArgs {
   const uint16_t* res;
   uint16_t* out;
   int64_t y_st, r_st, o_st;
-  int32_t hidden, top_k, num_experts, wide;
+  int32_t tokens, hidden, top_k, num_experts, wide;
 };
 
 // out[t] = the sum of its slots in their order (+ residual); slots of no expert are skipped.
@@ -231,9 +231,9 @@ struct CombineArgs {
 template <int DT, bool SCALED>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   constexpr int kAhead = 8;
-  const int64_t t = blockIdx.x;
-  const int h = 8 * (blockIdx.y * 256 + threadIdx.x);
-  if (h >= a.hidden) return;
+  const int64_t t = gemm::group_index();
+  const int h = 8 * (blockIdx.z * 256 + threadIdx.x);
+  if (h >= a.hidden || t >= a.tokens) return;
   const int32_t* ids = a.experts + t * a.top_k;
   float sum[8] = {};
   for (int j0 = 0; j0 < a.top_k; j0 += kAhead) {
@@ -332,9 +332,10 @@ int combine(const sgl_moe_t& x, const gemm::Args& down, hipStream_t s) {
   c.y = down.out, c.y_st = down.o_st, c.unit = down.unit, c.units = down.units, c.experts = x.experts;
   c.res = static_cast<const uint16_t*>(x.residual), c.r_st = x.residual_stride_row;
   c.out = static_cast<uint16_t*>(x.out), c.o_st = x.out_stride_row;
-  c.hidden = x.hidden, c.top_k = x.top_k, c.num_experts = x.num_experts;
+  c.tokens = static_cast<int32_t>(x.tokens), c.hidden = x.hidden, c.top_k = x.top_k, c.num_experts = x.num_experts;
   c.wide = aligned(x.out, x.out_stride_row, 16, 2) && aligned(x.residual, x.residual_stride_row, 16, 2);
-  const dim3 grid(static_cast<uint32_t>(x.tokens), (x.hidden + 2047) / 2048);
+  dim3 grid = gemm::rows_of(x.tokens);
+  grid.z = (x.hidden + 2047) / 2048;
   hipLaunchKernelGGL((combine_kernel<DT, SCALED>), grid, dim3(256), 0, s, c);
   return launch_status();
 }
@@ -373,7 +374,7 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   uint16_t* h = reinterpret_cast<uint16_t*>(ws + l.h);
   float* y = reinterpret_cast<float*>(ws + l.y);
   gemm::Args up{};
-  up.tiles = tiles, up.order = order, up.top_k = x.top_k, up.scale = x.weights;
+  up.places = tiles, up.order = order, up.top_k = x.top_k, up.scale = x.weights;
   gemm::Args down = up;
   up.x = static_cast<const uint16_t*>(x.x), up.x_st = x.tokens == 1 ? 0 : x.x_stride_row;
   up.w = static_cast<const uint16_t*>(x.gate_up);

@@ -292,7 +292,10 @@ __global__ __launch_bounds__(64 * NW, 2) void stream_kernel(const StreamArgs s) 
   const Args& a = s.g;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = static_cast<int>(blockIdx.x) * kOut;
+  // kLinear: rows of workgroups; experts have one of the grid's rows each.
+  const uint32_t group = MODE == kLinear ? group_index() : blockIdx.x;
+  if (group * kOut >= static_cast<uint32_t>(a.n)) return;
+  const int n0 = static_cast<int>(group) * kOut;
   int expert = 0, count = a.tokens;
   if constexpr (MODE != kLinear) {
     count = find_slots(s, list, expert);
@@ -461,7 +464,8 @@ __global__ __launch_bounds__(64 * NW) void down_few_kernel(const StreamArgs s, c
 template <int DT, int MODE, bool GATED, int MT, int NT, int NW>
 void launch_stream_as(const StreamArgs& s, int rows, hipStream_t st) {
   constexpr int kOut = (GATED ? MT / 2 : MT) * 16;
-  const dim3 grid((s.g.n + kOut - 1) / kOut, rows);
+  const int64_t groups = (static_cast<int64_t>(s.g.n) + kOut - 1) / kOut;
+  const dim3 grid = MODE == kLinear ? rows_of(groups) : dim3(static_cast<uint32_t>(groups), rows);
   hipLaunchKernelGGL((stream_kernel<DT, MODE, GATED, MT, NT, NW>), grid, dim3(64 * NW), 0, st, s);
 }
 

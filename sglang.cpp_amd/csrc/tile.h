@@ -214,8 +214,10 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void tile_kernel(const Args a) {
   static_assert(LA <= 2, "a wave's loads are of gate rows or of up rows");
   __shared__ __attribute__((aligned(1024))) char lds[S::kBytes];
   // Parts of k: all tiles of the first one, then of the next.
-  const int total = static_cast<int>(gridDim.x) / a.splits;
-  const int split = static_cast<int>(blockIdx.x) / total, block = blockIdx.x - split * total;
+  const int total = a.tiles;
+  const int split = group_index() / static_cast<uint32_t>(total);
+  if (split >= a.splits) return;
+  const int block = static_cast<int>(group_index()) - split * total;
   const Tile tile = tile_of(block, total, a.tiles_n);
   const int tn = tile.n, tt = tile.t;
   const Part p = part_of<MODE>(a, tt, S::kN);
@@ -447,17 +449,18 @@ int launch_tile(Args a, int64_t tiles_t, hipStream_t s) {
   using S = TileShape<WR, WC, AT, BT, D>;
   constexpr int out = GATED ? S::kM / 2 : S::kM;
   a.tiles_n = static_cast<int32_t>((static_cast<int64_t>(a.n) + out - 1) / out);
-  const int64_t grid = grid_of(a.tiles_n, tiles_t);
-  if (grid < 0) return SGL_ERR_UNSUPPORTED;
+  const int64_t tiles = all_tiles(a.tiles_n, tiles_t);
+  if (tiles < 0) return SGL_ERR_UNSUPPORTED;
+  a.tiles = static_cast<int32_t>(tiles);
   if (a.splits < 1) a.splits = 1;
-  hipLaunchKernelGGL((tile_kernel<DT, MODE, GATED, WR, WC, AT, BT, D>),
-                     dim3(static_cast<uint32_t>(grid * a.splits)), dim3(64 * S::kWaves), 0, s, a);
+  hipLaunchKernelGGL((tile_kernel<DT, MODE, GATED, WR, WC, AT, BT, D>), rows_of(tiles * a.splits),
+                     dim3(64 * S::kWaves), 0, s, a);
   if constexpr (MODE == kLinear) {
     if (a.splits > 1) {
       const int st = launch_status();
       if (st != SGL_OK) return st;
-      hipLaunchKernelGGL((fold_kernel<DT, GATED, WR, WC, AT, BT>), dim3(static_cast<uint32_t>(grid), 4 * BT * (GATED ? AT / 2 : AT)), dim3(64 * S::kWaves), 0,
-                         s, a);
+      hipLaunchKernelGGL((fold_kernel<DT, GATED, WR, WC, AT, BT>), dim3(a.tiles, 4 * BT * (GATED ? AT / 2 : AT)),
+                         dim3(64 * S::kWaves), 0, s, a);
     }
   }
   return launch_status();
