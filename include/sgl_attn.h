@@ -712,11 +712,9 @@ int sgl_moe_route(const void* logits, int64_t logits_stride_row, int logits_dtyp
  *   h = T(act(gate_up[e][:I] x[t]) * (gate_up[e][I:] x[t])), I = intermediate,
  * with x, out and residual [tokens, hidden], gate_up [num_experts, 2 I, hidden] and down
  * [num_experts, hidden, I] bf16 or fp16, weights fp32 and experts int32 [tokens, top_k]
- * contiguous. Sums in fp32; h is rounded to the type, as the matrix instructions take it,
- * and with many tokens the weighted terms of bf16 are rounded once more, by at most 2^-11 of
- * them (or 2^-25 of the largest of 64 outputs). A slot whose expert is outside [0,
- * num_experts) adds nothing (padding, experts of another device). An expert may be chosen
- * more than once.
+ * contiguous. Sums and weighted terms in fp32; h is rounded to the type, as the matrix
+ * instructions take it. A slot whose expert is outside [0, num_experts) adds nothing
+ * (padding, experts of another device). An expert may be chosen more than once.
  * activation: SGL_ACT_SILU_AND_MUL or SGL_ACT_GELU_AND_MUL. residual may be NULL, out may
  * be residual (same strides). workspace: sgl_moe_workspace_bytes, 16-byte aligned,
  * written before it is read; calls that share one must be stream-ordered. hidden and

@@ -37,8 +37,6 @@ struct Args {
   const int4* places;    // experts: {expert, first place, places, 0} of a tile of places
   const int32_t* order;  // experts: slot (token top_k + j) of each place
   const float* scale;    // kDown: weight of each slot
-  float* unit;           // kDown in 16 bits: unit of each 64 outputs of a slot, [slots, units]
-  int32_t units;
   float* part;           // sums of the parts of k, where a tile's is split
   int32_t splits;        // parts
 };
@@ -114,41 +112,9 @@ __device__ __forceinline__ f32x4_t activated4(const Args& a, int n0, f32x4_t g, 
   return g;
 }
 
-// A slot's weighted outputs n0 .. n0 + 7 in 16 bits, for their sum over a token's slots: as fp16
-// multiples of the power of two under the largest of 64, which 8 neighbouring lanes hold.
-// That is half of fp32's bytes for errors below 2^-11 of a value, an eighth of what rounding the
-// result to bf16 costs (rounded to bf16 the terms alone were off by as much as that). A result
-// in fp16 is rounded by 2^-11 itself: there the terms stay fp32 (error against 64 bits 0.00029,
-// not 0.00036; 8,192 tokens x 8 of 128 experts of 2,048 x 768 932 us, bf16 841). Infinite values and NaN stay
-// what they are and do not set the unit. out's rows are whole 64s.
-template <int DT>
-constexpr bool kScaledTerms = DT == SGL_DTYPE_BF16;
-
-__device__ __forceinline__ void store8_scaled(const Args& a, int n0, int64_t row, float scale,
-                                              const float (&y)[8]) {
-  if (n0 >= 64 * a.units) return;  // the same for 64 outputs
-  float v[8], most = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = n0 + i < a.n ? y[i] * scale : 0.f;
-    if (fabsf(v[i]) < INFINITY) most = fmaxf(most, fabsf(v[i]));
-  }
-  most = fmaxf(most, dpp_f32<0xB1>(most));
-  most = fmaxf(most, dpp_f32<0x4E>(most));
-  most = fmaxf(most, dpp_f32<0x141>(most));
-  // Exponent field 1 .. 253, so that the unit and its inverse are normal.
-  const uint32_t e = min(max(__float_as_uint(most) >> 23, 1u), 253u);
-  const float unit = __uint_as_float(e << 23), inverse = __uint_as_float((254u - e) << 23);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= inverse;
-  stg128(static_cast<uint16_t*>(a.out) + row * a.o_st + n0, pack8_t<SGL_DTYPE_F16>(v));
-  if (n0 % 64 == 0) a.unit[row * a.units + n0 / 64] = unit;
-}
-
 // Weight, residual and rounding of the activated outputs n0 .. n0 + 7 of one row.
 template <int DT, int MODE>
 __device__ __forceinline__ void store8(const Args& a, int n0, int64_t row, float scale, float (&y)[8]) {
-  if constexpr (MODE == kDown && kScaledTerms<DT>) return store8_scaled(a, n0, row, scale, y);
   if (n0 >= a.n) return;
   if constexpr (MODE == kDown) {
 #pragma unroll

@@ -215,9 +215,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const SortArgs a) {
 }
 
 struct CombineArgs {
-  const void* y;      // [slots, stride] weighted outputs of the slots
-  const float* unit;  // of each 64 of them where they are fp16, [slots, units]
-  int32_t units;
+  const float* y;  // [slots, stride] weighted outputs of the slots
   const int32_t* experts;
   const uint16_t* res;
   uint16_t* out;
@@ -226,9 +224,10 @@ struct CombineArgs {
 };
 
 // out[t] = the sum of its slots in their order (+ residual); slots of no expert are skipped.
-// Eight outputs a thread, eight slots' loads in flight. SCALED: y is fp16 in units, else fp32.
-// Bound by memory: 8 slots of 8,192 tokens x 2,048 47 us (6.4 TB/s).
-template <int DT, bool SCALED>
+// Eight outputs a thread, eight slots' loads in flight. y is fp32: a token's terms differ in size and
+// may cancel, so none is rounded before their sum.
+// Bound by memory: 8 slots of 8,192 tokens x 2,048 109 us (5.2 TB/s).
+template <int DT>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   constexpr int kAhead = 8;
   const int64_t t = gemm::group_index();
@@ -237,37 +236,20 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   const int32_t* ids = a.experts + t * a.top_k;
   float sum[8] = {};
   for (int j0 = 0; j0 < a.top_k; j0 += kAhead) {
-    u32x4_t v[kAhead][SCALED ? 1 : 2];
-    float unit[kAhead];
+    u32x4_t v[kAhead][2];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int j = j0 + u;
       const u32x4_t zero = {0, 0, 0, 0};
       const bool in = j < a.top_k && ids[j] >= 0 && ids[j] < a.num_experts;
       const int64_t at = (t * a.top_k + j) * a.y_st + h;
-      unit[u] = 1.f;
-      if constexpr (SCALED) {
-        v[u][0] = in ? ldg128_nt<true>(static_cast<const uint16_t*>(a.y) + at) : zero;
-        if (in) unit[u] = a.unit[(t * a.top_k + j) * a.units + h / 64];
-      } else {
-        v[u][0] = in ? ldg128_nt<true>(static_cast<const float*>(a.y) + at) : zero;
-        v[u][1] = in ? ldg128_nt<true>(static_cast<const float*>(a.y) + at + 4) : zero;
-      }
+      v[u][0] = in ? ldg128_nt<true>(a.y + at) : zero;
+      v[u][1] = in ? ldg128_nt<true>(a.y + at + 4) : zero;
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float f[8];
-      if constexpr (SCALED) {
-        unpack8_t<SGL_DTYPE_F16>(v[u][0], f);
+    for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= unit[u];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[u][i / 4][i % 4]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += f[i];
-    }
+      for (int i = 0; i < 8; ++i) sum[i] += __uint_as_float(v[u][i / 4][i % 4]);
   }
   uint16_t* o = a.out + t * a.o_st + h;
   const uint16_t* r = a.res ? a.res + t * a.r_st + h : nullptr;
@@ -299,7 +281,7 @@ constexpr int64_t kFewPlaces = 7;
 // The workspace: slots in order, tiles, the rows between the projections and the
 // weighted outputs. Rows are padded to whole 16 bytes.
 struct Layout {
-  int64_t num_tiles, h_st, y_st, units, order, tiles, h, y, unit, bytes;
+  int64_t num_tiles, h_st, y_st, order, tiles, h, y, bytes;
 };
 
 Layout layout_of(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) {
@@ -312,9 +294,7 @@ Layout layout_of(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) 
   l.tiles = up(slots * 4, 256);
   l.h = l.tiles + up(l.num_tiles * 16, 256);
   l.y = l.h + up(slots * l.h_st * 2, 256);
-  l.units = up(hidden, 64) / 64;
-  l.unit = l.y + up(slots * std::max(l.y_st * 4, l.units * 128), 256);
-  l.bytes = l.unit + up(slots * l.units * 4, 256);
+  l.bytes = l.y + up(slots * l.y_st * 4, 256);
   return l;
 }
 
@@ -326,17 +306,17 @@ bool sizes_built(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
          inter <= 1 << 20;
 }
 
-template <int DT, bool SCALED>
+template <int DT>
 int combine(const sgl_moe_t& x, const gemm::Args& down, hipStream_t s) {
   CombineArgs c{};
-  c.y = down.out, c.y_st = down.o_st, c.unit = down.unit, c.units = down.units, c.experts = x.experts;
+  c.y = static_cast<const float*>(down.out), c.y_st = down.o_st, c.experts = x.experts;
   c.res = static_cast<const uint16_t*>(x.residual), c.r_st = x.residual_stride_row;
   c.out = static_cast<uint16_t*>(x.out), c.o_st = x.out_stride_row;
   c.tokens = static_cast<int32_t>(x.tokens), c.hidden = x.hidden, c.top_k = x.top_k, c.num_experts = x.num_experts;
   c.wide = aligned(x.out, x.out_stride_row, 16, 2) && aligned(x.residual, x.residual_stride_row, 16, 2);
   dim3 grid = gemm::rows_of(x.tokens);
   grid.z = (x.hidden + 2047) / 2048;
-  hipLaunchKernelGGL((combine_kernel<DT, SCALED>), grid, dim3(256), 0, s, c);
+  hipLaunchKernelGGL(combine_kernel<DT>, grid, dim3(256), 0, s, c);
   return launch_status();
 }
 
@@ -363,7 +343,7 @@ int run_few(const sgl_moe_t& x, gemm::Args up, gemm::Args down, hipStream_t s) {
   }
   status = gemm::launch_experts<DT, gemm::kDown, false>(st, rows, s);
   if (status != SGL_OK) return status;
-  return combine<DT, false>(x, down, s);
+  return combine<DT>(x, down, s);
 }
 
 template <int DT>
@@ -400,11 +380,6 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   const int share = slots / x.num_experts;  // places of an expert, on average
   const int rows = !fast ? gemm::kAnyTile : share <= 64 ? 64 : share < 256 ? 128 : 256;
   const int num_tiles = slots / rows + x.num_experts;
-  const bool scaled = fast && gemm::kScaledTerms<DT>;
-  if (scaled) {
-    down.out_f32 = 0, down.o_st = l.units * 64;
-    down.unit = reinterpret_cast<float*>(ws + l.unit), down.units = static_cast<int32_t>(l.units);
-  }
   const SortArgs sort{x.experts, order, tiles, slots, x.num_experts, rows, num_tiles};
   hipLaunchKernelGGL(sort_kernel, dim3(x.num_experts), dim3(kSortThreads), 0, s, sort);
   int st = launch_status();
@@ -421,10 +396,7 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   if (st != SGL_OK) return st;
   st = product(std::integral_constant<int, gemm::kDown>{}, std::false_type{}, down);
   if (st != SGL_OK) return st;
-  if constexpr (gemm::kScaledTerms<DT>) {
-    if (scaled) return combine<DT, true>(x, down, s);
-  }
-  return combine<DT, false>(x, down, s);
+  return combine<DT>(x, down, s);
 }
 
 }  // namespace
