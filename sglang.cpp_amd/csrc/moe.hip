@@ -346,6 +346,20 @@ int run_few(const sgl_moe_t& x, gemm::Args up, gemm::Args down, hipStream_t s) {
   return combine<DT>(x, down, s);
 }
 
+// Elements of x that the tiles' 32-bit offsets reach (every expert's rows may be anywhere in
+// them). More are calls of their parts.
+constexpr int64_t kReach = (1ll << 30) - 1;
+
+// The call of `tokens` tokens from `first` on.
+sgl_moe_t tokens_of(sgl_moe_t x, int64_t first, int64_t tokens) {
+  x.x = static_cast<const uint16_t*>(x.x) + first * x.x_stride_row;
+  x.weights += first * x.top_k, x.experts += first * x.top_k;
+  if (x.residual) x.residual = static_cast<const uint16_t*>(x.residual) + first * x.residual_stride_row;
+  x.out = static_cast<uint16_t*>(x.out) + first * x.out_stride_row;
+  x.tokens = tokens;
+  return x;
+}
+
 template <int DT>
 int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
   const int slots = static_cast<int>(x.tokens * x.top_k);
@@ -375,8 +389,16 @@ int run(const sgl_moe_t& x, const Layout& l, char* ws, hipStream_t s) {
       std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride)
     return run_few<DT>(x, up, down, s);
 
-  const bool fast = up_vec && down_vec && x.tokens * up.x_st < (1ll << 30) &&
+  const bool fast = up_vec && down_vec &&
                     std::max({up.x_st, up.w_st, down.x_st, down.w_st}) <= gemm::kMostStride;
+  if (fast && x.tokens * up.x_st > kReach) {
+    const int64_t each = kReach / up.x_st;
+    for (int64_t t = 0; t < x.tokens; t += each) {
+      const int status = run<DT>(tokens_of(x, t, std::min(each, x.tokens - t)), l, ws, s);
+      if (status != SGL_OK) return status;
+    }
+    return SGL_OK;
+  }
   const int share = slots / x.num_experts;  // places of an expert, on average
   const int rows = !fast ? gemm::kAnyTile : share <= 64 ? 64 : share < 256 ? 128 : 256;
   const int num_tiles = slots / rows + x.num_experts;

@@ -86,3 +86,19 @@ def test_experts_past_a_grid(dev, H, I):
     many_gu[at], many_d[at] = gu, d
     got = capi.moe_experts(x, many_gu, many_d, w, at[ids.long()].int())
     ref.check(got, *ref.experts(x, gu, d, w, ids))
+
+
+# Of x 2^30 - 1 elements are in the tiles' reach: 1,023 rows of the first, 262,143 of the second.
+@pytest.mark.parametrize("T,H,I,stride,part", [(1100, 200, 72, 2 ** 20, 1023),
+                                               (262_200, 4096, 72, 4096, 262_143)])
+def test_rows_past_32_bit_offsets_are_calls_of_their_parts(dev, T, H, I, stride, part):
+    x, gu, d, w, ids = make_experts(dev, T, 4, 2, H, I)
+    far = torch.empty(T * stride, dtype=x.dtype, device=dev).as_strided((T, H), (stride, 1))
+    far.copy_(x)
+    out = x.clone()
+    assert capi.moe_experts(far, gu, d, w, ids, residual=out, out=out) is out
+    for s in (slice(0, part), slice(part, T)):
+        want = capi.moe_experts(x[s], gu, d, w[s].contiguous(), ids[s].contiguous(), residual=x[s])
+        assert torch.equal(out[s], want)
+    for s in (slice(0, 50), slice(part - 20, part + 20), slice(T - 50, T)):
+        ref.check(out[s], *ref.experts(x[s], gu, d, w[s], ids[s], x[s]))
