@@ -1155,6 +1155,7 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
 # ---------------------------------------------------------------- projections and experts
 
 _HALF = {torch.bfloat16: SGL_DTYPE_BF16, torch.float16: SGL_DTYPE_F16}
+_I32_MAX = 2 ** 31 - 1  # larger sizes would lose their upper bits on the way into an int32
 
 
 def _rows(t: torch.Tensor, shape, dtype, what: str) -> int:
@@ -1215,8 +1216,10 @@ def moe_route(logits: torch.Tensor, top_k: int,
     if logits.dim() != 2 or logits.dtype not in kinds:
         raise ValueError("logits must be a bf16, fp16 or float32 matrix")
     T, E = logits.shape
-    weights = torch.empty((T, max(top_k, 0)), dtype=torch.float32, device=dev)
-    experts = torch.empty((T, max(top_k, 0)), dtype=torch.int32, device=dev)
+    if not 1 <= top_k <= E or E > _I32_MAX:
+        raise ValueError("top_k must be in [1, num_experts], num_experts a 32-bit number")
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    experts = torch.empty((T, top_k), dtype=torch.int32, device=dev)
     with torch.cuda.device(dev):
         _check(lib().sgl_moe_route(_p(logits), _rows(logits, (T, E), logits.dtype, "logits"),
                                    kinds[logits.dtype], T, E, top_k, int(renormalize), _p(weights),
@@ -1244,9 +1247,11 @@ def moe_experts(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, weig
         raise ValueError("weights float32 and experts int32 must be contiguous [T, top_k]")
     if activation not in ("silu_and_mul", "gelu_and_mul"):
         raise ValueError("activation must be silu_and_mul or gelu_and_mul")
+    K = weights.shape[1]
+    if max(K, E, H, I) > _I32_MAX:
+        raise ValueError("top_k, num_experts, hidden and intermediate must be 32-bit numbers")
     if out is None:
         out = torch.empty((T, H), dtype=x.dtype, device=dev)
-    K = weights.shape[1]
     row = lambda t: max(t.stride(1), t.shape[2]) if t.shape[1] <= 1 else t.stride(1)
     args = MoeArgs(
         x.data_ptr(), gate_up.data_ptr(), down.data_ptr(), weights.data_ptr(), experts.data_ptr(),

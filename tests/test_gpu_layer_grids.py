@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import layer_refs as ref
-from conftest import capi
+from conftest import capi, pkg
 from test_gpu_moe import make as make_experts
 
 pytestmark = pytest.mark.gpu
@@ -102,3 +102,18 @@ def test_rows_past_32_bit_offsets_are_calls_of_their_parts(dev, T, H, I, stride,
         assert torch.equal(out[s], want)
     for s in (slice(0, 50), slice(part - 20, part + 20), slice(T - 50, T)):
         ref.check(out[s], *ref.experts(x[s], gu, d, w[s], ids[s], x[s]))
+
+
+def test_sizes_past_32_bits_are_refused(dev):
+    """2^32 + 8 is not 8: nothing is launched for a size that its 32-bit argument would cut."""
+    be = pkg.backend.load()
+    logits = torch.empty(0, 16, dtype=torch.float32, device=dev)
+    wide = torch.empty(0, 2 ** 32 + 8, dtype=torch.float32, device=dev)
+    x, gu, d, _, _ = make_experts(dev, 1, 4, 2, 16, 8)
+    choices = torch.empty(0, 2 ** 32 + 2, device=dev), torch.empty(0, 2 ** 32 + 2, dtype=torch.int32, device=dev)
+    for f in (capi, be):
+        for bad in ((logits, 2 ** 32 + 2), (logits, 17), (logits, 0), (wide, 2)):
+            with pytest.raises((ValueError, RuntimeError)):
+                f.moe_route(*bad)
+        with pytest.raises((ValueError, RuntimeError)):
+            f.moe_experts(x[:0], gu, d, *choices)
