@@ -660,7 +660,8 @@ int sgl_gelu_and_mul(void* out, const void* input, int64_t tokens, int64_t d,
  * t < tokens, j < n, i < k, and for the *_AND_MUL activations, whose weight and bias have
  * 2 n rows (gate, then up),
  *   out[t, j] = T(act(g_j) u_j + residual[t, j]), g and u the biased sums of rows j, n + j.
- * fp32 sums and arithmetic, one rounding. x, weight, bias and residual are bf16 or fp16
+ * fp32 sums and arithmetic, one rounding; act is off by at most (1 + |z|) 2^-21 of itself (or
+ * |x| 2^-126), z what its sigmoid is taken of. x, weight, bias and residual are bf16 or fp16
  * (dtype), out that type or fp32 (out_dtype SGL_DTYPE_F32: logits). bias and residual may
  * be NULL; out may be residual (same type and strides), other overlaps are the caller's
  * error. Any sizes up to 2^31 - 256, strides and alignment; fast where k is a multiple of 8 (best

@@ -892,14 +892,14 @@ void write_page_table(const torch::Tensor& page_table, const std::vector<int32_t
 // ---------------------------------------------------------------- layers
 
 namespace {
-// SGL_DTYPE_* of a 16-bit floating tensor; the reference's kernels take
-// fp16 and bf16 (normalization.cu:253-268,346-372, activation.cu:25-44,
-// rotary_embedding.cu:124-168).
 int32_t narrow_dim(int64_t v, const char* what) {
   TORCH_CHECK(v >= 0 && v <= 0x7fffffff, what, " out of range");
   return static_cast<int32_t>(v);
 }
 
+// SGL_DTYPE_* of a 16-bit floating tensor; the reference's kernels take
+// fp16 and bf16 (normalization.cu:253-268,346-372, activation.cu:25-44,
+// rotary_embedding.cu:124-168).
 int half_dtype(const torch::Tensor& t, const char* what) {
   if (t.scalar_type() == torch::kBFloat16) return SGL_DTYPE_BF16;
   TORCH_CHECK(t.scalar_type() == torch::kFloat16, what, " must be bf16 or fp16");

@@ -68,8 +68,9 @@ __device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, co
 }
 
 // x sigmoid(z), z = x (SiLU) or 2 * 0.7978845608 (x + 0.044715 x^3) (tanh GELU, since
-// (1 + tanh(u)) / 2 = sigmoid(2 u)), on the hardware exp2 and reciprocal: an fp32 ulp or
-// two, where the output is rounded to 16 bits.
+// (1 + tanh(u)) / 2 = sigmoid(2 u)), on the hardware exp2 and reciprocal. z log2(e) is rounded, so
+// the relative error grows with |z|, to (1 + |z|) 2^-21 at most: a small part of a 16-bit output's
+// rounding, all of an fp32 output's error. Below |x| 2^-126 the result is zero.
 __device__ __forceinline__ float activate(int act, float x) {
   if (act == SGL_ACT_NONE) return x;
   float z = x;

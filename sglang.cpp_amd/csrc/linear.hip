@@ -15,7 +15,7 @@ struct Shape {
   double alone, full;
 };
 constexpr Shape kShapes[] = {
-    {256, 256, 1, 1.55, 1.55},  // 1,384 TFLOP/s where they fill the CUs (8,192 x 24,576 x 4,096)
+    {256, 256, 1, 1.55, 1.55},  // 1,340 to 1,380 TFLOP/s where they fill the CUs (8,192 x 24,576 x 4,096)
     {128, 128, 2, 0.70, 1.05},  // 1,090 there; 2,048 x 4,096 x 4,096 takes 72 us, the larger ones 100
     {64, 128, 2, 0.40, 0.55},   // 512 x 4,096 x 4,096: 28 us, the others 48 and 92
 };

@@ -275,7 +275,9 @@ constexpr int64_t kMost = 1 << 30;  // choices: a workgroup's share of them stay
 constexpr int kTileRows = gemm::kAnyTile;
 // Slots an expert has on average at most where the weights are streamed: 16 at a time, more
 // take another pass (128 experts of 2,048 x 768, 8 a token: 96 tokens 215 us, tiles 234; 128
-// tokens 229 and 229).
+// tokens 229 and 229). How the choices fall is not known on the host; where all are at one expert
+// its passes come one behind the other (147 experts, one a token, spread and all at one: 128 tokens
+// 137 and 56 us, 512 222 and 259, 1,024 248 and 503; by tiles 1,025 260 and 83).
 constexpr int64_t kFewPlaces = 7;
 
 // The workspace: slots in order, tiles, the rows between the projections and the

@@ -12,7 +12,7 @@
 // each behind the reads of what it needs anew. Waves 4-7, the second one of each SIMD, run half
 // a phase behind waves 0-3: one reads while the other one multiplies. Four waves (smaller tiles,
 // two workgroups a CU): the operands of the next stage are read between the products of
-// this one. 8,192 x 24,576 x 4,096: 1,346 TFLOP/s, bound by the matrix instructions and the clock that
+// this one. 8,192 x 24,576 x 4,096: 1,340 to 1,380 TFLOP/s, bound by the matrix instructions and the clock that
 // they leave (1,830 alone on random operands).
 #pragma once
 
