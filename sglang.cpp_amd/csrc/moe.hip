@@ -280,8 +280,11 @@ constexpr int kTileRows = gemm::kAnyTile;
 // 137 and 56 us, 512 222 and 259, 1,024 248 and 503; by tiles 1,025 260 and 83).
 constexpr int64_t kFewPlaces = 7;
 
-// The workspace: slots in order, tiles, the rows between the projections and the
-// weighted outputs. Rows are padded to whole 16 bytes.
+// The workspace: slots in order, tiles, the rows h between the projections and the weighted
+// outputs. Rows are padded to whole 16 bytes. h is rounded to the type: the matrix instructions of the
+// down projection take 16-bit operands, and fp32 ones in two 16-bit parts would double its products.
+// That is as large an error as rounding the result (against 64 bits 0.0023 to 0.0024 in bf16, 0.0017
+// without it; fp16 0.00029 and 0.00021).
 struct Layout {
   int64_t num_tiles, h_st, y_st, order, tiles, h, y, bytes;
 };
